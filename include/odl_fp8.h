@@ -46,7 +46,7 @@ enum odl_status {
 };
 
 /* ABI version of this header; bumped when a signature changes or an entry point is added. */
-#define ODL_FP8_ABI_VERSION 30
+#define ODL_FP8_ABI_VERSION 31
 int odl_fp8_abi_version(void);
 
 /*
@@ -694,6 +694,73 @@ int odl_fp8_mx_gemm_splitk(const uint8_t *a, const uint8_t *sa, const uint8_t *b
 int odl_fp8_block_cast(const void *x, int src_dtype, int64_t rows, int64_t cols, int fmt, int margin, int two_d, uint8_t *out,
                        uint8_t *scales, uint8_t *out_t, uint8_t *scales_t, odl_stream_t stream);
 
+/*
+ * The residual stream between two blocks (no counterpart in the reference, whose blocks have a norm in front only and add
+ * as they are: optimus_dl/modules/model/llama2.py:121): the norm behind a block with its gate and the scaled residual, and the
+ * norm in front of the next block.
+ *   hh = h / sqrt(mean(h^2) + post_eps)  (hh = h where post_weight is NULL)
+ *   y  = residual_scale * x + gate * post_weight * hh        in the type of x
+ *   z  = bf16( y / sqrt(mean(y^2) + eps) * weight )          of the unrounded y; parts: partial maxima of |z|
+ * x [rows, cols] bf16 or fp32; h bf16, or fp32 beside an fp32 x; the weights and the gate fp32; gate: NULL, one element or cols
+ * (gate_size).  cols a multiple of 8, 8 to 8192.  stats[2 * rows]: the two reciprocal roots of every row, for the backward.
+ */
+int odl_fp8_residual_norm(const void *x, int x_dtype, const void *h, int h_dtype, const float *weight, const float *post_weight,
+                          const float *gate, int64_t gate_size, int64_t rows, int64_t cols, float residual_scale, float eps,
+                          float post_eps, void *y, void *z, float *stats, float *parts, odl_stream_t stream);
+/*
+ * Its backward for gradients dy (type of x) and dz (bf16), either of which may be NULL (zero).  dx in the type of x, dh in that of h,
+ * parts: partial maxima of |dh|; dweight[cols], dpost_weight[cols], dgate[gate_size] fp32.  dweight NULL: no gradients of weights;
+ * the other two may be NULL by themselves.  Sums over rows are fp32, in a fixed order on one device.
+ * workspace: ODL_FP8_RESIDUAL_NORM_SLABS * (2 * cols + 1) floats, contents irrelevant (needed with dweight).
+ */
+#define ODL_FP8_RESIDUAL_NORM_SLABS 512
+int odl_fp8_residual_norm_bwd(const void *dy, const void *dz, const void *x, int x_dtype, const void *h, int h_dtype,
+                              const float *weight, const float *post_weight, const float *gate, int64_t gate_size, int64_t rows,
+                              int64_t cols, float residual_scale, const float *stats, void *dx, void *dh, float *parts,
+                              float *dweight, float *dpost_weight, float *dgate, float *workspace, odl_stream_t stream);
+
+/*
+ * Log probabilities of given tokens (no counterpart in the reference: its criterion is the framework's cross entropy).
+ *   logprobs[r] = log_softmax(logits[r, :vocab] * inv_temperature)[targets[r]],  entropy[r] that of the same distribution,
+ *   top_logprobs / top_ids [rows, top_k]: the largest logits, ties to the lowest index.
+ * logits bf16 or fp32, rows `stride` elements apart, at any alignment; columns from vocab on are never read.
+ * targets[r] == ignore_index: the row is not read; 0, 0, top_logprobs 0 and top_ids -1.  Another target outside of [0, vocab): NaN.
+ * Rows of -inf only: -inf and entropy 0.  A row with NaN or +inf: NaN, top_ids -1.
+ * stats[2 * rows]: maximum and log of the sum, for the backward (may be NULL).
+ * splits: sections that the columns of a row are cut into (odl_fp8_token_logprobs_splits says how many pay); more than one need a
+ * workspace of rows * splits * (3 + 2 * top_k) floats and a second launch that joins them.
+ */
+#define ODL_FP8_LOGPROBS_MAX_TOP 64
+#define ODL_FP8_LOGPROBS_MAX_SPLITS 64
+int odl_fp8_token_logprobs_splits(int64_t rows, int64_t vocab);
+int odl_fp8_token_logprobs(const void *logits, int dtype, int64_t rows, int64_t stride, int64_t vocab, const int64_t *targets,
+                           int64_t ignore_index, float inv_temperature, int top_k, float *logprobs, float *entropy, float *stats,
+                           float *top_logprobs, int64_t *top_ids, int splits, float *workspace, odl_stream_t stream);
+/*
+ * Gradient of the logits for gradients of logprobs, entropy and top_logprobs (each may be NULL: zero), dense [rows, padded] in the
+ * type of the logits: zero for columns from vocab on and for ignored rows, NaN for rows whose target is no token.  parts: partial
+ * maxima of its magnitude, for the cast of the head's backward.  entropy, stats, top_ids as the forward wrote them.
+ */
+int odl_fp8_token_logprobs_bwd(const void *logits, int dtype, int64_t rows, int64_t stride, int64_t vocab, int64_t padded,
+                               const int64_t *targets, int64_t ignore_index, float inv_temperature, int top_k, const int64_t *top_ids,
+                               const float *stats, const float *entropy, const float *d_logprobs, const float *d_entropy,
+                               const float *d_top, void *dlogits, float *parts, odl_stream_t stream);
+
+/*
+ * Products with weights held in 4 bits (no counterpart in the reference).
+ *   y[m, n] = bf16( sum_g scales[n, g] * sum_{k in group g} x[m, k] * e2m1(codes[n, k]) + bias[n] ), fp32 accumulation
+ * codes [N, K / 2]: OCP E2M1 (sign, 2 bits of exponent, 1 of mantissa: 0, .5, 1, 1.5, 2, 3, 4, 6), two a byte, the even k in the low
+ * nibble; scales bf16 [N, K / group]; group 32, 64 or 128, a divisor of K.  x bf16 [M, K], rows ldx elements apart (a multiple of 8);
+ * bias bf16 or fp32 (bias_dtype), or NULL.  x and codes 16-byte aligned.
+ */
+int odl_fp8_fp4_linear(const void *x, int64_t ldx, const uint8_t *codes, const void *scales, int group, const void *bias,
+                       int bias_dtype, int64_t M, int64_t N, int64_t K, void *y, odl_stream_t stream);
+/*
+ * Weights [N, K] (bf16 or fp32) to such codes and scales: scale = the bf16 nearest to max|w| / 6 of the group, code = the E2M1 nearest to
+ * w / scale, ties to the even code, largest value 6.
+ */
+int odl_fp8_fp4_quantise(const void *w, int src_dtype, int64_t N, int64_t K, int group, uint8_t *codes, void *scales,
+                         odl_stream_t stream);
 
 #ifdef __cplusplus
 }

@@ -52,6 +52,12 @@ decltype(&odl_fp8_gemm_runs) runs_c;
 decltype(&odl_fp8_mx_cast_padded) mx_cast_c;
 decltype(&odl_fp8_block_cast) block_cast_c;
 decltype(&odl_fp8_mx_gemm_nt_hinted) mx_gemm_nt_c;
+decltype(&odl_fp8_residual_norm) residual_norm_c;
+decltype(&odl_fp8_residual_norm_bwd) residual_norm_bwd_c;
+decltype(&odl_fp8_token_logprobs_splits) logprobs_splits_c;
+decltype(&odl_fp8_token_logprobs) logprobs_c;
+decltype(&odl_fp8_token_logprobs_bwd) logprobs_bwd_c;
+decltype(&odl_fp8_fp4_linear) fp4_linear_c;
 
 template <class F>
 void take(F &f, const py::dict &d, const char *name) { f = reinterpret_cast<F>(py::cast<uintptr_t>(d[name])); }
@@ -88,6 +94,12 @@ void bind(const py::dict &d) {
     take(mx_cast_c, d, "odl_fp8_mx_cast_padded");
     take(block_cast_c, d, "odl_fp8_block_cast");
     take(mx_gemm_nt_c, d, "odl_fp8_mx_gemm_nt_hinted");
+    take(residual_norm_c, d, "odl_fp8_residual_norm");
+    take(residual_norm_bwd_c, d, "odl_fp8_residual_norm_bwd");
+    take(logprobs_splits_c, d, "odl_fp8_token_logprobs_splits");
+    take(logprobs_c, d, "odl_fp8_token_logprobs");
+    take(logprobs_bwd_c, d, "odl_fp8_token_logprobs_bwd");
+    take(fp4_linear_c, d, "odl_fp8_fp4_linear");
 }
 
 // as ctypes does: other Python threads run while a launch waits for room in its queue
@@ -460,6 +472,95 @@ py::object mx_gemm_nt(const Tensor &a, const Tensor &sa, const Tensor &b, const 
     return rc ? status(rc) : py::cast(c);
 }
 
+// the operands that both directions of the residual stream's step share
+bool residual_operands(const Tensor &x, const Tensor &h, const Tensor &w, const OptTensor &post, const OptTensor &gate) {
+    if (!norm_input(x) || !norm_input(h) || x.sizes() != h.sizes() || x.device() != h.device() || src_of(h) > src_of(x) || !norm_vector(w, x)) return false;
+    if (x.size(-1) % 8 || x.size(-1) < 8 || x.size(-1) > 8192) return false;
+    if (post && !norm_vector(*post, x)) return false;
+    return !gate || (gate->device() == x.device() && (floats(*gate, 1) || floats(*gate, x.size(-1))));
+}
+
+py::object residual_norm(const Tensor &x, const Tensor &h, const Tensor &w, const OptTensor &post, const OptTensor &gate, double scale, double eps,
+                         double post_eps, i64 stream) {
+    if (!residual_operands(x, h, w, post, gate)) return none();
+    const i64 cols = x.size(-1), rows = x.numel() / cols;
+    Tensor y = at::empty_like(x), z = at::empty(x.sizes(), x.options().dtype(at::kBFloat16)), stats = f32(x, {2, rows}), parts = f32(x, {kParts});
+    const int rc = call(residual_norm_c, ptr(x), src_of(x), ptr(h), src_of(h), ptr(w), ptr(post), ptr(gate), gate ? gate->numel() : 0, rows, cols,
+                        (float)scale, (float)eps, (float)post_eps, ptr(y), ptr(z), ptr(stats), ptr(parts), str(stream));
+    return rc ? status(rc) : py::make_tuple(y, z, stats, parts);
+}
+
+py::object residual_norm_bwd(const OptTensor &dy, const OptTensor &dz, const Tensor &x, const Tensor &h, const Tensor &w, const OptTensor &post,
+                             const OptTensor &gate, double scale, const Tensor &stats, bool weights, i64 stream) {
+    if (!residual_operands(x, h, w, post, gate)) return none();
+    if (dy && (!norm_input(*dy) || dy->sizes() != x.sizes() || dy->scalar_type() != x.scalar_type() || dy->device() != x.device())) return none();
+    if (dz && (!bf16(*dz) || dz->sizes() != x.sizes() || dz->device() != x.device())) return none();
+    const i64 cols = x.size(-1), rows = x.numel() / cols, g = gate ? gate->numel() : 0;
+    if (!floats(stats, 2 * rows) || stats.device() != x.device()) return none();
+    Tensor dx = at::empty_like(x), dh = at::empty_like(h), parts = f32(x, {kParts});
+    OptTensor dw, dpost, dgate, ws;
+    if (weights) {
+        dw = f32(x, {cols});
+        if (post) dpost = f32(x, {cols});
+        if (gate) dgate = f32(x, {g});
+        ws = f32(x, {ODL_FP8_RESIDUAL_NORM_SLABS * (2 * cols + 1)});
+    }
+    const int rc = call(residual_norm_bwd_c, ptr(dy), ptr(dz), ptr(x), src_of(x), ptr(h), src_of(h), ptr(w), ptr(post), ptr(gate), g, rows, cols,
+                        (float)scale, ptr(stats), ptr(dx), ptr(dh), ptr(parts), ptr(dw), ptr(dpost), ptr(dgate), ptr(ws), str(stream));
+    return rc ? status(rc) : py::make_tuple(dx, dh, parts, obj(dw), obj(dpost), obj(dgate));
+}
+
+// logits [rows, columns], rows at any distance; their other form, of any shape, goes the long way
+bool logits2d(const Tensor &l) { return l.is_cuda() && l.layout() == at::kStrided && l.dim() == 2 && src_of(l) >= 0 && l.numel() > 0 && l.stride(1) == 1 && l.stride(0) >= 0; }
+
+py::object token_logprobs(const Tensor &l, const Tensor &targets, i64 vocab, int top_k, double inv_t, i64 ignore, bool keep, i64 stream) {
+    if (!logits2d(l) || !dense(targets) || targets.scalar_type() != at::kLong || targets.numel() != l.size(0) || targets.device() != l.device()) return none();
+    const i64 rows = l.size(0);
+    if (vocab < 1 || vocab > l.size(1) || top_k < 0 || top_k > ODL_FP8_LOGPROBS_MAX_TOP) return none();
+    const int splits = logprobs_splits_c(rows, vocab);
+    Tensor out = f32(l, {2, rows});
+    OptTensor stats, top, ids, ws;
+    if (keep) stats = f32(l, {2, rows});
+    if (top_k) {
+        top = f32(l, {rows, top_k});
+        ids = at::empty({rows, top_k}, l.options().dtype(at::kLong));
+    }
+    if (splits > 1) ws = f32(l, {rows * splits * (3 + 2 * top_k)});
+    Tensor lp = out.select(0, 0), entropy = out.select(0, 1);
+    const int rc = call(logprobs_c, ptr(l), src_of(l), rows, l.stride(0), vocab, targets.data_ptr<i64>(), ignore, (float)inv_t, top_k, ptr(lp), ptr(entropy),
+                        ptr(stats), ptr(top), ptr(ids), splits, ptr(ws), str(stream));
+    return rc ? status(rc) : py::make_tuple(lp, entropy, obj(stats), obj(top), obj(ids));
+}
+
+bool row_gradient(const OptTensor &g, i64 n) { return !g || floats(*g, n); }
+
+py::object token_logprobs_bwd(const Tensor &l, const Tensor &targets, i64 vocab, int top_k, double inv_t, i64 ignore, const OptTensor &ids,
+                              const Tensor &stats, const Tensor &entropy, const OptTensor &dlp, const OptTensor &dent, const OptTensor &dtop, i64 stream) {
+    if (!logits2d(l) || !dense(targets) || targets.scalar_type() != at::kLong || targets.numel() != l.size(0)) return none();
+    const i64 rows = l.size(0), cols = l.size(1);
+    if (!floats(stats, 2 * rows) || !floats(entropy, rows) || !row_gradient(dlp, rows) || !row_gradient(dent, rows) || !row_gradient(dtop, rows * top_k))
+        return none();
+    if (dtop && (!ids || !dense(*ids) || ids->scalar_type() != at::kLong || ids->numel() != rows * top_k)) return none();
+    Tensor dl = at::empty({rows, cols}, l.options()), parts = f32(l, {kParts});
+    const int rc = call(logprobs_bwd_c, ptr(l), src_of(l), rows, l.stride(0), vocab, cols, targets.data_ptr<i64>(), ignore, (float)inv_t, top_k, ptr(ids),
+                        ptr(stats), ptr(entropy), ptr(dlp), ptr(dent), ptr(dtop), ptr(dl), ptr(parts), str(stream));
+    return rc ? status(rc) : py::make_tuple(dl, parts);
+}
+
+py::object fp4_linear(const Tensor &x, const Tensor &codes, const Tensor &scales, const OptTensor &bias, i64 stream) {
+    if (!x.is_cuda() || x.dim() != 2 || x.scalar_type() != at::kBFloat16 || x.stride(1) != 1 || x.stride(0) % 8 || !aligned(x) || !codes2d(codes) || !aligned(codes))
+        return none();
+    const i64 M = x.size(0), K = x.size(1), N = codes.size(0);
+    if (x.stride(0) < K || codes.size(1) * 2 != K || !dense(scales) || scales.scalar_type() != at::kBFloat16 || scales.dim() != 2 || scales.size(0) != N || scales.size(1) < 1 ||
+        K % scales.size(1) || codes.device() != x.device() || scales.device() != x.device())
+        return none();
+    if (bias && (!dense(*bias) || src_of(*bias) < 0 || bias->numel() != N || bias->device() != x.device())) return none();
+    Tensor y = at::empty({M, N}, x.options());
+    const int rc = call(fp4_linear_c, ptr(x), x.stride(0), ptr(codes), ptr(scales), (int)(K / scales.size(1)), ptr(bias), bias ? src_of(*bias) : 0, M, N, K, ptr(y),
+                        str(stream));
+    return rc ? status(rc) : py::cast(y);
+}
+
 }  // namespace
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
@@ -494,4 +595,9 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
     m.def("mx_cast", &mx_cast);
     m.def("block_cast", &block_cast);
     m.def("mx_gemm_nt", &mx_gemm_nt);
+    m.def("residual_norm", &residual_norm);
+    m.def("residual_norm_bwd", &residual_norm_bwd);
+    m.def("token_logprobs", &token_logprobs);
+    m.def("token_logprobs_bwd", &token_logprobs_bwd);
+    m.def("fp4_linear", &fp4_linear);
 }

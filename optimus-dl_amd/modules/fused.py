@@ -360,6 +360,84 @@ def fuse_rmsnorm(norm: nn.Module) -> bool:
     return True
 
 
+# ------------------------------------------------- residual stream between two blocks
+class _ResidualNormFn(torch.autograd.Function):
+    """y = residual_scale * x + gate * post_norm(h), z = bf16(norm(y)); x and h are kept for the backward, y is not."""
+
+    @staticmethod
+    def forward(ctx, x: torch.Tensor, h: torch.Tensor, weight: torch.Tensor, post_weight: torch.Tensor | None, gate: torch.Tensor | None,
+                residual_scale: float, eps: float, post_eps: float, recipe: FP8Recipe | None):
+        y, z, stats, parts = native.residual_norm(x, h, weight, eps, post_weight, post_eps, gate, residual_scale)
+        if recipe is not None:
+            recipe.offer_parts(z, parts)
+        ctx.save_for_backward(x, h, weight, post_weight, gate, stats)
+        ctx.set_materialize_grads(False)
+        ctx.residual_scale, ctx.recipe = residual_scale, recipe
+        return y, z
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dy: torch.Tensor | None, dz: torch.Tensor | None):
+        if dy is None and dz is None:
+            return (None,) * 9
+        x, h, weight, post_weight, gate, stats = ctx.saved_tensors
+        need = ctx.needs_input_grad
+        if dz is not None and dz.dtype != torch.bfloat16:
+            dz = dz.to(torch.bfloat16)
+        dx, dh, parts, dw, dpost, dgate = native.residual_norm_bwd(dy, dz, x, h, weight, post_weight, gate, ctx.residual_scale, stats,
+                                                                   want_weights=any(need[2:5]))
+        if ctx.recipe is not None and need[1]:
+            ctx.recipe.offer_parts(dh, parts)             # (the gradient of the Linear that ends the block)
+        given = lambda g, t, wanted: g.reshape(t.shape).to(t.dtype) if wanted and t is not None else None
+        return (dx if need[0] else None, dh if need[1] else None, given(dw, weight, need[2]), given(dpost, post_weight, need[3]),
+                given(dgate, gate, need[4]), None, None, None, None)
+
+
+def _rms(x: torch.Tensor, weight: torch.Tensor, eps: float) -> torch.Tensor:
+    return x * torch.rsqrt(x.pow(2).mean(-1, keepdim=True) + eps) * weight.to(x.dtype)
+
+
+def _residual_norm_plain(x, h, weight, eps, post_weight, post_eps, gate, residual_scale, out_dtype):
+    wide = torch.promote_types(x.dtype, torch.float32)
+    u = h.to(wide)
+    if post_weight is not None:
+        u = _rms(u, post_weight, post_eps)
+    if gate is not None:
+        u = (gate.reshape(()) if gate.numel() == 1 else gate.reshape(-1)).to(wide) * u
+    y = residual_scale * x.to(wide) + u
+    return y.to(x.dtype), _rms(y, weight, eps).to(out_dtype)
+
+
+@untraced
+def residual_norm(x: torch.Tensor, h: torch.Tensor, weight: torch.Tensor, eps: float, *, post_weight: torch.Tensor | None = None,
+                  post_eps: float | None = None, gate: torch.Tensor | None = None, residual_scale: float = 1.0,
+                  out_dtype: torch.dtype | None = None) -> tuple[torch.Tensor, torch.Tensor]:
+    """The residual stream between two blocks: ``y = residual_scale * x + gate * post_norm(h)`` and ``z = norm(y)``, norms over the last
+    axis by root mean square with weights ``post_weight`` (None: no norm behind the block) and ``weight``.  -> (y, z).
+
+    x is the stream, h what the block answered.  gate: None, one number or one for each channel, learned.  y has the type of x; z is of the
+    unrounded y and of ``out_dtype``: by default bf16 beside a bf16 stream, under an FP8 recipe and under bf16 autocast, else the type of
+    x.  One kernel each way on the GPU for z in bf16, h in bf16 (or fp32 beside an fp32 x) and up to 8192 channels, a multiple of 8; under an
+    FP8 recipe z hands its maxima to the next Linear's cast, and in the backward the gradient of h to that of the Linear before.
+    Anything else runs as torch operations in fp32."""
+    if x.shape != h.shape or x.dim() == 0:
+        raise ValueError(f"residual_norm: stream {tuple(x.shape)} and block output {tuple(h.shape)} differ")
+    cols = x.shape[-1]
+    if weight.numel() != cols or (post_weight is not None and post_weight.numel() != cols) or (gate is not None and gate.numel() not in (1, cols)):
+        raise ValueError(f"residual_norm: weights for {cols} channels, and a gate of 1 or {cols} elements")
+    recipe = _state.active_recipe()
+    if out_dtype is None:
+        bf16 = x.dtype == torch.bfloat16 or (x.is_cuda and (recipe is not None or (torch.is_autocast_enabled("cuda")
+                                                                                   and torch.get_autocast_dtype("cuda") == torch.bfloat16)))
+        out_dtype = torch.bfloat16 if bf16 else x.dtype
+    post_eps = eps if post_eps is None else post_eps
+    takes = (x.is_cuda and out_dtype == torch.bfloat16 and cols % 8 == 0 and 8 <= cols <= 8192 and x.numel() > 0
+             and (x.dtype == torch.float32 and h.dtype in (torch.bfloat16, torch.float32) or x.dtype == h.dtype == torch.bfloat16))
+    if not takes:
+        return _residual_norm_plain(x, h, weight, eps, post_weight, post_eps, gate, residual_scale, out_dtype)
+    return apply(_ResidualNormFn, x, h, weight, post_weight, gate, float(residual_scale), float(eps), float(post_eps), recipe)
+
+
 # ---------------------------------------------------------------------- LayerNorm
 class _LayerNormFn(torch.autograd.Function):
     """y = layer_norm(x) * weight + bias rounded once to bf16."""

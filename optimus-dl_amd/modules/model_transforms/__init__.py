@@ -5,6 +5,6 @@ from .config import ModelTransformConfig
 
 _MODEL_TRANSFORMS_REGISTRY, register_model_transform, build_model_transform = make_registry("model_transform")
 
-from . import fp8_linear_transform  # noqa: E402,F401  (registers "transformer_engine" and "fp8_linear")
+from . import fp4_linear_transform, fp8_linear_transform  # noqa: E402,F401  (registers "fp4_linear", "transformer_engine" and "fp8_linear")
 
 __all__ = ["BaseModelTransform", "ModelTransformConfig", "register_model_transform", "build_model_transform"]

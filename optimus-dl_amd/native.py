@@ -26,7 +26,7 @@ DT_BF16, DT_F32 = 0, 1
 AMAX_MAX, AMAX_MOST_RECENT = 0, 1
 FP8_MAX = {E4M3: 448.0, E5M2: 57344.0}
 TORCH_FP8 = {E4M3: torch.float8_e4m3fn, E5M2: torch.float8_e5m2}
-ABI_VERSION = 30
+ABI_VERSION = 31
 _OUT_DTYPES = {torch.bfloat16: DT_BF16, torch.float32: DT_F32}
 AMAX_PARTS = 512                       # ODL_FP8_AMAX_PARTS
 
@@ -104,6 +104,13 @@ EXPORTS = (
     "odl_fp8_mx_gemm_nt_hinted",
     "odl_fp8_block_cast",
     "odl_fp8_mx_gemm_splitk",
+    "odl_fp8_residual_norm",
+    "odl_fp8_residual_norm_bwd",
+    "odl_fp8_token_logprobs_splits",
+    "odl_fp8_token_logprobs",
+    "odl_fp8_token_logprobs_bwd",
+    "odl_fp8_fp4_linear",
+    "odl_fp8_fp4_quantise",
 )
 
 logger = logging.getLogger(__name__)
@@ -210,6 +217,15 @@ def load() -> ctypes.CDLL:
         L.odl_fp8_mx_gemm_nt_hinted.argtypes = [vp, vp, vp, vp, i32, i64, i64, i64, i32, i32, vp, vp, i32, i32, i32, vp]
         L.odl_fp8_block_cast.argtypes = [vp, i32, i64, i64, i32, i32, i32, vp, vp, vp, vp, vp]
         L.odl_fp8_mx_gemm_splitk.argtypes = [vp, vp, vp, vp, i64, i64, i64, i32, i32, vp, vp, i32, i32, i32, vp, i64, vp]
+        f32 = ctypes.c_float
+        L.odl_fp8_residual_norm.argtypes = [vp, i32, vp, i32, vp, vp, vp, i64, i64, i64, f32, f32, f32, vp, vp, vp, vp, vp]
+        L.odl_fp8_residual_norm_bwd.argtypes = [vp, vp, vp, i32, vp, i32, vp, vp, vp, i64, i64, i64, f32, vp, vp, vp, vp, vp, vp, vp, vp, vp]
+        L.odl_fp8_token_logprobs_splits.argtypes = [i64, i64]
+        L.odl_fp8_token_logprobs_splits.restype = i32
+        L.odl_fp8_token_logprobs.argtypes = [vp, i32, i64, i64, i64, vp, i64, f32, i32, vp, vp, vp, vp, vp, i32, vp, vp]
+        L.odl_fp8_token_logprobs_bwd.argtypes = [vp, i32, i64, i64, i64, i64, vp, i64, f32, i32, vp, vp, vp, vp, vp, vp, vp, vp, vp]
+        L.odl_fp8_fp4_linear.argtypes = [vp, i64, vp, vp, i32, vp, i32, i64, i64, i64, vp, vp]
+        L.odl_fp8_fp4_quantise.argtypes = [vp, i32, i64, i64, i32, vp, vp, vp]
         for name in EXPORTS:
             getattr(L, name)  # AttributeError here = the library does not match the header
         if L.odl_fp8_abi_version() != ABI_VERSION:
@@ -1603,3 +1619,220 @@ def gemm_set_clock_probe(records: torch.Tensor | None) -> None:
     if not (records.is_cuda and records.dtype == torch.int64 and records.dim() == 2 and records.shape[1] == 4 and records.is_contiguous()):
         raise NativeError("gemm_set_clock_probe: records must be a contiguous int64 CUDA tensor of shape [capacity, 4]")
     _check(load().odl_fp8_gemm_set_clock_probe(records.data_ptr(), records.shape[0]), "odl_fp8_gemm_set_clock_probe")
+
+
+# ------------------------------------------------------- operators around the Linear
+class _Elsewhere:
+    """Launches go to the stream of the device that holds the operands, whichever device is the current one."""
+
+    def __init__(self, *tensors: "torch.Tensor | None"):
+        devices = {t.device for t in tensors if t is not None}
+        if len(devices) != 1 or next(iter(devices)).type != "cuda":
+            raise NativeError(f"the operands have to be on one GPU; got {', '.join(sorted(map(str, devices)))}")
+        self._guard = torch.cuda.device(next(iter(devices)))
+
+    def __enter__(self) -> None:
+        load()
+        self._guard.__enter__()
+
+    def __exit__(self, *exc) -> None:
+        self._guard.__exit__(*exc)
+
+
+def _here(t: torch.Tensor) -> bool:
+    return t.is_cuda and t.get_device() == _current_device()
+
+
+def _residual_operands(x, h, weight, post_weight, gate):
+    if x.dtype not in _OUT_DTYPES or h.dtype not in _OUT_DTYPES or (x.dtype == torch.bfloat16 and h.dtype != torch.bfloat16):
+        raise NativeError(f"residual_norm: a stream of {x.dtype} with a block output of {h.dtype} (bf16 or fp32; fp32 beside fp32 only)")
+    if x.shape != h.shape or x.dim() == 0:
+        raise NativeError(f"residual_norm: shapes {tuple(x.shape)} and {tuple(h.shape)} differ")
+    cols = x.shape[-1]
+    if cols % 8 or not 8 <= cols <= 8192:
+        raise NativeError(f"residual_norm: {cols} columns (a multiple of 8 from 8 to 8192)")
+    w = _f32_vector(weight, cols, x.device, "residual_norm weight")
+    post = _f32_vector(post_weight, cols, x.device, "residual_norm post_weight")
+    g = None if gate is None else _f32_vector(gate, 1 if gate.numel() == 1 else cols, x.device, "residual_norm gate")
+    return _dense_16(x), _dense_16(h), w, post, g
+
+
+def residual_norm(x: torch.Tensor, h: torch.Tensor, weight: torch.Tensor, eps: float, post_weight: torch.Tensor | None = None,
+                  post_eps: float | None = None, gate: torch.Tensor | None = None, residual_scale: float = 1.0):
+    """y = residual_scale * x + gate * norm(h) * post_weight (h itself without post_weight) in the type of x, z = bf16(norm(y) * weight),
+    norms over the last axis by root mean square.  -> (y, z, stats fp32 [2, rows], partial maxima of |z|)."""
+    post_eps = eps if post_eps is None else post_eps
+    if _here(x):
+        load()
+        r = _host.residual_norm(x, h, weight, post_weight, gate, residual_scale, eps, post_eps, _stream())
+        if r is not None:
+            return _done(r, "odl_fp8_residual_norm")
+    with _Elsewhere(x, h, weight, post_weight, gate):
+        x, h, w, post, g = _residual_operands(x, h, weight, post_weight, gate)
+        cols = x.shape[-1]
+        rows = x.numel() // cols
+        y, z = torch.empty_like(x), torch.empty(x.shape, dtype=torch.bfloat16, device=x.device)
+        stats = torch.empty((2, rows), dtype=torch.float32, device=x.device)
+        parts = torch.empty(AMAX_PARTS, dtype=torch.float32, device=x.device)
+        _check(load().odl_fp8_residual_norm(x.data_ptr(), _src_dtype(x), h.data_ptr(), _src_dtype(h), w.data_ptr(), post.data_ptr() if post is not None else None,
+                                            g.data_ptr() if g is not None else None, g.numel() if g is not None else 0, rows, cols,
+                                            float(residual_scale), float(eps), float(post_eps), y.data_ptr(), z.data_ptr(), stats.data_ptr(),
+                                            parts.data_ptr(), _stream()), "odl_fp8_residual_norm")
+    return y, z, stats, parts
+
+
+RESIDUAL_NORM_SLABS = 512
+
+
+def residual_norm_bwd(dy: torch.Tensor | None, dz: torch.Tensor | None, x: torch.Tensor, h: torch.Tensor, weight: torch.Tensor,
+                      post_weight: torch.Tensor | None, gate: torch.Tensor | None, residual_scale: float, stats: torch.Tensor,
+                      want_weights: bool = True):
+    """Gradients of :func:`residual_norm` for those of y and z (None: zero).
+    -> (dx, dh, partial maxima of |dh|, d_weight, d_post_weight, d_gate), the last three fp32, None where there is nothing to want."""
+    if _here(x):
+        load()
+        r = _host.residual_norm_bwd(dy, dz, x, h, weight, post_weight, gate, residual_scale, stats, want_weights, _stream())
+        if r is not None:
+            return _done(r, "odl_fp8_residual_norm_bwd")
+    with _Elsewhere(x, h, weight, post_weight, gate, dy, dz, stats):
+        x, h, w, post, g = _residual_operands(x, h, weight, post_weight, gate)
+        for t, dtype, name in ((dy, x.dtype, "dy"), (dz, torch.bfloat16, "dz")):
+            if t is not None and (t.shape != x.shape or t.dtype != dtype):
+                raise NativeError(f"residual_norm backward: {name} is {t.dtype} {tuple(t.shape)}, expected {dtype} {tuple(x.shape)}")
+        dy, dz = (None if t is None else _dense_16(t) for t in (dy, dz))
+        cols = x.shape[-1]
+        rows = x.numel() // cols
+        stats = _f32_dev(stats, 2 * rows, "residual_norm backward stats")
+        dx, dh = torch.empty_like(x), torch.empty_like(h)
+        parts = torch.empty(AMAX_PARTS, dtype=torch.float32, device=x.device)
+        new = lambda n: torch.empty(n, dtype=torch.float32, device=x.device)
+        dw = dpost = dgate = ws = None
+        if want_weights:
+            dw, dpost, dgate = new(cols), None if post is None else new(cols), None if g is None else new(g.numel())
+            ws = new(RESIDUAL_NORM_SLABS * (2 * cols + 1))
+        p = lambda t: None if t is None else t.data_ptr()
+        _check(load().odl_fp8_residual_norm_bwd(p(dy), p(dz), p(x), _src_dtype(x), p(h), _src_dtype(h), p(w), p(post), p(g),
+                                                0 if g is None else g.numel(), rows, cols, float(residual_scale), p(stats), p(dx), p(dh), p(parts),
+                                                p(dw), p(dpost), p(dgate), p(ws), _stream()), "odl_fp8_residual_norm_bwd")
+    return dx, dh, parts, dw, dpost, dgate
+
+
+LOGPROBS_MAX_TOP = 64
+
+
+def _logits_operands(logits, targets, n_vocab, top_k, temperature):
+    if logits.dtype not in _OUT_DTYPES or logits.dim() != 2:
+        raise NativeError(f"token_logprobs: logits are {logits.dtype} {tuple(logits.shape)}, expected bf16 or fp32 [rows, columns]")
+    if not 1 <= n_vocab <= logits.shape[1] or logits.shape[1] > 1 << 24:
+        raise NativeError(f"token_logprobs: n_vocab {n_vocab} of {logits.shape[1]} columns (1 to 2^24)")
+    if not 0 <= top_k <= min(LOGPROBS_MAX_TOP, n_vocab):
+        raise NativeError(f"token_logprobs: top_k {top_k} (0 to {LOGPROBS_MAX_TOP}, and to the vocabulary)")
+    if not (0.0 < temperature < float("inf")) or not 0.0 < np.float32(1.0 / temperature) < np.inf:
+        raise NativeError(f"token_logprobs: temperature {temperature} (positive and finite, its inverse in fp32 too)")
+    if targets.dtype != torch.int64 or targets.numel() != logits.shape[0]:
+        raise NativeError(f"token_logprobs: targets are {targets.dtype} {tuple(targets.shape)}, expected an int64 for each of {logits.shape[0]} rows")
+    if logits.stride(1) != 1 or logits.stride(0) < 0:
+        logits = logits.contiguous()
+    return logits, targets.reshape(-1).contiguous()
+
+
+def token_logprobs(logits: torch.Tensor, targets: torch.Tensor, n_vocab: int, top_k: int = 0, temperature: float = 1.0,
+                   ignore_index: int = -100, keep_stats: bool = False):
+    """Log probabilities of targets [rows] from logits [rows, columns >= n_vocab] (bf16 or fp32, rows at any distance), with the entropy of
+    each row and its top_k largest logits (``odl_fp8_token_logprobs`` says what ignored, empty and unsound rows answer).
+    -> (logprobs, entropy, stats or None, top_logprobs or None, top_ids or None)."""
+    if _here(logits) and 0.0 < temperature < float("inf") and top_k <= n_vocab:
+        load()
+        r = _host.token_logprobs(logits, targets, n_vocab, top_k, 1.0 / temperature, ignore_index, keep_stats, _stream())
+        if r is not None:
+            return _done(r, "odl_fp8_token_logprobs")
+    with _Elsewhere(logits, targets):
+        logits, targets = _logits_operands(logits, targets, n_vocab, top_k, temperature)
+        rows = logits.shape[0]
+        new = lambda *shape: torch.empty(shape, dtype=torch.float32, device=logits.device)
+        splits = load().odl_fp8_token_logprobs_splits(rows, n_vocab)
+        out, stats = new(2, rows), new(2, rows) if keep_stats else None
+        top, ids = (new(rows, top_k), torch.empty((rows, top_k), dtype=torch.int64, device=logits.device)) if top_k else (None, None)
+        ws = new(rows * splits * (3 + 2 * top_k)) if splits > 1 else None
+        p = lambda t: None if t is None else t.data_ptr()
+        _check(load().odl_fp8_token_logprobs(p(logits), _src_dtype(logits), rows, logits.stride(0), n_vocab, p(targets), ignore_index,
+                                             1.0 / temperature, top_k, out[0].data_ptr(), out[1].data_ptr(), p(stats), p(top), p(ids), splits,
+                                             p(ws), _stream()), "odl_fp8_token_logprobs")
+    return out[0], out[1], stats, top, ids
+
+
+def token_logprobs_bwd(logits: torch.Tensor, targets: torch.Tensor, n_vocab: int, top_k: int, temperature: float, ignore_index: int,
+                       top_ids: torch.Tensor | None, stats: torch.Tensor, entropy: torch.Tensor, d_logprobs: torch.Tensor | None,
+                       d_entropy: torch.Tensor | None, d_top: torch.Tensor | None):
+    """Gradient of the logits, dense and in their type, for gradients of what :func:`token_logprobs` answered (None: zero), and the partial
+    maxima of its magnitude."""
+    if _here(logits):
+        load()
+        r = _host.token_logprobs_bwd(logits, targets, n_vocab, top_k, 1.0 / temperature, ignore_index, top_ids, stats, entropy, d_logprobs, d_entropy,
+                                     d_top, _stream())
+        if r is not None:
+            return _done(r, "odl_fp8_token_logprobs_bwd")
+    with _Elsewhere(logits, targets, top_ids, stats, entropy, d_logprobs, d_entropy, d_top):
+        logits, targets = _logits_operands(logits, targets, n_vocab, top_k, temperature)
+        rows, cols = logits.shape
+        f32 = lambda t, n, what: None if t is None else _f32_dev(t.float().contiguous(), n, "token_logprobs backward " + what)
+        d_logprobs, d_entropy, d_top = (f32(t, n, what) for t, n, what in ((d_logprobs, rows, "d_logprobs"), (d_entropy, rows, "d_entropy"),
+                                                                           (d_top, rows * top_k, "d_top_logprobs")))
+        stats, entropy = f32(stats, 2 * rows, "stats"), f32(entropy, rows, "entropy")
+        if d_top is not None:
+            if top_ids is None or top_ids.dtype != torch.int64 or top_ids.numel() != rows * top_k:
+                raise NativeError("token_logprobs backward: a gradient of the top alternatives needs their ids")
+            top_ids = top_ids.contiguous()
+        dlogits = torch.empty((rows, cols), dtype=logits.dtype, device=logits.device)
+        parts = torch.empty(AMAX_PARTS, dtype=torch.float32, device=logits.device)
+        p = lambda t: None if t is None else t.data_ptr()
+        _check(load().odl_fp8_token_logprobs_bwd(p(logits), _src_dtype(logits), rows, logits.stride(0), n_vocab, cols, p(targets), ignore_index,
+                                                 1.0 / temperature, top_k, p(top_ids), p(stats), p(entropy), p(d_logprobs), p(d_entropy), p(d_top),
+                                                 p(dlogits), p(parts), _stream()), "odl_fp8_token_logprobs_bwd")
+    return dlogits, parts
+
+
+FP4_GROUPS = (32, 64, 128)
+
+
+def fp4_linear(x: torch.Tensor, codes: torch.Tensor, scales: torch.Tensor, bias: torch.Tensor | None = None) -> torch.Tensor:
+    """x [M, K] bf16 times weights held as codes uint8 [N, K / 2] and scales bf16 [N, K / group] (``odl_fp8_fp4_linear``), plus bias [N]
+    (bf16 or fp32).  -> bf16 [M, N]."""
+    if _here(x):
+        load()
+        r = _host.fp4_linear(x, codes, scales, bias, _stream())
+        if r is not None:
+            return _done(r, "odl_fp8_fp4_linear")
+    with _Elsewhere(x, codes, scales, bias):
+        if x.dtype != torch.bfloat16 or x.dim() != 2:
+            raise NativeError(f"fp4_linear: x is {x.dtype} {tuple(x.shape)}, expected bf16 [rows, K]")
+        M, K = x.shape
+        if codes.dtype != torch.uint8 or codes.dim() != 2 or 2 * codes.shape[1] != K:
+            raise NativeError(f"fp4_linear: codes are {codes.dtype} {tuple(codes.shape)}, expected uint8 [N, {K} / 2]")
+        N = codes.shape[0]
+        if scales.dtype != torch.bfloat16 or scales.dim() != 2 or scales.shape[0] != N or not any(scales.shape[1] * g == K for g in FP4_GROUPS):
+            raise NativeError(f"fp4_linear: scales are {scales.dtype} {tuple(scales.shape)}, expected bf16 [{N}, {K} / group], group 32, 64 or 128")
+        if bias is not None and (bias.dtype not in _OUT_DTYPES or bias.shape != (N,)):
+            raise NativeError(f"fp4_linear: bias is {bias.dtype} {tuple(bias.shape)}, expected bf16 or fp32 [{N}]")
+        if x.stride(1) != 1 or x.stride(0) % 8 or x.stride(0) < K or x.data_ptr() % 16:
+            x = _dense_16(x)
+        codes, scales, bias = _dense_16(codes), scales.contiguous(), None if bias is None else bias.contiguous()
+        y = torch.empty((M, N), dtype=torch.bfloat16, device=x.device)
+        _check(load().odl_fp8_fp4_linear(x.data_ptr(), x.stride(0), codes.data_ptr(), scales.data_ptr(), K // scales.shape[1],
+                                         None if bias is None else bias.data_ptr(), DT_BF16 if bias is None else _src_dtype(bias), M, N, K, y.data_ptr(),
+                                         _stream()), "odl_fp8_fp4_linear")
+    return y
+
+
+def fp4_quantise(w: torch.Tensor, group: int):
+    """Weights [N, K] (bf16 or fp32) as :func:`fp4_linear` takes them.  -> (codes uint8 [N, K / 2], scales bf16 [N, K / group])."""
+    if group not in FP4_GROUPS or w.dim() != 2 or w.shape[1] == 0 or w.shape[1] % group:
+        raise NativeError(f"fp4_quantise: weights {tuple(w.shape)} in groups of {group} (32, 64 or 128, a divisor of the columns)")
+    with _Elsewhere(w):
+        src = _src_dtype(w)
+        w = _dense_16(w)
+        N, K = w.shape
+        codes = torch.empty((N, K // 2), dtype=torch.uint8, device=w.device)
+        scales = torch.empty((N, K // group), dtype=torch.bfloat16, device=w.device)
+        _check(load().odl_fp8_fp4_quantise(w.data_ptr(), src, N, K, group, codes.data_ptr(), scales.data_ptr(), _stream()), "odl_fp8_fp4_quantise")
+    return codes, scales

@@ -47,112 +47,403 @@ struct Fp4Args {
     const uint8_t *codes;
     const void *bias;
     uint16_t *y;
+    float *partial;                              // [runs][M][N] where K is cut into runs of several blocks
     int64_t M, N, K, ldx;
     int bias_f32;
 };
 
-template <int G, int MT, int NT, int WAVES>
-__global__ __launch_bounds__(WAVES *kWave) void fp4_linear_kernel(const Fp4Args a) {
+__device__ __forceinline__ float bias_of(const Fp4Args &a, int64_t n) {
+    if (!a.bias) return 0.0f;
+    return a.bias_f32 ? reinterpret_cast<const float *>(a.bias)[n] : bits_to_float((uint32_t)reinterpret_cast<const uint16_t *>(a.bias)[n] << 16);
+}
+
+// What a block of the thin kernel reads through LDS: the scales of its columns, and x where it is small (XLDS).  Scales are fetched by the
+// lanes of one column at a time otherwise, 16 lines of memory for 64 bytes; x in four times as many loads as the codes.  (One row, 4096 -> 14336:
+// 12.2 us with both from memory, 10.2 so; without any x and scales, which is not the product, 9.3.)
+struct Fp4Tile {
+    int groups, whole, pitch, xpitch;            // groups of a row, whole chunks, elements of a staged row of scales and of x
+};
+
+template <int G>
+__host__ __device__ inline Fp4Tile fp4_tile(int K) {
+    Fp4Tile t;
+    t.groups = K / G;
+    t.whole = K / kChunk;
+    t.pitch = ((t.whole + 1) * (kChunk / G) + 7) / 8 * 8 + 2;         // (an odd number of dwords: the 16 columns lie in different banks)
+    t.xpitch = (t.whole + 1) * kChunk + 8;
+    return t;
+}
+
+// Up to 16 * MT rows a block.  Rows and columns past the end are read as the last ones are and not stored, so that nothing is masked on
+// the way; the K behind the last whole chunk is.  Codes of the next DEPTH chunks are on their way, x (from memory) of the next half chunk.
+template <int G, int MT, int NT, int WAVES, int DEPTH, bool XLDS>
+__global__ __launch_bounds__(WAVES *kWave) void fp4_thin_kernel(const Fp4Args a) {
     constexpr int kGroups = kChunk / G;          // groups of a chunk
-    __shared__ f32x4 part[WAVES][MT * NT][kWave];
-    const int lane = threadIdx.x % kWave, wave = threadIdx.x / kWave, col = lane % 16, quarter = lane / 16;
+    constexpr int kSteps = G / 32;               // instructions of a group
+    extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
+    const int lane = threadIdx.x % kWave, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave), col = lane % 16, quarter = lane / 16;
+    const int K = (int)a.K;
+    const Fp4Tile tile = fp4_tile<G>(K);
     const int64_t n0 = (int64_t)blockIdx.x * (16 * NT), m0 = (int64_t)blockIdx.y * (16 * MT);
-    const int64_t groups = a.K / G, chunks = (a.K + kChunk - 1) / kChunk;
+    const uint8_t *cbase = a.codes + n0 * (a.K / 2);
+    const uint16_t *sbase = a.scales + n0 * tile.groups, *xbase = a.x + m0 * a.ldx;
+    uint16_t *slds = reinterpret_cast<uint16_t *>(lds), *xlds = slds + 16 * NT * tile.pitch;
+    uint32_t coff[NT], xoff[MT];
+#pragma unroll
+    for (int j = 0; j < NT; ++j) coff[j] = (uint32_t)(min(n0 + 16 * j + col, a.N - 1) - n0) * (uint32_t)(K / 2) + quarter * 16;
+#pragma unroll
+    for (int i = 0; i < MT; ++i) {
+        const uint32_t m = (uint32_t)(min(m0 + 16 * i + col, a.M - 1) - m0);
+        xoff[i] = m * (uint32_t)(XLDS ? tile.xpitch : a.ldx) + quarter * (G < 128 ? 8 : 32);
+    }
+
     f32x4 acc[MT][NT];
 #pragma unroll
     for (int i = 0; i < MT; ++i)
 #pragma unroll
         for (int j = 0; j < NT; ++j) acc[i][j] = f32x4{0, 0, 0, 0};
 
-    u32x4 codes[NT][2];
-    uint16_t scales[NT][kGroups];
-    auto fetch = [&](int64_t ch) {
+    u32x4 codes[DEPTH][NT][2], xv[XLDS ? 1 : 2][MT][4];
+    auto fetch = [&](int slot, int ch) {
+#pragma unroll
+        for (int j = 0; j < NT; ++j)
+#pragma unroll
+            for (int t = 0; t < 2; ++t) codes[slot][j][t] = *reinterpret_cast<const u32x4 *>(cbase + (uint32_t)(ch * (kChunk / 2) + t * 64) + coff[j]);
+    };
+    auto fetch_x = [&](int t, int ch) {
+#pragma unroll
+        for (int i = 0; i < MT; ++i)
+#pragma unroll
+            for (int s = 0; s < 4; ++s) {
+                const uint32_t k = ch * kChunk + t * 128 + s * (G < 128 ? 32 : 8);
+                if constexpr (XLDS) xv[0][i][s] = *reinterpret_cast<const u32x4 *>(xlds + k + xoff[i]);
+                else xv[t][i][s] = *reinterpret_cast<const u32x4 *>(xbase + k + xoff[i]);
+            }
+    };
+    auto multiply = [&](int slot, int t, int ch) {
 #pragma unroll
         for (int j = 0; j < NT; ++j) {
-            const int64_t n = n0 + 16 * j + col;
+            const u32x4 w = G < 128 ? exchange(codes[slot][j][t]) : codes[slot][j][t];
+            const uint16_t *sc = slds + (16 * j + col) * tile.pitch + ch * kGroups;
+            uint32_t pair = 0;
+            f32x4 p[MT];
 #pragma unroll
-            for (int t = 0; t < 2; ++t) {
-                const int64_t k = ch * kChunk + t * 128 + quarter * 32;
-                codes[j][t] = n < a.N && k < a.K ? *reinterpret_cast<const u32x4 *>(a.codes + (n * a.K + k) / 2) : u32x4{0, 0, 0, 0};
+            for (int s = 0; s < 4; ++s) {
+                const bf16x8 b = widen_codes(w[s]);
+                const int g = (t * 4 + s) / kSteps;
+                if (s == 0 || (s % kSteps == 0 && g % 2 == 0)) pair = *reinterpret_cast<const uint32_t *>(sc + g / 2 * 2);
+                const float scale = g % 2 ? bf16_hi(pair) : bf16_lo(pair);
+#pragma unroll
+                for (int i = 0; i < MT; ++i) {
+                    const f32x4 from = s % kSteps == 0 ? f32x4{0, 0, 0, 0} : p[i];
+                    p[i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, xv[XLDS ? 0 : t][i][s]), b, from, 0, 0, 0);
+                    if (s % kSteps == kSteps - 1)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) acc[i][j][e] = __fmaf_rn(scale, p[i][e], acc[i][j][e]);
+                }
             }
-            const uint16_t *s = a.scales + n * groups + ch * kGroups;
-            if ((ch + 1) * kChunk <= a.K) {      // (the same for every lane)
-                if (n < a.N) __builtin_memcpy(scales[j], s, sizeof(scales[j]));
-            } else {
-#pragma unroll
-                for (int g = 0; g < kGroups; ++g) scales[j][g] = n < a.N && ch * kGroups + g < groups ? s[g] : (uint16_t)0;
-            }
-            if (n >= a.N)
-#pragma unroll
-                for (int g = 0; g < kGroups; ++g) scales[j][g] = 0;
         }
     };
-    if (wave < chunks) fetch(wave);
-    for (int64_t ch = wave; ch < chunks; ch += WAVES) {
-        u32x4 now[NT][2];
-        float sc[NT][kGroups];
+    const int first = wave, last = first < tile.whole ? first + (tile.whole - 1 - first) / WAVES * WAVES : 0;
+    if (first < tile.whole) {
 #pragma unroll
-        for (int j = 0; j < NT; ++j) {
-            now[j][0] = codes[j][0];
-            now[j][1] = codes[j][1];
-#pragma unroll
-            for (int g = 0; g < kGroups; ++g) sc[j][g] = bits_to_float((uint32_t)scales[j][g] << 16);
-        }
-        bf16x8 xf[2][MT][4];
-#pragma unroll
-        for (int t = 0; t < 2; ++t)
-#pragma unroll
-            for (int i = 0; i < MT; ++i)
-#pragma unroll
-                for (int s = 0; s < 4; ++s) {
-                    const int64_t m = m0 + 16 * i + col;
-                    const int64_t k = ch * kChunk + t * 128 + (G < 128 ? s * 32 + quarter * 8 : quarter * 32 + s * 8);
-                    u32x4 v = {0, 0, 0, 0};
-                    if (m < a.M && k < a.K) v = *reinterpret_cast<const u32x4 *>(a.x + m * a.ldx + k);
-                    xf[t][i][s] = __builtin_bit_cast(bf16x8, v);
-                }
-        if (ch + WAVES < chunks) fetch(ch + WAVES);
-#pragma unroll
-        for (int t = 0; t < 2; ++t) {
-            constexpr int kSteps = G / 32;       // instructions of a group
-#pragma unroll
-            for (int j = 0; j < NT; ++j) {
-                const u32x4 w = G < 128 ? exchange(now[j][t]) : now[j][t];
-                f32x4 p[MT];
-#pragma unroll
-                for (int s = 0; s < 4; ++s) {
-                    const bf16x8 b = widen_codes(w[s]);
-#pragma unroll
-                    for (int i = 0; i < MT; ++i) {
-                        const f32x4 from = s % kSteps == 0 ? f32x4{0, 0, 0, 0} : p[i];
-                        p[i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(xf[t][i][s], b, from, 0, 0, 0);
-                        if (s % kSteps == kSteps - 1)
-#pragma unroll
-                            for (int e = 0; e < 4; ++e) acc[i][j][e] = __fmaf_rn(sc[j][(t * 4 + s) / kSteps], p[i][e], acc[i][j][e]);
-                    }
-                }
+        for (int d = 0; d < DEPTH; ++d) fetch(d, min(first + d * WAVES, last));          // (chunks behind the last are that one, and not used)
+        if constexpr (!XLDS) fetch_x(0, first);
+    }
+    {                                            // rows of scales, eight at a time; groups and columns past the end are zero
+        const int per = (tile.pitch - 2) / 8, rows = 16 * NT, have = tile.groups;
+        for (int i = threadIdx.x; i < rows * per; i += WAVES * kWave) {
+            const int r = i / per, g = i % per * 8;
+            u32x4 v = {0, 0, 0, 0};
+            const uint16_t *from = sbase + (uint32_t)(r * tile.groups + g);
+            if (n0 + r < a.N) {
+                if (g + 8 <= have) __builtin_memcpy(&v, from, 16);
+                else
+                    for (int e = 0; e < 8; ++e)
+                        if (g + e < have) v[e / 2] |= (uint32_t)from[e] << (e % 2 * 16);
             }
+            uint32_t *to = reinterpret_cast<uint32_t *>(slds + r * tile.pitch + g);
+            to[0] = v.x; to[1] = v.y; to[2] = v.z; to[3] = v.w;
         }
     }
+    if constexpr (XLDS) {                        // rows of x, the K past the end zero
+        const int rows = (int)min((int64_t)(16 * MT), a.M - m0), per = (tile.xpitch - 8) / 8;
+        for (int i = threadIdx.x; i < rows * per; i += WAVES * kWave) {
+            const int r = i / per, k = i % per * 8;
+            u32x4 v = {0, 0, 0, 0};
+            if (k < K) v = *reinterpret_cast<const u32x4 *>(xbase + (uint32_t)(r * (uint32_t)a.ldx + k));
+            *reinterpret_cast<u32x4 *>(xlds + r * tile.xpitch + k) = v;
+        }
+    }
+    __syncthreads();
+    for (int ch0 = first; ch0 < tile.whole; ch0 += DEPTH * WAVES) {
+#pragma unroll
+        for (int d = 0; d < DEPTH; ++d) {
+            const int ch = ch0 + d * WAVES;
+            if (ch >= tile.whole) break;
+            if constexpr (XLDS) fetch_x(0, ch);
+            else fetch_x(1, ch);
+            multiply(d, 0, ch);
+            if constexpr (XLDS) fetch_x(1, ch);
+            else fetch_x(0, min(ch + WAVES, last));
+            multiply(d, 1, ch);
+            fetch(d, min(ch + DEPTH * WAVES, last));
+        }
+    }
+    if (K % kChunk && wave == tile.whole % WAVES) {      // the rest of K, shorter than a chunk
+#pragma unroll
+        for (int j = 0; j < NT; ++j)
+#pragma unroll
+            for (int t = 0; t < 2; ++t) {
+                const int k = tile.whole * kChunk + t * 128 + quarter * 32;
+                codes[0][j][t] = k < K ? *reinterpret_cast<const u32x4 *>(cbase + (uint32_t)(tile.whole * (kChunk / 2) + t * 64) + coff[j]) : u32x4{0, 0, 0, 0};
+            }
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+            if constexpr (XLDS) {
+                fetch_x(t, tile.whole);
+            } else {
+#pragma unroll
+                for (int i = 0; i < MT; ++i)
+#pragma unroll
+                    for (int s = 0; s < 4; ++s) {
+                        const int k = tile.whole * kChunk + t * 128 + s * (G < 128 ? 32 : 8), from = k + quarter * (G < 128 ? 8 : 32);
+                        xv[t][i][s] = from < K ? *reinterpret_cast<const u32x4 *>(xbase + (uint32_t)k + xoff[i]) : u32x4{0, 0, 0, 0};
+                    }
+            }
+            multiply(0, t, tile.whole);
+        }
+    }
+    __syncthreads();                             // what was staged has been read
+    f32x4 *part = reinterpret_cast<f32x4 *>(lds);
 #pragma unroll
     for (int i = 0; i < MT; ++i)
 #pragma unroll
-        for (int j = 0; j < NT; ++j) part[wave][i * NT + j][lane] = acc[i][j];
+        for (int j = 0; j < NT; ++j) part[(wave * MT * NT + i * NT + j) * kWave + lane] = acc[i][j];
     __syncthreads();
     for (int o = threadIdx.x; o < MT * NT * kWave; o += WAVES * kWave) {
-        const int tile = o / kWave, l = o % kWave;
-        f32x4 s = part[0][tile][l];
+        const int t = o / kWave, l = o % kWave;
+        f32x4 s = part[o];
 #pragma unroll
-        for (int w = 1; w < WAVES; ++w) s += part[w][tile][l];
-        const int64_t n = n0 + 16 * (tile % NT) + l % 16, m = m0 + 16 * (tile / NT) + l / 16 * 4;
-        if (n < a.N) {
-            float b = 0.0f;
-            if (a.bias) b = a.bias_f32 ? reinterpret_cast<const float *>(a.bias)[n] : bits_to_float((uint32_t)reinterpret_cast<const uint16_t *>(a.bias)[n] << 16);
+        for (int w = 1; w < WAVES; ++w) s += part[w * MT * NT * kWave + o];
+        const int64_t n = n0 + 16 * (t % NT) + l % 16, m = m0 + 16 * (t / NT) + l / 16 * 4;
+        if (n >= a.N) continue;
+        const float b = bias_of(a, n);
 #pragma unroll
-            for (int e = 0; e < 4; ++e)
-                if (m + e < a.M) a.y[(m + e) * a.N + n] = (uint16_t)pack_bf16x2(a.bias ? s[e] + b : s[e], 0.0f);
+        for (int e = 0; e < 4; ++e)
+            if (m + e < a.M) a.y[(m + e) * a.N + n] = (uint16_t)pack_bf16x2(a.bias ? s[e] + b : s[e], 0.0f);
+    }
+}
+
+template <int G, int MT, int NT, int WAVES, int DEPTH, bool XLDS>
+void launch_thin(const Fp4Args &a, hipStream_t stream) {
+    const Fp4Tile t = fp4_tile<G>((int)a.K);
+    const int64_t rows = a.M < 16 * MT ? a.M : 16 * MT;
+    const int64_t staged = 2 * (16 * NT * (int64_t)t.pitch + (XLDS ? rows * t.xpitch : 0)), sums = (int64_t)WAVES * MT * NT * kWave * 16;
+    hipLaunchKernelGGL((fp4_thin_kernel<G, MT, NT, WAVES, DEPTH, XLDS>), dim3((unsigned)((a.N + 16 * NT - 1) / (16 * NT)), (unsigned)((a.M + 16 * MT - 1) / (16 * MT))),
+                       dim3(WAVES * kWave), (size_t)(staged > sums ? staged : sums), stream, a);
+}
+
+// Up to 16 * MT rows, many of them: x goes through LDS in phases of kPhase k, double-buffered, and eight waves share it, four times 32
+// columns and two halves of a phase.  Codes, scales and x of the next phase are on their way while the waves multiply.
+template <int G, int MT>
+struct Fp4Wide {
+    static constexpr int kNT = 2, kWaves = 8, kPhase = MT >= 8 ? 256 : MT >= 4 ? 512 : 1024, kHalf = kPhase / 2, kSteps = kHalf / 128, kPitch = kPhase + 8;
+    static constexpr int kPieces = 16 * MT * kPhase / 8 / (kWaves * kWave), kGroups = kHalf / G, kPairs = (kGroups + 1) / 2;
+    static constexpr int kStage = 16 * MT * kPitch;          // elements of a buffer
+};
+
+template <int G, int MT>
+__global__ __launch_bounds__(512) void fp4_wide_kernel(const Fp4Args a, int run_k, int runs) {
+    typedef Fp4Wide<G, MT> W;
+    constexpr int NT = W::kNT, kPer = G / 32;                // instructions of a group
+    __shared__ __attribute__((aligned(16))) uint16_t stage[2][W::kStage];
+    const int lane = threadIdx.x % kWave, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave), col = lane % 16, quarter = lane / 16;
+    const int half = wave / 4, K = (int)a.K, groups = K / G;
+    const int64_t n0 = (int64_t)blockIdx.x * (4 * 16 * NT) + wave % 4 * (16 * NT), m0 = (int64_t)blockIdx.y * (16 * MT);
+    const int k0 = blockIdx.z * run_k, k1 = min(K, k0 + run_k);
+    // (columns and rows past the end are the last ones and not stored)
+    const int64_t nb = min(n0, a.N - 1);
+    const uint8_t *cbase = a.codes + nb * (a.K / 2);
+    const uint16_t *sbase = a.scales + nb * groups, *xbase = a.x + m0 * a.ldx;
+    uint32_t coff[NT], soff[NT], xoff[W::kPieces];
+#pragma unroll
+    for (int j = 0; j < NT; ++j) {
+        const uint32_t n = (uint32_t)min((int64_t)(16 * j + col), a.N - 1 - nb);
+        coff[j] = n * (uint32_t)(K / 2) + quarter * 16;
+        soff[j] = n * (uint32_t)groups;
+    }
+#pragma unroll
+    for (int i = 0; i < W::kPieces; ++i) {
+        const int piece = i * 512 + threadIdx.x;
+        xoff[i] = (uint32_t)min((int64_t)(piece / (W::kPhase / 8)), a.M - 1 - m0) * (uint32_t)a.ldx + piece % (W::kPhase / 8) * 8;
+    }
+    f32x4 acc[MT][NT];
+#pragma unroll
+    for (int i = 0; i < MT; ++i)
+#pragma unroll
+        for (int j = 0; j < NT; ++j) acc[i][j] = f32x4{0, 0, 0, 0};
+
+    struct Next {
+        u32x4 codes[W::kSteps][NT], x[W::kPieces];
+        uint32_t scales[NT][W::kPairs];
+    } next;
+    auto fetch = [&](int k) {
+        const int kc = k + half * W::kHalf;
+#pragma unroll
+        for (int j = 0; j < NT; ++j) {
+#pragma unroll
+            for (int s = 0; s < W::kSteps; ++s) next.codes[s][j] = *reinterpret_cast<const u32x4 *>(cbase + (uint32_t)(kc / 2 + s * 64) + coff[j]);
+            if constexpr (W::kGroups == 1) next.scales[j][0] = sbase[(uint32_t)(kc / G) + soff[j]];
+            else __builtin_memcpy(next.scales[j], sbase + (uint32_t)(kc / G) + soff[j], sizeof(next.scales[j]));
+        }
+#pragma unroll
+        for (int i = 0; i < W::kPieces; ++i) next.x[i] = *reinterpret_cast<const u32x4 *>(xbase + (uint32_t)k + xoff[i]);
+    };
+    auto fetch_end = [&](int k) {                            // a phase that k1 ends: what is behind it is zero
+        const int kc = k + half * W::kHalf;
+#pragma unroll
+        for (int j = 0; j < NT; ++j) {
+#pragma unroll
+            for (int s = 0; s < W::kSteps; ++s) {
+                next.codes[s][j] = u32x4{0, 0, 0, 0};
+                if (kc + s * 128 + quarter * 32 < k1) next.codes[s][j] = *reinterpret_cast<const u32x4 *>(cbase + (uint32_t)(kc / 2 + s * 64) + coff[j]);
+            }
+            uint32_t v[2 * W::kPairs];                       // (all asked for before any is looked at)
+#pragma unroll
+            for (int g = 0; g < 2 * W::kPairs; ++g) v[g] = sbase[(uint32_t)min(kc / G + g, groups - 1) + soff[j]];
+#pragma unroll
+            for (int g = 0; g < W::kPairs; ++g)
+                next.scales[j][g] = (kc + 2 * g * G < k1 ? v[2 * g] : 0u) | (kc + (2 * g + 1) * G < k1 ? v[2 * g + 1] << 16 : 0u);
+        }
+#pragma unroll
+        for (int i = 0; i < W::kPieces; ++i) {
+            next.x[i] = u32x4{0, 0, 0, 0};
+            if (k + (int)((i * 512 + threadIdx.x) % (W::kPhase / 8)) * 8 < k1) next.x[i] = *reinterpret_cast<const u32x4 *>(xbase + (uint32_t)k + xoff[i]);
+        }
+    };
+    auto put = [&](uint16_t *to) {
+#pragma unroll
+        for (int i = 0; i < W::kPieces; ++i) {
+            const int piece = i * 512 + threadIdx.x, r = piece / (W::kPhase / 8), p = piece % (W::kPhase / 8) * 8;
+            *reinterpret_cast<u32x4 *>(to + r * W::kPitch + p) = next.x[i];
+        }
+    };
+    if (k0 + W::kPhase <= k1) fetch(k0);
+    else fetch_end(k0);
+    put(stage[0]);
+    __syncthreads();
+    int buf = 0;
+    for (int k = k0; k < k1; k += W::kPhase, buf ^= 1) {
+        u32x4 codes[W::kSteps][NT];
+        uint32_t scales[NT][W::kPairs];
+#pragma unroll
+        for (int j = 0; j < NT; ++j) {
+#pragma unroll
+            for (int s = 0; s < W::kSteps; ++s) codes[s][j] = next.codes[s][j];
+#pragma unroll
+            for (int g = 0; g < W::kPairs; ++g) scales[j][g] = next.scales[j][g];
+        }
+        const bool more = k + W::kPhase < k1;
+        if (k + 2 * W::kPhase <= k1) fetch(k + W::kPhase);
+        else if (more) fetch_end(k + W::kPhase);
+        const uint16_t *xs = stage[buf] + col * W::kPitch + half * W::kHalf + quarter * (G < 128 ? 8 : 32);
+        // Units of 16 rows and one group of k, software-pipelined: x is asked for kAhead units before its products, and the products of a
+        // unit are scaled onto the sums behind the products of the next kBehind.
+        constexpr int kUnits = W::kSteps * (4 / kPer) * MT, kAhead = 4 / kPer, kBehind = kPer > 2 ? 1 : 2;
+        bf16x8 xq[kAhead + 1][kPer], b[NT][kPer];
+        f32x4 p[kBehind + 1][NT];
+        float scale[4][NT];
+        auto ask = [&](int u) {                  // (every index is known at compile time)
+            const int i = u % MT, s0 = u / MT * kPer;
+#pragma unroll
+            for (int s = 0; s < kPer; ++s)
+                xq[u % (kAhead + 1)][s] = __builtin_bit_cast(
+                    bf16x8, *reinterpret_cast<const u32x4 *>(xs + i * 16 * W::kPitch + (s0 + s) / 4 * 128 + (s0 + s) % 4 * (G < 128 ? 32 : 8)));
+        };
+#pragma unroll
+        for (int u = 0; u < (kAhead < kUnits ? kAhead : kUnits); ++u) ask(u);
+        u32x4 w[NT];
+#pragma unroll
+        for (int u = 0; u < kUnits + kBehind; ++u) {
+            if (u + kAhead < kUnits) ask(u + kAhead);
+            if (u < kUnits) {
+                const int g = u / MT, s0 = g * kPer;
+                if (u % MT == 0) {
+#pragma unroll
+                    for (int j = 0; j < NT; ++j) {
+                        if (s0 % 4 == 0) w[j] = G < 128 ? exchange(codes[s0 / 4][j]) : codes[s0 / 4][j];
+                        scale[g % 4][j] = g % 2 ? bf16_hi(scales[j][g / 2]) : bf16_lo(scales[j][g / 2]);
+#pragma unroll
+                        for (int s = 0; s < kPer; ++s) b[j][s] = widen_codes(w[j][(s0 + s) % 4]);
+                    }
+                }
+#pragma unroll
+                for (int s = 0; s < kPer; ++s)
+#pragma unroll
+                    for (int j = 0; j < NT; ++j)
+                        p[u % (kBehind + 1)][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(xq[u % (kAhead + 1)][s], b[j][s], s == 0 ? f32x4{0, 0, 0, 0} : p[u % (kBehind + 1)][j], 0, 0, 0);
+            }
+            if (u >= kBehind) {
+                const int v = u - kBehind, i = v % MT;
+#pragma unroll
+                for (int j = 0; j < NT; ++j) {
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) acc[i][j][e] = __fmaf_rn(scale[v / MT % 4][j], p[v % (kBehind + 1)][j][e], acc[i][j][e]);
+                    asm volatile("" : "+v"(acc[i][j]));      // (not put off behind the loop, which would spill the products)
+                }
+            }
+            __builtin_amdgcn_sched_barrier(0);
+        }
+        if (more) put(stage[buf ^ 1]);
+        __syncthreads();
+    }
+    // the second half's sums onto the first's
+    f32x4 *part = reinterpret_cast<f32x4 *>(stage[0]) + (wave % 4) * (MT * NT * kWave) + lane;
+    static_assert(sizeof(stage) >= 4 * MT * NT * kWave * sizeof(f32x4), "the sums fit into the stage");
+    if (half) {
+#pragma unroll
+        for (int i = 0; i < MT; ++i)
+#pragma unroll
+            for (int j = 0; j < NT; ++j) part[(i * NT + j) * kWave] = acc[i][j];
+    }
+    __syncthreads();
+    if (half) return;
+#pragma unroll
+    for (int j = 0; j < NT; ++j) {
+        const int64_t n = n0 + 16 * j + col;
+        if (n >= a.N) continue;
+        const float b = bias_of(a, n);
+#pragma unroll
+        for (int i = 0; i < MT; ++i) {
+            const f32x4 s = acc[i][j] + part[(i * NT + j) * kWave];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const int64_t m = m0 + 16 * i + quarter * 4 + e;
+                if (m >= a.M) continue;
+                if (runs > 1) a.partial[(blockIdx.z * a.M + m) * a.N + n] = s[e];
+                else a.y[m * a.N + n] = (uint16_t)pack_bf16x2(a.bias ? s[e] + b : s[e], 0.0f);
+            }
         }
     }
+}
+
+template <int G, int MT>
+int launch_wide(const Fp4Args &a, int runs, hipStream_t stream) {
+    const int phase = Fp4Wide<G, MT>::kPhase, run_k = (int)((a.K + runs - 1) / runs + phase - 1) / phase * phase;
+    runs = (int)((a.K + run_k - 1) / run_k);                 // (no run is empty)
+    hipLaunchKernelGGL((fp4_wide_kernel<G, MT>), dim3((unsigned)((a.N + 127) / 128), (unsigned)((a.M + 16 * MT - 1) / (16 * MT)), (unsigned)runs), dim3(512), 0, stream, a, run_k, runs);
+    return runs;
+}
+
+// Runs of K of several blocks, added in their order.
+__global__ __launch_bounds__(256) void fp4_join_kernel(const Fp4Args a, int runs) {
+    const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x, total = a.M * a.N;
+    if (i >= total) return;
+    float s = a.partial[i];
+    for (int r = 1; r < runs; ++r) s += a.partial[r * total + i];
+    if (a.bias) s += bias_of(a, i % a.N);
+    a.y[i] = (uint16_t)pack_bf16x2(s, 0.0f);
 }
 
 // Weights to codes.  A group's scale is the bf16 nearest to max|w| / 6 (6 is the largest E2M1); a code is the E2M1 nearest to w / scale, ties to
@@ -208,14 +499,47 @@ __global__ __launch_bounds__(256) void fp4_quantise_kernel(const void *__restric
 bool aligned16(const void *p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 bool group_known(int group) { return group == 32 || group == 64 || group == 128; }
 
+// Which kernel, by what it was measured to take (us):
+//   up to 4 rows, thin with x in LDS: 4096 -> 14336 10.2 (wide 17), 768 -> 2304 3.2 (10)
+//   matrices of less than 4 M weights, thin: 24 rows 768 -> 2304 4.7 (wide 10.4: its phases do not pay for themselves)
+//   else wide: 16 rows 4096 -> 14336 14.8 (thin 16.3), 32 rows 14336 -> 4096 20.9 (22.9), 120 rows 8192 -> 28672 109 (174)
+// The thin kernel stages the scales of whole rows, which for a very long K do not fit.
+constexpr int64_t kThinLds = 64 * 1024;
+
 template <int G>
-void launch_linear(const Fp4Args &a, hipStream_t stream) {
-#define ODL_FP4(MT, NT, WAVES)                                                                                                              \
-    hipLaunchKernelGGL((fp4_linear_kernel<G, MT, NT, WAVES>), dim3((unsigned)((a.N + 16 * NT - 1) / (16 * NT)), (unsigned)((a.M + 16 * MT - 1) / (16 * MT))), \
-                       dim3(WAVES * kWave), 0, stream, a)
-    if (a.M <= 16) ODL_FP4(1, 1, 8);
-    else ODL_FP4(2, 1, 8);
-#undef ODL_FP4
+bool takes_thin(int64_t M, int64_t N, int64_t K) {
+    return 2 * 16 * (int64_t)fp4_tile<G>((int)K).pitch <= kThinLds && (M <= 4 || N * K < (int64_t)4 << 20);
+}
+
+// rows of a block of the wide kernel, in 16s
+int wide_rows(int64_t M) { return M <= 16 ? 1 : M <= 64 ? 2 : 8; }
+
+// Runs of K that fill the chip with blocks of the wide kernel, none shorter than a phase.
+int wide_runs(int64_t M, int64_t N, int64_t K) {
+    const int mt = wide_rows(M);
+    const int64_t blocks = (N + 127) / 128 * ((M + 16 * mt - 1) / (16 * mt)), most = K / (mt == 8 ? 256 : 1024);
+    int64_t r = device_cu_count() / blocks;
+    r = r < most ? r : most;
+    return (int)(r < 1 ? 1 : r);
+}
+
+template <int G>
+void launch_linear(const Fp4Args &a, int runs, hipStream_t stream) {
+    if (takes_thin<G>(a.M, a.N, a.K)) {
+        const Fp4Tile t = fp4_tile<G>((int)a.K);
+        const bool lds = a.M <= 4 && 2 * (16 * (int64_t)t.pitch + a.M * t.xpitch) <= kThinLds, deep = t.whole >= 32;
+        // long rows: 16 waves share them (14336 -> 4096 11.5 -> 10.5, 4096 -> 14336 no faster)
+        if (lds && deep) launch_thin<G, 1, 1, 16, 1, true>(a, stream);
+        else if (lds) launch_thin<G, 1, 1, 8, 1, true>(a, stream);
+        else if (a.M <= 16) launch_thin<G, 1, 1, 8, 1, false>(a, stream);
+        else launch_thin<G, 2, 1, 4, 1, false>(a, stream);
+        return;
+    }
+    const int mt = wide_rows(a.M);
+    if (mt == 1) runs = launch_wide<G, 1>(a, runs, stream);
+    else if (mt == 2) runs = launch_wide<G, 2>(a, runs, stream);
+    else runs = launch_wide<G, 8>(a, runs, stream);
+    if (runs > 1) hipLaunchKernelGGL(fp4_join_kernel, dim3((unsigned)((a.M * a.N + 255) / 256)), dim3(256), 0, stream, a, runs);
 }
 
 }  // namespace
@@ -223,8 +547,16 @@ void launch_linear(const Fp4Args &a, hipStream_t stream) {
 
 using namespace odl;
 
+// Partial results that a call writes: its workspace is as many times M * N floats; 0 needs none.
+extern "C" int odl_fp8_fp4_linear_runs(int64_t M, int64_t N, int64_t K, int group) {
+    if (M < 1 || N < 1 || K < 1 || K > (int64_t)1 << 24) return 0;
+    const bool thin = group == 32 ? takes_thin<32>(M, N, K) : group == 64 ? takes_thin<64>(M, N, K) : takes_thin<128>(M, N, K);
+    const int runs = thin ? 1 : wide_runs(M, N, K);
+    return runs > 1 ? runs : 0;
+}
+
 extern "C" int odl_fp8_fp4_linear(const void *x, int64_t ldx, const uint8_t *codes, const void *scales, int group, const void *bias, int bias_dtype,
-                                  int64_t M, int64_t N, int64_t K, void *y, odl_stream_t stream_) {
+                                  int64_t M, int64_t N, int64_t K, void *y, float *workspace, int64_t workspace_bytes, odl_stream_t stream_) {
     hipStream_t stream = reinterpret_cast<hipStream_t>(stream_);
     if (M < 0 || N < 0 || K < 0) return set_error(ODL_ERR_ARG, "odl_fp8_fp4_linear: negative shape");
     if (!group_known(group)) return set_error(ODL_ERR_ARG, "odl_fp8_fp4_linear: group %d (32, 64 or 128)", group);
@@ -232,15 +564,20 @@ extern "C" int odl_fp8_fp4_linear(const void *x, int64_t ldx, const uint8_t *cod
     if (K < group || K % group != 0) return set_error(ODL_ERR_SHAPE, "odl_fp8_fp4_linear: K must be a multiple of the group");
     if (M == 0 || N == 0) return ODL_OK;
     if (!x || !codes || !scales || !y) return set_error(ODL_ERR_ARG, "odl_fp8_fp4_linear: null pointer");
-    if (ldx % 8 != 0 || (M > 1 && ldx < K) || !aligned16(x) || !aligned16(codes))
-        return set_error(ODL_ERR_SHAPE, "odl_fp8_fp4_linear: x and codes must be 16-byte aligned, rows of x too");
-    if (N > (int64_t)1 << 24 || M > (int64_t)1 << 20) return set_error(ODL_ERR_SHAPE, "odl_fp8_fp4_linear: up to 2^24 columns and 2^20 rows");
+    if (ldx % 8 != 0 || (M > 1 && ldx < K) || ldx > (int64_t)1 << 24 || !aligned16(x) || !aligned16(codes))
+        return set_error(ODL_ERR_SHAPE, "odl_fp8_fp4_linear: x and codes must be 16-byte aligned, rows of x too, at most 2^24 elements apart");
+    if (N > (int64_t)1 << 22 || M > (int64_t)1 << 16 || K > (int64_t)1 << 24)
+        return set_error(ODL_ERR_SHAPE, "odl_fp8_fp4_linear: up to 2^16 rows, 2^22 columns and 2^24 inputs");
+    const int runs = odl_fp8_fp4_linear_runs(M, N, K, group);
+    if (runs && (!workspace || workspace_bytes / 4 / M / N < runs))
+        return set_error(ODL_ERR_ARG, "odl_fp8_fp4_linear: a workspace of %d * M * N floats is needed", runs);
+    if (runs && M * N >= (int64_t)1 << 32) return set_error(ODL_ERR_SHAPE, "odl_fp8_fp4_linear: an output of that size is not cut over K");
     Fp4Args a = {};
     a.x = static_cast<const uint16_t *>(x); a.scales = static_cast<const uint16_t *>(scales); a.codes = codes; a.bias = bias; a.y = static_cast<uint16_t *>(y);
-    a.M = M; a.N = N; a.K = K; a.ldx = ldx; a.bias_f32 = bias_dtype == ODL_F32;
-    if (group == 32) launch_linear<32>(a, stream);
-    else if (group == 64) launch_linear<64>(a, stream);
-    else launch_linear<128>(a, stream);
+    a.partial = workspace; a.M = M; a.N = N; a.K = K; a.ldx = M > 1 ? ldx : 0; a.bias_f32 = bias_dtype == ODL_F32;
+    if (group == 32) launch_linear<32>(a, runs ? runs : 1, stream);
+    else if (group == 64) launch_linear<64>(a, runs ? runs : 1, stream);
+    else launch_linear<128>(a, runs ? runs : 1, stream);
     return check_launch("odl_fp8_fp4_linear");
 }
 

@@ -57,6 +57,7 @@ decltype(&odl_fp8_residual_norm_bwd) residual_norm_bwd_c;
 decltype(&odl_fp8_token_logprobs_splits) logprobs_splits_c;
 decltype(&odl_fp8_token_logprobs) logprobs_c;
 decltype(&odl_fp8_token_logprobs_bwd) logprobs_bwd_c;
+decltype(&odl_fp8_fp4_linear_runs) fp4_runs_c;
 decltype(&odl_fp8_fp4_linear) fp4_linear_c;
 
 template <class F>
@@ -99,6 +100,7 @@ void bind(const py::dict &d) {
     take(logprobs_splits_c, d, "odl_fp8_token_logprobs_splits");
     take(logprobs_c, d, "odl_fp8_token_logprobs");
     take(logprobs_bwd_c, d, "odl_fp8_token_logprobs_bwd");
+    take(fp4_runs_c, d, "odl_fp8_fp4_linear_runs");
     take(fp4_linear_c, d, "odl_fp8_fp4_linear");
 }
 
@@ -551,12 +553,16 @@ py::object fp4_linear(const Tensor &x, const Tensor &codes, const Tensor &scales
     if (!x.is_cuda() || x.dim() != 2 || x.scalar_type() != at::kBFloat16 || x.stride(1) != 1 || x.stride(0) % 8 || !aligned(x) || !codes2d(codes) || !aligned(codes))
         return none();
     const i64 M = x.size(0), K = x.size(1), N = codes.size(0);
-    if (x.stride(0) < K || codes.size(1) * 2 != K || !dense(scales) || scales.scalar_type() != at::kBFloat16 || scales.dim() != 2 || scales.size(0) != N || scales.size(1) < 1 ||
+    if (x.stride(0) < K || x.stride(0) > (1 << 24) || codes.size(1) * 2 != K || !dense(scales) || scales.scalar_type() != at::kBFloat16 || scales.dim() != 2 || scales.size(0) != N || scales.size(1) < 1 ||
         K % scales.size(1) || codes.device() != x.device() || scales.device() != x.device())
         return none();
     if (bias && (!dense(*bias) || src_of(*bias) < 0 || bias->numel() != N || bias->device() != x.device())) return none();
+    const int group = (int)(K / scales.size(1));
+    const i64 partial = (i64)fp4_runs_c(M, N, K, group) * M * N;
     Tensor y = at::empty({M, N}, x.options());
-    const int rc = call(fp4_linear_c, ptr(x), x.stride(0), ptr(codes), ptr(scales), (int)(K / scales.size(1)), ptr(bias), bias ? src_of(*bias) : 0, M, N, K, ptr(y),
+    OptTensor ws;
+    if (partial) ws = f32(x, {partial});
+    const int rc = call(fp4_linear_c, ptr(x), x.stride(0), ptr(codes), ptr(scales), group, ptr(bias), bias ? src_of(*bias) : 0, M, N, K, ptr(y), ptr(ws), 4 * partial,
                         str(stream));
     return rc ? status(rc) : py::cast(y);
 }

@@ -109,6 +109,7 @@ EXPORTS = (
     "odl_fp8_token_logprobs_splits",
     "odl_fp8_token_logprobs",
     "odl_fp8_token_logprobs_bwd",
+    "odl_fp8_fp4_linear_runs",
     "odl_fp8_fp4_linear",
     "odl_fp8_fp4_quantise",
 )
@@ -224,7 +225,9 @@ def load() -> ctypes.CDLL:
         L.odl_fp8_token_logprobs_splits.restype = i32
         L.odl_fp8_token_logprobs.argtypes = [vp, i32, i64, i64, i64, vp, i64, f32, i32, vp, vp, vp, vp, vp, i32, vp, vp]
         L.odl_fp8_token_logprobs_bwd.argtypes = [vp, i32, i64, i64, i64, i64, vp, i64, f32, i32, vp, vp, vp, vp, vp, vp, vp, vp, vp]
-        L.odl_fp8_fp4_linear.argtypes = [vp, i64, vp, vp, i32, vp, i32, i64, i64, i64, vp, vp]
+        L.odl_fp8_fp4_linear_runs.argtypes = [i64, i64, i64, i32]
+        L.odl_fp8_fp4_linear_runs.restype = i32
+        L.odl_fp8_fp4_linear.argtypes = [vp, i64, vp, vp, i32, vp, i32, i64, i64, i64, vp, vp, i64, vp]
         L.odl_fp8_fp4_quantise.argtypes = [vp, i32, i64, i64, i32, vp, vp, vp]
         for name in EXPORTS:
             getattr(L, name)  # AttributeError here = the library does not match the header
@@ -1814,13 +1817,16 @@ def fp4_linear(x: torch.Tensor, codes: torch.Tensor, scales: torch.Tensor, bias:
             raise NativeError(f"fp4_linear: scales are {scales.dtype} {tuple(scales.shape)}, expected bf16 [{N}, {K} / group], group 32, 64 or 128")
         if bias is not None and (bias.dtype not in _OUT_DTYPES or bias.shape != (N,)):
             raise NativeError(f"fp4_linear: bias is {bias.dtype} {tuple(bias.shape)}, expected bf16 or fp32 [{N}]")
-        if x.stride(1) != 1 or x.stride(0) % 8 or x.stride(0) < K or x.data_ptr() % 16:
+        if x.stride(1) != 1 or x.stride(0) % 8 or not K <= x.stride(0) <= 1 << 24 or x.data_ptr() % 16:
             x = _dense_16(x)
         codes, scales, bias = _dense_16(codes), scales.contiguous(), None if bias is None else bias.contiguous()
         y = torch.empty((M, N), dtype=torch.bfloat16, device=x.device)
-        _check(load().odl_fp8_fp4_linear(x.data_ptr(), x.stride(0), codes.data_ptr(), scales.data_ptr(), K // scales.shape[1],
-                                         None if bias is None else bias.data_ptr(), DT_BF16 if bias is None else _src_dtype(bias), M, N, K, y.data_ptr(),
-                                         _stream()), "odl_fp8_fp4_linear")
+        group = K // scales.shape[1]
+        runs = load().odl_fp8_fp4_linear_runs(M, N, K, group)
+        ws = torch.empty(runs * M * N, dtype=torch.float32, device=x.device) if runs else None
+        _check(load().odl_fp8_fp4_linear(x.data_ptr(), x.stride(0), codes.data_ptr(), scales.data_ptr(), group, None if bias is None else bias.data_ptr(),
+                                         DT_BF16 if bias is None else _src_dtype(bias), M, N, K, y.data_ptr(), None if ws is None else ws.data_ptr(),
+                                         4 * runs * M * N, _stream()), "odl_fp8_fp4_linear")
     return y
 
 

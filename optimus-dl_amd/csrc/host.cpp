@@ -54,7 +54,6 @@ decltype(&odl_fp8_block_cast) block_cast_c;
 decltype(&odl_fp8_mx_gemm_nt_hinted) mx_gemm_nt_c;
 decltype(&odl_fp8_residual_norm) residual_norm_c;
 decltype(&odl_fp8_residual_norm_bwd) residual_norm_bwd_c;
-decltype(&odl_fp8_token_logprobs_splits) logprobs_splits_c;
 decltype(&odl_fp8_token_logprobs) logprobs_c;
 decltype(&odl_fp8_token_logprobs_bwd) logprobs_bwd_c;
 decltype(&odl_fp8_fp4_linear_runs) fp4_runs_c;
@@ -97,7 +96,6 @@ void bind(const py::dict &d) {
     take(mx_gemm_nt_c, d, "odl_fp8_mx_gemm_nt_hinted");
     take(residual_norm_c, d, "odl_fp8_residual_norm");
     take(residual_norm_bwd_c, d, "odl_fp8_residual_norm_bwd");
-    take(logprobs_splits_c, d, "odl_fp8_token_logprobs_splits");
     take(logprobs_c, d, "odl_fp8_token_logprobs");
     take(logprobs_bwd_c, d, "odl_fp8_token_logprobs_bwd");
     take(fp4_runs_c, d, "odl_fp8_fp4_linear_runs");
@@ -519,18 +517,16 @@ py::object token_logprobs(const Tensor &l, const Tensor &targets, i64 vocab, int
     if (!logits2d(l) || !dense(targets) || targets.scalar_type() != at::kLong || targets.numel() != l.size(0) || targets.device() != l.device()) return none();
     const i64 rows = l.size(0);
     if (vocab < 1 || vocab > l.size(1) || top_k < 0 || top_k > ODL_FP8_LOGPROBS_MAX_TOP) return none();
-    const int splits = logprobs_splits_c(rows, vocab);
     Tensor out = f32(l, {2, rows});
-    OptTensor stats, top, ids, ws;
+    OptTensor stats, top, ids;
     if (keep) stats = f32(l, {2, rows});
     if (top_k) {
         top = f32(l, {rows, top_k});
         ids = at::empty({rows, top_k}, l.options().dtype(at::kLong));
     }
-    if (splits > 1) ws = f32(l, {rows * splits * (3 + 2 * top_k)});
     Tensor lp = out.select(0, 0), entropy = out.select(0, 1);
     const int rc = call(logprobs_c, ptr(l), src_of(l), rows, l.stride(0), vocab, targets.data_ptr<i64>(), ignore, (float)inv_t, top_k, ptr(lp), ptr(entropy),
-                        ptr(stats), ptr(top), ptr(ids), splits, ptr(ws), str(stream));
+                        ptr(stats), ptr(top), ptr(ids), str(stream));
     return rc ? status(rc) : py::make_tuple(lp, entropy, obj(stats), obj(top), obj(ids));
 }
 

@@ -4,9 +4,9 @@
 //   p_j = e^d_j / s,  dl_j = [A (j == t) + sum_i C_i (j == id_i) - p_j (A + sum_i C_i) - B p_j (ln p_j + entropy)] / T
 // for gradients A of the logprob, B of the entropy, C_i of the top alternatives.
 //
-// The forward reads a row once, with a running maximum and the two sums of it per lane.  The top k cost no work in that pass:
-// the k-th largest of the lanes' maxima is a lower bound of the k-th largest logit, and only lanes whose maximum reaches it can hold
-// one; their share of the row (k lanes of 256, mostly) is read again and what reaches the bound is ranked.
+// The forward reads a row once, a block a row, with a running maximum and the two sums of it per lane.  The top k cost no work in that
+// pass: the lanes' maxima are folded to 64, the k-th largest of those is a lower bound of the k-th largest logit, and only lanes whose
+// maximum reaches it can hold one; their share of the row is read again and what reaches the bound is ranked.
 // Rows are read and written with 16-byte accesses at any alignment (rows of an odd number of columns begin anywhere).
 // Bound by HBM for large calls (8 to 12 operations an element, one of them an exponential), by latency for a few rows.
 #include "common.h"
@@ -17,10 +17,8 @@ namespace odl {
 namespace {
 
 constexpr int kParts = ODL_FP8_AMAX_PARTS;
-constexpr int kThreads = 256;
 constexpr int kMaxTop = ODL_FP8_LOGPROBS_MAX_TOP;
-constexpr int kMaxSplits = ODL_FP8_LOGPROBS_MAX_SPLITS;
-constexpr int kCand = 1024;                      // candidates of a section that are ranked at once
+constexpr int kCand = 1024;                      // candidates that are ranked at once
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 constexpr float kFar = 1e30f;                    // exponents are cut off here: finite times e^-far is 0, infinity times 0 is not
 
@@ -55,59 +53,64 @@ struct Chunk {
     }
 };
 
-// Running maximum m (never below -FLT_MAX, so that differences stay finite), s = sum 2^d, q = sum 2^d d, d = (l - m) * c,
-// c = log2(e) / T.
-struct Softmax {
-    float m = -FLT_MAX, s = 0.0f, q = 0.0f;
-    __device__ __forceinline__ void move_to(float to, float c) {
-        const float delta = fminf((to - m) * c, kFar), f = __builtin_amdgcn_exp2f(-delta);
-        q = f * __fmaf_rn(-delta, s, q);
-        s *= f;
-        m = to;
-    }
-    __device__ __forceinline__ void add(const Softmax &o, float c) {
-        Softmax b = o;
-        const float to = fmaxf(m, b.m);
-        move_to(to, c);
-        b.move_to(to, c);
-        s += b.s;
-        q += b.q;
-    }
-    __device__ __forceinline__ void take(float l, float c) {       // l <= m
-        const float d = (l - m) * c, e = __builtin_amdgcn_exp2f(d);
-        s += e;
-        q = __fmaf_rn(e, fmaxf(d, -kFar), q);
-    }
+// The exponent of an element, in powers of two, against a running maximum m: d = (l - m) * c, c = log2(e) / T.  With mc = m * c rounded it is one
+// fused multiply-add, l * c - mc: the rounding of mc is the same for every element and for the maximum itself, so nothing is lost by
+// it as long as sums are held against mc and not against m.  Maxima beyond 2^96 (rows masked by the lowest value of a type), where
+// products overflow, take the difference first.
+struct Exponent {
+    float m, mc, c;
+    bool near;
+    __device__ __forceinline__ Exponent(float m_, float c_) : m(m_), mc(m_ * c_), c(c_), near(__builtin_fabsf(m_ * c_) < 0x1p96f) {}
+    __device__ __forceinline__ float operator()(float l) const { return near ? __fmaf_rn(l, c, -mc) : (l - m) * c; }
 };
 
-__device__ __forceinline__ Softmax wave_softmax(Softmax a, float c) {
-#pragma unroll
-    for (int off = kWave / 2; off > 0; off >>= 1) {
-        Softmax b;
-        b.m = __shfl_xor(a.m, off, kWave);
-        b.s = __shfl_xor(a.s, off, kWave);
-        b.q = __shfl_xor(a.q, off, kWave);
-        a.add(b, c);
-    }
-    return a;
+// How far down it is from maximum m to maximum `to`, >= 0 (and finite: what was summed against m is then 0).
+__device__ __forceinline__ float descent(float m, float to, float c) {
+    const Exponent a(m, c), b(to, c);
+    return fminf(a.near && b.near ? b.mc - a.mc : (to - m) * c, kFar);
 }
 
-struct Row {                                     // what a row answers
-    float m, log_s, entropy;
+// sums over a wave, in every lane
+template <int CTRL>
+__device__ __forceinline__ float add_dpp(float v) {
+    return v + bits_to_float((uint32_t)__builtin_amdgcn_update_dpp(0, (int)float_to_bits(v), CTRL, 0xf, 0xf, false));
+}
+__device__ __forceinline__ float wave_sum(float v) {
+    v = add_dpp<0xB1>(v);                        // lane ^ 1, ^ 2, the other quad of 8, the other half of 16
+    v = add_dpp<0x4E>(v);
+    v = add_dpp<0x141>(v);
+    v = add_dpp<0x140>(v);
+    const auto r = __builtin_amdgcn_permlane16_swap(float_to_bits(v), float_to_bits(v), false, false);
+    v = bits_to_float(r[0]) + bits_to_float(r[1]);
+    const auto q = __builtin_amdgcn_permlane32_swap(float_to_bits(v), float_to_bits(v), false, false);
+    return bits_to_float(q[0]) + bits_to_float(q[1]);
+}
+template <int CTRL>
+__device__ __forceinline__ float max_dpp(float v) {
+    return fmaxf(v, bits_to_float((uint32_t)__builtin_amdgcn_update_dpp(0, (int)float_to_bits(v), CTRL, 0xf, 0xf, false)));
+}
+// maxima over groups of 4, 8, 16 or 64 lanes
+template <int LANES>
+__device__ __forceinline__ float group_max(float v) {
+    v = max_dpp<0x4E>(max_dpp<0xB1>(v));
+    if constexpr (LANES >= 8) v = max_dpp<0x141>(v);
+    if constexpr (LANES >= 16) v = max_dpp<0x140>(v);
+    if constexpr (LANES >= 64) {
+        const auto r = __builtin_amdgcn_permlane16_swap(float_to_bits(v), float_to_bits(v), false, false);
+        v = fmaxf(bits_to_float(r[0]), bits_to_float(r[1]));
+        const auto q = __builtin_amdgcn_permlane32_swap(float_to_bits(v), float_to_bits(v), false, false);
+        v = fmaxf(bits_to_float(q[0]), bits_to_float(q[1]));
+    }
+    return v;
+}
+
+struct Row {                                     // what a row answers: its maximum, log2 of the sum against it, its entropy
+    float m, log2_s, entropy;
 };
 
-// (a sum of 0: every logit is -inf)
-__device__ __forceinline__ Row answer(const Softmax &a) {
-    Row r;
-    r.m = a.m;
-    r.log_s = a.s == 0.0f ? -INFINITY : logf(a.s);
-    r.entropy = a.s == 0.0f ? 0.0f : r.log_s - a.q * kLn2 / a.s;
-    return r;
-}
-
-__device__ __forceinline__ float log_prob(float l, const Row &r, float inv_t) {
-    if (r.log_s == -INFINITY) return -INFINITY;
-    return (l - r.m) * inv_t - r.log_s;
+__device__ __forceinline__ float log_prob(float l, const Row &r, float c) {
+    if (r.log2_s == -INFINITY) return -INFINITY; // every logit is -inf
+    return (Exponent(r.m, c)(l) - r.log2_s) * kLn2;
 }
 
 __device__ __forceinline__ bool before(float v, int i, float w, int j) { return v > w || (v == w && i < j); }
@@ -116,69 +119,63 @@ struct Forward {
     const void *logits;
     const int64_t *targets;
     int64_t rows, stride, ignore_index;
-    int vocab, top_k, splits, section;           // a section: columns of a block, a multiple of 8
-    float inv_t;
+    int vocab, top_k;
+    float c;                                     // log2(e) / T
     float *logprobs, *entropy, *stats, *top_logprobs;
     int64_t *top_ids;
-    float *part_sums, *part_values;              // splits > 1: [rows][splits][3], [rows][splits][top_k]
-    int *part_ids;
 };
 
-__device__ __forceinline__ void write_ignored(const Forward &a, int64_t row) {
-    if (threadIdx.x == 0) {
-        a.logprobs[row] = 0.0f;
-        a.entropy[row] = 0.0f;
-        if (a.stats) { a.stats[row] = 0.0f; a.stats[a.rows + row] = 0.0f; }
+// How many of n candidates come before (v, id).  The arrays are filled up to a multiple of 8 with what comes before nothing.
+__device__ __forceinline__ int rank_of(const float *values, const int *ids, int n, float v, int id) {
+    int rank = 0;
+    for (int j = 0; j < n; j += 8) {
+        float w[8];
+        int i[8];
+#pragma unroll
+        for (int u = 0; u < 8; ++u) { w[u] = values[j + u]; i[u] = ids[j + u]; }
+#pragma unroll
+        for (int u = 0; u < 8; ++u) rank += before(w[u], i[u], v, id);
     }
-    for (int i = threadIdx.x; i < a.top_k; i += kThreads) {
-        a.top_logprobs[row * a.top_k + i] = 0.0f;
-        a.top_ids[row * a.top_k + i] = -1;
-    }
+    return rank;
 }
 
-template <int DT>
-__device__ __forceinline__ void write_row(const Forward &a, int64_t row, int64_t target, const Row &r) {
-    float lp = __builtin_nanf("");
-    if (target >= 0 && target < a.vocab)
-        lp = log_prob(one<DT>(reinterpret_cast<const typename Elem<DT>::T *>(a.logits) + row * a.stride + target), r, a.inv_t);
-    a.logprobs[row] = lp;
-    a.entropy[row] = r.entropy;
-    if (a.stats) { a.stats[row] = r.m; a.stats[a.rows + row] = r.log_s; }
-}
-
-__device__ __forceinline__ void write_top(const Forward &a, int64_t row, int rank, float v, int id, const Row &r) {
-    const bool sound = r.log_s == r.log_s;       // a row with NaN or +inf has no order
-    a.top_logprobs[row * a.top_k + rank] = sound ? log_prob(v, r, a.inv_t) : __builtin_nanf("");
-    a.top_ids[row * a.top_k + rank] = sound ? id : -1;
-}
-
-// One block for each row and section of its columns.
-template <int DT>
-__global__ __launch_bounds__(kThreads) void token_logprobs_kernel(const Forward a) {
+template <int DT, int THREADS>
+__global__ __launch_bounds__(THREADS) void token_logprobs_kernel(const Forward a) {
     typedef typename Elem<DT>::T T;
-    constexpr int U = 4;
-    __shared__ float sums[kThreads / kWave][3], cand_v[kCand], bound;
-    __shared__ __attribute__((aligned(16))) float lane_top[kThreads];
-    __shared__ int cand_i[kCand], lanes[kThreads], n_lanes, n_cand;
-    const int tid = threadIdx.x;
-    const int64_t row = blockIdx.x / a.splits;
-    const int sec = (int)(blockIdx.x - row * a.splits);
+    constexpr int U = 4, kWaves = THREADS / kWave;
+    __shared__ float wave_m[kWaves], wave_s[kWaves], wave_q[kWaves], cand_v[kCand];
+    __shared__ __attribute__((aligned(16))) float group_top[kWave];
+    __shared__ int cand_i[kCand], lanes[THREADS], n_lanes, n_cand;
+    const int tid = threadIdx.x, lane = tid % kWave;
+    const int64_t row = blockIdx.x;
     const int64_t target = a.targets[row];
     if (target == a.ignore_index) {              // (not read)
-        if (a.splits == 1) write_ignored(a, row);
+        if (tid == 0) {
+            a.logprobs[row] = 0.0f;
+            a.entropy[row] = 0.0f;
+            if (a.stats) { a.stats[row] = 0.0f; a.stats[a.rows + row] = 0.0f; }
+        }
+        if (tid < a.top_k) {
+            a.top_logprobs[row * a.top_k + tid] = 0.0f;
+            a.top_ids[row * a.top_k + tid] = -1;
+        }
         return;
     }
-    const int first = sec * a.section, cols = min(a.section, a.vocab - first);
-    const T *p = reinterpret_cast<const T *>(a.logits) + row * a.stride + first;
-    const int n = cols / 8, tail = cols % 8;
-    const float c = a.inv_t * kLog2e;
-    Softmax run;
-    float top = -INFINITY;
-    for (int i = tid; i < n; i += U * kThreads) {
+    const T *p = reinterpret_cast<const T *>(a.logits) + row * a.stride;
+    const int n = a.vocab / 8, tail = a.vocab % 8;
+    // running maximum (never below -FLT_MAX, so that differences from it are finite or -inf), sum 2^d, sum 2^d d
+    float m = -FLT_MAX, s = 0.0f, q = 0.0f, top = -INFINITY;
+    auto move_to = [&](float to) {
+        const float down = descent(m, to, a.c), f = __builtin_amdgcn_exp2f(-down);
+        q = f * __fmaf_rn(-down, s, q);
+        s *= f;
+        m = to;
+    };
+    for (int i = tid; i < n; i += U * THREADS) {
         Chunk<DT> in[U];
 #pragma unroll
         for (int u = 0; u < U; ++u) {
-            if (i + u * kThreads < n) in[u].load(p + (int64_t)(i + u * kThreads) * 8);
+            if (i + u * THREADS < n) in[u].load(p + (int64_t)(i + u * THREADS) * 8);
             else in[u].fill();
         }
         float f[U][8], most = -INFINITY;
@@ -188,73 +185,98 @@ __global__ __launch_bounds__(kThreads) void token_logprobs_kernel(const Forward 
 #pragma unroll
             for (int e = 0; e < 8; ++e) most = fmaxf(most, f[u][e]);
         }
-        top = fmaxf(top, most);
-        run.move_to(fmaxf(run.m, most), c);
+        if (most > top) {                        // (rare behind the first trips; -inf and NaN move nothing)
+            top = most;
+            move_to(fmaxf(m, most));
+        }
+        const Exponent x(m, a.c);
+        if (x.near) {
 #pragma unroll
-        for (int u = 0; u < U; ++u)
+            for (int u = 0; u < U; ++u)
 #pragma unroll
-            for (int e = 0; e < 8; ++e) run.take(f[u][e], c);
+                for (int e = 0; e < 8; ++e) {
+                    const float d = __fmaf_rn(f[u][e], x.c, -x.mc), w = __builtin_amdgcn_exp2f(d);
+                    s += w;
+                    q = __fmaf_rn(w, fmaxf(d, -kFar), q);
+                }
+        } else {
+#pragma unroll
+            for (int u = 0; u < U; ++u)
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    const float d = (f[u][e] - m) * x.c, w = __builtin_amdgcn_exp2f(d);
+                    s += w;
+                    q = __fmaf_rn(w, fmaxf(d, -kFar), q);
+                }
+        }
     }
     if (tid < tail) {
         const float l = one<DT>(p + n * 8 + tid);
         top = fmaxf(top, l);
-        run.move_to(fmaxf(run.m, l), c);
-        run.take(l, c);
+        move_to(fmaxf(m, l));
+        const float d = Exponent(m, a.c)(l), w = __builtin_amdgcn_exp2f(d);
+        s += w;
+        q = __fmaf_rn(w, fmaxf(d, -kFar), q);
     }
-    run = wave_softmax(run, c);
-    if (tid % kWave == 0) {
-        sums[tid / kWave][0] = run.m;
-        sums[tid / kWave][1] = run.s;
-        sums[tid / kWave][2] = run.q;
-    }
+    // the block's maximum, every lane's sums against it, their sums
+    const float wm = group_max<kWave>(m);
+    if (lane == 0) wave_m[tid / kWave] = wm;
     if (a.top_k) {
-        lane_top[tid] = top;
+        const float g = group_max<THREADS / kWave>(top);
+        if (tid % (THREADS / kWave) == 0) group_top[tid / (THREADS / kWave)] = g;
         if (tid == 0) n_lanes = n_cand = 0;
     }
     __syncthreads();
-    run = Softmax{sums[0][0], sums[0][1], sums[0][2]};
+    float to = wave_m[0];
 #pragma unroll
-    for (int w = 1; w < kThreads / kWave; ++w) run.add(Softmax{sums[w][0], sums[w][1], sums[w][2]}, c);
-    const Row r = answer(run);
-    if (tid == 0) {
-        if (a.splits == 1) {
-            write_row<DT>(a, row, target, r);
-        } else {
-            float *o = a.part_sums + blockIdx.x * (int64_t)3;
-            o[0] = run.m; o[1] = run.s; o[2] = run.q;
+    for (int w = 1; w < kWaves; ++w) to = fmaxf(to, wave_m[w]);
+    move_to(to);
+    const float ws = wave_sum(s), wq = wave_sum(q);
+    if (lane == 0) { wave_s[tid / kWave] = ws; wave_q[tid / kWave] = wq; }
+    float least = 0.0f;
+    if (a.top_k) {                               // the k-th largest of the 64 maxima; every wave finds it for itself
+        const float v = group_top[lane];
+        int above = 0, equal = 0;
+#pragma unroll
+        for (int j = 0; j < kWave; j += 4) {
+            const float4 o = *reinterpret_cast<const float4 *>(group_top + j);
+            above += (o.x > v) + (o.y > v) + (o.z > v) + (o.w > v);
+            equal += (o.x == v) + (o.y == v) + (o.z == v) + (o.w == v);
         }
+        const uint64_t kth = __ballot(above < a.top_k && a.top_k <= above + equal);
+        least = __shfl(v, __ffsll((unsigned long long)kth) - 1, kWave);
+        if (top >= least) lanes[atomicAdd(&n_lanes, 1)] = tid;
+    }
+    __syncthreads();
+    s = wave_s[0];
+    q = wave_q[0];
+#pragma unroll
+    for (int w = 1; w < kWaves; ++w) { s += wave_s[w]; q += wave_q[w]; }
+    Row r;
+    r.m = m;
+    r.log2_s = s == 0.0f ? -INFINITY : log2f(s);
+    r.entropy = s == 0.0f ? 0.0f : (r.log2_s - q / s) * kLn2;
+    if (tid == 0) {
+        a.logprobs[row] = target >= 0 && target < a.vocab ? log_prob(one<DT>(p + target), r, a.c) : __builtin_nanf("");
+        a.entropy[row] = r.entropy;
+        if (a.stats) { a.stats[row] = r.m; a.stats[a.rows + row] = r.log2_s; }
     }
     if (!a.top_k) return;
 
+    const bool sound = r.log2_s == r.log2_s;     // a row with NaN or +inf has no order
     auto put = [&](int rank, float v, int id) {
-        if (a.splits == 1) {
-            write_top(a, row, rank, v, id, r);
-        } else {
-            a.part_values[blockIdx.x * (int64_t)a.top_k + rank] = v;
-            a.part_ids[blockIdx.x * (int64_t)a.top_k + rank] = id;
-        }
+        a.top_logprobs[row * a.top_k + rank] = sound ? log_prob(v, r, a.c) : __builtin_nanf("");
+        a.top_ids[row * a.top_k + rank] = sound ? id : -1;
     };
-    {                                            // the k-th largest of the lanes' maxima
-        int rank = 0;
-        for (int j = 0; j < kThreads; j += 4) {
-            const float4 o = *reinterpret_cast<const float4 *>(lane_top + j);
-            rank += before(o.x, j, top, tid) + before(o.y, j + 1, top, tid) + before(o.z, j + 2, top, tid) + before(o.w, j + 3, top, tid);
-        }
-        if (rank == a.top_k - 1) bound = top;
-    }
-    __syncthreads();
-    const float least = bound;
-    if (top >= least) lanes[atomicAdd(&n_lanes, 1)] = tid;
-    __syncthreads();
     auto offer = [&](float v, int col) {
         if (v >= least) {
             const int at = atomicAdd(&n_cand, 1);
-            if (at < kCand) { cand_v[at] = v; cand_i[at] = first + col; }
+            if (at < kCand) { cand_v[at] = v; cand_i[at] = col; }
         }
     };
-    const int per = (n + kThreads - 1) / kThreads, total = n_lanes * per;
-    for (int i = tid; i < total; i += kThreads) {
-        const int chunk = lanes[i / per] + (i % per) * kThreads;
+    const int per = (n + THREADS - 1) / THREADS, total = n_lanes * per;
+    for (int i = tid; i < total; i += THREADS) {
+        const int chunk = lanes[i / per] + (i % per) * THREADS;
         if (chunk < n) {
             Chunk<DT> in;
             in.load(p + (int64_t)chunk * 8);
@@ -268,15 +290,14 @@ __global__ __launch_bounds__(kThreads) void token_logprobs_kernel(const Forward 
     __syncthreads();
     const int found = n_cand;
     if (found <= kCand) {
-        for (int i = tid; i < found; i += kThreads) {
+        if (tid < 8 && found + tid < kCand) { cand_v[found + tid] = -INFINITY; cand_i[found + tid] = INT_MAX; }
+        __syncthreads();
+        for (int i = tid; i < found; i += THREADS) {
             const float v = cand_v[i];
-            const int id = cand_i[i];
-            int rank = 0;
-            for (int j = 0; j < found; ++j) rank += before(cand_v[j], cand_i[j], v, id);
+            const int id = cand_i[i], rank = rank_of(cand_v, cand_i, found, v, id);
             if (rank < a.top_k) put(rank, v, id);
         }
-        // (fewer than k: a section of fewer columns, or NaN in the row)
-        for (int i = found + tid; i < a.top_k; i += kThreads) put(i, -INFINITY, INT_MAX);
+        if (tid >= found && tid < a.top_k) put(tid, -INFINITY, -1);        // (fewer than k: NaN in the row)
         return;
     }
     // More than a thousand logits share the bound (rows that are masked almost everywhere, say): the largest behind the last one
@@ -289,15 +310,15 @@ __global__ __launch_bounds__(kThreads) void token_logprobs_kernel(const Forward 
         auto look = [&](float v, int id) {
             if (before(last_v, last_i, v, id) && before(v, id, best_v, best_i)) { best_v = v; best_i = id; }
         };
-        for (int i = tid; i < n; i += kThreads) {
+        for (int i = tid; i < n; i += THREADS) {
             Chunk<DT> in;
             in.load(p + (int64_t)i * 8);
             float f[8];
             in.widen(f);
 #pragma unroll
-            for (int e = 0; e < 8; ++e) look(f[e], first + i * 8 + e);
+            for (int e = 0; e < 8; ++e) look(f[e], i * 8 + e);
         }
-        if (tid < tail) look(one<DT>(p + n * 8 + tid), first + n * 8 + tid);
+        if (tid < tail) look(one<DT>(p + n * 8 + tid), n * 8 + tid);
 #pragma unroll
         for (int off = kWave / 2; off > 0; off >>= 1) {
             const float v = __shfl_xor(best_v, off, kWave);
@@ -305,64 +326,16 @@ __global__ __launch_bounds__(kThreads) void token_logprobs_kernel(const Forward 
             if (before(v, id, best_v, best_i)) { best_v = v; best_i = id; }
         }
         __syncthreads();                         // (cand_v and cand_i are read by everybody in the round before)
-        if (tid % kWave == 0) { cand_v[tid / kWave] = best_v; cand_i[tid / kWave] = best_i; }
+        if (lane == 0) { cand_v[tid / kWave] = best_v; cand_i[tid / kWave] = best_i; }
         __syncthreads();
         best_v = cand_v[0];
         best_i = cand_i[0];
-        for (int w = 1; w < kThreads / kWave; ++w)
+        for (int w = 1; w < kWaves; ++w)
             if (before(cand_v[w], cand_i[w], best_v, best_i)) { best_v = cand_v[w]; best_i = cand_i[w]; }
         last_v = best_v;
         last_i = best_i;
         if (tid == 0) put(k, best_v, best_i);
     }
-}
-
-// Rows whose columns were split: one block joins the sections of a row, in their order.
-template <int DT>
-__global__ __launch_bounds__(kThreads) void token_logprobs_join_kernel(const Forward a) {
-    __shared__ float cand_v[kMaxSplits * kMaxTop], least;
-    __shared__ int cand_i[kMaxSplits * kMaxTop], n_cand;
-    const int tid = threadIdx.x;
-    const int64_t row = blockIdx.x, target = a.targets[row];
-    if (target == a.ignore_index) {
-        write_ignored(a, row);
-        return;
-    }
-    const float c = a.inv_t * kLog2e;
-    Softmax run;
-    if (tid % kWave < a.splits) {                // a lane for each section, at most a wave of them; every wave does the same
-        const float *o = a.part_sums + (row * a.splits + tid % kWave) * 3;
-        run.m = o[0]; run.s = o[1]; run.q = o[2];
-    }
-    run = wave_softmax(run, c);
-    const Row r = answer(run);
-    if (tid == 0) write_row<DT>(a, row, target, r);
-    if (!a.top_k) return;
-    const float *values = a.part_values + row * a.splits * a.top_k;
-    const int *ids = a.part_ids + row * a.splits * a.top_k;
-    if (tid < kWave) {                           // the k-th largest of any section is a lower bound
-        float v = tid < a.splits ? values[tid * a.top_k + a.top_k - 1] : -INFINITY;
-#pragma unroll
-        for (int off = kWave / 2; off > 0; off >>= 1) v = fmaxf(v, __shfl_xor(v, off, kWave));
-        if (tid == 0) { least = v; n_cand = 0; }
-    }
-    __syncthreads();
-    for (int i = tid; i < a.splits * a.top_k; i += kThreads)
-        if (values[i] >= least && ids[i] != INT_MAX) {
-            const int at = atomicAdd(&n_cand, 1);
-            cand_v[at] = values[i];
-            cand_i[at] = ids[i];
-        }
-    __syncthreads();
-    const int found = n_cand;
-    for (int i = tid; i < found; i += kThreads) {
-        const float v = cand_v[i];
-        const int id = cand_i[i];
-        int rank = 0;
-        for (int j = 0; j < found; ++j) rank += before(cand_v[j], cand_i[j], v, id);
-        if (rank < a.top_k) write_top(a, row, rank, v, id, r);
-    }
-    for (int i = found + tid; i < a.top_k; i += kThreads) write_top(a, row, i, -INFINITY, -1, r);
 }
 
 struct Backward {
@@ -376,7 +349,9 @@ struct Backward {
     float *parts;
 };
 
-constexpr int kBwdThreads = 512, kMarks = 128;
+// 1024 lanes keep more of a row on its way than 512: 8192 x 50304 bf16 388 -> 347 us (2 sections a row; with stores that bypass the caches 338, but then
+// the cast behind finds nothing there, and 1004 x 50257 fp32 goes 86 -> 89)
+constexpr int kBwdThreads = 1024, kMarks = 128;
 
 // An item is a section of a row; blocks take them round-robin (at most one block for each partial maximum).
 template <int DT, bool TOP>
@@ -394,8 +369,9 @@ __global__ __launch_bounds__(kBwdThreads) void token_logprobs_bwd_kernel(const B
         const T *in = reinterpret_cast<const T *>(a.logits) + row * a.stride;
         T *out = reinterpret_cast<T *>(a.dlogits) + row * a.padded;
         const int64_t target = a.targets[row];
-        const float m = a.stats[row], log_s = a.stats[a.rows + row];
-        const bool nothing = target == a.ignore_index || log_s == -INFINITY;
+        const float l2 = a.stats[a.rows + row];
+        const Exponent x(a.stats[row], a.inv_t * kLog2e);
+        const bool nothing = target == a.ignore_index || l2 == -INFINITY;
         float sum = a.d_logprobs ? a.d_logprobs[row] : 0.0f;
         const float given = sum * a.inv_t, b = a.d_entropy ? a.d_entropy[row] : 0.0f;
         if constexpr (TOP) {
@@ -411,13 +387,14 @@ __global__ __launch_bounds__(kBwdThreads) void token_logprobs_bwd_kernel(const B
             __syncthreads();
             for (int i = 0; i < a.top_k; ++i) sum += top_d[i];
         }
-        float k0 = -a.inv_t * __fmaf_rn(b, a.entropy[row] - log_s, sum);
-        const float k1 = -a.inv_t * b * a.inv_t, c = a.inv_t * kLog2e, l2 = log_s * kLog2e;
+        // gradient of an element = p * (k0 + k1 * log2 p)
+        float k0 = -a.inv_t * __fmaf_rn(b, a.entropy[row], sum);
+        const float k1 = -a.inv_t * b * kLn2;
         if (target < 0 || target >= a.vocab) k0 = __builtin_nanf("");          // no such token: its log probability is NaN too
         const int t_chunk = target >= 0 && target < a.vocab ? (int)target / 8 : -1;
         auto gradient = [&](float l) {
-            const float d = l - m, p = __builtin_amdgcn_exp2f(__fmaf_rn(d, c, -l2));
-            return p * __fmaf_rn(fmaxf(d, -kFar), k1, k0);
+            const float y = x(l) - l2;
+            return __builtin_amdgcn_exp2f(y) * __fmaf_rn(fmaxf(y, -kFar), k1, k0);
         };
         // gradients of a chunk in which the target or a top alternative may lie, or that ends behind the vocabulary
         auto special = [&](int chunk, float (&f)[8]) {
@@ -507,7 +484,7 @@ int check(const char *who, int dtype, int64_t rows, int64_t stride, int64_t padd
     if (rows < 0 || stride < 0) return set_error(ODL_ERR_ARG, "%s: negative shape", who);
     if (dtype != ODL_BF16 && dtype != ODL_F32) return set_error(ODL_ERR_ARG, "%s: dtype %d", who, dtype);
     if (vocab < 1 || vocab > padded || padded > (1 << 24)) return set_error(ODL_ERR_SHAPE, "%s: %lld of %lld columns (1 to 2^24)", who, (long long)vocab, (long long)padded);
-    if (rows >= (1 << 24)) return set_error(ODL_ERR_SHAPE, "%s: %lld rows (up to 2^24 - 1)", who, (long long)rows);
+    if (rows >= (1 << 22)) return set_error(ODL_ERR_SHAPE, "%s: %lld rows (up to 2^22 - 1)", who, (long long)rows);   // (lanes of a launch are counted in 32 bits)
     if (top_k < 0 || top_k > kMaxTop || top_k > vocab) return set_error(ODL_ERR_ARG, "%s: top_k %d (0 to %d, and to the vocabulary)", who, top_k, kMaxTop);
     if (!(inv_t > 0.0f) || __builtin_isinf(inv_t)) return set_error(ODL_ERR_ARG, "%s: the temperature must be positive and finite", who);
     return ODL_OK;
@@ -518,45 +495,30 @@ int check(const char *who, int dtype, int64_t rows, int64_t stride, int64_t padd
 
 using namespace odl;
 
-// Sections of a row: enough blocks for four on every compute unit, none of fewer than 2048 columns (a chunk for every lane).
-extern "C" int odl_fp8_token_logprobs_splits(int64_t rows, int64_t vocab) {
-    if (rows < 1 || vocab < 1) return 1;
-    const int64_t want = (4 * (int64_t)device_cu_count() + rows - 1) / rows, most = (vocab + 2047) / 2048;
-    int64_t s = want < most ? want : most;
-    s = s < kMaxSplits ? s : kMaxSplits;
-    return (int)(s < 1 ? 1 : s);
-}
-
 extern "C" int odl_fp8_token_logprobs(const void *logits, int dtype, int64_t rows, int64_t stride, int64_t vocab, const int64_t *targets,
                                       int64_t ignore_index, float inv_temperature, int top_k, float *logprobs, float *entropy, float *stats,
-                                      float *top_logprobs, int64_t *top_ids, int splits, float *workspace, odl_stream_t stream_) {
+                                      float *top_logprobs, int64_t *top_ids, odl_stream_t stream_) {
     hipStream_t stream = reinterpret_cast<hipStream_t>(stream_);
     if (const int rc = check("odl_fp8_token_logprobs", dtype, rows, stride, vocab, vocab, top_k, inv_temperature)) return rc;
     if (rows == 0) return ODL_OK;
     if (!logits || !targets || !logprobs || !entropy || (top_k && (!top_logprobs || !top_ids)))
         return set_error(ODL_ERR_ARG, "odl_fp8_token_logprobs: null pointer");
-    if (splits < 1 || splits > kMaxSplits || (splits > 1 && !workspace))
-        return set_error(ODL_ERR_ARG, "odl_fp8_token_logprobs: %d sections (1 to %d; more than one need a workspace)", splits, kMaxSplits);
-    if (rows * splits >= (1 << 24))              // (lanes of a launch are counted in 32 bits)
-        return set_error(ODL_ERR_SHAPE, "odl_fp8_token_logprobs: %lld rows of %d sections (up to 2^24 - 1 blocks)", (long long)rows, splits);
-    const int64_t chunks = (vocab + 7) / 8, section = (chunks + splits - 1) / splits * 8;
-    splits = (int)((vocab + section - 1) / section);              // (no section is empty)
     Forward a = {};
     a.logits = logits; a.targets = targets; a.rows = rows; a.stride = stride; a.ignore_index = ignore_index;
-    a.vocab = (int)vocab; a.top_k = top_k; a.splits = splits; a.section = (int)section; a.inv_t = inv_temperature;
+    a.vocab = (int)vocab; a.top_k = top_k; a.c = inv_temperature * kLog2e;
     a.logprobs = logprobs; a.entropy = entropy; a.stats = stats; a.top_logprobs = top_logprobs; a.top_ids = top_ids;
-    a.part_sums = workspace;
-    if (splits > 1 && top_k) {
-        a.part_values = workspace + rows * splits * 3;
-        a.part_ids = reinterpret_cast<int *>(a.part_values + rows * splits * top_k);
-    }
-    const dim3 grid((unsigned)(rows * splits));
-    if (dtype == ODL_BF16) hipLaunchKernelGGL(token_logprobs_kernel<ODL_BF16>, grid, dim3(kThreads), 0, stream, a);
-    else hipLaunchKernelGGL(token_logprobs_kernel<ODL_F32>, grid, dim3(kThreads), 0, stream, a);
-    if (splits > 1) {
-        if (dtype == ODL_BF16) hipLaunchKernelGGL(token_logprobs_join_kernel<ODL_BF16>, dim3((unsigned)rows), dim3(kThreads), 0, stream, a);
-        else hipLaunchKernelGGL(token_logprobs_join_kernel<ODL_F32>, dim3((unsigned)rows), dim3(kThreads), 0, stream, a);
-    }
+    const dim3 grid((unsigned)rows);
+    // Lanes of a row's block, us with 256 / 512 / 1024: 8192 x 50257 bf16 160 / 155 / 190, 2048 rows 44.8 / 42.5 / 46.4, 16 x 32000 (top 20) 10.1 / 9.4 / 10.6;
+    // short rows, and rows of middle length where there are many, have less to do than a wide block to agree on: 2000 x 1000
+    // 11.4 / 17.5 / 30.5, 700 x 32000 15.3 / 17.1 / 20.5; few long ones more: 1 x 131072 20.2 / 16.2 / 14.9
+    const int threads = vocab <= 4096 || (vocab <= 40000 && rows >= 512) ? 256 : vocab >= 65536 && rows <= 64 ? 1024 : 512;
+#define ODL_LPF(DT, THREADS) hipLaunchKernelGGL((token_logprobs_kernel<DT, THREADS>), grid, dim3(THREADS), 0, stream, a)
+#define ODL_LPF_DT(THREADS) do { if (dtype == ODL_BF16) ODL_LPF(ODL_BF16, THREADS); else ODL_LPF(ODL_F32, THREADS); } while (0)
+    if (threads == 256) ODL_LPF_DT(256);
+    else if (threads == 512) ODL_LPF_DT(512);
+    else ODL_LPF_DT(1024);
+#undef ODL_LPF_DT
+#undef ODL_LPF
     return check_launch("odl_fp8_token_logprobs");
 }
 

@@ -97,20 +97,33 @@ struct Rows {
 template <int CPT, int LPR>
 __device__ __forceinline__ void lane_weights(const float *weight, const float *post_weight, const float *gate, bool gate_scalar, int lane,
                                              int nchunk, float (&wv)[CPT][8], float (&wn)[CPT][8]) {
+    auto take = [&](const float *from, float (&to)[CPT][8], float past) {
 #pragma unroll
-    for (int j = 0; j < CPT; ++j) {
-        const int c = lane + j * LPR;
+        for (int j = 0; j < CPT; ++j) {
+            const int c = lane + j * LPR;
+            if (c < nchunk) __builtin_memcpy(to[j], from + c * 8, sizeof(to[j]));
+            else
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-            float b = 0.0f, n = 0.0f;
-            if (c < nchunk) {
-                b = post_weight ? post_weight[c * 8 + e] : 1.0f;
-                if (gate && !gate_scalar) b *= gate[c * 8 + e];
-                n = weight[c * 8 + e];
-            }
-            wv[j][e] = b;
-            wn[j][e] = n;
+                for (int e = 0; e < 8; ++e) to[j][e] = past;
         }
+    };
+    float g[CPT][8];
+    take(weight, wn, 0.0f);
+    const bool channels = gate && !gate_scalar;
+    if (channels) take(gate, g, 0.0f);
+    if (post_weight) {
+        take(post_weight, wv, 0.0f);
+    } else {
+#pragma unroll
+        for (int j = 0; j < CPT; ++j)
+#pragma unroll
+            for (int e = 0; e < 8; ++e) wv[j][e] = 1.0f;
+    }
+    if (channels) {
+#pragma unroll
+        for (int j = 0; j < CPT; ++j)
+#pragma unroll
+            for (int e = 0; e < 8; ++e) wv[j][e] *= g[j][e];
     }
 }
 
@@ -125,9 +138,6 @@ __global__ __launch_bounds__(Rows<LPR>::kThreads) void residual_norm_kernel(
     const int lane = threadIdx.x % LPR, nchunk = cols / 8;
     const int64_t step = (int64_t)gridDim.x * RPB;
     const float gs = gate && gate_scalar ? gate[0] : 1.0f;
-    float wv[CPT][8], wn[CPT][8];
-    lane_weights<CPT, LPR>(weight, post_weight, gate, gate_scalar, lane, nchunk, wv, wn);
-
     u32x4 nx[CPT][kVecs<XT>], nh[CPT][kVecs<HT>];
     auto fetch = [&](int64_t row) {
 #pragma unroll
@@ -142,6 +152,8 @@ __global__ __launch_bounds__(Rows<LPR>::kThreads) void residual_norm_kernel(
     uint32_t am = 0;
     int64_t row = (int64_t)blockIdx.x * RPB + threadIdx.x / LPR;
     fetch(row);
+    float wv[CPT][8], wn[CPT][8];
+    lane_weights<CPT, LPR>(weight, post_weight, gate, gate_scalar, lane, nchunk, wv, wn);
     for (int64_t row0 = (int64_t)blockIdx.x * RPB; row0 < rows; row0 += step, row += step) {      // the same trips for every lane
         float yf[CPT][8], hf[CPT][8];
 #pragma unroll
@@ -206,11 +218,12 @@ __global__ __launch_bounds__(Rows<LPR>::kThreads) void residual_norm_bwd_kernel(
     constexpr int kThreads = Rows<LPR>::kThreads, RPB = Rows<LPR>::kPerBlock;
     __shared__ float lds[2 * 3 * (LPR / kWave + 1)];
     __shared__ uint32_t red[kThreads / kWave];
-    __shared__ float fold[RPB > 1 ? kThreads * 8 : kThreads / kWave];
+    __shared__ float fold[RPB > 1 ? kThreads * 8 : 1];
     const int lane = threadIdx.x % LPR, nchunk = cols / 8;
     const int64_t step = (int64_t)gridDim.x * RPB;
     const float gs = gate && gate_scalar ? gate[0] : 1.0f;
-    float wv[CPT][8], wn[CPT][8], dw[CPT][8], dd[CPT][8], dg = 0.0f;
+    float wv[CPT][8], wn[CPT][8], dw[CPT][8], dd[CPT][8];
+    double dg = 0.0;                                           // (a sum of everything, of both signs: held in 64 bits from row to row)
     lane_weights<CPT, LPR>(weight, post_weight, gate, gate_scalar, lane, nchunk, wv, wn);
 #pragma unroll
     for (int j = 0; j < CPT; ++j)
@@ -267,6 +280,7 @@ __global__ __launch_bounds__(Rows<LPR>::kThreads) void residual_norm_bwd_kernel(
             }
         row_sums<LPR, 3>(s, lds, turn);
         const float c2 = ry * (s[0] / (float)cols);
+        float dg_row = 0.0f;
         const float c3 = post_weight ? __fmaf_rn(-c2, s[2], s[1]) / (float)cols : 0.0f;
         if (row < rows) {
 #pragma unroll
@@ -279,7 +293,7 @@ __global__ __launch_bounds__(Rows<LPR>::kThreads) void residual_norm_bwd_kernel(
                         const float ey = __fmaf_rn(-c2, yf[j][e], ef[j][e]);
                         const float eh = ey * hf[j][e];
                         dd[j][e] += eh;
-                        dg = __fmaf_rn(eh, wv[j][e], dg);
+                        dg_row = __fmaf_rn(eh, wv[j][e], dg_row);
                         ox[e] = a * ey;
                         oh[e] = rh * __fmaf_rn(-c3, hf[j][e], ey * (gs * wv[j][e]));
                     }
@@ -295,6 +309,7 @@ __global__ __launch_bounds__(Rows<LPR>::kThreads) void residual_norm_bwd_kernel(
                 }
             }
         }
+        dg += dg_row;
     }
     am = block_max_u32(HT == ODL_BF16 ? fold_u16x2_to_f32bits(am) : am, red);
     if (threadIdx.x == 0) parts[blockIdx.x] = bits_to_float(am);
@@ -335,15 +350,15 @@ __global__ __launch_bounds__(Rows<LPR>::kThreads) void residual_norm_bwd_kernel(
             }
     }
     if (gate_sums) {
-        __syncthreads();
+        __shared__ double sums[kThreads / kWave];
 #pragma unroll
         for (int off = kWave / 2; off > 0; off >>= 1) dg += __shfl_xor(dg, off, kWave);
-        if (threadIdx.x % kWave == 0) fold[threadIdx.x / kWave] = dg;
+        if (threadIdx.x % kWave == 0) sums[threadIdx.x / kWave] = dg;
         __syncthreads();
         if (threadIdx.x == 0) {
-            float s = fold[0];
-            for (int w = 1; w < kThreads / kWave; ++w) s += fold[w];
-            gate_sums[blockIdx.x] = s;
+            double s = sums[0];
+            for (int w = 1; w < kThreads / kWave; ++w) s += sums[w];
+            gate_sums[blockIdx.x] = (float)s;
         }
     }
 }
@@ -358,11 +373,11 @@ __global__ __launch_bounds__(1024) void residual_norm_sums_kernel(const float *_
     const int cx = threadIdx.x % 64, grp = threadIdx.x / 64;
     if ((int)blockIdx.x == (2 * cols + 63) / 64) {
         if (grp == 0) {
-            float a = 0.0f;
+            double a = 0.0;
             for (int b = cx; b < nslab; b += 64) a += gate_sums[b];
 #pragma unroll
             for (int off = kWave / 2; off > 0; off >>= 1) a += __shfl_xor(a, off, kWave);
-            if (cx == 0) dgate[0] = a;
+            if (cx == 0) dgate[0] = (float)a;
         }
         return;
     }

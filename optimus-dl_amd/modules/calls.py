@@ -68,3 +68,15 @@ def apply(function: "type[torch.autograd.Function]", *args):
     if not no_graph():
         return function.apply(*args)
     return function.forward(_NoGraph(len(args)), *args)
+
+
+def once_differentiable(backward):
+    """``torch.autograd.function.once_differentiable`` for a backward whose kernels autograd cannot see into: a gradient of its gradient raises.
+    Its wrapper (3 us a call) only where a graph of the backward is recorded."""
+    careful = torch.autograd.function.once_differentiable(backward)
+
+    @functools.wraps(backward)
+    def call(ctx, *grads):
+        return careful(ctx, *grads) if torch.is_grad_enabled() else backward(ctx, *grads)
+
+    return call

@@ -22,7 +22,7 @@ import torch.nn.functional as F
 from .. import native
 from .amp import state as _state
 from .amp.fp8 import FP8Recipe
-from .calls import apply, no_graph, untraced
+from .calls import apply, no_graph, once_differentiable, untraced
 from .fp8_linear import (ROLE_G, ROLE_X, FP8Linear, _converted_input, _Fp8LinearFn, _Fp8LinearGroupFn, _MemberCtx, _product_jobs,
                          _quantise_delayed_for_all, _run_jobs, _wgrad_jobs)
 
@@ -376,7 +376,7 @@ class _ResidualNormFn(torch.autograd.Function):
         return y, z
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
+    @once_differentiable
     def backward(ctx, dy: torch.Tensor | None, dz: torch.Tensor | None):
         if dy is None and dz is None:
             return (None,) * 9
@@ -388,7 +388,12 @@ class _ResidualNormFn(torch.autograd.Function):
                                                                    want_weights=any(need[2:5]))
         if ctx.recipe is not None and need[1]:
             ctx.recipe.offer_parts(dh, parts)             # (the gradient of the Linear that ends the block)
-        given = lambda g, t, wanted: g.reshape(t.shape).to(t.dtype) if wanted and t is not None else None
+
+        def given(g, t, wanted):
+            if not wanted or t is None or (g.dtype == t.dtype and g.shape == t.shape):
+                return g if wanted else None
+            return g.reshape(t.shape).to(t.dtype)
+
         return (dx if need[0] else None, dh if need[1] else None, given(dw, weight, need[2]), given(dpost, post_weight, need[3]),
                 given(dgate, gate, need[4]), None, None, None, None)
 

@@ -14,7 +14,7 @@ import torch
 
 from .. import native
 from .amp import state as _state
-from .calls import apply, untraced
+from .calls import no_graph, once_differentiable, untraced
 
 MAX_TOP = native.LOGPROBS_MAX_TOP
 
@@ -46,7 +46,7 @@ class _TokenLogProbsFn(torch.autograd.Function):
         return logprobs.reshape(lead), entropy.reshape(lead), top.reshape(*lead, top_k), ids_out
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
+    @once_differentiable
     def backward(ctx, d_logprobs, d_entropy, d_top, _):
         if d_logprobs is None and d_entropy is None and d_top is None:
             return (None,) * 7
@@ -109,4 +109,7 @@ def token_logprobs(logits: torch.Tensor, targets: torch.Tensor, *, n_vocab: int 
         raise ValueError(f"token_logprobs: temperature {temperature} (positive and finite)")
     if not logits.is_cuda:
         return _plain(logits, targets, n_vocab, top_k, float(temperature), ignore_index)
-    return TokenLogProbs(*apply(_TokenLogProbsFn, logits, targets, n_vocab, top_k, float(temperature), ignore_index, _state.active_recipe()))
+    if logits.dim() == 2 and no_graph():
+        logprobs, entropy, _, top, ids = native.token_logprobs(logits, targets, n_vocab, top_k, temperature, ignore_index)
+        return TokenLogProbs(logprobs, entropy, top, ids)
+    return TokenLogProbs(*_TokenLogProbsFn.apply(logits, targets, n_vocab, top_k, float(temperature), ignore_index, _state.active_recipe()))

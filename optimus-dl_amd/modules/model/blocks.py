@@ -11,6 +11,8 @@ import torch
 import torch.nn as nn
 import torch.nn.functional as F
 
+from ..fused import residual_norm
+
 
 class RMSNorm(nn.Module):
     def __init__(self, dim: int, eps: float = 1e-5):
@@ -104,27 +106,48 @@ class GELUMLP(nn.Module):
 
 
 class LlamaBlock(nn.Module):
-    """Pre-norm block: x + attn(ln_1(x)); x + mlp(ln_2(x))."""
+    """Pre-norm block: x + attn(ln_1(x)); x + mlp(ln_2(x)).
+
+    post_norms, layer_scale, residual_scale (not in the reference): a norm behind each half (``post_ln_1``, ``post_ln_2``), a learned gate for each
+    channel of it that begins at ``layer_scale`` (``gate_1``, ``gate_2``) and a factor on the stream that it is added to.  With any of them a
+    half ends in ``residual_norm``, one kernel that also is the norm in front of the next half: a model hands the block what the step before
+    made of ``ln_1`` (``z``) and the norm that comes behind it (``next_norm``), and gets the stream and that norm of it."""
 
     def __init__(self, n_embd: int, n_head: int, n_kv_head: int | None, intermediate_size: int | None,
-                 use_qk_norm: bool = False, head_dim: int | None = None, eps: float = 1e-5, rope_theta: float = 10000.0):
+                 use_qk_norm: bool = False, head_dim: int | None = None, eps: float = 1e-5, rope_theta: float = 10000.0,
+                 post_norms: bool = False, layer_scale: float | None = None, residual_scale: float = 1.0):
         super().__init__()
         self.ln_1 = RMSNorm(n_embd, eps)
         self.attn = CausalSelfAttention(n_embd, n_head, n_kv_head, head_dim, bias=False, use_qk_norm=use_qk_norm,
                                         rope_theta=rope_theta, rmsnorm_eps=eps)
         self.ln_2 = RMSNorm(n_embd, eps)
         self.mlp = SwiGLUMLP(n_embd, intermediate_size)
+        self.residual_scale = residual_scale
+        self.stepped = post_norms or layer_scale is not None or residual_scale != 1.0
+        self.post_ln_1, self.post_ln_2 = (RMSNorm(n_embd, eps) if post_norms else None for _ in range(2))
+        self.gate_1, self.gate_2 = (None if layer_scale is None else nn.Parameter(torch.full((n_embd,), float(layer_scale))) for _ in range(2))
 
-    def forward(self, x: torch.Tensor) -> torch.Tensor:
-        x = x + self.attn(self.ln_1(x))
-        return x + self.mlp(self.ln_2(x))
+    def _step(self, x: torch.Tensor, h: torch.Tensor, post: "RMSNorm | None", gate: torch.Tensor | None, norm: RMSNorm):
+        return residual_norm(x, h, norm.weight, norm.eps, post_weight=None if post is None else post.weight, post_eps=None if post is None else post.eps,
+                             gate=gate, residual_scale=self.residual_scale)
+
+    def forward(self, x: torch.Tensor, z: torch.Tensor | None = None, next_norm: RMSNorm | None = None):
+        if not self.stepped:
+            x = x + self.attn(self.ln_1(x))
+            return x + self.mlp(self.ln_2(x))
+        x, z = self._step(x, self.attn(self.ln_1(x) if z is None else z), self.post_ln_1, self.gate_1, self.ln_2)
+        h = self.mlp(z)
+        if next_norm is not None:
+            return self._step(x, h, self.post_ln_2, self.gate_2, next_norm)
+        h = (h if self.post_ln_2 is None else self.post_ln_2(h)).to(x.dtype)
+        return self.residual_scale * x + (h if self.gate_2 is None else (self.gate_2 * h).to(x.dtype))
 
 
 class Qwen3Block(LlamaBlock):
     def __init__(self, n_embd: int, n_head: int, n_kv_head: int | None, intermediate_size: int | None,
-                 head_dim: int | None = None, eps: float = 1e-6, rope_theta: float = 1e6):
+                 head_dim: int | None = None, eps: float = 1e-6, rope_theta: float = 1e6, **step):
         super().__init__(n_embd, n_head, n_kv_head, intermediate_size, use_qk_norm=True, head_dim=head_dim, eps=eps,
-                         rope_theta=rope_theta)
+                         rope_theta=rope_theta, **step)
 
 
 class GPT2Block(nn.Module):

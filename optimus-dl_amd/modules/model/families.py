@@ -1,7 +1,8 @@
 """Llama / Qwen3 / GPT-2 shaped models (``transformer.{wte,h,ln_f}`` + ``lm_head``
 as in optimus_dl/modules/model/{llama2,qwen3,gpt2}.py), random-initialised with
 the reference's standard deviations (gpt2.py:167-180: 0.02, and 0.02/sqrt(2*n_layer)
-for the residual projections ``c_proj`` / ``wo``)."""
+for the residual projections ``c_proj`` / ``wo``).  Not in the reference: norms behind the blocks, gates and a scaled stream
+(``post_norms``, ``layer_scale``, ``residual_scale``), and ``score``, the log probabilities that a model gives to tokens."""
 
 from __future__ import annotations
 
@@ -11,6 +12,7 @@ from dataclasses import dataclass
 import torch
 import torch.nn as nn
 
+from ..logprobs import TokenLogProbs, token_logprobs
 from .blocks import GPT2Block, LlamaBlock, Qwen3Block, RMSNorm
 
 
@@ -26,6 +28,12 @@ class LlamaConfig:
     rmsnorm_eps: float = 1e-5
     rope_theta: float = 10000.0
     tie_word_embeddings: bool = False
+    post_norms: bool = False                # a norm behind each half of a block as well
+    layer_scale: float | None = None        # a learned gate for each channel of a half's output, beginning at this
+    residual_scale: float = 1.0             # factor on the residual stream where a half's output is added
+
+    def step(self) -> dict:
+        return {"post_norms": self.post_norms, "layer_scale": self.layer_scale, "residual_scale": self.residual_scale}
 
 
 @dataclass
@@ -71,10 +79,23 @@ class _DecoderLM(nn.Module):
         return self.transformer.wte(input_ids)
 
     def forward(self, input_ids: torch.Tensor, **kwargs) -> dict:
-        x = self.embed(input_ids)
-        for block in self.transformer.h:
-            x = block(x)
-        return {"logits": self.lm_head(self.transformer.ln_f(x))}
+        x, z = self.embed(input_ids), None
+        blocks, ln_f = self.transformer.h, self.transformer.ln_f
+        for i, block in enumerate(blocks):
+            if getattr(block, "stepped", False):        # the end of a block and the norm in front of the next in one
+                x, z = block(x, z, blocks[i + 1].ln_1 if i + 1 < len(blocks) else ln_f)
+            else:
+                x, z = block(x), None
+        return {"logits": self.lm_head(ln_f(x) if z is None else z)}
+
+    def score(self, input_ids: torch.Tensor, targets: torch.Tensor | None = None, top_k: int = 0, temperature: float = 1.0,
+              ignore_index: int = -100) -> TokenLogProbs:
+        """Log probabilities of ``targets`` [batch, tokens], with entropy and ``top_k`` alternatives of every position.  Without targets each
+        position is asked for the token behind it, and the last one is ignored.  ``-score(ids).logprobs.sum() / n`` is the loss of training."""
+        if targets is None:
+            targets = torch.cat((input_ids[:, 1:], torch.full_like(input_ids[:, :1], ignore_index)), dim=1)
+        return token_logprobs(self(input_ids)["logits"], targets, n_vocab=self.config.vocab_size, top_k=top_k, temperature=temperature,
+                              ignore_index=ignore_index)
 
 
 class Llama(_DecoderLM):
@@ -84,7 +105,7 @@ class Llama(_DecoderLM):
         self.transformer = nn.ModuleDict({
             "wte": nn.Embedding(config.vocab_size, config.n_embd),
             "h": nn.ModuleList([LlamaBlock(config.n_embd, config.n_head, config.n_kv_head, config.intermediate_size,
-                                           eps=config.rmsnorm_eps, rope_theta=config.rope_theta)
+                                           eps=config.rmsnorm_eps, rope_theta=config.rope_theta, **config.step())
                                 for _ in range(config.n_layer)]),
             "ln_f": RMSNorm(config.n_embd, config.rmsnorm_eps),
         })
@@ -99,7 +120,7 @@ class Qwen3(_DecoderLM):
             "wte": nn.Embedding(config.vocab_size, config.n_embd),
             "h": nn.ModuleList([Qwen3Block(config.n_embd, config.n_head, config.n_kv_head, config.intermediate_size,
                                            head_dim=config.head_dim, eps=config.rmsnorm_eps,
-                                           rope_theta=config.rope_theta) for _ in range(config.n_layer)]),
+                                           rope_theta=config.rope_theta, **config.step()) for _ in range(config.n_layer)]),
             "ln_f": RMSNorm(config.n_embd, config.rmsnorm_eps),
         })
         self._finish(config)

@@ -149,3 +149,72 @@ def test_transform_replaces_linears_of_whole_groups(monkeypatch):
     assert build_model_transform({"_name": "fp4_linear", "enabled": False}).apply(torch.nn.Sequential(torch.nn.Linear(64, 64)))[0].__class__ is torch.nn.Linear
     with pytest.raises(ValueError):
         t.apply(torch.nn.Linear(64, 64))
+
+
+def small_llama(**kwargs):
+    from optimus_dl_amd.modules.model import Llama, LlamaConfig
+
+    torch.manual_seed(0)
+    return Llama(LlamaConfig(vocab_size=50, n_layer=2, n_head=2, n_kv_head=1, n_embd=16, intermediate_size=24, **kwargs))
+
+
+def test_plain_models_are_what_they_were_and_stepped_ones_chain_their_norms():
+    ids = torch.arange(12).reshape(2, 6)
+    plain = small_llama()
+    assert not any("post_ln" in n or "gate" in n for n, _ in plain.named_parameters())
+    x = plain.embed(ids)
+    for block in plain.transformer.h:
+        x = x + block.attn(block.ln_1(x))
+        x = x + block.mlp(block.ln_2(x))
+    assert torch.equal(plain(ids)["logits"], plain.lm_head(plain.transformer.ln_f(x)))
+    m = small_llama(post_norms=True, layer_scale=0.3, residual_scale=0.9)
+    assert {"transformer.h.0.post_ln_1.weight", "transformer.h.1.post_ln_2.weight", "transformer.h.0.gate_1", "transformer.h.1.gate_2"} <= set(m.state_dict())
+    x = m.embed(ids)
+    for block in m.transformer.h:
+        alone = block(x)
+        x = 0.9 * x + block.gate_1 * block.post_ln_1(block.attn(block.ln_1(x)))
+        x = 0.9 * x + block.gate_2 * block.post_ln_2(block.mlp(block.ln_2(x)))
+        assert torch.allclose(alone, x, rtol=1e-5, atol=1e-6)
+    assert torch.allclose(m(ids)["logits"], m.lm_head(m.transformer.ln_f(x)), rtol=1e-4, atol=1e-5)
+
+
+@pytest.mark.parametrize("kwargs", [dict(post_norms=True), dict(layer_scale=0.5), dict(residual_scale=0.7), dict(post_norms=True, layer_scale=0.3, residual_scale=0.9)])
+def test_loss_of_a_stepped_model_against_differences(monkeypatch, kwargs):
+    """In 64 bits (the RMSNorm module, which a model begins with, computes in 32 by itself): central differences of size h are off by h^2 times a
+    third derivative, and by 1e-16 / h."""
+    from optimus_dl_amd.modules.model import blocks
+
+    monkeypatch.setattr(blocks.RMSNorm, "forward", lambda self, x: x * torch.rsqrt(x.pow(2).mean(-1, keepdim=True) + self.eps) * self.weight)
+    m = small_llama(**kwargs).double()
+    ids = torch.arange(12).reshape(2, 6) % 50
+
+    def loss():
+        r = m.score(ids, top_k=2)
+        return -(r.logprobs.sum() + 0.1 * r.entropy.sum() + 0.01 * r.top_logprobs.sum())
+
+    params = list(m.parameters())
+    grads = torch.autograd.grad(loss(), params)
+    g = torch.Generator().manual_seed(1)
+    along = [torch.randn(p.shape, generator=g, dtype=p.dtype) for p in params]
+    ends = []
+    for sign in (1, -1):
+        with torch.no_grad():
+            for p, v in zip(params, along):
+                p.add_(v, alpha=sign * 1e-5)
+            ends.append(loss().item())
+            for p, v in zip(params, along):
+                p.sub_(v, alpha=sign * 1e-5)
+    want = sum((gr * v).sum().item() for gr, v in zip(grads, along))
+    assert abs((ends[0] - ends[1]) / 2e-5 - want) < 1e-5 * (1 + abs(want)) and all(gr.abs().max() > 0 for gr in grads)
+
+
+def test_score_asks_for_the_next_token():
+    m = small_llama()
+    ids = torch.arange(12).reshape(2, 6)
+    with torch.no_grad():
+        r = m.score(ids, top_k=3, temperature=0.5)
+        logp = torch.log_softmax(m(ids)["logits"] / 0.5, -1)
+        assert torch.allclose(r.logprobs[:, :-1], logp[:, :-1].gather(-1, ids[:, 1:, None]).squeeze(-1), atol=1e-5) and not r.logprobs[:, -1].any()
+        assert torch.equal(r.top_ids[:, :-1], logp[:, :-1].topk(3).indices) and (r.top_ids[:, -1] == -1).all()
+        one = m.score(ids[:, :1], targets=ids[:, 1:2])
+        assert torch.allclose(one.logprobs, torch.log_softmax(m(ids[:, :1])["logits"], -1).gather(-1, ids[:, 1:2, None]).squeeze(-1), atol=1e-6)

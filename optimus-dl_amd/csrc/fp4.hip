@@ -244,23 +244,25 @@ void launch_thin(const Fp4Args &a, hipStream_t stream) {
                        dim3(WAVES * kWave), (size_t)(staged > sums ? staged : sums), stream, a);
 }
 
-// Up to 16 * MT rows, many of them: x goes through LDS in phases of kPhase k, double-buffered, and eight waves share it, four times 32
-// columns and two halves of a phase.  Codes, scales and x of the next phase are on their way while the waves multiply.
-template <int G, int MT>
+// Up to 16 * MT rows, many of them: x goes through LDS in phases of kPhase k, double-buffered, and the waves of a block share it, 16 * NT columns each
+// of 128 and one of two halves of a phase.  Codes, scales and x of the next phase are on their way while the waves multiply.
+// Bound by no single thing: of 106 us for 120 rows 8192 -> 28672, groups of 64, the products are 18 to 22, scaling them 16, reading x from LDS 15 and
+// bringing it there 25 to 30 (each left out by itself); of 20 us for 32 rows 14336 -> 4096, groups of 32, scaling is 4 and adding up the runs 4.
+template <int G, int MT, int NT>
 struct Fp4Wide {
-    static constexpr int kNT = 2, kWaves = 8, kPhase = MT >= 8 ? 256 : MT >= 4 ? 512 : 1024, kHalf = kPhase / 2, kSteps = kHalf / 128, kPitch = kPhase + 8;
+    static constexpr int kSlots = 8 / NT, kWaves = 2 * kSlots, kThreads = kWaves * kWave, kPhase = MT >= 8 ? 256 : MT >= 4 ? 512 : 1024, kHalf = kPhase / 2, kSteps = kHalf / 128, kPitch = kPhase + 8;
     static constexpr int kPieces = 16 * MT * kPhase / 8 / (kWaves * kWave), kGroups = kHalf / G, kPairs = (kGroups + 1) / 2;
     static constexpr int kStage = 16 * MT * kPitch;          // elements of a buffer
 };
 
-template <int G, int MT>
-__global__ __launch_bounds__(512) void fp4_wide_kernel(const Fp4Args a, int run_k, int runs) {
-    typedef Fp4Wide<G, MT> W;
-    constexpr int NT = W::kNT, kPer = G / 32;                // instructions of a group
+template <int G, int MT, int NT>
+__global__ __launch_bounds__((Fp4Wide<G, MT, NT>::kThreads)) void fp4_wide_kernel(const Fp4Args a, int run_k, int runs) {
+    typedef Fp4Wide<G, MT, NT> W;
+    constexpr int kPer = G / 32;                // instructions of a group
     __shared__ __attribute__((aligned(16))) uint16_t stage[2][W::kStage];
     const int lane = threadIdx.x % kWave, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave), col = lane % 16, quarter = lane / 16;
-    const int half = wave / 4, K = (int)a.K, groups = K / G;
-    const int64_t n0 = (int64_t)blockIdx.x * (4 * 16 * NT) + wave % 4 * (16 * NT), m0 = (int64_t)blockIdx.y * (16 * MT);
+    const int half = wave / W::kSlots, K = (int)a.K, groups = K / G;
+    const int64_t n0 = (int64_t)blockIdx.x * 128 + wave % W::kSlots * (16 * NT), m0 = (int64_t)blockIdx.y * (16 * MT);
     const int k0 = blockIdx.z * run_k, k1 = min(K, k0 + run_k);
     // (columns and rows past the end are the last ones and not stored)
     const int64_t nb = min(n0, a.N - 1);
@@ -275,7 +277,7 @@ __global__ __launch_bounds__(512) void fp4_wide_kernel(const Fp4Args a, int run_
     }
 #pragma unroll
     for (int i = 0; i < W::kPieces; ++i) {
-        const int piece = i * 512 + threadIdx.x;
+        const int piece = i * W::kThreads + threadIdx.x;
         xoff[i] = (uint32_t)min((int64_t)(piece / (W::kPhase / 8)), a.M - 1 - m0) * (uint32_t)a.ldx + piece % (W::kPhase / 8) * 8;
     }
     f32x4 acc[MT][NT];
@@ -319,13 +321,13 @@ __global__ __launch_bounds__(512) void fp4_wide_kernel(const Fp4Args a, int run_
 #pragma unroll
         for (int i = 0; i < W::kPieces; ++i) {
             next.x[i] = u32x4{0, 0, 0, 0};
-            if (k + (int)((i * 512 + threadIdx.x) % (W::kPhase / 8)) * 8 < k1) next.x[i] = *reinterpret_cast<const u32x4 *>(xbase + (uint32_t)k + xoff[i]);
+            if (k + (int)((i * W::kThreads + threadIdx.x) % (W::kPhase / 8)) * 8 < k1) next.x[i] = *reinterpret_cast<const u32x4 *>(xbase + (uint32_t)k + xoff[i]);
         }
     };
     auto put = [&](uint16_t *to) {
 #pragma unroll
         for (int i = 0; i < W::kPieces; ++i) {
-            const int piece = i * 512 + threadIdx.x, r = piece / (W::kPhase / 8), p = piece % (W::kPhase / 8) * 8;
+            const int piece = i * W::kThreads + threadIdx.x, r = piece / (W::kPhase / 8), p = piece % (W::kPhase / 8) * 8;
             *reinterpret_cast<u32x4 *>(to + r * W::kPitch + p) = next.x[i];
         }
     };
@@ -399,8 +401,8 @@ __global__ __launch_bounds__(512) void fp4_wide_kernel(const Fp4Args a, int run_
         __syncthreads();
     }
     // the second half's sums onto the first's
-    f32x4 *part = reinterpret_cast<f32x4 *>(stage[0]) + (wave % 4) * (MT * NT * kWave) + lane;
-    static_assert(sizeof(stage) >= 4 * MT * NT * kWave * sizeof(f32x4), "the sums fit into the stage");
+    f32x4 *part = reinterpret_cast<f32x4 *>(stage[0]) + (wave % W::kSlots) * (MT * NT * kWave) + lane;
+    static_assert(sizeof(stage) >= W::kSlots * MT * NT * kWave * sizeof(f32x4), "the sums fit into the stage");
     if (half) {
 #pragma unroll
         for (int i = 0; i < MT; ++i)
@@ -428,11 +430,13 @@ __global__ __launch_bounds__(512) void fp4_wide_kernel(const Fp4Args a, int run_
     }
 }
 
-template <int G, int MT>
+template <int G, int MT, int NT>
 int launch_wide(const Fp4Args &a, int runs, hipStream_t stream) {
-    const int phase = Fp4Wide<G, MT>::kPhase, run_k = (int)((a.K + runs - 1) / runs + phase - 1) / phase * phase;
+    typedef Fp4Wide<G, MT, NT> W;
+    const int phase = W::kPhase, run_k = (int)((a.K + runs - 1) / runs + phase - 1) / phase * phase;
     runs = (int)((a.K + run_k - 1) / run_k);                 // (no run is empty)
-    hipLaunchKernelGGL((fp4_wide_kernel<G, MT>), dim3((unsigned)((a.N + 127) / 128), (unsigned)((a.M + 16 * MT - 1) / (16 * MT)), (unsigned)runs), dim3(512), 0, stream, a, run_k, runs);
+    hipLaunchKernelGGL((fp4_wide_kernel<G, MT, NT>), dim3((unsigned)((a.N + 127) / 128), (unsigned)((a.M + 16 * MT - 1) / (16 * MT)), (unsigned)runs), dim3(W::kThreads), 0, stream, a,
+                       run_k, runs);
     return runs;
 }
 
@@ -440,8 +444,14 @@ int launch_wide(const Fp4Args &a, int runs, hipStream_t stream) {
 __global__ __launch_bounds__(256) void fp4_join_kernel(const Fp4Args a, int runs) {
     const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x, total = a.M * a.N;
     if (i >= total) return;
-    float s = a.partial[i];
-    for (int r = 1; r < runs; ++r) s += a.partial[r * total + i];
+    float s = 0.0f;
+    for (int r = 0; r < runs; r += 8) {
+        float v[8];                              // (eight on their way at once)
+#pragma unroll
+        for (int u = 0; u < 8; ++u) v[u] = r + u < runs ? a.partial[(r + u) * total + i] : 0.0f;
+#pragma unroll
+        for (int u = 0; u < 8; ++u) s += v[u];
+    }
     if (a.bias) s += bias_of(a, i % a.N);
     a.y[i] = (uint16_t)pack_bf16x2(s, 0.0f);
 }
@@ -536,9 +546,11 @@ void launch_linear(const Fp4Args &a, int runs, hipStream_t stream) {
         return;
     }
     const int mt = wide_rows(a.M);
-    if (mt == 1) runs = launch_wide<G, 1>(a, runs, stream);
-    else if (mt == 2) runs = launch_wide<G, 2>(a, runs, stream);
-    else runs = launch_wide<G, 8>(a, runs, stream);
+    // Sixteen waves of 16 columns hide more of each other than eight of 32 and read x from LDS twice as often: 120 rows 8192 -> 28672 101 us (106),
+    // 32 rows 4096 -> 14336 18.4 (17.8).  Groups of 128 keep more of x on its way than their 128 registers hold.
+    if (mt == 1) runs = launch_wide<G, 1, 2>(a, runs, stream);
+    else if (mt == 2) runs = launch_wide<G, 2, 2>(a, runs, stream);
+    else runs = launch_wide<G, 8, G == 128 ? 2 : 1>(a, runs, stream);
     if (runs > 1) hipLaunchKernelGGL(fp4_join_kernel, dim3((unsigned)((a.M * a.N + 255) / 256)), dim3(256), 0, stream, a, runs);
 }
 

@@ -486,7 +486,7 @@ int check(const char *who, int dtype, int64_t rows, int64_t stride, int64_t padd
     if (vocab < 1 || vocab > padded || padded > (1 << 24)) return set_error(ODL_ERR_SHAPE, "%s: %lld of %lld columns (1 to 2^24)", who, (long long)vocab, (long long)padded);
     if (rows >= (1 << 22)) return set_error(ODL_ERR_SHAPE, "%s: %lld rows (up to 2^22 - 1)", who, (long long)rows);   // (lanes of a launch are counted in 32 bits)
     if (top_k < 0 || top_k > kMaxTop || top_k > vocab) return set_error(ODL_ERR_ARG, "%s: top_k %d (0 to %d, and to the vocabulary)", who, top_k, kMaxTop);
-    if (!(inv_t > 0.0f) || __builtin_isinf(inv_t)) return set_error(ODL_ERR_ARG, "%s: the temperature must be positive and finite", who);
+    if (!(inv_t >= 0.99e-30f && inv_t <= 1.01e30f)) return set_error(ODL_ERR_ARG, "%s: a temperature from 1e-30 to 1e30", who);
     return ODL_OK;
 }
 

@@ -372,7 +372,7 @@ class _ResidualNormFn(torch.autograd.Function):
             recipe.offer_parts(z, parts)
         ctx.save_for_backward(x, h, weight, post_weight, gate, stats)
         ctx.set_materialize_grads(False)
-        ctx.residual_scale, ctx.recipe = residual_scale, recipe
+        ctx.residual_scale, ctx.recipe = residual_scale, recipe if gradient_is_cast(h, recipe) else None
         return y, z
 
     @staticmethod
@@ -387,7 +387,7 @@ class _ResidualNormFn(torch.autograd.Function):
         dx, dh, parts, dw, dpost, dgate = native.residual_norm_bwd(dy, dz, x, h, weight, post_weight, gate, ctx.residual_scale, stats,
                                                                    want_weights=any(need[2:5]))
         if ctx.recipe is not None and need[1]:
-            ctx.recipe.offer_parts(dh, parts)             # (the gradient of the Linear that ends the block)
+            ctx.recipe.offer_parts(dh, parts)
 
         def given(g, t, wanted):
             if not wanted or t is None or (g.dtype == t.dtype and g.shape == t.shape):
@@ -532,6 +532,17 @@ class _GeluFn(torch.autograd.Function):
 
 # what ``_forward_fp8`` may put between a Linear's product and what its caller gets
 _VIEW_NODES = frozenset(("ViewBackward0", "UnsafeViewBackward0", "ReshapeAliasBackward0", "AliasBackward0"))
+
+
+def gradient_is_cast(x: torch.Tensor, recipe: FP8Recipe | None) -> bool:
+    """Whether the gradient of x goes, as it is, to an FP8 Linear whose cast wants its maxima.  Maxima of any other gradient would be
+    offered to nobody, and the offer keeps the gradient alive until the backward is over."""
+    if recipe is None or recipe.recipe.kind != "tensorwise" or x.grad_fn is None:
+        return False
+    node = x.grad_fn
+    if type(node).__name__ in _VIEW_NODES:
+        node = node.next_functions[0][0]
+    return isinstance(getattr(node, "module", None), FP8Linear)
 
 
 def _gradient_is_summed(x: torch.Tensor, recipe: FP8Recipe) -> bool:

@@ -15,6 +15,7 @@ import torch
 from .. import native
 from .amp import state as _state
 from .calls import no_graph, once_differentiable, untraced
+from .fused import gradient_is_cast
 
 MAX_TOP = native.LOGPROBS_MAX_TOP
 
@@ -37,7 +38,7 @@ class _TokenLogProbsFn(torch.autograd.Function):
                                                                    keep_stats=ctx.needs_input_grad[0])
         ctx.save_for_backward(logits, targets, entropy, stats, ids)
         ctx.set_materialize_grads(False)
-        ctx.asked, ctx.recipe = (n_vocab, top_k, temperature, ignore_index), recipe
+        ctx.asked, ctx.recipe = (n_vocab, top_k, temperature, ignore_index), recipe if gradient_is_cast(logits, recipe) else None
         lead = logits.shape[:-1]
         if top is None:
             return logprobs.reshape(lead), entropy.reshape(lead), None, None
@@ -105,8 +106,8 @@ def token_logprobs(logits: torch.Tensor, targets: torch.Tensor, *, n_vocab: int 
         raise ValueError(f"token_logprobs: n_vocab {n_vocab} of {columns} columns")
     if not 0 <= top_k <= min(MAX_TOP, n_vocab):
         raise ValueError(f"token_logprobs: top_k {top_k} (0 to {MAX_TOP}, and to the vocabulary)")
-    if not 0.0 < temperature < float("inf"):
-        raise ValueError(f"token_logprobs: temperature {temperature} (positive and finite)")
+    if not 1e-30 <= temperature <= 1e30:
+        raise ValueError(f"token_logprobs: temperature {temperature} (1e-30 to 1e30)")
     if not logits.is_cuda:
         return _plain(logits, targets, n_vocab, top_k, float(temperature), ignore_index)
     if logits.dim() == 2 and no_graph():

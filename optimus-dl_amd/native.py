@@ -1727,8 +1727,8 @@ def _logits_operands(logits, targets, n_vocab, top_k, temperature):
         raise NativeError(f"token_logprobs: n_vocab {n_vocab} of {logits.shape[1]} columns (1 to 2^24)")
     if not 0 <= top_k <= min(LOGPROBS_MAX_TOP, n_vocab):
         raise NativeError(f"token_logprobs: top_k {top_k} (0 to {LOGPROBS_MAX_TOP}, and to the vocabulary)")
-    if not (0.0 < temperature < float("inf")) or not 0.0 < np.float32(1.0 / temperature) < np.inf:
-        raise NativeError(f"token_logprobs: temperature {temperature} (positive and finite, its inverse in fp32 too)")
+    if not 1e-30 <= temperature <= 1e30:
+        raise NativeError(f"token_logprobs: temperature {temperature} (1e-30 to 1e30)")
     if targets.dtype != torch.int64 or targets.numel() != logits.shape[0]:
         raise NativeError(f"token_logprobs: targets are {targets.dtype} {tuple(targets.shape)}, expected an int64 for each of {logits.shape[0]} rows")
     if logits.stride(1) != 1 or logits.stride(0) < 0:
@@ -1741,7 +1741,7 @@ def token_logprobs(logits: torch.Tensor, targets: torch.Tensor, n_vocab: int, to
     """Log probabilities of targets [rows] from logits [rows, columns >= n_vocab] (bf16 or fp32, rows at any distance), with the entropy of
     each row and its top_k largest logits (``odl_fp8_token_logprobs`` says what ignored, empty and unsound rows answer).
     -> (logprobs, entropy, stats or None, top_logprobs or None, top_ids or None)."""
-    if _here(logits) and 0.0 < temperature < float("inf") and top_k <= n_vocab:
+    if _here(logits) and 1e-30 <= temperature <= 1e30 and top_k <= n_vocab:
         load()
         r = _host.token_logprobs(logits, targets, n_vocab, top_k, 1.0 / temperature, ignore_index, keep_stats, _stream())
         if r is not None:

@@ -117,3 +117,59 @@ def test_decode_step_with_4_bit_weights(group):
         build_model_transform({"_name": "fp8_linear"}).apply(m)
         with fp8_autocast(CUDA, create_fp8_recipe("tensorwise", "hybrid")):
             assert m.score(ids).logprobs.isfinite().all() and len([x for x in m.modules() if isinstance(x, FP4Linear)]) == 14
+
+
+def test_a_step_of_the_operators_captured_with_its_backward():
+    """The public functions and autograd under capture; replays on new data, with eager passes and synchronizations between them, give the eager bits."""
+    from optimus_dl_amd.modules.fused import residual_norm
+    from optimus_dl_amd.modules.logprobs import token_logprobs
+
+    g = torch.Generator(device="cuda").manual_seed(4)
+    n = lambda *s: torch.randn(s, device=CUDA, generator=g)
+    x, h, w, wp, gate = n(40, 256).requires_grad_(True), n(40, 256).bfloat16().requires_grad_(True), *(n(256).requires_grad_(True) for _ in range(3))
+    head = (n(256, 1003) * 0.05).bfloat16()
+    targets = torch.randint(0, 1003, (40,), device=CUDA, generator=g)
+
+    def step():
+        y, z = residual_norm(x, h, w, 1e-6, post_weight=wp, gate=gate, residual_scale=0.9, out_dtype=torch.bfloat16)
+        r = token_logprobs(z @ head, targets, n_vocab=1000, top_k=3, temperature=0.8)
+        loss = r.logprobs.clamp(min=-20).sum() + r.entropy.sum() + r.top_logprobs.sum() + y.sum()
+        return loss.detach(), r.top_ids, *torch.autograd.grad(loss, (x, h, w, wp, gate))
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        for _ in range(2):
+            step()
+    torch.cuda.current_stream().wait_stream(side)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        held = step()
+    for _ in range(3):
+        with torch.no_grad():
+            for t in (x, h, w):
+                t.copy_(n(*t.shape))
+            targets.copy_(torch.randint(0, 1003, (40,), device=CUDA, generator=g).clamp(max=999))
+        graph.replay()
+        torch.cuda.synchronize()
+        kept = [t.clone() for t in held]
+        eager = step()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(kept, eager))
+
+
+def test_an_unconverted_head_is_offered_nothing():
+    """A gradient that no FP8 Linear takes is not kept for one."""
+    m = model(post_norms=True)
+    head, m.lm_head = m.lm_head, torch.nn.Identity()
+    build_model_transform({"_name": "fp8_linear"}).apply(m)
+    m.lm_head = head
+    ids = torch.randint(0, 1024, (2, 32), device=CUDA)
+    recipe = create_fp8_recipe("tensorwise", "hybrid")
+    with fp8_autocast(CUDA, recipe):
+        loss = -m.score(ids).logprobs.sum()
+    with fp8_backward(recipe):
+        loss.backward()
+        assert not any(t.shape[-1] == 1024 for _, t, *_ in recipe.producer_parts)
+    assert all(p.grad.isfinite().all() for p in m.parameters())

@@ -80,7 +80,7 @@ def test_arguments_are_checked():
     t = torch.zeros(4, dtype=torch.int64)
     for args, kwargs in (((x, t[:3]), {}), ((x, t.int()), {}), ((x.long(), t), {}), ((x, t), {"n_vocab": 0}), ((x, t), {"n_vocab": 65}), ((x, t), {"top_k": 65}),
                          ((x, t), {"top_k": -1}), ((x, t), {"n_vocab": 3, "top_k": 4}), ((x, t), {"temperature": 0.0}), ((x, t), {"temperature": float("inf")}),
-                         ((x, t), {"temperature": float("nan")}), ((x, t.unsqueeze(1)), {})):
+                         ((x, t), {"temperature": float("nan")}), ((x, t), {"temperature": -1.0}), ((x, t), {"temperature": 1e-31}), ((x, t.unsqueeze(1)), {})):
         with pytest.raises(ValueError, match="token_logprobs"):
             token_logprobs(*args, **kwargs)
     codes, scales, xb = torch.zeros(8, 32, dtype=torch.uint8), torch.zeros(8, 2, dtype=torch.bfloat16), x.bfloat16()

@@ -4,6 +4,7 @@
 // dense, aligned or of the expected type, an output of the caller's that does not fit): the wrapper then goes the long way,
 // which copies or refuses.  An int is the status of a C entry that refused.  A step of a few hundred tokens waits for
 // the host, and of its time a third went into the wrappers: per call 5 to 9 us of Python around 3.7 us of launch, here 1 to 2.
+#include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/extension.h>
 #include <torch/version.h>
 
@@ -52,6 +53,7 @@ decltype(&odl_fp8_gemm_runs) runs_c;
 decltype(&odl_fp8_mx_cast_padded) mx_cast_c;
 decltype(&odl_fp8_block_cast) block_cast_c;
 decltype(&odl_fp8_mx_gemm_nt_hinted) mx_gemm_nt_c;
+decltype(&odl_fp8_last_error) last_error_c;
 decltype(&odl_fp8_residual_norm) residual_norm_c;
 decltype(&odl_fp8_residual_norm_bwd) residual_norm_bwd_c;
 decltype(&odl_fp8_token_logprobs) logprobs_c;
@@ -94,6 +96,7 @@ void bind(const py::dict &d) {
     take(mx_cast_c, d, "odl_fp8_mx_cast_padded");
     take(block_cast_c, d, "odl_fp8_block_cast");
     take(mx_gemm_nt_c, d, "odl_fp8_mx_gemm_nt_hinted");
+    take(last_error_c, d, "odl_fp8_last_error");
     take(residual_norm_c, d, "odl_fp8_residual_norm");
     take(residual_norm_bwd_c, d, "odl_fp8_residual_norm_bwd");
     take(logprobs_c, d, "odl_fp8_token_logprobs");
@@ -563,6 +566,155 @@ py::object fp4_linear(const Tensor &x, const Tensor &codes, const Tensor &scales
     return rc ? status(rc) : py::cast(y);
 }
 
+// ---- The same two as autograd nodes, for graphs without a recipe (which would be handed maxima, in Python).  Python's part of a
+// node is 60 to 100 us of a step that computes for 20; these take 25.
+using torch::autograd::AutogradContext;
+using torch::autograd::variable_list;
+
+// an entry's answer where no Python is on the way (the thread of a backward does not hold its lock)
+void done(int rc, const char *what) {
+    if (rc) throw std::runtime_error(std::string(what) + " refused: " + last_error_c());
+}
+OptTensor given(const Tensor &t) { return t.defined() ? OptTensor(t) : OptTensor(); }
+// dense and aligned, as the kernels read it
+OptTensor dense_gradient(const Tensor &t) {
+    if (!t.defined()) return {};
+    Tensor d = t.contiguous();
+    return aligned(d) ? d : d.clone(at::MemoryFormat::Contiguous);
+}
+// Gradients of kernels that autograd cannot see into: where a graph of the backward is recorded, what would differentiate them raises.
+variable_list once(variable_list grads, const char *what) {
+    if (!at::GradMode::is_enabled()) return grads;
+    for (Tensor &g : grads)
+        if (g.defined()) {
+            variable_list in{g.detach().set_requires_grad(true)};
+            g = (*std::make_shared<torch::autograd::DelayedError>(std::string(what) + " can be differentiated once only", 1))(std::move(in))[0];
+        }
+    return grads;
+}
+
+struct ResidualNormNode : torch::autograd::Function<ResidualNormNode> {
+    static variable_list forward(AutogradContext *ctx, const Tensor &x, const Tensor &h, const Tensor &w, const OptTensor &post, const OptTensor &gate, double scale,
+                                 double eps, double post_eps, i64 stream) {
+        const i64 cols = x.size(-1), rows = x.numel() / cols;
+        Tensor y = at::empty_like(x), z = at::empty(x.sizes(), x.options().dtype(at::kBFloat16)), stats = f32(x, {2, rows}), parts = f32(x, {kParts});
+        done(residual_norm_c(ptr(x), src_of(x), ptr(h), src_of(h), ptr(w), ptr(post), ptr(gate), gate ? gate->numel() : 0, rows, cols, (float)scale, (float)eps,
+                             (float)post_eps, ptr(y), ptr(z), static_cast<float *>(ptr(stats)), static_cast<float *>(ptr(parts)), str(stream)),
+             "odl_fp8_residual_norm");
+        ctx->save_for_backward({x, h, w, post.value_or(Tensor()), gate.value_or(Tensor()), stats});
+        ctx->set_materialize_grads(false);
+        ctx->saved_data["scale"] = scale;
+        ctx->saved_data["stream"] = stream;
+        return {y, z};
+    }
+
+    static variable_list backward(AutogradContext *ctx, variable_list out) {
+        variable_list grads(9);
+        if (!out[0].defined() && !out[1].defined()) return grads;
+        const variable_list saved = ctx->get_saved_variables();
+        const Tensor &x = saved[0], &h = saved[1], &w = saved[2], &stats = saved[5];
+        const OptTensor post = given(saved[3]), gate = given(saved[4]), dy = dense_gradient(out[0]), dz = dense_gradient(out[1]);
+        {
+            at::NoGradGuard quiet;
+            const i64 cols = x.size(-1), rows = x.numel() / cols, g = gate ? gate->numel() : 0;
+            const bool weights = ctx->needs_input_grad(2) || (post && ctx->needs_input_grad(3)) || (gate && ctx->needs_input_grad(post ? 4 : 3));
+            Tensor dx = at::empty_like(x), dh = at::empty_like(h), parts = f32(x, {kParts});
+            OptTensor dw, dpost, dgate, ws;
+            if (weights) {
+                dw = f32(x, w.sizes());
+                if (post) dpost = f32(x, post->sizes());
+                if (gate) dgate = f32(x, gate->sizes());
+                ws = f32(x, {ODL_FP8_RESIDUAL_NORM_SLABS * (2 * cols + 1)});
+            }
+            // (a node runs on the stream that its forward ran on)
+            done(residual_norm_bwd_c(ptr(dy), ptr(dz), ptr(x), src_of(x), ptr(h), src_of(h), ptr(w), ptr(post), ptr(gate), g, rows, cols,
+                                     (float)ctx->saved_data["scale"].toDouble(), ptr(stats), ptr(dx), ptr(dh), ptr(parts), ptr(dw), ptr(dpost), ptr(dgate), ptr(ws),
+                                     str(ctx->saved_data["stream"].toInt())),
+                 "odl_fp8_residual_norm_bwd");
+            grads[0] = dx;
+            grads[1] = dh;
+            if (dw) grads[2] = *dw;
+            if (dpost) grads[3] = *dpost;
+            if (dgate) grads[4] = *dgate;
+        }
+        return once(std::move(grads), "residual_norm");
+    }
+};
+
+py::object residual_norm_node(const Tensor &x, const Tensor &h, const Tensor &w, const OptTensor &post, const OptTensor &gate, double scale, double eps,
+                              double post_eps, i64 stream) {
+    if (!residual_operands(x, h, w, post, gate) || x.numel() == 0) return none();
+    variable_list out;
+    {
+        py::gil_scoped_release unlocked;
+        out = ResidualNormNode::apply(x, h, w, post, gate, scale, eps, post_eps, stream);
+    }
+    return py::make_tuple(out[0], out[1]);
+}
+
+struct TokenLogprobsNode : torch::autograd::Function<TokenLogprobsNode> {
+    static variable_list forward(AutogradContext *ctx, const Tensor &logits, const Tensor &targets, i64 vocab, i64 top_k, double inv_t, i64 ignore, i64 stream) {
+        const Tensor l = logits.reshape({-1, logits.size(-1)});
+        const i64 rows = l.size(0);
+        const auto lead = logits.sizes().slice(0, logits.dim() - 1);
+        Tensor lp = f32(l, lead), entropy = f32(l, lead), stats = f32(l, {2, rows}), top, ids;
+        if (top_k) {
+            std::vector<i64> shape(lead.begin(), lead.end());
+            shape.push_back(top_k);
+            top = f32(l, shape);
+            ids = at::empty(shape, l.options().dtype(at::kLong));
+        }
+        done(logprobs_c(ptr(l), src_of(l), rows, l.stride(0), vocab, targets.data_ptr<i64>(), ignore, (float)inv_t, (int)top_k, ptr(lp), ptr(entropy), ptr(stats),
+                        ptr(given(top)), ptr(given(ids)), str(stream)),
+             "odl_fp8_token_logprobs");
+        ctx->save_for_backward({logits, targets, entropy, stats, ids});
+        ctx->set_materialize_grads(false);
+        ctx->saved_data["vocab"] = vocab;
+        ctx->saved_data["top_k"] = top_k;
+        ctx->saved_data["inv_t"] = inv_t;
+        ctx->saved_data["ignore"] = ignore;
+        ctx->saved_data["stream"] = stream;
+        if (!top_k) return {lp, entropy};
+        ctx->mark_non_differentiable({ids});
+        return {lp, entropy, top, ids};
+    }
+
+    static variable_list backward(AutogradContext *ctx, variable_list out) {
+        variable_list grads(7);
+        const i64 top_k = ctx->saved_data["top_k"].toInt();
+        const bool tops = top_k && out[2].defined();
+        if (!out[0].defined() && !out[1].defined() && !tops) return grads;
+        const variable_list saved = ctx->get_saved_variables();
+        const Tensor &logits = saved[0], &targets = saved[1], &entropy = saved[2], &stats = saved[3];
+        const OptTensor dlp = dense_gradient(out[0]), dent = dense_gradient(out[1]), dtop = tops ? dense_gradient(out[2]) : OptTensor(), ids = given(saved[4]);
+        {
+            at::NoGradGuard quiet;
+            const Tensor l = logits.reshape({-1, logits.size(-1)});
+            const i64 rows = l.size(0), cols = l.size(1);
+            Tensor dl = at::empty({rows, cols}, l.options()), parts = f32(l, {kParts});
+            done(logprobs_bwd_c(ptr(l), src_of(l), rows, l.stride(0), ctx->saved_data["vocab"].toInt(), cols, targets.data_ptr<i64>(), ctx->saved_data["ignore"].toInt(),
+                                (float)ctx->saved_data["inv_t"].toDouble(), (int)top_k, ptr(ids), ptr(stats), ptr(entropy), ptr(dlp), ptr(dent), ptr(dtop), ptr(dl), ptr(parts),
+                                str(ctx->saved_data["stream"].toInt())),
+                 "odl_fp8_token_logprobs_bwd");
+            grads[0] = dl.view(logits.sizes());
+        }
+        return once(std::move(grads), "token_logprobs");
+    }
+};
+
+py::object token_logprobs_node(const Tensor &logits, const Tensor &targets, i64 vocab, i64 top_k, double inv_t, i64 ignore, i64 stream) {
+    if (logits.dim() < 1 || logits.numel() == 0 || !dense(targets) || targets.scalar_type() != at::kLong || targets.device() != logits.device()) return none();
+    if (!(logits.dim() == 2 ? logits2d(logits) : dense(logits) && src_of(logits) >= 0)) return none();
+    if (vocab < 1 || vocab > logits.size(-1) || top_k < 0 || top_k > ODL_FP8_LOGPROBS_MAX_TOP || top_k > vocab) return none();
+    variable_list out;
+    {
+        py::gil_scoped_release unlocked;
+        out = TokenLogprobsNode::apply(logits, targets, vocab, top_k, inv_t, ignore, stream);
+    }
+    if (!top_k) return py::make_tuple(out[0], out[1], py::none(), py::none());
+    return py::make_tuple(out[0], out[1], out[2], out[3]);
+}
+
 }  // namespace
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
@@ -602,4 +754,6 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
     m.def("token_logprobs", &token_logprobs);
     m.def("token_logprobs_bwd", &token_logprobs_bwd);
     m.def("fp4_linear", &fp4_linear);
+    m.def("residual_norm_node", &residual_norm_node);
+    m.def("token_logprobs_node", &token_logprobs_node);
 }

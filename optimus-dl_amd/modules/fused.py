@@ -440,6 +440,10 @@ def residual_norm(x: torch.Tensor, h: torch.Tensor, weight: torch.Tensor, eps: f
              and (x.dtype == torch.float32 and h.dtype in (torch.bfloat16, torch.float32) or x.dtype == h.dtype == torch.bfloat16))
     if not takes:
         return _residual_norm_plain(x, h, weight, eps, post_weight, post_eps, gate, residual_scale, out_dtype)
+    if recipe is None and torch.is_grad_enabled():            # nobody to hand maxima to
+        pair = native.residual_norm_node(x, h, weight, eps, post_weight, post_eps, gate, residual_scale)
+        if pair is not None:
+            return pair
     return apply(_ResidualNormFn, x, h, weight, post_weight, gate, float(residual_scale), float(eps), float(post_eps), recipe)
 
 

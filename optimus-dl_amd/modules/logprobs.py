@@ -113,4 +113,9 @@ def token_logprobs(logits: torch.Tensor, targets: torch.Tensor, *, n_vocab: int 
     if logits.dim() == 2 and no_graph():
         logprobs, entropy, _, top, ids = native.token_logprobs(logits, targets, n_vocab, top_k, temperature, ignore_index)
         return TokenLogProbs(logprobs, entropy, top, ids)
-    return TokenLogProbs(*_TokenLogProbsFn.apply(logits, targets, n_vocab, top_k, float(temperature), ignore_index, _state.active_recipe()))
+    recipe = _state.active_recipe()
+    if not gradient_is_cast(logits, recipe) and torch.is_grad_enabled():     # nobody to hand maxima to
+        r = native.token_logprobs_node(logits, targets, n_vocab, top_k, temperature, ignore_index)
+        if r is not None:
+            return TokenLogProbs(*r)
+    return TokenLogProbs(*_TokenLogProbsFn.apply(logits, targets, n_vocab, top_k, float(temperature), ignore_index, recipe))

@@ -1681,6 +1681,14 @@ def residual_norm(x: torch.Tensor, h: torch.Tensor, weight: torch.Tensor, eps: f
     return y, z, stats, parts
 
 
+def residual_norm_node(x, h, weight, eps: float, post_weight, post_eps: float, gate, residual_scale: float):
+    """(y, z) of :func:`residual_norm` as one autograd node on the C++ side, which leaves no maxima; None where the call is not a plain one."""
+    if not _here(x):
+        return None
+    load()
+    return _host.residual_norm_node(x, h, weight, post_weight, gate, residual_scale, eps, post_eps, _stream())
+
+
 RESIDUAL_NORM_SLABS = 512
 
 
@@ -1757,6 +1765,15 @@ def token_logprobs(logits: torch.Tensor, targets: torch.Tensor, n_vocab: int, to
                                              1.0 / temperature, top_k, out[0].data_ptr(), out[1].data_ptr(), p(stats), p(top), p(ids),
                                              _stream()), "odl_fp8_token_logprobs")
     return out[0], out[1], stats, top, ids
+
+
+def token_logprobs_node(logits, targets, n_vocab: int, top_k: int, temperature: float, ignore_index: int):
+    """(logprobs, entropy, top_logprobs or None, top_ids or None) as one autograd node on the C++ side, which leaves no maxima; None where the call is not
+    a plain one."""
+    if not _here(logits):
+        return None
+    load()
+    return _host.token_logprobs_node(logits, targets, n_vocab, top_k, 1.0 / temperature, ignore_index, _stream())
 
 
 def token_logprobs_bwd(logits: torch.Tensor, targets: torch.Tensor, n_vocab: int, top_k: int, temperature: float, ignore_index: int,

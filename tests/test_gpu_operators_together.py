@@ -173,3 +173,52 @@ def test_an_unconverted_head_is_offered_nothing():
         loss.backward()
         assert not any(t.shape[-1] == 1024 for _, t, *_ in recipe.producer_parts)
     assert all(p.grad.isfinite().all() for p in m.parameters())
+
+
+@pytest.mark.parametrize("stream", [torch.float32, torch.bfloat16])
+def test_nodes_of_either_side_give_the_same_bits(monkeypatch, stream):
+    """The autograd node in C++, which graphs without a recipe get, and the one in Python: values, gradients, what is left out, what is refused."""
+    from optimus_dl_amd.modules.fused import residual_norm
+    from optimus_dl_amd.modules.logprobs import token_logprobs
+
+    g = torch.Generator(device="cuda").manual_seed(5)
+    n = lambda *s: torch.randn(s, device=CUDA, generator=g)
+    x, h, dy, dz = n(3, 20, 512).to(stream), n(3, 20, 512).bfloat16(), n(3, 20, 512).to(stream), n(3, 20, 512).bfloat16()
+    w, wp, gates = n(512), n(512), (None, n(512), n(1), torch.tensor(0.3, device=CUDA))
+    logits, targets, dl = n(3, 20, 1003).to(stream), torch.randint(0, 1000, (3, 20), device=CUDA, generator=g), n(3, 20)
+
+    def everything():
+        out = []
+        for gate in gates:
+            for post in (None, wp):
+                for frozen in (False, True):
+                    leaves = [t.clone().requires_grad_(True) for t in (x, h)] + [None if t is None else t.clone().requires_grad_(not frozen) for t in (w, post, gate)]
+                    y, z = residual_norm(leaves[0], leaves[1], leaves[2], 1e-5, post_weight=leaves[3], gate=leaves[4], residual_scale=0.5, out_dtype=torch.bfloat16)
+                    asked = [t for t in leaves if t is not None and t.requires_grad]
+                    for outs, grads in (((y, z), (dy, dz)), ((y,), (dy,)), ((z,), (dz,))):
+                        out += [o.detach() for o in outs] + list(torch.autograd.grad(outs, asked, grads, retain_graph=True))
+        for k in (0, 4):
+            leaf = logits.clone().requires_grad_(True)
+            r = token_logprobs(leaf, targets, n_vocab=1000, top_k=k, temperature=0.5)
+            out += [t.detach() for t in r if t is not None]
+            out += torch.autograd.grad(r.logprobs, leaf, dl, retain_graph=True) + torch.autograd.grad(r.entropy.sum(), leaf, retain_graph=True)
+            if k:
+                out += torch.autograd.grad((r.logprobs, r.top_logprobs), leaf, (dl, n(3, 20, 4).fill_(0.25)), retain_graph=True)
+        return out, type(y.grad_fn).__name__, type(r.logprobs.grad_fn).__name__
+
+    here, *names = everything()
+    monkeypatch.setattr(native, "residual_norm_node", lambda *a: None)
+    monkeypatch.setattr(native, "token_logprobs_node", lambda *a: None)
+    there, *others = everything()
+    assert names != others and len(here) == len(there)
+    for a, b in zip(here, there):
+        assert a.dtype == b.dtype and torch.equal(a, b)
+    monkeypatch.undo()
+    leaf = logits.clone().requires_grad_(True)
+    r = token_logprobs(leaf, targets, n_vocab=1000)
+    leaf.data_ptr(), leaf.detach().add_(1.0)               # changed since it was kept
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        r.logprobs.sum().backward()
+    (first,) = torch.autograd.grad(token_logprobs(logits.requires_grad_(True), targets).entropy.sum(), logits, create_graph=True)
+    with pytest.raises(RuntimeError, match="once"):
+        first.sum().backward()

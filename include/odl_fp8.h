@@ -702,7 +702,8 @@ int odl_fp8_block_cast(const void *x, int src_dtype, int64_t rows, int64_t cols,
  *   y  = residual_scale * x + gate * post_weight * hh        in the type of x
  *   z  = bf16( y / sqrt(mean(y^2) + eps) * weight )          of the unrounded y; parts: partial maxima of |z|
  * x [rows, cols] bf16 or fp32; h bf16, or fp32 beside an fp32 x; the weights and the gate fp32; gate: NULL, one element or cols
- * (gate_size).  cols a multiple of 8, 8 to 8192.  stats[2 * rows]: the two reciprocal roots of every row, for the backward.
+ * (gate_size).  cols a multiple of 8, 8 to 8192.  stats[2 * rows]: the two reciprocal roots of every row, for the backward; stats and
+ * parts may be NULL.
  */
 int odl_fp8_residual_norm(const void *x, int x_dtype, const void *h, int h_dtype, const float *weight, const float *post_weight,
                           const float *gate, int64_t gate_size, int64_t rows, int64_t cols, float residual_scale, float eps,

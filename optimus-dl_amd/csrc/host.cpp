@@ -484,13 +484,18 @@ bool residual_operands(const Tensor &x, const Tensor &h, const Tensor &w, const 
 }
 
 py::object residual_norm(const Tensor &x, const Tensor &h, const Tensor &w, const OptTensor &post, const OptTensor &gate, double scale, double eps,
-                         double post_eps, i64 stream) {
+                         double post_eps, bool keep, i64 stream) {
     if (!residual_operands(x, h, w, post, gate)) return none();
     const i64 cols = x.size(-1), rows = x.numel() / cols;
-    Tensor y = at::empty_like(x), z = at::empty(x.sizes(), x.options().dtype(at::kBFloat16)), stats = f32(x, {2, rows}), parts = f32(x, {kParts});
+    Tensor y = at::empty_like(x), z = at::empty(x.sizes(), x.options().dtype(at::kBFloat16));
+    OptTensor stats, parts;
+    if (keep) {
+        stats = f32(x, {2, rows});
+        parts = f32(x, {kParts});
+    }
     const int rc = call(residual_norm_c, ptr(x), src_of(x), ptr(h), src_of(h), ptr(w), ptr(post), ptr(gate), gate ? gate->numel() : 0, rows, cols,
                         (float)scale, (float)eps, (float)post_eps, ptr(y), ptr(z), ptr(stats), ptr(parts), str(stream));
-    return rc ? status(rc) : py::make_tuple(y, z, stats, parts);
+    return rc ? status(rc) : py::make_tuple(y, z, obj(stats), obj(parts));
 }
 
 py::object residual_norm_bwd(const OptTensor &dy, const OptTensor &dz, const Tensor &x, const Tensor &h, const Tensor &w, const OptTensor &post,

@@ -183,7 +183,7 @@ __global__ __launch_bounds__(Rows<LPR>::kThreads) void residual_norm_kernel(
         row_sums<LPR, 1>(s, lds, turn);
         const float ry = 1.0f / __builtin_sqrtf(s[0] / (float)cols + eps);
         if (row < rows) {
-            if (lane == 0) {
+            if (lane == 0 && stats) {
                 stats[row] = rh;
                 stats[rows + row] = ry;
             }
@@ -203,6 +203,7 @@ __global__ __launch_bounds__(Rows<LPR>::kThreads) void residual_norm_kernel(
             }
         }
     }
+    if (!parts) return;
     am = block_max_u32(fold_u16x2_to_f32bits(am), red);
     if (threadIdx.x == 0) parts[blockIdx.x] = bits_to_float(am);
     if (blockIdx.x == 0)
@@ -460,7 +461,7 @@ extern "C" int odl_fp8_residual_norm(const void *x, int x_dtype, const void *h, 
                                      float post_eps, void *y, void *z, float *stats, float *parts, odl_stream_t stream_) {
     hipStream_t stream = reinterpret_cast<hipStream_t>(stream_);
     if (const int rc = check_shape("odl_fp8_residual_norm", x_dtype, h_dtype, rows, cols, gate_size, gate)) return rc;
-    if (!parts || !weight || (rows > 0 && (!x || !h || !y || !z || !stats))) return set_error(ODL_ERR_ARG, "odl_fp8_residual_norm: null pointer");
+    if (!weight || (rows > 0 && (!x || !h || !y || !z))) return set_error(ODL_ERR_ARG, "odl_fp8_residual_norm: null pointer");
     if (!aligned16(x) || !aligned16(h) || !aligned16(y) || !aligned16(z))
         return set_error(ODL_ERR_SHAPE, "odl_fp8_residual_norm: x, h, y and z must be 16-byte aligned");
     const int lanes = lanes_of(cols);

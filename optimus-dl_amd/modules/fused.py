@@ -440,6 +440,8 @@ def residual_norm(x: torch.Tensor, h: torch.Tensor, weight: torch.Tensor, eps: f
              and (x.dtype == torch.float32 and h.dtype in (torch.bfloat16, torch.float32) or x.dtype == h.dtype == torch.bfloat16))
     if not takes:
         return _residual_norm_plain(x, h, weight, eps, post_weight, post_eps, gate, residual_scale, out_dtype)
+    if recipe is None and no_graph():
+        return native.residual_norm(x, h, weight, eps, post_weight, post_eps, gate, residual_scale, keep=False)[:2]
     if recipe is None and torch.is_grad_enabled():            # nobody to hand maxima to
         pair = native.residual_norm_node(x, h, weight, eps, post_weight, post_eps, gate, residual_scale)
         if pair is not None:

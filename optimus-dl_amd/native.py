@@ -1658,13 +1658,13 @@ def _residual_operands(x, h, weight, post_weight, gate):
 
 
 def residual_norm(x: torch.Tensor, h: torch.Tensor, weight: torch.Tensor, eps: float, post_weight: torch.Tensor | None = None,
-                  post_eps: float | None = None, gate: torch.Tensor | None = None, residual_scale: float = 1.0):
+                  post_eps: float | None = None, gate: torch.Tensor | None = None, residual_scale: float = 1.0, keep: bool = True):
     """y = residual_scale * x + gate * norm(h) * post_weight (h itself without post_weight) in the type of x, z = bf16(norm(y) * weight),
-    norms over the last axis by root mean square.  -> (y, z, stats fp32 [2, rows], partial maxima of |z|)."""
+    norms over the last axis by root mean square.  -> (y, z, stats fp32 [2, rows], partial maxima of |z|), the last two None without keep."""
     post_eps = eps if post_eps is None else post_eps
     if _here(x):
         load()
-        r = _host.residual_norm(x, h, weight, post_weight, gate, residual_scale, eps, post_eps, _stream())
+        r = _host.residual_norm(x, h, weight, post_weight, gate, residual_scale, eps, post_eps, keep, _stream())
         if r is not None:
             return _done(r, "odl_fp8_residual_norm")
     with _Elsewhere(x, h, weight, post_weight, gate):
@@ -1672,12 +1672,12 @@ def residual_norm(x: torch.Tensor, h: torch.Tensor, weight: torch.Tensor, eps: f
         cols = x.shape[-1]
         rows = x.numel() // cols
         y, z = torch.empty_like(x), torch.empty(x.shape, dtype=torch.bfloat16, device=x.device)
-        stats = torch.empty((2, rows), dtype=torch.float32, device=x.device)
-        parts = torch.empty(AMAX_PARTS, dtype=torch.float32, device=x.device)
+        stats = torch.empty((2, rows), dtype=torch.float32, device=x.device) if keep else None
+        parts = torch.empty(AMAX_PARTS, dtype=torch.float32, device=x.device) if keep else None
         _check(load().odl_fp8_residual_norm(x.data_ptr(), _src_dtype(x), h.data_ptr(), _src_dtype(h), w.data_ptr(), post.data_ptr() if post is not None else None,
                                             g.data_ptr() if g is not None else None, g.numel() if g is not None else 0, rows, cols,
-                                            float(residual_scale), float(eps), float(post_eps), y.data_ptr(), z.data_ptr(), stats.data_ptr(),
-                                            parts.data_ptr(), _stream()), "odl_fp8_residual_norm")
+                                            float(residual_scale), float(eps), float(post_eps), y.data_ptr(), z.data_ptr(),
+                                            stats.data_ptr() if keep else None, parts.data_ptr() if keep else None, _stream()), "odl_fp8_residual_norm")
     return y, z, stats, parts
 
 

@@ -168,6 +168,8 @@ def test_parts_are_the_maxima_and_weights_in_bf16_get_their_gradients():
             t, dy, dz = case(rows, 1024, stream, branch, True, "channel")
             y, z, stats, parts = N.residual_norm(t["x"], t["h"], t["weight"], EPS, t["post_weight"], None, t["gate"], 1.0)
             assert parts.shape == (N.AMAX_PARTS,) and parts.max().item() == z.float().abs().max().item()
+            bare = N.residual_norm(t["x"], t["h"], t["weight"], EPS, t["post_weight"], None, t["gate"], 1.0, keep=False)
+            assert torch.equal(bare[0], y) and torch.equal(bare[1], z) and bare[2:] == (None, None)
             dx, dh, parts, dw, dpost, dgate = N.residual_norm_bwd(dy, dz, t["x"], t["h"], t["weight"], t["post_weight"], t["gate"], 1.0, stats)
             assert parts.max().item() == dh.float().abs().max().item()
             frozen = N.residual_norm_bwd(dy, dz, t["x"], t["h"], t["weight"], t["post_weight"], t["gate"], 1.0, stats, want_weights=False)

@@ -21,8 +21,8 @@ def refused(name, args, word):
 def test_residual_norm_entry_refuses():
     ok = dict(x=P, xd=1, h=P, hd=0, w=P, post=P, gate=P, gs=64, rows=4, cols=64, a=1.0, eps=1e-6, pe=1e-6, y=P, z=P, stats=P, parts=P, stream=None)
     for change, word in ((dict(rows=-1), "negative"), (dict(xd=2), "x_dtype"), (dict(xd=0, hd=1), "h_dtype"), (dict(cols=60, gs=60), "multiple of 8"), (dict(cols=0), "multiple of 8"),
-                         (dict(cols=8200), "8192"), (dict(gs=2), "gate"), (dict(w=None), "null"), (dict(parts=None), "null"), (dict(x=None), "null"),
-                         (dict(stats=None), "null"), (dict(x=P + 8), "aligned"), (dict(z=P + 2), "aligned")):
+                         (dict(cols=8200), "8192"), (dict(gs=2), "gate"), (dict(w=None), "null"), (dict(y=None), "null"), (dict(x=None), "null"),
+                         (dict(x=P + 8), "aligned"), (dict(z=P + 2), "aligned")):
         refused("odl_fp8_residual_norm", tuple({**ok, **change}.values()), word)
     ok = dict(dy=P, dz=P, x=P, xd=1, h=P, hd=0, w=P, post=P, gate=P, gs=1, rows=4, cols=64, a=1.0, stats=P, dx=P, dh=P, parts=P, dw=P, dpost=P, dgate=P, ws=P,
               stream=None)

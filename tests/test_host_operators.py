@@ -218,3 +218,15 @@ def test_score_asks_for_the_next_token():
         assert torch.equal(r.top_ids[:, :-1], logp[:, :-1].topk(3).indices) and (r.top_ids[:, -1] == -1).all()
         one = m.score(ids[:, :1], targets=ids[:, 1:2])
         assert torch.allclose(one.logprobs, torch.log_softmax(m(ids[:, :1])["logits"], -1).gather(-1, ids[:, 1:2, None]).squeeze(-1), atol=1e-6)
+
+
+def test_only_conversions_that_widen_codes_need_no_saturating_mode():
+    from optimus_dl_amd.build import check_saturating_conversions
+
+    def found(instruction):
+        return len(check_saturating_conversions(f"_Z1kv:\n\t{instruction}\n", "x.s"))
+
+    assert found("v_cvt_scalef32_pk_bf16_fp4 v0, v1, 1.0") == 0
+    assert found("v_cvt_scalef32_pk_fp4_bf16 v0, v1, 1.0") == 1
+    assert found("v_cvt_scalef32_pk_bf16_fp8 v0, v1, 1.0") == 1
+    assert found("v_cvt_scalef32_pk_bf8_f32 v0, v1, v2, 1.0") == 1

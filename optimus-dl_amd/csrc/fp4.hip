@@ -509,16 +509,19 @@ __global__ __launch_bounds__(256) void fp4_quantise_kernel(const void *__restric
 bool aligned16(const void *p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 bool group_known(int group) { return group == 32 || group == 64 || group == 128; }
 
-// Which kernel, by what it was measured to take (us):
-//   up to 4 rows, thin with x in LDS: 4096 -> 14336 10.2 (wide 17), 768 -> 2304 3.2 (10)
-//   matrices of less than 4 M weights, thin: 24 rows 768 -> 2304 4.7 (wide 10.4: its phases do not pay for themselves)
-//   else wide: 16 rows 4096 -> 14336 14.8 (thin 16.3), 32 rows 14336 -> 4096 20.9 (22.9), 120 rows 8192 -> 28672 109 (174)
+// Which kernel.  Up to 4 rows the thin one, x in LDS: 4096 -> 14336 10 us (wide 17), 768 -> 2304 3.2 (10).  For more, its blocks of up to 32 rows by
+// 16 columns take K * (10 + rows) / 20000 us each and 256 of them run at a time, while the wide kernel begins at 9 to 12 us and grows
+// little.  Thin / wide, us, either side of where they meet: 4096 -> 4096 16 rows 8.4 / 9.5, 32 rows 11.5 / 11.0; 2048 -> 8192 8 rows 7.5 / 8.3, 24 rows
+// 11.0 / 10.2; 8192 -> 1024 5 rows 8.3 / 8.8, 8 rows 9.7 / 8.8; 4096 -> 14336 5 rows 16.3 / 11.4; 768 -> 2304 128 rows 9.5 / 11.4, 512 rows 27 / 18.6,
+// 2048 rows 95 / 31.
 // The thin kernel stages the scales of whole rows, which for a very long K do not fit.
 constexpr int64_t kThinLds = 64 * 1024;
 
 template <int G>
 bool takes_thin(int64_t M, int64_t N, int64_t K) {
-    return 2 * 16 * (int64_t)fp4_tile<G>((int)K).pitch <= kThinLds && (M <= 4 || N * K < (int64_t)4 << 20);
+    if (2 * 16 * (int64_t)fp4_tile<G>((int)K).pitch > kThinLds) return false;
+    const int64_t blocks = (N + 15) / 16 * ((M + 31) / 32);
+    return M <= 4 || K * (10 + (M < 32 ? M : 32)) * (blocks > 256 ? blocks : 256) < (int64_t)1 << 25;
 }
 
 // rows of a block of the wide kernel, in 16s

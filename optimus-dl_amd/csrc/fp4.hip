@@ -509,36 +509,42 @@ __global__ __launch_bounds__(256) void fp4_quantise_kernel(const void *__restric
 bool aligned16(const void *p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 bool group_known(int group) { return group == 32 || group == 64 || group == 128; }
 
-// Which kernel.  Up to 4 rows the thin one, x in LDS: 4096 -> 14336 10 us (wide 17), 768 -> 2304 3.2 (10).  For more, its blocks of up to 32 rows by
-// 16 columns take K * (10 + rows) / 20000 us each and 256 of them run at a time, while the wide kernel begins at 9 to 12 us and grows
-// little.  Thin / wide, us, either side of where they meet: 4096 -> 4096 16 rows 8.4 / 9.5, 32 rows 11.5 / 11.0; 2048 -> 8192 8 rows 7.5 / 8.3, 24 rows
-// 11.0 / 10.2; 8192 -> 1024 5 rows 8.3 / 8.8, 8 rows 9.7 / 8.8; 4096 -> 14336 5 rows 16.3 / 11.4; 768 -> 2304 128 rows 9.5 / 11.4, 512 rows 27 / 18.6,
-// 2048 rows 95 / 31.
 // The thin kernel stages the scales of whole rows, which for a very long K do not fit.
 constexpr int64_t kThinLds = 64 * 1024;
 
+// How a product is done: rows of a block of the wide kernel in 16s (0: the thin kernel), and runs of K.
+struct Fp4Plan {
+    int mt, runs;
+};
+
+// Up to 4 rows the thin kernel, x in LDS: 4096 -> 14336 10 us (wide 17), 768 -> 2304 3.2 (10).  For more the cheapest by what a block was measured
+// to take: thin 0.39 + 0.058 a row, ns for each k; wide 3.0, 4.1, 5.4 and 9.8 for 16, 32, 64 and 128 rows and some 2 us besides, with as many
+// blocks at a time as there are compute units; a join 1.6 us and 1.6 ps for each number.  Over 195 products of 5 to 1024 rows, 768 -> 768 to
+// 28672 -> 8192, what this takes is 1 % off the best of them all on average and 13 % at worst.  (By rows and size of the weights alone, as it
+// was: 20 % and 95 %.)
 template <int G>
-bool takes_thin(int64_t M, int64_t N, int64_t K) {
-    if (2 * 16 * (int64_t)fp4_tile<G>((int)K).pitch > kThinLds) return false;
-    const int64_t blocks = (N + 15) / 16 * ((M + 31) / 32);
-    return M <= 4 || K * (10 + (M < 32 ? M : 32)) * (blocks > 256 ? blocks : 256) < (int64_t)1 << 25;
+Fp4Plan plan(int64_t M, int64_t N, int64_t K) {
+    const bool fits = 2 * 16 * (int64_t)fp4_tile<G>((int)K).pitch <= kThinLds;
+    if (fits && M <= 4) return {0, 1};
+    const int64_t cus = device_cu_count(), thin = (N + 15) / 16 * (M <= 16 ? 1 : (M + 31) / 32);
+    Fp4Plan best = {0, 1};
+    int64_t least = fits ? 4100000 + K * (390 + 58 * (M < 32 ? M : 32)) * (thin > cus ? thin : cus) / cus : INT64_MAX;      // ps
+    static constexpr struct { int mt, phase, per_k, start; } kinds[] = {{1, 1024, 3000, 1500000}, {2, 1024, 4100, 2000000}, {4, 512, 5400, 2000000}, {8, 256, 9800, 3000000}};
+    for (const auto &kind : kinds) {
+        const int64_t tiles = (N + 127) / 128 * ((M + 16 * kind.mt - 1) / (16 * kind.mt));
+        for (const int runs : {1, 2, 3, 4, 6, 8, 12, 16, 24, 32}) {
+            if (runs > 1 && (runs * kind.phase > K || M * N >= (int64_t)1 << 32)) break;
+            const int64_t k = ((K + runs - 1) / runs + kind.phase - 1) / kind.phase * kind.phase, rounds = (tiles * ((K + k - 1) / k) + cus - 1) / cus;
+            const int64_t cost = 3300000 + rounds * (kind.start + k * kind.per_k) + (runs > 1 ? 1600000 + runs * M * N * 8 / 5 : 0);
+            if (cost < least) { least = cost; best = {kind.mt, runs}; }
+        }
+    }
+    return best;
 }
 
-// rows of a block of the wide kernel, in 16s
-int wide_rows(int64_t M) { return M <= 16 ? 1 : M <= 64 ? 2 : 8; }
-
-// Runs of K that fill the chip with blocks of the wide kernel, none shorter than a phase.
-int wide_runs(int64_t M, int64_t N, int64_t K) {
-    const int mt = wide_rows(M);
-    const int64_t blocks = (N + 127) / 128 * ((M + 16 * mt - 1) / (16 * mt)), most = K / (mt == 8 ? 256 : 1024);
-    int64_t r = device_cu_count() / blocks;
-    r = r < most ? r : most;
-    return (int)(r < 1 ? 1 : r);
-}
-
 template <int G>
-void launch_linear(const Fp4Args &a, int runs, hipStream_t stream) {
-    if (takes_thin<G>(a.M, a.N, a.K)) {
+void launch_linear(const Fp4Args &a, const Fp4Plan how, hipStream_t stream) {
+    if (how.mt == 0) {
         const Fp4Tile t = fp4_tile<G>((int)a.K);
         const bool lds = a.M <= 4 && 2 * (16 * (int64_t)t.pitch + a.M * t.xpitch) <= kThinLds, deep = t.whole >= 32;
         // long rows: 16 waves share them (14336 -> 4096 11.5 -> 10.5, 4096 -> 14336 no faster)
@@ -548,13 +554,19 @@ void launch_linear(const Fp4Args &a, int runs, hipStream_t stream) {
         else launch_thin<G, 2, 1, 4, 1, false>(a, stream);
         return;
     }
-    const int mt = wide_rows(a.M);
     // Sixteen waves of 16 columns hide more of each other than eight of 32 and read x from LDS twice as often: 120 rows 8192 -> 28672 101 us (106),
-    // 32 rows 4096 -> 14336 18.4 (17.8).  Groups of 128 keep more of x on its way than their 128 registers hold.
-    if (mt == 1) runs = launch_wide<G, 1, 2>(a, runs, stream);
-    else if (mt == 2) runs = launch_wide<G, 2, 2>(a, runs, stream);
+    // 64 rows 14336 -> 4096 21.2 (23.9), but 32 rows 4096 -> 14336 18.4 (17.8).  Groups of 128 keep more of x on its way than the 128 registers of sixteen
+    // waves hold beside 128 rows.
+    int runs = how.runs;
+    if (how.mt == 1) runs = launch_wide<G, 1, 2>(a, runs, stream);
+    else if (how.mt == 2) runs = launch_wide<G, 2, 2>(a, runs, stream);
+    else if (how.mt == 4) runs = launch_wide<G, 4, 1>(a, runs, stream);
     else runs = launch_wide<G, 8, G == 128 ? 2 : 1>(a, runs, stream);
     if (runs > 1) hipLaunchKernelGGL(fp4_join_kernel, dim3((unsigned)((a.M * a.N + 255) / 256)), dim3(256), 0, stream, a, runs);
+}
+
+Fp4Plan plan_of(int64_t M, int64_t N, int64_t K, int group) {
+    return group == 32 ? plan<32>(M, N, K) : group == 64 ? plan<64>(M, N, K) : plan<128>(M, N, K);
 }
 
 }  // namespace
@@ -564,9 +576,8 @@ using namespace odl;
 
 // Partial results that a call writes: its workspace is as many times M * N floats; 0 needs none.
 extern "C" int odl_fp8_fp4_linear_runs(int64_t M, int64_t N, int64_t K, int group) {
-    if (M < 1 || N < 1 || K < 1 || K > (int64_t)1 << 24) return 0;
-    const bool thin = group == 32 ? takes_thin<32>(M, N, K) : group == 64 ? takes_thin<64>(M, N, K) : takes_thin<128>(M, N, K);
-    const int runs = thin ? 1 : wide_runs(M, N, K);
+    if (M < 1 || N < 1 || K < 1 || M > (int64_t)1 << 16 || N > (int64_t)1 << 22 || K > (int64_t)1 << 24) return 0;
+    const int runs = plan_of(M, N, K, group).runs;
     return runs > 1 ? runs : 0;
 }
 
@@ -583,16 +594,15 @@ extern "C" int odl_fp8_fp4_linear(const void *x, int64_t ldx, const uint8_t *cod
         return set_error(ODL_ERR_SHAPE, "odl_fp8_fp4_linear: x and codes must be 16-byte aligned, rows of x too, at most 2^24 elements apart");
     if (N > (int64_t)1 << 22 || M > (int64_t)1 << 16 || K > (int64_t)1 << 24)
         return set_error(ODL_ERR_SHAPE, "odl_fp8_fp4_linear: up to 2^16 rows, 2^22 columns and 2^24 inputs");
-    const int runs = odl_fp8_fp4_linear_runs(M, N, K, group);
-    if (runs && (!workspace || workspace_bytes / 4 / M / N < runs))
-        return set_error(ODL_ERR_ARG, "odl_fp8_fp4_linear: a workspace of %d * M * N floats is needed", runs);
-    if (runs && M * N >= (int64_t)1 << 32) return set_error(ODL_ERR_SHAPE, "odl_fp8_fp4_linear: an output of that size is not cut over K");
+    const Fp4Plan how = plan_of(M, N, K, group);
+    if (how.runs > 1 && (!workspace || workspace_bytes / 4 / M / N < how.runs))
+        return set_error(ODL_ERR_ARG, "odl_fp8_fp4_linear: a workspace of %d * M * N floats is needed", how.runs);
     Fp4Args a = {};
     a.x = static_cast<const uint16_t *>(x); a.scales = static_cast<const uint16_t *>(scales); a.codes = codes; a.bias = bias; a.y = static_cast<uint16_t *>(y);
     a.partial = workspace; a.M = M; a.N = N; a.K = K; a.ldx = M > 1 ? ldx : 0; a.bias_f32 = bias_dtype == ODL_F32;
-    if (group == 32) launch_linear<32>(a, runs ? runs : 1, stream);
-    else if (group == 64) launch_linear<64>(a, runs ? runs : 1, stream);
-    else launch_linear<128>(a, runs ? runs : 1, stream);
+    if (group == 32) launch_linear<32>(a, how, stream);
+    else if (group == 64) launch_linear<64>(a, how, stream);
+    else launch_linear<128>(a, how, stream);
     return check_launch("odl_fp8_fp4_linear");
 }
 

@@ -52,7 +52,7 @@ def fp4_linear(x: torch.Tensor, codes: torch.Tensor, scales: torch.Tensor, bias:
     """``x @ weight.T + bias`` for x [..., in] in bf16 and weights as :func:`quantise_fp4` makes them; bias bf16 or fp32 [out] or None.  Accumulated in
     fp32, rounded once.  -> bf16 [..., out].
 
-    Made for up to some hundred rows: the weights are read again for every 64.  For inference: an input that wants a gradient is refused."""
+    Made for up to some hundred rows: the weights are read again for every 16 to 128 of them.  For inference: an input that wants a gradient is refused."""
     if torch.is_grad_enabled() and (x.requires_grad or (bias is not None and bias.requires_grad)):
         raise RuntimeError("fp4_linear has no backward: call it under torch.no_grad()")
     _check_weight(codes, scales)

@@ -70,6 +70,18 @@ def test_layers_of_models(n, k, group):
         check(torch.randn((rows, k), device="cuda", generator=g).bfloat16(), codes, scales)
 
 
+# blocks of 16, 32, 64 and 128 rows, K in one run and in several, the last ones ragged
+@pytest.mark.parametrize("group", [32, 64, 128])
+@pytest.mark.parametrize("rows,n,k", [(33, 4100, 1664), (63, 8200, 1664), (257, 4100, 1664), (200, 8200, 1664), (33, 4100, 2176), (257, 100, 4224),
+                                      (13, 1030, 8320), (31, 8200, 3200), (17, 8200, 6272), (130, 4100, 2176), (50, 4100, 3200), (65, 8200, 4224),
+                                      (65, 4100, 6272)])
+def test_ways_of_cutting_a_product(rows, n, k, group):
+    codes, scales, g = weight_of(n, k, group, rows)
+    x = torch.randn((rows, k), device="cuda", generator=g).bfloat16()
+    bias = torch.randn(n, device="cuda", generator=g)
+    assert torch.equal(check(x, codes, scales, bias), fp4_linear(x, codes, scales, bias))
+
+
 def test_whole_numbers_are_exact_and_every_group_has_its_own_scale():
     for group in (32, 64, 128):
         codes, _, g = weight_of(70, 1280, group)

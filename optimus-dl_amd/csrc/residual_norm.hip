@@ -14,7 +14,11 @@
 // c3 needs e and e needs c2; with k = b * hh it is ((S1 - ry * c2 * S2) / cols, S1 = sum k * (dy + ry * t), S2 = sum k * yh, so
 // that one round of three row sums does for both means.
 //
-// Bound by HBM: 12 and 18 bytes an element against some 10 and 40 operations.
+// Bound by HBM: 12 and 18 bytes an element (fp32 stream, bf16 block output) against some 10 and 40 operations.  16 to 512 lanes hold a row, two
+// chunks of 8 elements a lane at most: the row is read once, the next one is on its way, and the weights of a lane's columns and the sums of
+// their gradients stay in its registers from row to row.  8192 x 4096, fp32 / bf16: forward 76 us (5.3 TB/s; a copy reaches 5.1), backward
+// 112 us (5.4 TB/s) and 5 us for the sums of its slabs; 4016 x 2048 in bf16 16, 23 and 4; one row of 4096 3.4, latency of its loads and sums.
+// (fp32 rows of more than 4096 beside an fp32 block output spill 60 bytes a lane in the backward: 16 columns of six arrays.)
 #include "common.h"
 
 #pragma clang fp contract(off)

@@ -252,16 +252,18 @@ void launch_thin(const Fp4Args &a, hipStream_t stream) {
 // bringing it there 25 to 30 (each left out by itself); of 20 us for 32 rows 14336 -> 4096, groups of 32, scaling is 4 and adding up the runs 4.
 template <int G, int MT, int NT>
 struct Fp4Wide {
-    static constexpr int kSlots = 8 / NT, kWaves = 2 * kSlots, kThreads = kWaves * kWave, kPhase = MT >= 8 ? 256 : MT >= 4 ? 512 : 1024, kHalf = kPhase / 2, kSteps = kHalf / 128, kPitch = kPhase + 8;
+    static constexpr int kSlots = 8 / NT, kWaves = 2 * kSlots, kThreads = kWaves * kWave, kPhase = MT >= 8 ? 256 : MT >= 4 ? 512 : 1024, kHalf = kPhase / 2, kSteps = kHalf / 128;
     static constexpr int kPieces = 16 * MT * kPhase / 8 / (kWaves * kWave), kGroups = kHalf / G, kPairs = (kGroups + 1) / 2;
-    static constexpr int kStage = 16 * MT * kPitch;          // elements of a buffer
+    static constexpr int kStage = 16 * MT * kPhase;          // elements of a buffer
+    static constexpr int kRow = kPhase / 8;                  // 16-byte pieces of a row
+    static_assert(kPieces * kThreads * 8 == kStage, "the lanes' pieces are the buffer");
 };
 
 template <int G, int MT, int NT>
 __global__ __launch_bounds__((Fp4Wide<G, MT, NT>::kThreads)) void fp4_wide_kernel(const Fp4Args a, int run_k, int runs) {
     typedef Fp4Wide<G, MT, NT> W;
     constexpr int kPer = G / 32;                // instructions of a group
-    __shared__ __attribute__((aligned(16))) uint16_t stage[2][W::kStage];
+    __shared__ __attribute__((aligned(1024))) uint16_t stage[2][W::kStage];
     const int lane = threadIdx.x % kWave, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave), col = lane % 16, quarter = lane / 16;
     const int half = wave / W::kSlots, K = (int)a.K, groups = K / G;
     const int64_t n0 = (int64_t)blockIdx.x * 128 + wave % W::kSlots * (16 * NT), m0 = (int64_t)blockIdx.y * (16 * MT);
@@ -270,18 +272,34 @@ __global__ __launch_bounds__((Fp4Wide<G, MT, NT>::kThreads)) void fp4_wide_kerne
     const int64_t nb = min(n0, a.N - 1);
     const uint8_t *cbase = a.codes + nb * (a.K / 2);
     const uint16_t *sbase = a.scales + nb * groups, *xbase = a.x + m0 * a.ldx;
-    uint32_t coff[NT], soff[NT], xoff[W::kPieces];
+    uint32_t coff[NT], soff[NT], xrow[W::kPieces];
+    int xk[W::kPieces];
 #pragma unroll
     for (int j = 0; j < NT; ++j) {
         const uint32_t n = (uint32_t)min((int64_t)(16 * j + col), a.N - 1 - nb);
         coff[j] = n * (uint32_t)(K / 2) + quarter * 16;
         soff[j] = n * (uint32_t)groups;
     }
+    // x goes to LDS without passing registers: 64 lanes' pieces of 16 bytes land one behind the other, so what can be chosen is what a lane reads.  Place
+    // s of row r holds piece s ^ (r % 16) of it: the 16 rows that are read at a time then lie in different banks.
 #pragma unroll
     for (int i = 0; i < W::kPieces; ++i) {
-        const int piece = i * W::kThreads + threadIdx.x;
-        xoff[i] = (uint32_t)min((int64_t)(piece / (W::kPhase / 8)), a.M - 1 - m0) * (uint32_t)a.ldx + piece % (W::kPhase / 8) * 8;
+        const int place = i * W::kThreads + threadIdx.x, r = place / W::kRow;
+        xrow[i] = (uint32_t)min((int64_t)r, a.M - 1 - m0) * (uint32_t)a.ldx;
+        xk[i] = ((place % W::kRow) ^ (r % 16)) * 8;
     }
+    int xread[4];                                // where a lane finds the four k of a step
+#pragma unroll
+    for (int s = 0; s < 4; ++s) xread[s] = col * W::kPhase + half * W::kHalf + ((G < 128 ? s * 4 + quarter : quarter * 4 + s) ^ col) * 8;
+    const uint32_t stage_at = (uint32_t)(uintptr_t)(const __attribute__((address_space(3))) uint16_t *)stage[0];
+    auto load_x = [&](int to, int k, int last) {
+#pragma unroll
+        for (int i = 0; i < W::kPieces; ++i) {
+            const uint16_t *from = xbase + xrow[i] + min(k + xk[i], last);
+            asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off"
+                         ::"s"(stage_at + 2 * to * W::kStage + (i * W::kWaves + wave) * 1024), "v"(from) : "memory");
+        }
+    };
     f32x4 acc[MT][NT];
 #pragma unroll
     for (int i = 0; i < MT; ++i)
@@ -289,7 +307,7 @@ __global__ __launch_bounds__((Fp4Wide<G, MT, NT>::kThreads)) void fp4_wide_kerne
         for (int j = 0; j < NT; ++j) acc[i][j] = f32x4{0, 0, 0, 0};
 
     struct Next {
-        u32x4 codes[W::kSteps][NT], x[W::kPieces];
+        u32x4 codes[W::kSteps][NT];
         uint32_t scales[NT][W::kPairs];
     } next;
     auto fetch = [&](int k) {
@@ -301,8 +319,6 @@ __global__ __launch_bounds__((Fp4Wide<G, MT, NT>::kThreads)) void fp4_wide_kerne
             if constexpr (W::kGroups == 1) next.scales[j][0] = sbase[(uint32_t)(kc / G) + soff[j]];
             else __builtin_memcpy(next.scales[j], sbase + (uint32_t)(kc / G) + soff[j], sizeof(next.scales[j]));
         }
-#pragma unroll
-        for (int i = 0; i < W::kPieces; ++i) next.x[i] = *reinterpret_cast<const u32x4 *>(xbase + (uint32_t)k + xoff[i]);
     };
     auto fetch_end = [&](int k) {                            // a phase that k1 ends: what is behind it is zero
         const int kc = k + half * W::kHalf;
@@ -320,22 +336,21 @@ __global__ __launch_bounds__((Fp4Wide<G, MT, NT>::kThreads)) void fp4_wide_kerne
             for (int g = 0; g < W::kPairs; ++g)
                 next.scales[j][g] = (kc + 2 * g * G < k1 ? v[2 * g] : 0u) | (kc + (2 * g + 1) * G < k1 ? v[2 * g + 1] << 16 : 0u);
         }
-#pragma unroll
-        for (int i = 0; i < W::kPieces; ++i) {
-            next.x[i] = u32x4{0, 0, 0, 0};
-            if (k + (int)((i * W::kThreads + threadIdx.x) % (W::kPhase / 8)) * 8 < k1) next.x[i] = *reinterpret_cast<const u32x4 *>(xbase + (uint32_t)k + xoff[i]);
-        }
     };
-    auto put = [&](uint16_t *to) {
-#pragma unroll
-        for (int i = 0; i < W::kPieces; ++i) {
-            const int piece = i * W::kThreads + threadIdx.x, r = piece / (W::kPhase / 8), p = piece % (W::kPhase / 8) * 8;
-            *reinterpret_cast<u32x4 *>(to + r * W::kPitch + p) = next.x[i];
-        }
+    auto ask_for = [&](int to, int k) {
+        if (k + W::kPhase <= k1) fetch(k);
+        else fetch_end(k);
+        load_x(to, k, k1 - 8);                   // (pieces behind k1: the last one, zeroed below)
     };
-    if (k0 + W::kPhase <= k1) fetch(k0);
-    else fetch_end(k0);
-    put(stage[0]);
+    auto arrived = [&](int to, int k) {          // this lane's own pieces
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        if (k + W::kPhase <= k1) return;
+#pragma unroll
+        for (int i = 0; i < W::kPieces; ++i)
+            if (k + xk[i] >= k1) *reinterpret_cast<u32x4 *>(stage[to] + (i * W::kThreads + threadIdx.x) * 8) = u32x4{0, 0, 0, 0};
+    };
+    ask_for(0, k0);
+    arrived(0, k0);
     __syncthreads();
     int buf = 0;
     for (int k = k0; k < k1; k += W::kPhase, buf ^= 1) {
@@ -349,9 +364,8 @@ __global__ __launch_bounds__((Fp4Wide<G, MT, NT>::kThreads)) void fp4_wide_kerne
             for (int g = 0; g < W::kPairs; ++g) scales[j][g] = next.scales[j][g];
         }
         const bool more = k + W::kPhase < k1;
-        if (k + 2 * W::kPhase <= k1) fetch(k + W::kPhase);
-        else if (more) fetch_end(k + W::kPhase);
-        const uint16_t *xs = stage[buf] + col * W::kPitch + half * W::kHalf + quarter * (G < 128 ? 8 : 32);
+        if (more) ask_for(buf ^ 1, k + W::kPhase);
+        const uint16_t *xs = stage[buf];
         // Units of 16 rows and one group of k, software-pipelined: x is asked for kAhead units before its products, and the products of a
         // unit are scaled onto the sums behind the products of the next kBehind.
         constexpr int kUnits = W::kSteps * (4 / kPer) * MT, kAhead = 4 / kPer, kBehind = kPer > 2 ? 1 : 2;
@@ -363,7 +377,7 @@ __global__ __launch_bounds__((Fp4Wide<G, MT, NT>::kThreads)) void fp4_wide_kerne
 #pragma unroll
             for (int s = 0; s < kPer; ++s)
                 xq[u % (kAhead + 1)][s] = __builtin_bit_cast(
-                    bf16x8, *reinterpret_cast<const u32x4 *>(xs + i * 16 * W::kPitch + (s0 + s) / 4 * 128 + (s0 + s) % 4 * (G < 128 ? 32 : 8)));
+                    bf16x8, *reinterpret_cast<const u32x4 *>(xs + xread[(s0 + s) % 4] + i * 16 * W::kPhase + (s0 + s) / 4 * 128));
         };
 #pragma unroll
         for (int u = 0; u < (kAhead < kUnits ? kAhead : kUnits); ++u) ask(u);
@@ -399,7 +413,7 @@ __global__ __launch_bounds__((Fp4Wide<G, MT, NT>::kThreads)) void fp4_wide_kerne
             }
             __builtin_amdgcn_sched_barrier(0);
         }
-        if (more) put(stage[buf ^ 1]);
+        if (more) arrived(buf ^ 1, k + W::kPhase);
         __syncthreads();
     }
     // the second half's sums onto the first's

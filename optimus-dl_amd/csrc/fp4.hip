@@ -246,42 +246,40 @@ void launch_thin(const Fp4Args &a, hipStream_t stream) {
                        dim3(WAVES * kWave), (size_t)(staged > sums ? staged : sums), stream, a);
 }
 
-// Up to 16 * MT rows, many of them: x goes through LDS in phases of kPhase k, double-buffered, and the waves of a block share it, 16 * NT columns each
-// of 128 and one of two halves of a phase.  Codes, scales and x of the next phase are on their way while the waves multiply.
-// Bound by no single thing: of 106 us for 120 rows 8192 -> 28672, groups of 64, the products are 18 to 22, scaling them 16, reading x from LDS 15 and
-// bringing it there 25 to 30 (each left out by itself); of 20 us for 32 rows 14336 -> 4096, groups of 32, scaling is 4 and adding up the runs 4.
-template <int G, int MT, int NT>
+// Up to 16 * MT rows, many of them: x goes through LDS in phases of kPhase k, double-buffered, and the sixteen waves of a block share it, 16 columns each of
+// 16 * kSlots and one of SHARES parts of a phase.  Codes, scales and x of the next phase are on their way while the waves multiply.
+// Eight waves of 32 columns, which read x from LDS half as often, are slower: 32 rows 14336 -> 4096 18.0 us (15.9), 8192 -> 28672 38.7 (33.1), 120 rows 95 (90).
+// x through registers on its way to LDS: 120 rows 8192 -> 28672 94.8 (85.8).  128 rows by 256 columns bring x to LDS half as often as 128 by 128: 512
+// rows 4096 -> 14336 77 (90); for 120 rows of 8192 -> 28672 they are too few blocks, 129 (90).
+// Bound by no single thing: products, their scaling and the reads of x from LDS take some 20 us each of 86 for 120 rows 8192 -> 28672, groups of 64.
+template <int G, int MT, int SHARES>
 struct Fp4Wide {
-    static constexpr int kSlots = 8 / NT, kWaves = 2 * kSlots, kThreads = kWaves * kWave, kPhase = MT >= 8 ? 256 : MT >= 4 ? 512 : 1024, kHalf = kPhase / 2, kSteps = kHalf / 128;
-    static constexpr int kPieces = 16 * MT * kPhase / 8 / (kWaves * kWave), kGroups = kHalf / G, kPairs = (kGroups + 1) / 2;
+    static constexpr int kWaves = 16, kThreads = kWaves * kWave, kSlots = kWaves / SHARES, kColumns = 16 * kSlots;
+    static constexpr int kPhase = MT >= 8 ? 256 : MT >= 4 ? 512 : 1024, kShare = kPhase / SHARES, kSteps = kShare / 128;
+    static constexpr int kPieces = 16 * MT * kPhase / 8 / kThreads, kGroups = kShare / G, kPairs = (kGroups + 1) / 2;
     static constexpr int kStage = 16 * MT * kPhase;          // elements of a buffer
     static constexpr int kRow = kPhase / 8;                  // 16-byte pieces of a row
     static_assert(kPieces * kThreads * 8 == kStage, "the lanes' pieces are the buffer");
 };
 
-template <int G, int MT, int NT>
-__global__ __launch_bounds__((Fp4Wide<G, MT, NT>::kThreads)) void fp4_wide_kernel(const Fp4Args a, int run_k, int runs) {
-    typedef Fp4Wide<G, MT, NT> W;
+template <int G, int MT, int SHARES>
+__global__ __launch_bounds__((Fp4Wide<G, MT, SHARES>::kThreads)) void fp4_wide_kernel(const Fp4Args a, int run_k, int runs) {
+    typedef Fp4Wide<G, MT, SHARES> W;
     constexpr int kPer = G / 32;                // instructions of a group
     __shared__ __attribute__((aligned(1024))) uint16_t stage[2][W::kStage];
     const int lane = threadIdx.x % kWave, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave), col = lane % 16, quarter = lane / 16;
-    const int half = wave / W::kSlots, K = (int)a.K, groups = K / G;
-    const int64_t n0 = (int64_t)blockIdx.x * 128 + wave % W::kSlots * (16 * NT), m0 = (int64_t)blockIdx.y * (16 * MT);
+    const int share = wave / W::kSlots, K = (int)a.K, groups = K / G;
+    const int64_t n0 = (int64_t)blockIdx.x * W::kColumns + wave % W::kSlots * 16, m0 = (int64_t)blockIdx.y * (16 * MT);
     const int k0 = blockIdx.z * run_k, k1 = min(K, k0 + run_k);
     // (columns and rows past the end are the last ones and not stored)
     const int64_t nb = min(n0, a.N - 1);
+    const uint32_t n = (uint32_t)min((int64_t)col, a.N - 1 - nb), coff = n * (uint32_t)(K / 2) + quarter * 16, soff = n * (uint32_t)groups;
     const uint8_t *cbase = a.codes + nb * (a.K / 2);
     const uint16_t *sbase = a.scales + nb * groups, *xbase = a.x + m0 * a.ldx;
-    uint32_t coff[NT], soff[NT], xrow[W::kPieces];
-    int xk[W::kPieces];
-#pragma unroll
-    for (int j = 0; j < NT; ++j) {
-        const uint32_t n = (uint32_t)min((int64_t)(16 * j + col), a.N - 1 - nb);
-        coff[j] = n * (uint32_t)(K / 2) + quarter * 16;
-        soff[j] = n * (uint32_t)groups;
-    }
     // x goes to LDS without passing registers: 64 lanes' pieces of 16 bytes land one behind the other, so what can be chosen is what a lane reads.  Place
     // s of row r holds piece s ^ (r % 16) of it: the 16 rows that are read at a time then lie in different banks.
+    uint32_t xrow[W::kPieces];
+    int xk[W::kPieces];
 #pragma unroll
     for (int i = 0; i < W::kPieces; ++i) {
         const int place = i * W::kThreads + threadIdx.x, r = place / W::kRow;
@@ -290,59 +288,46 @@ __global__ __launch_bounds__((Fp4Wide<G, MT, NT>::kThreads)) void fp4_wide_kerne
     }
     int xread[4];                                // where a lane finds the four k of a step
 #pragma unroll
-    for (int s = 0; s < 4; ++s) xread[s] = col * W::kPhase + half * W::kHalf + ((G < 128 ? s * 4 + quarter : quarter * 4 + s) ^ col) * 8;
+    for (int s = 0; s < 4; ++s) xread[s] = col * W::kPhase + share * W::kShare + ((G < 128 ? s * 4 + quarter : quarter * 4 + s) ^ col) * 8;
     const uint32_t stage_at = (uint32_t)(uintptr_t)(const __attribute__((address_space(3))) uint16_t *)stage[0];
-    auto load_x = [&](int to, int k, int last) {
+    f32x4 acc[MT];
 #pragma unroll
-        for (int i = 0; i < W::kPieces; ++i) {
-            const uint16_t *from = xbase + xrow[i] + min(k + xk[i], last);
-            asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off"
-                         ::"s"(stage_at + 2 * to * W::kStage + (i * W::kWaves + wave) * 1024), "v"(from) : "memory");
-        }
-    };
-    f32x4 acc[MT][NT];
-#pragma unroll
-    for (int i = 0; i < MT; ++i)
-#pragma unroll
-        for (int j = 0; j < NT; ++j) acc[i][j] = f32x4{0, 0, 0, 0};
+    for (int i = 0; i < MT; ++i) acc[i] = f32x4{0, 0, 0, 0};
 
-    struct Next {
-        u32x4 codes[W::kSteps][NT];
-        uint32_t scales[NT][W::kPairs];
-    } next;
+    u32x4 next_codes[W::kSteps];
+    uint32_t next_scales[W::kPairs];
     auto fetch = [&](int k) {
-        const int kc = k + half * W::kHalf;
+        const int kc = k + share * W::kShare;
 #pragma unroll
-        for (int j = 0; j < NT; ++j) {
-#pragma unroll
-            for (int s = 0; s < W::kSteps; ++s) next.codes[s][j] = *reinterpret_cast<const u32x4 *>(cbase + (uint32_t)(kc / 2 + s * 64) + coff[j]);
-            if constexpr (W::kGroups == 1) next.scales[j][0] = sbase[(uint32_t)(kc / G) + soff[j]];
-            else __builtin_memcpy(next.scales[j], sbase + (uint32_t)(kc / G) + soff[j], sizeof(next.scales[j]));
-        }
+        for (int s = 0; s < W::kSteps; ++s) next_codes[s] = *reinterpret_cast<const u32x4 *>(cbase + (uint32_t)(kc / 2 + s * 64) + coff);
+        if constexpr (W::kGroups == 1) next_scales[0] = sbase[(uint32_t)(kc / G) + soff];
+        else __builtin_memcpy(next_scales, sbase + (uint32_t)(kc / G) + soff, sizeof(next_scales));
     };
     auto fetch_end = [&](int k) {                            // a phase that k1 ends: what is behind it is zero
-        const int kc = k + half * W::kHalf;
+        const int kc = k + share * W::kShare;
 #pragma unroll
-        for (int j = 0; j < NT; ++j) {
-#pragma unroll
-            for (int s = 0; s < W::kSteps; ++s) {
-                next.codes[s][j] = u32x4{0, 0, 0, 0};
-                if (kc + s * 128 + quarter * 32 < k1) next.codes[s][j] = *reinterpret_cast<const u32x4 *>(cbase + (uint32_t)(kc / 2 + s * 64) + coff[j]);
-            }
-            uint32_t v[2 * W::kPairs];                       // (all asked for before any is looked at)
-#pragma unroll
-            for (int g = 0; g < 2 * W::kPairs; ++g) v[g] = sbase[(uint32_t)min(kc / G + g, groups - 1) + soff[j]];
-#pragma unroll
-            for (int g = 0; g < W::kPairs; ++g)
-                next.scales[j][g] = (kc + 2 * g * G < k1 ? v[2 * g] : 0u) | (kc + (2 * g + 1) * G < k1 ? v[2 * g + 1] << 16 : 0u);
+        for (int s = 0; s < W::kSteps; ++s) {
+            next_codes[s] = u32x4{0, 0, 0, 0};
+            if (kc + s * 128 + quarter * 32 < k1) next_codes[s] = *reinterpret_cast<const u32x4 *>(cbase + (uint32_t)(kc / 2 + s * 64) + coff);
         }
+        uint32_t v[2 * W::kPairs];                           // (all asked for before any is looked at)
+#pragma unroll
+        for (int g = 0; g < 2 * W::kPairs; ++g) v[g] = sbase[(uint32_t)min(kc / G + g, groups - 1) + soff];
+#pragma unroll
+        for (int g = 0; g < W::kPairs; ++g)
+            next_scales[g] = (kc + 2 * g * G < k1 ? v[2 * g] : 0u) | (kc + (2 * g + 1) * G < k1 ? v[2 * g + 1] << 16 : 0u);
     };
     auto ask_for = [&](int to, int k) {
         if (k + W::kPhase <= k1) fetch(k);
         else fetch_end(k);
-        load_x(to, k, k1 - 8);                   // (pieces behind k1: the last one, zeroed below)
+#pragma unroll
+        for (int i = 0; i < W::kPieces; ++i) {               // (pieces behind k1: the last one, zeroed below)
+            const uint16_t *from = xbase + xrow[i] + min(k + xk[i], k1 - 8);
+            asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off"
+                         ::"s"(stage_at + 2 * to * W::kStage + (i * W::kWaves + wave) * 1024), "v"(from) : "memory");
+        }
     };
-    auto arrived = [&](int to, int k) {          // this lane's own pieces
+    auto arrived = [&](int to, int k) {                      // this lane's own pieces
         asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
         if (k + W::kPhase <= k1) return;
 #pragma unroll
@@ -354,24 +339,21 @@ __global__ __launch_bounds__((Fp4Wide<G, MT, NT>::kThreads)) void fp4_wide_kerne
     __syncthreads();
     int buf = 0;
     for (int k = k0; k < k1; k += W::kPhase, buf ^= 1) {
-        u32x4 codes[W::kSteps][NT];
-        uint32_t scales[NT][W::kPairs];
+        u32x4 codes[W::kSteps];
+        uint32_t scales[W::kPairs];
 #pragma unroll
-        for (int j = 0; j < NT; ++j) {
+        for (int s = 0; s < W::kSteps; ++s) codes[s] = next_codes[s];
 #pragma unroll
-            for (int s = 0; s < W::kSteps; ++s) codes[s][j] = next.codes[s][j];
-#pragma unroll
-            for (int g = 0; g < W::kPairs; ++g) scales[j][g] = next.scales[j][g];
-        }
+        for (int g = 0; g < W::kPairs; ++g) scales[g] = next_scales[g];
         const bool more = k + W::kPhase < k1;
         if (more) ask_for(buf ^ 1, k + W::kPhase);
         const uint16_t *xs = stage[buf];
         // Units of 16 rows and one group of k, software-pipelined: x is asked for kAhead units before its products, and the products of a
         // unit are scaled onto the sums behind the products of the next kBehind.
         constexpr int kUnits = W::kSteps * (4 / kPer) * MT, kAhead = 4 / kPer, kBehind = kPer > 2 ? 1 : 2;
-        bf16x8 xq[kAhead + 1][kPer], b[NT][kPer];
-        f32x4 p[kBehind + 1][NT];
-        float scale[4][NT];
+        bf16x8 xq[kAhead + 1][kPer], b[kPer];
+        f32x4 p[kBehind + 1];
+        float scale[4];
         auto ask = [&](int u) {                  // (every index is known at compile time)
             const int i = u % MT, s0 = u / MT * kPer;
 #pragma unroll
@@ -381,78 +363,66 @@ __global__ __launch_bounds__((Fp4Wide<G, MT, NT>::kThreads)) void fp4_wide_kerne
         };
 #pragma unroll
         for (int u = 0; u < (kAhead < kUnits ? kAhead : kUnits); ++u) ask(u);
-        u32x4 w[NT];
+        u32x4 w;
 #pragma unroll
         for (int u = 0; u < kUnits + kBehind; ++u) {
             if (u + kAhead < kUnits) ask(u + kAhead);
             if (u < kUnits) {
                 const int g = u / MT, s0 = g * kPer;
                 if (u % MT == 0) {
+                    if (s0 % 4 == 0) w = G < 128 ? exchange(codes[s0 / 4]) : codes[s0 / 4];
+                    scale[g % 4] = g % 2 ? bf16_hi(scales[g / 2]) : bf16_lo(scales[g / 2]);
 #pragma unroll
-                    for (int j = 0; j < NT; ++j) {
-                        if (s0 % 4 == 0) w[j] = G < 128 ? exchange(codes[s0 / 4][j]) : codes[s0 / 4][j];
-                        scale[g % 4][j] = g % 2 ? bf16_hi(scales[j][g / 2]) : bf16_lo(scales[j][g / 2]);
-#pragma unroll
-                        for (int s = 0; s < kPer; ++s) b[j][s] = widen_codes(w[j][(s0 + s) % 4]);
-                    }
+                    for (int s = 0; s < kPer; ++s) b[s] = widen_codes(w[(s0 + s) % 4]);
                 }
+                f32x4 &to = p[u % (kBehind + 1)];
 #pragma unroll
                 for (int s = 0; s < kPer; ++s)
-#pragma unroll
-                    for (int j = 0; j < NT; ++j)
-                        p[u % (kBehind + 1)][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(xq[u % (kAhead + 1)][s], b[j][s], s == 0 ? f32x4{0, 0, 0, 0} : p[u % (kBehind + 1)][j], 0, 0, 0);
+                    to = __builtin_amdgcn_mfma_f32_16x16x32_bf16(xq[u % (kAhead + 1)][s], b[s], s == 0 ? f32x4{0, 0, 0, 0} : to, 0, 0, 0);
             }
             if (u >= kBehind) {
                 const int v = u - kBehind, i = v % MT;
 #pragma unroll
-                for (int j = 0; j < NT; ++j) {
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) acc[i][j][e] = __fmaf_rn(scale[v / MT % 4][j], p[v % (kBehind + 1)][j][e], acc[i][j][e]);
-                    asm volatile("" : "+v"(acc[i][j]));      // (not put off behind the loop, which would spill the products)
-                }
+                for (int e = 0; e < 4; ++e) acc[i][e] = __fmaf_rn(scale[v / MT % 4], p[v % (kBehind + 1)][e], acc[i][e]);
+                asm volatile("" : "+v"(acc[i]));             // (not put off behind the loop, which would spill the products)
             }
             __builtin_amdgcn_sched_barrier(0);
         }
         if (more) arrived(buf ^ 1, k + W::kPhase);
         __syncthreads();
     }
-    // the second half's sums onto the first's
-    f32x4 *part = reinterpret_cast<f32x4 *>(stage[0]) + (wave % W::kSlots) * (MT * NT * kWave) + lane;
-    static_assert(sizeof(stage) >= W::kSlots * MT * NT * kWave * sizeof(f32x4), "the sums fit into the stage");
-    if (half) {
+    if constexpr (SHARES == 2) {                 // the second share's sums onto the first's
+        f32x4 *part = reinterpret_cast<f32x4 *>(stage[0]) + wave % W::kSlots * (MT * kWave) + lane;
+        static_assert(sizeof(stage) >= W::kSlots * MT * kWave * sizeof(f32x4), "the sums fit into the stage");
+        if (share) {
 #pragma unroll
-        for (int i = 0; i < MT; ++i)
-#pragma unroll
-            for (int j = 0; j < NT; ++j) part[(i * NT + j) * kWave] = acc[i][j];
-    }
-    __syncthreads();
-    if (half) return;
-#pragma unroll
-    for (int j = 0; j < NT; ++j) {
-        const int64_t n = n0 + 16 * j + col;
-        if (n >= a.N) continue;
-        const float b = bias_of(a, n);
-#pragma unroll
-        for (int i = 0; i < MT; ++i) {
-            const f32x4 s = acc[i][j] + part[(i * NT + j) * kWave];
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                const int64_t m = m0 + 16 * i + quarter * 4 + e;
-                if (m >= a.M) continue;
-                if (runs > 1) a.partial[(blockIdx.z * a.M + m) * a.N + n] = s[e];
-                else a.y[m * a.N + n] = (uint16_t)pack_bf16x2(a.bias ? s[e] + b : s[e], 0.0f);
-            }
+            for (int i = 0; i < MT; ++i) part[i * kWave] = acc[i];
         }
+        __syncthreads();
+        if (share) return;
+#pragma unroll
+        for (int i = 0; i < MT; ++i) acc[i] += part[i * kWave];
     }
+    if (n0 + col >= a.N) return;
+    const float bias = bias_of(a, n0 + col);
+#pragma unroll
+    for (int i = 0; i < MT; ++i)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            const int64_t m = m0 + 16 * i + quarter * 4 + e;
+            if (m >= a.M) continue;
+            if (runs > 1) a.partial[(blockIdx.z * a.M + m) * a.N + n0 + col] = acc[i][e];
+            else a.y[m * a.N + n0 + col] = (uint16_t)pack_bf16x2(a.bias ? acc[i][e] + bias : acc[i][e], 0.0f);
+        }
 }
 
-template <int G, int MT, int NT>
+template <int G, int MT, int SHARES>
 int launch_wide(const Fp4Args &a, int runs, hipStream_t stream) {
-    typedef Fp4Wide<G, MT, NT> W;
+    typedef Fp4Wide<G, MT, SHARES> W;
     const int phase = W::kPhase, run_k = (int)((a.K + runs - 1) / runs + phase - 1) / phase * phase;
     runs = (int)((a.K + run_k - 1) / run_k);                 // (no run is empty)
-    hipLaunchKernelGGL((fp4_wide_kernel<G, MT, NT>), dim3((unsigned)((a.N + 127) / 128), (unsigned)((a.M + 16 * MT - 1) / (16 * MT)), (unsigned)runs), dim3(W::kThreads), 0, stream, a,
-                       run_k, runs);
+    hipLaunchKernelGGL((fp4_wide_kernel<G, MT, SHARES>), dim3((unsigned)((a.N + W::kColumns - 1) / W::kColumns), (unsigned)((a.M + 16 * MT - 1) / (16 * MT)), (unsigned)runs),
+                       dim3(W::kThreads), 0, stream, a, run_k, runs);
     return runs;
 }
 
@@ -528,31 +498,33 @@ bool group_known(int group) { return group == 32 || group == 64 || group == 128;
 // The thin kernel stages the scales of whole rows, which for a very long K do not fit.
 constexpr int64_t kThinLds = 64 * 1024;
 
-// How a product is done: rows of a block of the wide kernel in 16s (0: the thin kernel), and runs of K.
+// How a product is done: rows of a block of the wide kernel in 16s (0: the thin kernel), in how many parts its waves share a phase, and runs of K.
 struct Fp4Plan {
-    int mt, runs;
+    int mt, shares, runs;
 };
 
 // Up to 4 rows the thin kernel, x in LDS: 4096 -> 14336 10 us (wide 17), 768 -> 2304 3.2 (10).  For more the cheapest by what a block was measured
-// to take: thin 0.39 + 0.058 a row, ns for each k; wide 3.0, 4.1, 5.4 and 9.8 for 16, 32, 64 and 128 rows and some 2 us besides, with as many
-// blocks at a time as there are compute units; a join 1.6 us and 1.6 ps for each number.  Over 195 products of 5 to 1024 rows, 768 -> 768 to
-// 28672 -> 8192, what this takes is 1 % off the best of them all on average and 13 % at worst.  (By rows and size of the weights alone, as it
-// was: 20 % and 95 %.)
+// to take: thin 0.39 + 0.058 a row, ns for each k; wide 3.1, 3.7, 5.0 and 9.2 for 16, 32, 64 and 128 rows, 15 for 128 rows by 256 columns, and 1.3 to
+// 4.6 us besides, with as many blocks at a time as there are compute units; a join 1.5 us and 0.86 ps for each number.  Over 182 products of 5 to 2048
+// rows, 768 -> 768 to 28672 -> 8192, what this takes is 1.5 % off the best of them all on average and 24 % at worst.  (By rows and size of the
+// weights alone: 20 % and 95 %.  Blocks of 16 rows were timed for up to 48.)
 template <int G>
 Fp4Plan plan(int64_t M, int64_t N, int64_t K) {
     const bool fits = 2 * 16 * (int64_t)fp4_tile<G>((int)K).pitch <= kThinLds;
-    if (fits && M <= 4) return {0, 1};
+    if (fits && M <= 4) return {0, 1, 1};
     const int64_t cus = device_cu_count(), thin = (N + 15) / 16 * (M <= 16 ? 1 : (M + 31) / 32);
-    Fp4Plan best = {0, 1};
+    Fp4Plan best = {0, 1, 1};
     int64_t least = fits ? 4100000 + K * (390 + 58 * (M < 32 ? M : 32)) * (thin > cus ? thin : cus) / cus : INT64_MAX;      // ps
-    static constexpr struct { int mt, phase, per_k, start; } kinds[] = {{1, 1024, 3000, 1500000}, {2, 1024, 4100, 2000000}, {4, 512, 5400, 2000000}, {8, 256, 9800, 3000000}};
+    static constexpr struct { int mt, shares, phase, per_k, start; } kinds[] = {
+        {1, 2, 1024, 3100, 1300000}, {2, 2, 1024, 3700, 1700000}, {4, 2, 512, 5000, 3000000}, {8, 2, 256, 9200, 4500000}, {8, 1, 256, 15000, 4600000}};
     for (const auto &kind : kinds) {
-        const int64_t tiles = (N + 127) / 128 * ((M + 16 * kind.mt - 1) / (16 * kind.mt));
+        if (kind.mt == 1 && M > 48) continue;
+        const int64_t columns = 256 / kind.shares, tiles = (N + columns - 1) / columns * ((M + 16 * kind.mt - 1) / (16 * kind.mt));
         for (const int runs : {1, 2, 3, 4, 6, 8, 12, 16, 24, 32}) {
             if (runs > 1 && (runs * kind.phase > K || M * N >= (int64_t)1 << 32)) break;
             const int64_t k = ((K + runs - 1) / runs + kind.phase - 1) / kind.phase * kind.phase, rounds = (tiles * ((K + k - 1) / k) + cus - 1) / cus;
-            const int64_t cost = 3300000 + rounds * (kind.start + k * kind.per_k) + (runs > 1 ? 1600000 + runs * M * N * 8 / 5 : 0);
-            if (cost < least) { least = cost; best = {kind.mt, runs}; }
+            const int64_t cost = 2400000 + rounds * (kind.start + k * kind.per_k) + (runs > 1 ? 1500000 + runs * M * N * 43 / 50 : 0);
+            if (cost < least) { least = cost; best = {kind.mt, kind.shares, runs}; }
         }
     }
     return best;
@@ -570,14 +542,12 @@ void launch_linear(const Fp4Args &a, const Fp4Plan how, hipStream_t stream) {
         else launch_thin<G, 2, 1, 4, 1, false>(a, stream);
         return;
     }
-    // Sixteen waves of 16 columns hide more of each other than eight of 32 and read x from LDS twice as often: 120 rows 8192 -> 28672 101 us (106),
-    // 64 rows 14336 -> 4096 21.2 (23.9), but 32 rows 4096 -> 14336 18.4 (17.8).  Groups of 128 keep more of x on its way than the 128 registers of sixteen
-    // waves hold beside 128 rows.
     int runs = how.runs;
     if (how.mt == 1) runs = launch_wide<G, 1, 2>(a, runs, stream);
     else if (how.mt == 2) runs = launch_wide<G, 2, 2>(a, runs, stream);
-    else if (how.mt == 4) runs = launch_wide<G, 4, 1>(a, runs, stream);
-    else runs = launch_wide<G, 8, G == 128 ? 2 : 1>(a, runs, stream);
+    else if (how.mt == 4) runs = launch_wide<G, 4, 2>(a, runs, stream);
+    else if (how.shares == 2) runs = launch_wide<G, 8, 2>(a, runs, stream);
+    else runs = launch_wide<G, 8, 1>(a, runs, stream);
     if (runs > 1) hipLaunchKernelGGL(fp4_join_kernel, dim3((unsigned)((a.M * a.N + 255) / 256)), dim3(256), 0, stream, a, runs);
 }
 

@@ -70,11 +70,11 @@ def test_layers_of_models(n, k, group):
         check(torch.randn((rows, k), device="cuda", generator=g).bfloat16(), codes, scales)
 
 
-# blocks of 16, 32, 64 and 128 rows, K in one run and in several, the last ones ragged
+# blocks of 16, 32, 64 and 128 rows, of 128 and 256 columns, K in one run and in several, the last ones ragged
 @pytest.mark.parametrize("group", [32, 64, 128])
 @pytest.mark.parametrize("rows,n,k", [(33, 4100, 1664), (63, 8200, 1664), (257, 4100, 1664), (200, 8200, 1664), (33, 4100, 2176), (257, 100, 4224),
                                       (13, 1030, 8320), (31, 8200, 3200), (17, 8200, 6272), (130, 4100, 2176), (50, 4100, 3200), (65, 8200, 4224),
-                                      (65, 4100, 6272)])
+                                      (65, 4100, 6272), (257, 8200, 1664), (530, 8200, 1664), (530, 2050, 3200)])
 def test_ways_of_cutting_a_product(rows, n, k, group):
     codes, scales, g = weight_of(n, k, group, rows)
     x = torch.randn((rows, k), device="cuda", generator=g).bfloat16()

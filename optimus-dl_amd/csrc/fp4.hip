@@ -251,7 +251,8 @@ void launch_thin(const Fp4Args &a, hipStream_t stream) {
 // Eight waves of 32 columns, which read x from LDS half as often, are slower: 32 rows 14336 -> 4096 18.0 us (15.9), 8192 -> 28672 38.7 (33.1), 120 rows 95 (90).
 // x through registers on its way to LDS: 120 rows 8192 -> 28672 94.8 (85.8).  128 rows by 256 columns bring x to LDS half as often as 128 by 128: 512
 // rows 4096 -> 14336 77 (90); for 120 rows of 8192 -> 28672 they are too few blocks, 129 (90).
-// Bound by no single thing: products, their scaling and the reads of x from LDS take some 20 us each of 86 for 120 rows 8192 -> 28672, groups of 64.
+// 120 rows 8192 -> 28672, groups of 64, 82 us: 690 TFLOP/s, a large bf16 product 1235.  Bound by the products (half of them left out: 24 us of 94 in a row of
+// twenty; scaling 11, bringing x to LDS 7, reading it there nothing); 32 rows 14336 -> 4096, 15.3 us, by the latency of two phases and of the join (4 us).
 template <int G, int MT, int SHARES>
 struct Fp4Wide {
     static constexpr int kWaves = 16, kThreads = kWaves * kWave, kSlots = kWaves / SHARES, kColumns = 16 * kSlots;

@@ -110,9 +110,13 @@ def token_logprobs(logits: torch.Tensor, targets: torch.Tensor, *, n_vocab: int 
         raise ValueError(f"token_logprobs: temperature {temperature} (1e-30 to 1e30)")
     if not logits.is_cuda:
         return _plain(logits, targets, n_vocab, top_k, float(temperature), ignore_index)
-    if logits.dim() == 2 and no_graph():
-        logprobs, entropy, _, top, ids = native.token_logprobs(logits, targets, n_vocab, top_k, temperature, ignore_index)
-        return TokenLogProbs(logprobs, entropy, top, ids)
+    if no_graph():
+        if logits.dim() == 2:
+            logprobs, entropy, _, top, ids = native.token_logprobs(logits, targets, n_vocab, top_k, temperature, ignore_index)
+            return TokenLogProbs(logprobs, entropy, top, ids)
+        lead = logits.shape[:-1]
+        logprobs, entropy, _, top, ids = native.token_logprobs(logits.reshape(-1, columns), targets.reshape(-1), n_vocab, top_k, temperature, ignore_index)
+        return TokenLogProbs(logprobs.view(lead), entropy.view(lead), *((None, None) if top is None else (t.view(*lead, top_k) for t in (top, ids))))
     recipe = _state.active_recipe()
     if not gradient_is_cast(logits, recipe) and torch.is_grad_enabled():     # nobody to hand maxima to
         r = native.token_logprobs_node(logits, targets, n_vocab, top_k, temperature, ignore_index)

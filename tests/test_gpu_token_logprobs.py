@@ -241,3 +241,20 @@ def test_no_rows():
     r = token_logprobs(torch.zeros((0, 100), device="cuda", requires_grad=True), torch.zeros(0, dtype=torch.int64, device="cuda"), top_k=3)
     assert r.logprobs.shape == (0,) and r.top_ids.shape == (0, 3)
     r.logprobs.sum().backward()
+
+
+@pytest.mark.parametrize("lead", [(), (6,), (2, 3), (2, 1, 3), (2, 0)])
+@pytest.mark.parametrize("top_k", [0, 4])
+def test_any_number_of_axes_with_and_without_a_graph(lead, top_k):
+    rows = math.prod(lead)
+    l, t, _ = logits_of(max(rows, 1), 300, BF16)
+    l, t = l[:rows].reshape(*lead, 300), t[:rows].reshape(lead)
+    with torch.no_grad():
+        r = token_logprobs(l, t, top_k=top_k)
+    live = token_logprobs(l.clone().requires_grad_(True), t, top_k=top_k)
+    assert r.logprobs.shape == r.entropy.shape == lead and torch.equal(r.logprobs, live.logprobs) and torch.equal(r.entropy, live.entropy)
+    if top_k:
+        assert r.top_ids.shape == r.top_logprobs.shape == (*lead, top_k)
+        assert torch.equal(r.top_ids, live.top_ids) and torch.equal(r.top_logprobs, live.top_logprobs)
+    else:
+        assert r.top_ids is None and r.top_logprobs is None

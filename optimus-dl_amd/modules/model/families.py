@@ -81,11 +81,14 @@ class _DecoderLM(nn.Module):
     def forward(self, input_ids: torch.Tensor, **kwargs) -> dict:
         x, z = self.embed(input_ids), None
         blocks, ln_f = self.transformer.h, self.transformer.ln_f
+        stepped = [getattr(block, "stepped", False) for block in blocks]      # (a wrapper around a block has the stream alone)
         for i, block in enumerate(blocks):
-            if getattr(block, "stepped", False):        # the end of a block and the norm in front of the next in one
-                x, z = block(x, z, blocks[i + 1].ln_1 if i + 1 < len(blocks) else ln_f)
-            else:
+            if not stepped[i]:
                 x, z = block(x), None
+            elif i + 1 == len(blocks) or stepped[i + 1]:                      # the end of a block and the norm in front of the next in one
+                x, z = block(x, z, ln_f if i + 1 == len(blocks) else blocks[i + 1].ln_1)
+            else:
+                x, z = block(x, z), None
         return {"logits": self.lm_head(ln_f(x) if z is None else z)}
 
     def score(self, input_ids: torch.Tensor, targets: torch.Tensor | None = None, top_k: int = 0, temperature: float = 1.0,

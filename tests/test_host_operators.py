@@ -230,3 +230,26 @@ def test_only_conversions_that_widen_codes_need_no_saturating_mode():
     assert found("v_cvt_scalef32_pk_fp4_bf16 v0, v1, 1.0") == 1
     assert found("v_cvt_scalef32_pk_bf16_fp8 v0, v1, 1.0") == 1
     assert found("v_cvt_scalef32_pk_bf8_f32 v0, v1, v2, 1.0") == 1
+
+
+@pytest.mark.parametrize("wrapped", [(0,), (1,), (2,), (0, 2), (0, 1, 2)])
+def test_blocks_behind_a_wrapper_take_and_give_the_stream_alone(wrapped):
+    from optimus_dl_amd.modules.model.families import Llama, LlamaConfig
+
+    class Wrapper(torch.nn.Module):
+        def __init__(self, inner):
+            super().__init__()
+            self.inner = inner
+
+        def forward(self, x):
+            return self.inner(x)
+
+    torch.manual_seed(0)
+    model = Llama(LlamaConfig(vocab_size=50, n_layer=3, n_embd=32, n_head=2, n_kv_head=2, intermediate_size=64, post_norms=True,
+                              layer_scale=0.5, residual_scale=0.9))
+    ids = torch.randint(0, 50, (2, 7))
+    want = model(ids)["logits"]
+    for i in wrapped:
+        model.transformer.h[i] = Wrapper(model.transformer.h[i])
+    # the same fp32 operations, some in another order: a few roundings of values near one
+    torch.testing.assert_close(model(ids)["logits"], want, rtol=0, atol=64 * 2.0 ** -24 * float(want.abs().max()))

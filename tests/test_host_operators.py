@@ -54,7 +54,7 @@ def test_fp4_entries_refuse():
                          (dict(M=32, N=4096, K=14336, ldx=14336), "workspace"), (dict(M=32, N=4096, K=14336, ldx=14336, ws=P, wsb=1 << 20), "workspace")):
         refused("odl_fp8_fp4_linear", tuple({**ok, **change}.values()), word)
     runs = native.load().odl_fp8_fp4_linear_runs
-    assert runs(1, 14336, 4096, 128) == runs(24, 2304, 768, 32) == runs(120, 28672, 8192, 64) == runs(0, 4096, 4096, 32) == 0 and 1 < runs(32, 4096, 14336, 32) <= 14
+    assert runs(1, 14336, 4096, 128) == runs(24, 2304, 768, 32) == runs(64, 28672, 8192, 64) == runs(0, 4096, 4096, 32) == 0 and 1 < runs(32, 4096, 14336, 32) <= 14
     ok = dict(w=P, src=0, N=16, K=128, group=64, codes=P, scales=P, stream=None)
     for change, word in ((dict(N=-1), "negative"), (dict(src=2), "src_dtype"), (dict(group=0), "group"), (dict(K=96), "multiple"), (dict(codes=None), "null"), (dict(w=P + 4), "aligned")):
         refused("odl_fp8_fp4_quantise", tuple({**ok, **change}.values()), word)

@@ -250,8 +250,8 @@ void launch_thin(const Fp4Args &a, hipStream_t stream) {
 // 16 * kSlots and one of SHARES parts of a phase.  Codes, scales and x of the next phase are on their way while the waves multiply.
 // Eight waves of 32 columns, which read x from LDS half as often, are slower: 32 rows 14336 -> 4096 18.0 us (15.9), 8192 -> 28672 38.7 (33.1), 120 rows 95 (90).
 // x through registers on its way to LDS: 120 rows 8192 -> 28672 94.8 (85.8).  128 rows by 256 columns bring x to LDS half as often as 128 by 128: 512
-// rows 4096 -> 14336 77 (90); for 120 rows of 8192 -> 28672 they are too few blocks, 129 (90).
-// 120 rows 8192 -> 28672, groups of 64, 82 us: 690 TFLOP/s, a large bf16 product 1235.  Bound by the products (half of them left out: 24 us of 94 in a row of
+// rows 4096 -> 14336 77 (90); for 120 rows of 8192 -> 28672 they are too few blocks, 129 (90), unless K is cut in two, 79 (81).
+// 120 rows 8192 -> 28672, groups of 64, 79 us: 710 TFLOP/s, a large bf16 product 1235.  Bound by the products (half of them left out: 24 us of 94 in a row of
 // twenty; scaling 11, bringing x to LDS 7, reading it there nothing); 32 rows 14336 -> 4096, 15.3 us, by the latency of two phases and of the join (4 us).
 template <int G, int MT, int SHARES>
 struct Fp4Wide {

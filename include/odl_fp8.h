@@ -710,7 +710,7 @@ int odl_fp8_residual_norm(const void *x, int x_dtype, const void *h, int h_dtype
                           float post_eps, void *y, void *z, float *stats, float *parts, odl_stream_t stream);
 /*
  * Its backward for gradients dy (type of x) and dz (bf16), either of which may be NULL (zero).  dx in the type of x, dh in that of h,
- * parts: partial maxima of |dh|; dweight[cols], dpost_weight[cols], dgate[gate_size] fp32.  dweight NULL: no gradients of weights;
+ * parts: partial maxima of |dh| (may be NULL); dweight[cols], dpost_weight[cols], dgate[gate_size] fp32.  dweight NULL: no gradients of weights;
  * the other two may be NULL by themselves.  Sums over rows are fp32, in a fixed order on one device.
  * workspace: ODL_FP8_RESIDUAL_NORM_SLABS * (2 * cols + 1) floats, contents irrelevant (needed with dweight).
  */
@@ -737,7 +737,7 @@ int odl_fp8_token_logprobs(const void *logits, int dtype, int64_t rows, int64_t 
 /*
  * Gradient of the logits for gradients of logprobs, entropy and top_logprobs (each may be NULL: zero), dense [rows, padded] in the
  * type of the logits: zero for columns from vocab on and for ignored rows, NaN for rows whose target is no token.  parts: partial
- * maxima of its magnitude, for the cast of the head's backward.  entropy, stats, top_ids as the forward wrote them.
+ * maxima of its magnitude, for the cast of the head's backward (may be NULL).  entropy, stats, top_ids as the forward wrote them.
  */
 int odl_fp8_token_logprobs_bwd(const void *logits, int dtype, int64_t rows, int64_t stride, int64_t vocab, int64_t padded,
                                const int64_t *targets, int64_t ignore_index, float inv_temperature, int top_k, const int64_t *top_ids,

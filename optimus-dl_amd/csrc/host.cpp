@@ -602,9 +602,9 @@ struct ResidualNormNode : torch::autograd::Function<ResidualNormNode> {
     static variable_list forward(AutogradContext *ctx, const Tensor &x, const Tensor &h, const Tensor &w, const OptTensor &post, const OptTensor &gate, double scale,
                                  double eps, double post_eps, i64 stream) {
         const i64 cols = x.size(-1), rows = x.numel() / cols;
-        Tensor y = at::empty_like(x), z = at::empty(x.sizes(), x.options().dtype(at::kBFloat16)), stats = f32(x, {2, rows}), parts = f32(x, {kParts});
+        Tensor y = at::empty_like(x), z = at::empty(x.sizes(), x.options().dtype(at::kBFloat16)), stats = f32(x, {2, rows});
         done(residual_norm_c(ptr(x), src_of(x), ptr(h), src_of(h), ptr(w), ptr(post), ptr(gate), gate ? gate->numel() : 0, rows, cols, (float)scale, (float)eps,
-                             (float)post_eps, ptr(y), ptr(z), static_cast<float *>(ptr(stats)), static_cast<float *>(ptr(parts)), str(stream)),
+                             (float)post_eps, ptr(y), ptr(z), static_cast<float *>(ptr(stats)), nullptr, str(stream)),
              "odl_fp8_residual_norm");
         ctx->save_for_backward({x, h, w, post.value_or(Tensor()), gate.value_or(Tensor()), stats});
         ctx->set_materialize_grads(false);
@@ -623,7 +623,7 @@ struct ResidualNormNode : torch::autograd::Function<ResidualNormNode> {
             at::NoGradGuard quiet;
             const i64 cols = x.size(-1), rows = x.numel() / cols, g = gate ? gate->numel() : 0;
             const bool weights = ctx->needs_input_grad(2) || (post && ctx->needs_input_grad(3)) || (gate && ctx->needs_input_grad(post ? 4 : 3));
-            Tensor dx = at::empty_like(x), dh = at::empty_like(h), parts = f32(x, {kParts});
+            Tensor dx = at::empty_like(x), dh = at::empty_like(h);
             OptTensor dw, dpost, dgate, ws;
             if (weights) {
                 dw = f32(x, w.sizes());
@@ -633,7 +633,7 @@ struct ResidualNormNode : torch::autograd::Function<ResidualNormNode> {
             }
             // (a node runs on the stream that its forward ran on)
             done(residual_norm_bwd_c(ptr(dy), ptr(dz), ptr(x), src_of(x), ptr(h), src_of(h), ptr(w), ptr(post), ptr(gate), g, rows, cols,
-                                     (float)ctx->saved_data["scale"].toDouble(), ptr(stats), ptr(dx), ptr(dh), ptr(parts), ptr(dw), ptr(dpost), ptr(dgate), ptr(ws),
+                                     (float)ctx->saved_data["scale"].toDouble(), ptr(stats), ptr(dx), ptr(dh), nullptr, ptr(dw), ptr(dpost), ptr(dgate), ptr(ws),
                                      str(ctx->saved_data["stream"].toInt())),
                  "odl_fp8_residual_norm_bwd");
             grads[0] = dx;
@@ -696,9 +696,9 @@ struct TokenLogprobsNode : torch::autograd::Function<TokenLogprobsNode> {
             at::NoGradGuard quiet;
             const Tensor l = logits.reshape({-1, logits.size(-1)});
             const i64 rows = l.size(0), cols = l.size(1);
-            Tensor dl = at::empty({rows, cols}, l.options()), parts = f32(l, {kParts});
+            Tensor dl = at::empty({rows, cols}, l.options());
             done(logprobs_bwd_c(ptr(l), src_of(l), rows, l.stride(0), ctx->saved_data["vocab"].toInt(), cols, targets.data_ptr<i64>(), ctx->saved_data["ignore"].toInt(),
-                                (float)ctx->saved_data["inv_t"].toDouble(), (int)top_k, ptr(ids), ptr(stats), ptr(entropy), ptr(dlp), ptr(dent), ptr(dtop), ptr(dl), ptr(parts),
+                                (float)ctx->saved_data["inv_t"].toDouble(), (int)top_k, ptr(ids), ptr(stats), ptr(entropy), ptr(dlp), ptr(dent), ptr(dtop), ptr(dl), nullptr,
                                 str(ctx->saved_data["stream"].toInt())),
                  "odl_fp8_token_logprobs_bwd");
             grads[0] = dl.view(logits.sizes());

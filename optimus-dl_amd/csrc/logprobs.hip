@@ -477,6 +477,7 @@ __global__ __launch_bounds__(kBwdThreads) void token_logprobs_bwd_kernel(const B
             }
         }
     }
+    if (!a.parts) return;
     am = block_max_u32(DT == ODL_BF16 ? fold_u16x2_to_f32bits(am) : am, red);
     if (tid == 0) a.parts[blockIdx.x] = bits_to_float(am);
     if (blockIdx.x == 0)
@@ -531,7 +532,7 @@ extern "C" int odl_fp8_token_logprobs_bwd(const void *logits, int dtype, int64_t
                                           const float *d_top, void *dlogits, float *parts, odl_stream_t stream_) {
     hipStream_t stream = reinterpret_cast<hipStream_t>(stream_);
     if (const int rc = check("odl_fp8_token_logprobs_bwd", dtype, rows, stride, padded, vocab, top_k, inv_temperature)) return rc;
-    if (!parts || (rows > 0 && (!logits || !targets || !stats || !entropy || !dlogits)) || (d_top && top_k && !top_ids))
+    if ((rows > 0 && (!logits || !targets || !stats || !entropy || !dlogits)) || (d_top && top_k && !top_ids))
         return set_error(ODL_ERR_ARG, "odl_fp8_token_logprobs_bwd: null pointer");
     Backward a = {};
     a.logits = logits; a.targets = targets; a.top_ids = top_ids; a.d_logprobs = d_logprobs; a.d_entropy = d_entropy; a.d_top = d_top;

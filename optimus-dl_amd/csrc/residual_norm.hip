@@ -18,7 +18,7 @@
 // chunks of 8 elements a lane at most: the row is read once, the next one is on its way, and the weights of a lane's columns and the sums of
 // their gradients stay in its registers from row to row.  8192 x 4096, fp32 / bf16: forward 76 us (5.3 TB/s; a copy reaches 5.1), backward
 // 112 us (5.4 TB/s) and 5 us for the sums of its slabs; 4016 x 2048 in bf16 16, 23 and 4; one row of 4096 3.4, latency of its loads and sums.
-// (fp32 rows of more than 4096 beside an fp32 block output spill 60 bytes a lane in the backward: 16 columns of six arrays.)
+// (fp32 rows of more than 4096 beside an fp32 block output spill 52 bytes a lane in the backward: 16 columns of six arrays.)
 #include "common.h"
 
 #pragma clang fp contract(off)
@@ -316,10 +316,12 @@ __global__ __launch_bounds__(Rows<LPR>::kThreads) void residual_norm_bwd_kernel(
         }
         dg += dg_row;
     }
-    am = block_max_u32(HT == ODL_BF16 ? fold_u16x2_to_f32bits(am) : am, red);
-    if (threadIdx.x == 0) parts[blockIdx.x] = bits_to_float(am);
-    if (blockIdx.x == 0)
-        for (int j = (int)gridDim.x + threadIdx.x; j < kParts; j += kThreads) parts[j] = 0.0f;
+    if (parts) {
+        am = block_max_u32(HT == ODL_BF16 ? fold_u16x2_to_f32bits(am) : am, red);
+        if (threadIdx.x == 0) parts[blockIdx.x] = bits_to_float(am);
+        if (blockIdx.x == 0)
+            for (int j = (int)gridDim.x + threadIdx.x; j < kParts; j += kThreads) parts[j] = 0.0f;
+    }
     if (!slabs) return;                                        // (uniform: none of the weights wants a gradient)
 
     // the block's sums of its columns as one slab: [d_weight, D]
@@ -484,7 +486,7 @@ extern "C" int odl_fp8_residual_norm_bwd(const void *dy, const void *dz, const v
                                          float *dpost_weight, float *dgate, float *workspace, odl_stream_t stream_) {
     hipStream_t stream = reinterpret_cast<hipStream_t>(stream_);
     if (const int rc = check_shape("odl_fp8_residual_norm_bwd", x_dtype, h_dtype, rows, cols, gate_size, gate)) return rc;
-    if (!parts || !weight || (rows > 0 && (!x || !h || !dx || !dh || !stats))) return set_error(ODL_ERR_ARG, "odl_fp8_residual_norm_bwd: null pointer");
+    if (!weight || (rows > 0 && (!x || !h || !dx || !dh || !stats))) return set_error(ODL_ERR_ARG, "odl_fp8_residual_norm_bwd: null pointer");
     if (dweight && !workspace) return set_error(ODL_ERR_ARG, "odl_fp8_residual_norm_bwd: gradients of the weights need a workspace");
     if ((dpost_weight || dgate) && !dweight) return set_error(ODL_ERR_ARG, "odl_fp8_residual_norm_bwd: dweight comes with the other weights' gradients");
     if ((dpost_weight && !post_weight) || (dgate && !gate)) return set_error(ODL_ERR_ARG, "odl_fp8_residual_norm_bwd: a gradient of a weight that is not there");

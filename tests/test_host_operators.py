@@ -41,7 +41,7 @@ def test_token_logprobs_entry_refuses():
         refused("odl_fp8_token_logprobs", tuple({**ok, **change}.values()), word)
     assert native.load().odl_fp8_token_logprobs(*{**ok, "rows": 0}.values()) == 0
     ok = dict(l=P, dt=1, rows=4, stride=100, vocab=90, padded=100, t=P, ign=-100, it=1.0, k=5, ids=P, st=P, H=P, a=P, b=P, c=P, dl=P, parts=P, stream=None)
-    for change, word in ((dict(vocab=101), "columns"), (dict(dt=-1), "dtype"), (dict(k=91), "top_k"), (dict(ids=None), "null"), (dict(dl=None), "null"), (dict(parts=None), "null")):
+    for change, word in ((dict(vocab=101), "columns"), (dict(dt=-1), "dtype"), (dict(k=91), "top_k"), (dict(ids=None), "null"), (dict(dl=None), "null"), (dict(st=None), "null")):
         refused("odl_fp8_token_logprobs_bwd", tuple({**ok, **change}.values()), word)
 
 

@@ -206,3 +206,48 @@ def test_streams_and_captured_products():
         eager = fp4_linear(x, codes, scales)
         torch.cuda.synchronize()
         assert torch.equal(held[0], eager) and torch.equal(held[1], eager)
+
+
+@pytest.mark.parametrize("group", [32, 64, 128])
+@pytest.mark.parametrize("rows,n,k", [(7, 100, 384), (20, 1030, 8320), (50, 4100, 3200), (130, 1030, 4224), (65, 8200, 4224)])
+def test_nan_and_infinity_stay_in_their_rows_and_what_is_behind_k_is_nothing(rows, n, k, group):
+    """With codes of zero among the weights an infinity makes infinities and NaN, each where the definition has them; x beyond K, here NaN, is not looked at."""
+    codes, scales, g = weight_of(n, k, group, rows)
+    wide = torch.full((rows, k + 128), float("nan"), device="cuda", dtype=torch.bfloat16)
+    x = wide[:, :k]
+    x.copy_(torch.randn((rows, k), device="cuda", generator=g))
+    want = check(x, codes, scales)
+    x[1, k - 1], x[3, 0], x[rows - 2, k // 2], x[rows - 1, k - 33] = float("inf"), -float("inf"), float("nan"), float("inf")
+    got = fp4_linear(x, codes, scales)
+    whole = [i for i in range(rows) if i not in (1, 3, rows - 2, rows - 1)]
+    assert torch.equal(got[whole], want[whole])
+    w = dequantise_fp4(codes, scales)
+    for i, at in ((1, k - 1), (3, 0), (rows - 1, k - 33)):
+        line = torch.where(w[:, at] == 0, float("nan"), w[:, at] * x[i, at].float())
+        assert torch.equal(got[i].isnan(), line.isnan()) and torch.equal(got[i][~line.isnan()].float(), line[~line.isnan()])
+    assert got[rows - 2].isnan().all()
+
+
+def test_captured_products_of_several_runs_on_two_streams():
+    """Each capture has a workspace of its own: replayed in turn, and at the same time."""
+    rows, n, k = 50, 4100, 3200
+    made = []
+    for seed in range(2):
+        codes, scales, g = weight_of(n, k, 64, seed)
+        x = torch.randn((rows, k), device="cuda", generator=g).bfloat16()
+        want = check(x, codes, scales)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            y = fp4_linear(x, codes, scales)
+        made.append((graph, torch.cuda.Stream(), x, codes, scales, want, y))
+    for trip in range(4):
+        for graph, stream, *_, y in made:
+            y.zero_()
+        torch.cuda.synchronize()
+        for graph, stream, *_ in made:
+            with torch.cuda.stream(stream):
+                graph.replay()
+        eager = [fp4_linear(x, codes, scales) for _, _, x, codes, scales, *_ in made]
+        torch.cuda.synchronize()
+        for (*_, want, y), e in zip(made, eager):
+            assert torch.equal(y, want) and torch.equal(e, want)

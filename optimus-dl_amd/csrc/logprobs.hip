@@ -58,19 +58,20 @@ struct Chunk {
 
 // The exponent of an element, in powers of two, against a running maximum m: d = (l - m) * c, c = log2(e) / T.  With mc = m * c rounded it is one
 // fused multiply-add, l * c - mc: the rounding of mc is the same for every element and for the maximum itself, so nothing is lost by
-// it as long as sums are held against mc and not against m.  Maxima beyond 2^96 (rows masked by the lowest value of a type), where
-// products overflow, take the difference first.
+// it as long as sums are held against mc and not against m.  It moves every exponent by up to 2^-25 |mc|, though, and the sums by as many
+// powers of two: maxima beyond 2^24, where that is more than a half, take the difference first, and sums are held against m * c itself.
 struct Exponent {
     float m, mc, c;
     bool near;
-    __device__ __forceinline__ Exponent(float m_, float c_) : m(m_), mc(m_ * c_), c(c_), near(__builtin_fabsf(m_ * c_) < 0x1p96f) {}
+    __device__ __forceinline__ Exponent(float m_, float c_) : m(m_), mc(m_ * c_), c(c_), near(__builtin_fabsf(m_ * c_) < 0x1p24f) {}
     __device__ __forceinline__ float operator()(float l) const { return near ? __fmaf_rn(l, c, -mc) : (l - m) * c; }
 };
 
-// How far down it is from maximum m to maximum `to`, >= 0 (and finite: what was summed against m is then 0).
+// How far down it is from what is held against maximum m to what is held against `to` (and finite: what was summed against m is 0 then).
 __device__ __forceinline__ float descent(float m, float to, float c) {
     const Exponent a(m, c), b(to, c);
-    return fminf(a.near && b.near ? b.mc - a.mc : (to - m) * c, kFar);
+    const float down = a.near ? (b.near ? b.mc - a.mc : __fmaf_rn(to, c, -a.mc)) : (b.near ? -__fmaf_rn(m, c, -b.mc) : (to - m) * c);
+    return fminf(down, kFar);
 }
 
 // sums over a wave, in every lane

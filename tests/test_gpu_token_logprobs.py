@@ -258,3 +258,32 @@ def test_any_number_of_axes_with_and_without_a_graph(lead, top_k):
         assert torch.equal(r.top_ids, live.top_ids) and torch.equal(r.top_logprobs, live.top_logprobs)
     else:
         assert r.top_ids is None and r.top_logprobs is None
+
+
+@pytest.mark.parametrize("temperature", [1.0, 1e-10, 1e-25, 1e10])
+@pytest.mark.parametrize("log2_size", [-20, 0, 10, 20, 27, 29, 34, 50, 80, 95, 97, 120])
+def test_logits_of_any_size(log2_size, temperature):
+    """Bounds as above, C = 48: the exponents of what is drawn here are off by u (4 |d| + 2), d = (l - max) / T, whose product is rounded before or behind the
+    subtraction.  What lies beyond the range of fp32 is -inf.  Rows of one sign, around a number by its last places, and with a step up for every lane."""
+    g = torch.Generator(device="cuda").manual_seed(log2_size + 100)
+    l = torch.randn((5, 3000), device="cuda", generator=g) * 2.0 ** log2_size
+    l[1] = l[1].abs()
+    l[2] = -l[2].abs()
+    l[3] = l[3].abs().max() * (1 + torch.randint(0, 9, (3000,), device="cuda", generator=g) * 2.0 ** -23)      # the last places of one number
+    l[4] = torch.sort(l[4]).values
+    t = torch.randint(0, 3000, (5,), device="cuda", generator=g)
+    live = l.clone().requires_grad_(True)
+    r = token_logprobs(live, t, top_k=3, temperature=temperature)
+    logp = torch.log_softmax(l.double() / temperature, 1)
+    want = logp.gather(1, t.unsqueeze(1)).squeeze(1)
+    fits = want > -2e38
+    assert not r.logprobs.isnan().any() and bool(((r.logprobs - want).abs()[fits] <= (U * (8 * want.abs() + 250))[fits]).all())
+    assert (r.logprobs[~fits] < -1e38).all()
+    H = -(logp.exp() * logp.clamp_min(-1e300)).sum(1)
+    assert bool(((r.entropy - H).abs() <= U * 250 * (1 + H)).all())
+    assert torch.equal(r.top_ids, l.sort(dim=1, descending=True, stable=True).indices[:, :3])
+    r.logprobs.sum().backward()
+    p = logp.exp()
+    want = -p / temperature
+    want[torch.arange(5), t] += 1 / temperature
+    assert bool(((live.grad * temperature - want * temperature).abs() <= U * (200 + 16 * logp.abs().clamp_max(1e3)) * p + 4 * U).all())

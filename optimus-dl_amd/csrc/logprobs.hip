@@ -22,6 +22,7 @@ namespace {
 constexpr int kParts = ODL_FP8_AMAX_PARTS;
 constexpr int kMaxTop = ODL_FP8_LOGPROBS_MAX_TOP;
 constexpr int kCand = 1024;                      // candidates that are ranked at once
+constexpr int kFolded = 32;                      // up to so many alternatives 64 folded maxima give a good bound
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 constexpr float kFar = 1e30f;                    // exponents are cut off here: finite times e^-far is 0, infinity times 0 is not
 
@@ -117,6 +118,16 @@ __device__ __forceinline__ float log_prob(float l, const Row &r, float c) {
     return (Exponent(r.m, c)(l) - r.log2_s) * kLn2;
 }
 
+// A float as a number that is larger where it is (no NaN), and the least float whose number has these upper 16 bits.
+__device__ __forceinline__ uint32_t order_key(float v) {
+    const uint32_t u = float_to_bits(v);
+    return u >> 31 ? ~u : u | 0x80000000u;
+}
+__device__ __forceinline__ float order_least(uint32_t upper) {
+    const uint32_t key = upper << 16;
+    return fmaxf(bits_to_float(key >> 31 ? key & 0x7fffffffu : ~key), -INFINITY);          // (below -inf: all of them)
+}
+
 __device__ __forceinline__ bool before(float v, int i, float w, int j) { return v > w || (v == w && i < j); }
 
 struct Forward {
@@ -148,7 +159,7 @@ __global__ __launch_bounds__(THREADS) void token_logprobs_kernel(const Forward a
     typedef typename Elem<DT>::T T;
     constexpr int U = 4, kWaves = THREADS / kWave;
     __shared__ float wave_m[kWaves], wave_s[kWaves], wave_q[kWaves], cand_v[kCand];
-    __shared__ __attribute__((aligned(16))) float group_top[kWave];
+    __shared__ __attribute__((aligned(16))) float group_top[THREADS];
     __shared__ int cand_i[kCand], lanes[THREADS], n_lanes, n_cand;
     const int tid = threadIdx.x, lane = tid % kWave;
     const int64_t row = blockIdx.x;
@@ -226,8 +237,12 @@ __global__ __launch_bounds__(THREADS) void token_logprobs_kernel(const Forward a
     const float wm = group_max<kWave>(m);
     if (lane == 0) wave_m[tid / kWave] = wm;
     if (a.top_k) {
-        const float g = group_max<THREADS / kWave>(top);
-        if (tid % (THREADS / kWave) == 0) group_top[tid / (THREADS / kWave)] = g;
+        if (a.top_k <= kFolded) {
+            const float g = group_max<THREADS / kWave>(top);
+            if (tid % (THREADS / kWave) == 0) group_top[tid / (THREADS / kWave)] = g;
+        } else {
+            group_top[tid] = top;
+        }
         if (tid == 0) n_lanes = n_cand = 0;
     }
     __syncthreads();
@@ -238,7 +253,20 @@ __global__ __launch_bounds__(THREADS) void token_logprobs_kernel(const Forward a
     const float ws = wave_sum(s), wq = wave_sum(q);
     if (lane == 0) { wave_s[tid / kWave] = ws; wave_q[tid / kWave] = wq; }
     float least = 0.0f;
-    if (a.top_k) {                               // the k-th largest of the 64 maxima; every wave finds it for itself
+    if (a.top_k > kFolded) {
+        // a bound of the k-th largest of all lanes' maxima: the largest number of 16 bits that k of them reach, bit by bit
+        uint32_t key[THREADS / kWave], reach = 0;
+#pragma unroll
+        for (int j = 0; j < THREADS / kWave; ++j) key[j] = order_key(group_top[j * kWave + lane]) >> 16;
+        for (uint32_t bit = 1u << 15; bit; bit >>= 1) {
+            int count = 0;
+#pragma unroll
+            for (int j = 0; j < THREADS / kWave; ++j) count += __popcll(__ballot(key[j] >= (reach | bit)));
+            if (count >= a.top_k) reach |= bit;
+        }
+        least = order_least(reach);
+        if (top >= least) lanes[atomicAdd(&n_lanes, 1)] = tid;
+    } else if (a.top_k) {                        // the k-th largest of the 64 maxima; every wave finds it for itself
         const float v = group_top[lane];
         int above = 0, equal = 0;
 #pragma unroll

@@ -287,3 +287,23 @@ def test_logits_of_any_size(log2_size, temperature):
     want = -p / temperature
     want[torch.arange(5), t] += 1 / temperature
     assert bool(((live.grad * temperature - want * temperature).abs() <= U * (200 + 16 * logp.abs().clamp_max(1e3)) * p + 4 * U).all())
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("cols", [64, 100, 4097, 50257])
+def test_many_alternatives_wherever_the_logits_lie(dtype, cols):
+    """The ids are those of a stable sort, for values of one sign, of both, around zero (of either sign, subnormal too), with infinities below and with ties."""
+    l, t, _ = logits_of(9, cols, dtype, seed=cols)
+    l[1] = l[1].abs() + 1
+    l[2] = -l[2].abs() - 1
+    l[3] *= 1e-39
+    l[4] = torch.where(l[4] > 0, 0.0, -0.0).to(dtype)
+    l[5, 40:] = float("-inf")
+    l[6] = (l[6] * 4).round() / 4
+    l[7] *= 1e30
+    l[8] = -3.0 - torch.arange(cols, device="cuda").flip(0).to(dtype) / cols
+    want = l.float().sort(dim=1, descending=True, stable=True).indices
+    for top_k in (31, 32, 33, 48, 64):
+        r = token_logprobs(l, t, top_k=top_k)
+        assert torch.equal(r.top_ids, want[:, :top_k])
+        assert bool((r.top_logprobs[:, 1:] <= r.top_logprobs[:, :-1]).all())

@@ -728,12 +728,14 @@ int odl_fp8_residual_norm_bwd(const void *dy, const void *dz, const void *x, int
  * targets[r] == ignore_index: the row is not read; 0, 0, top_logprobs 0 and top_ids -1.  Another target outside of [0, vocab): NaN.
  * Rows of -inf only: -inf and entropy 0.  A row with NaN or +inf: NaN, top_ids -1.
  * stats[2 * rows]: of each row the maximum and log2 of the sum against it, for the backward (may be NULL).
- * Up to 2^22 - 1 rows and 2^24 columns.
+ * Up to 2^22 - 1 rows and 2^24 columns.  workspace: odl_fp8_token_logprobs_workspace(rows, vocab, top_k) floats, contents irrelevant; where that is
+ * 0 it may be NULL.
  */
 #define ODL_FP8_LOGPROBS_MAX_TOP 64
+int64_t odl_fp8_token_logprobs_workspace(int64_t rows, int64_t vocab, int top_k);
 int odl_fp8_token_logprobs(const void *logits, int dtype, int64_t rows, int64_t stride, int64_t vocab, const int64_t *targets,
                            int64_t ignore_index, float inv_temperature, int top_k, float *logprobs, float *entropy, float *stats,
-                           float *top_logprobs, int64_t *top_ids, odl_stream_t stream);
+                           float *top_logprobs, int64_t *top_ids, float *workspace, int64_t workspace_bytes, odl_stream_t stream);
 /*
  * Gradient of the logits for gradients of logprobs, entropy and top_logprobs (each may be NULL: zero), dense [rows, padded] in the
  * type of the logits: zero for columns from vocab on and for ignored rows, NaN for rows whose target is no token.  parts: partial

@@ -56,6 +56,7 @@ decltype(&odl_fp8_mx_gemm_nt_hinted) mx_gemm_nt_c;
 decltype(&odl_fp8_last_error) last_error_c;
 decltype(&odl_fp8_residual_norm) residual_norm_c;
 decltype(&odl_fp8_residual_norm_bwd) residual_norm_bwd_c;
+decltype(&odl_fp8_token_logprobs_workspace) logprobs_workspace_c;
 decltype(&odl_fp8_token_logprobs) logprobs_c;
 decltype(&odl_fp8_token_logprobs_bwd) logprobs_bwd_c;
 decltype(&odl_fp8_fp4_linear_runs) fp4_runs_c;
@@ -99,6 +100,7 @@ void bind(const py::dict &d) {
     take(last_error_c, d, "odl_fp8_last_error");
     take(residual_norm_c, d, "odl_fp8_residual_norm");
     take(residual_norm_bwd_c, d, "odl_fp8_residual_norm_bwd");
+    take(logprobs_workspace_c, d, "odl_fp8_token_logprobs_workspace");
     take(logprobs_c, d, "odl_fp8_token_logprobs");
     take(logprobs_bwd_c, d, "odl_fp8_token_logprobs_bwd");
     take(fp4_runs_c, d, "odl_fp8_fp4_linear_runs");
@@ -532,9 +534,12 @@ py::object token_logprobs(const Tensor &l, const Tensor &targets, i64 vocab, int
         top = f32(l, {rows, top_k});
         ids = at::empty({rows, top_k}, l.options().dtype(at::kLong));
     }
+    const i64 need = logprobs_workspace_c(rows, vocab, top_k);
+    OptTensor ws;
+    if (need) ws = f32(l, {need});
     Tensor lp = out.select(0, 0), entropy = out.select(0, 1);
     const int rc = call(logprobs_c, ptr(l), src_of(l), rows, l.stride(0), vocab, targets.data_ptr<i64>(), ignore, (float)inv_t, top_k, ptr(lp), ptr(entropy),
-                        ptr(stats), ptr(top), ptr(ids), str(stream));
+                        ptr(stats), ptr(top), ptr(ids), ptr(ws), 4 * need, str(stream));
     return rc ? status(rc) : py::make_tuple(lp, entropy, obj(stats), obj(top), obj(ids));
 }
 
@@ -669,8 +674,11 @@ struct TokenLogprobsNode : torch::autograd::Function<TokenLogprobsNode> {
             top = f32(l, shape);
             ids = at::empty(shape, l.options().dtype(at::kLong));
         }
+        const i64 need = logprobs_workspace_c(rows, vocab, (int)top_k);
+        OptTensor ws;
+        if (need) ws = f32(l, {need});
         done(logprobs_c(ptr(l), src_of(l), rows, l.stride(0), vocab, targets.data_ptr<i64>(), ignore, (float)inv_t, (int)top_k, ptr(lp), ptr(entropy), ptr(stats),
-                        ptr(given(top)), ptr(given(ids)), str(stream)),
+                        ptr(given(top)), ptr(given(ids)), ptr(ws), 4 * need, str(stream)),
              "odl_fp8_token_logprobs");
         ctx->save_for_backward({logits, targets, entropy, stats, ids});
         ctx->set_materialize_grads(false);

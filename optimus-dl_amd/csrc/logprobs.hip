@@ -4,14 +4,14 @@
 //   p_j = e^d_j / s,  dl_j = [A (j == t) + sum_i C_i (j == id_i) - p_j (A + sum_i C_i) - B p_j (ln p_j + entropy)] / T
 // for gradients A of the logprob, B of the entropy, C_i of the top alternatives.
 //
-// The forward reads a row once, a block a row, with a running maximum and the two sums of it per lane.  The top k cost no work in that
+// The forward reads a row once, a block a row or a part of it, with a running maximum and the two sums of it per lane.  The top k cost no work in that
 // pass: the lanes' maxima are folded to 64, the k-th largest of those is a lower bound of the k-th largest logit, and only lanes whose
 // maximum reaches it can hold one; their share of the row is read again and what reaches the bound is ranked.
 // Rows are read and written with 16-byte accesses at any alignment (rows of an odd number of columns begin anywhere).
 // Bound by HBM for large calls (8 to 12 operations an element, one of them an exponential), by latency for a few rows.  8192 x 50257 bf16: forward
 // 155 to 165 us (5.0 to 5.3 TB/s), backward 340 us (4.8 TB/s read and written); 2048 rows with the top 5 47 us (4.3); 1004 rows of fp32 at odd addresses
-// 50 (4.1) and 74; 16 rows of 32000 with the top 20 9.3.  A row is one block's: cut over
-// several and joined by a second launch, 16 rows took 18 + 26 us, most of it the top k of the parts.
+// 50 (4.1) and 74; 16 rows of 32000 with the top 20 9.3.  A row is one block's, but for few
+// rows of a large vocabulary, which are cut over several blocks and joined by a second launch (parts_of).
 #include "common.h"
 
 #pragma clang fp contract(off)
@@ -22,6 +22,7 @@ namespace {
 constexpr int kParts = ODL_FP8_AMAX_PARTS;
 constexpr int kMaxTop = ODL_FP8_LOGPROBS_MAX_TOP;
 constexpr int kCand = 1024;                      // candidates that are ranked at once
+constexpr int kMaxParts = 16;                    // (their top k are ranked at once)
 constexpr int kFolded = 32;                      // up to so many alternatives 64 folded maxima give a good bound
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 constexpr float kFar = 1e30f;                    // exponents are cut off here: finite times e^-far is 0, infinity times 0 is not
@@ -138,7 +139,46 @@ struct Forward {
     float c;                                     // log2(e) / T
     float *logprobs, *entropy, *stats, *top_logprobs;
     int64_t *top_ids;
+    float *partial;                              // of rows that several blocks share: [rows][parts][3 + 2 top_k]
+    int parts, span;                             // parts of a row, columns of one (a multiple of 8)
 };
+
+// A row that is not read.
+__device__ __forceinline__ void ignored(const Forward &a, int64_t row, int tid) {
+    if (tid == 0) {
+        a.logprobs[row] = 0.0f;
+        a.entropy[row] = 0.0f;
+        if (a.stats) { a.stats[row] = 0.0f; a.stats[a.rows + row] = 0.0f; }
+    }
+    if (tid < a.top_k) {
+        a.top_logprobs[row * a.top_k + tid] = 0.0f;
+        a.top_ids[row * a.top_k + tid] = -1;
+    }
+}
+
+// What sum and weighted sum against the maximum say.
+__device__ __forceinline__ Row row_of(float m, float s, float q) {
+    Row r;
+    r.m = m;
+    r.log2_s = s == 0.0f ? -INFINITY : log2f(s);
+    r.entropy = s == 0.0f ? 0.0f : (r.log2_s - q / s) * kLn2;
+    return r;
+}
+
+template <int DT>
+__device__ __forceinline__ void answer(const Forward &a, int64_t row, int64_t target, const Row &r) {
+    const typename Elem<DT>::T *p = reinterpret_cast<const typename Elem<DT>::T *>(a.logits) + row * a.stride;
+    a.logprobs[row] = target >= 0 && target < a.vocab ? log_prob(one<DT>(p + target), r, a.c) : __builtin_nanf("");
+    a.entropy[row] = r.entropy;
+    if (a.stats) { a.stats[row] = r.m; a.stats[a.rows + row] = r.log2_s; }
+}
+
+// An alternative of its rank; a row with NaN or +inf has no order.
+__device__ __forceinline__ void alternative(const Forward &a, int64_t row, const Row &r, int rank, float v, int id) {
+    const bool sound = r.log2_s == r.log2_s;
+    a.top_logprobs[row * a.top_k + rank] = sound ? log_prob(v, r, a.c) : __builtin_nanf("");
+    a.top_ids[row * a.top_k + rank] = sound ? id : -1;
+}
 
 // How many of n candidates come before (v, id).  The arrays are filled up to a multiple of 8 with what comes before nothing.
 __device__ __forceinline__ int rank_of(const float *values, const int *ids, int n, float v, int id) {
@@ -154,7 +194,8 @@ __device__ __forceinline__ int rank_of(const float *values, const int *ids, int 
     return rank;
 }
 
-template <int DT, int THREADS>
+// PART: a block has one of the parts of a row, and leaves its maximum, its sums and its top k for the join.
+template <int DT, int THREADS, bool PART>
 __global__ __launch_bounds__(THREADS) void token_logprobs_kernel(const Forward a) {
     typedef typename Elem<DT>::T T;
     constexpr int U = 4, kWaves = THREADS / kWave;
@@ -164,20 +205,14 @@ __global__ __launch_bounds__(THREADS) void token_logprobs_kernel(const Forward a
     const int tid = threadIdx.x, lane = tid % kWave;
     const int64_t row = blockIdx.x;
     const int64_t target = a.targets[row];
-    if (target == a.ignore_index) {              // (not read)
-        if (tid == 0) {
-            a.logprobs[row] = 0.0f;
-            a.entropy[row] = 0.0f;
-            if (a.stats) { a.stats[row] = 0.0f; a.stats[a.rows + row] = 0.0f; }
-        }
-        if (tid < a.top_k) {
-            a.top_logprobs[row * a.top_k + tid] = 0.0f;
-            a.top_ids[row * a.top_k + tid] = -1;
-        }
+    if (target == a.ignore_index) {
+        if (!PART) ignored(a, row, tid);
         return;
     }
-    const T *p = reinterpret_cast<const T *>(a.logits) + row * a.stride;
-    const int n = a.vocab / 8, tail = a.vocab % 8;
+    const int first = PART ? (int)blockIdx.y * a.span : 0, end = PART ? min(first + a.span, a.vocab) : a.vocab;
+    float *mine = a.partial + (row * a.parts + blockIdx.y) * (3 + 2 * a.top_k);
+    const T *p = reinterpret_cast<const T *>(a.logits) + row * a.stride + first;
+    const int n = (end - first) / 8, tail = (end - first) % 8;
     // running maximum (never below -FLT_MAX, so that differences from it are finite or -inf), sum 2^d, sum 2^d d
     float m = -FLT_MAX, s = 0.0f, q = 0.0f, top = -INFINITY;
     auto move_to = [&](float to) {
@@ -284,21 +319,16 @@ __global__ __launch_bounds__(THREADS) void token_logprobs_kernel(const Forward a
     q = wave_q[0];
 #pragma unroll
     for (int w = 1; w < kWaves; ++w) { s += wave_s[w]; q += wave_q[w]; }
-    Row r;
-    r.m = m;
-    r.log2_s = s == 0.0f ? -INFINITY : log2f(s);
-    r.entropy = s == 0.0f ? 0.0f : (r.log2_s - q / s) * kLn2;
+    const Row r = row_of(m, s, q);
     if (tid == 0) {
-        a.logprobs[row] = target >= 0 && target < a.vocab ? log_prob(one<DT>(p + target), r, a.c) : __builtin_nanf("");
-        a.entropy[row] = r.entropy;
-        if (a.stats) { a.stats[row] = r.m; a.stats[a.rows + row] = r.log2_s; }
+        if constexpr (PART) { mine[0] = m; mine[1] = s; mine[2] = q; }
+        else answer<DT>(a, row, target, r);
     }
     if (!a.top_k) return;
 
-    const bool sound = r.log2_s == r.log2_s;     // a row with NaN or +inf has no order
     auto put = [&](int rank, float v, int id) {
-        a.top_logprobs[row * a.top_k + rank] = sound ? log_prob(v, r, a.c) : __builtin_nanf("");
-        a.top_ids[row * a.top_k + rank] = sound ? id : -1;
+        if constexpr (PART) { mine[3 + rank] = v; reinterpret_cast<uint32_t *>(mine)[3 + a.top_k + rank] = (uint32_t)first + (uint32_t)id; }
+        else alternative(a, row, r, rank, v, id);
     };
     auto offer = [&](float v, int col) {
         if (v >= least) {
@@ -329,7 +359,7 @@ __global__ __launch_bounds__(THREADS) void token_logprobs_kernel(const Forward a
             const int id = cand_i[i], rank = rank_of(cand_v, cand_i, found, v, id);
             if (rank < a.top_k) put(rank, v, id);
         }
-        if (tid >= found && tid < a.top_k) put(tid, -INFINITY, -1);        // (fewer than k: NaN in the row)
+        if (tid >= found && tid < a.top_k) put(tid, -INFINITY, 0);         // (fewer than k: NaN in the row, which has no order)
         return;
     }
     // More than a thousand logits share the bound (rows that are masked almost everywhere, say): the largest behind the last one
@@ -367,6 +397,68 @@ __global__ __launch_bounds__(THREADS) void token_logprobs_kernel(const Forward a
         last_v = best_v;
         last_i = best_i;
         if (tid == 0) put(k, best_v, best_i);
+    }
+}
+
+// Rows that several blocks share: the maxima and sums of their parts and the largest of their top k.  Each part has at least
+// ceil(k / parts) logits that reach its own one of that rank, and k that reach its last: the smallest of the former and the largest of the latter are bounds
+// of the k-th largest of the row, and little more than k candidates reach them.
+template <int DT>
+__global__ __launch_bounds__(256) void token_logprobs_join_kernel(const Forward a) {
+    __shared__ float cand_v[kCand];
+    __shared__ int cand_i[kCand], n_cand;
+    const int tid = threadIdx.x, record = 3 + 2 * a.top_k;
+    const int64_t row = blockIdx.x, target = a.targets[row];
+    if (target == a.ignore_index) return ignored(a, row, tid);
+    const float *from = a.partial + row * a.parts * record;
+    if (tid == 0) n_cand = 0;
+    // a part a lane, sixteen lanes at a time; every wave for itself
+    const bool have = tid % 16 < a.parts;
+    const float *part = from + tid % 16 * record;
+    const float pm = have ? part[0] : -FLT_MAX, ps = have ? part[1] : 0.0f, pq = have ? part[2] : 0.0f;
+    float m = pm, each = INFINITY, last = -INFINITY;
+    if (have && a.top_k) {
+        each = part[3 + (a.top_k + a.parts - 1) / a.parts - 1];
+        last = part[3 + a.top_k - 1];
+    }
+    static_assert(kMaxParts == 16, "a group of lanes has the parts");
+#pragma unroll
+    for (int off = 8; off > 0; off >>= 1) {
+        m = fmaxf(m, __shfl_xor(m, off, kWave));
+        each = fminf(each, __shfl_xor(each, off, kWave));
+        last = fmaxf(last, __shfl_xor(last, off, kWave));
+    }
+    const float least = fmaxf(each, last), down = descent(pm, m, a.c), f = __builtin_amdgcn_exp2f(-down);
+    float s = f * ps, q = f * __fmaf_rn(-down, ps, pq);
+#pragma unroll
+    for (int off = 8; off > 0; off >>= 1) {
+        s += __shfl_xor(s, off, kWave);
+        q += __shfl_xor(q, off, kWave);
+    }
+    __syncthreads();
+    for (int i = tid; i < a.parts * a.top_k; i += 256) {
+        const float *at = from + i / a.top_k * record + 3 + i % a.top_k;
+        const float v = at[0];
+        const int id = reinterpret_cast<const int *>(at)[a.top_k];
+        if (v >= least) {
+            const int to = atomicAdd(&n_cand, 1);
+            cand_v[to] = v;
+            cand_i[to] = id;
+        }
+    }
+    const Row r = row_of(m, s, q);
+    if (tid == 0) answer<DT>(a, row, target, r);
+    __syncthreads();
+    const int n = n_cand;
+    if (r.log2_s != r.log2_s) {                  // (candidates of such a row may be fewer)
+        if (tid < a.top_k) alternative(a, row, r, tid, 0.0f, 0);
+        return;
+    }
+    if (tid < 8 && n + tid < kCand) { cand_v[n + tid] = -INFINITY; cand_i[n + tid] = INT_MAX; }
+    __syncthreads();
+    for (int i = tid; i < n; i += 256) {
+        const int rank = rank_of(cand_v, cand_i, n, cand_v[i], cand_i[i]);
+        if (rank < a.top_k) alternative(a, row, r, rank, cand_v[i], cand_i[i]);
     }
 }
 
@@ -523,29 +615,63 @@ int check(const char *who, int dtype, int64_t rows, int64_t stride, int64_t padd
     return ODL_OK;
 }
 
+// Blocks that share a row: few rows of a large vocabulary keep a compute unit each busy with their exponentials alone.  us, one block a row / shared,
+// no alternatives and 20: 1 x 151936 12.3, 16.9 / 6.2, 12.1; 64 x 128256 10.7, 15.5 / 7.7, 13.9; 100 x 151936 15.4, 20.3 / 12.1, 18.2; 1 x 100352 8.5, 13.2 / 6.0,
+// 11.7; 1 x 65536, 32 x 65536 6.3, 11.0 and 6.7, 11.4 / 5.7, 11.6 and 6.4, 12.1, which pays for no second launch.  Parts of 8192: 13.2 to 14.7 for 16.
+int parts_of(int64_t rows, int64_t vocab) {
+    if (vocab < 98304) return 1;
+    int64_t p = device_cu_count() / rows;
+    p = p < vocab / 16384 ? p : vocab / 16384;
+    return p < 2 ? 1 : p < kMaxParts ? (int)p : kMaxParts;
+}
+
 }  // namespace
 }  // namespace odl
 
 using namespace odl;
 
+// Floats of the workspace that a call needs; 0: none.
+extern "C" int64_t odl_fp8_token_logprobs_workspace(int64_t rows, int64_t vocab, int top_k) {
+    if (rows < 1 || rows >= (1 << 22) || vocab < 1 || top_k < 0 || top_k > kMaxTop) return 0;
+    const int parts = parts_of(rows, vocab);
+    return parts > 1 ? rows * parts * (3 + 2 * top_k) : 0;
+}
+
 extern "C" int odl_fp8_token_logprobs(const void *logits, int dtype, int64_t rows, int64_t stride, int64_t vocab, const int64_t *targets,
                                       int64_t ignore_index, float inv_temperature, int top_k, float *logprobs, float *entropy, float *stats,
-                                      float *top_logprobs, int64_t *top_ids, odl_stream_t stream_) {
+                                      float *top_logprobs, int64_t *top_ids, float *workspace, int64_t workspace_bytes, odl_stream_t stream_) {
     hipStream_t stream = reinterpret_cast<hipStream_t>(stream_);
     if (const int rc = check("odl_fp8_token_logprobs", dtype, rows, stride, vocab, vocab, top_k, inv_temperature)) return rc;
     if (rows == 0) return ODL_OK;
     if (!logits || !targets || !logprobs || !entropy || (top_k && (!top_logprobs || !top_ids)))
         return set_error(ODL_ERR_ARG, "odl_fp8_token_logprobs: null pointer");
+    const int64_t needed = odl_fp8_token_logprobs_workspace(rows, vocab, top_k);
+    if (needed && (!workspace || workspace_bytes / 4 < needed))
+        return set_error(ODL_ERR_ARG, "odl_fp8_token_logprobs: a workspace of %lld floats is needed", (long long)needed);
     Forward a = {};
     a.logits = logits; a.targets = targets; a.rows = rows; a.stride = stride; a.ignore_index = ignore_index;
     a.vocab = (int)vocab; a.top_k = top_k; a.c = inv_temperature * kLog2e;
     a.logprobs = logprobs; a.entropy = entropy; a.stats = stats; a.top_logprobs = top_logprobs; a.top_ids = top_ids;
+    a.parts = needed ? parts_of(rows, vocab) : 1;
+    a.span = (int)((vocab + a.parts - 1) / a.parts + 7) / 8 * 8;
+    a.partial = workspace;
+    if (needed) {
+        const dim3 shared((unsigned)rows, (unsigned)a.parts);
+        if (dtype == ODL_BF16) {
+            hipLaunchKernelGGL((token_logprobs_kernel<ODL_BF16, 512, true>), shared, dim3(512), 0, stream, a);
+            hipLaunchKernelGGL(token_logprobs_join_kernel<ODL_BF16>, dim3((unsigned)rows), dim3(256), 0, stream, a);
+        } else {
+            hipLaunchKernelGGL((token_logprobs_kernel<ODL_F32, 512, true>), shared, dim3(512), 0, stream, a);
+            hipLaunchKernelGGL(token_logprobs_join_kernel<ODL_F32>, dim3((unsigned)rows), dim3(256), 0, stream, a);
+        }
+        return check_launch("odl_fp8_token_logprobs");
+    }
     const dim3 grid((unsigned)rows);
     // Lanes of a row's block, us with 256 / 512 / 1024: 8192 x 50257 bf16 160 / 155 / 190, 2048 rows 44.8 / 42.5 / 46.4, 16 x 32000 (top 20) 10.1 / 9.4 / 10.6;
     // short rows, and rows of middle length where there are many, have less to do than a wide block to agree on: 2000 x 1000
     // 11.4 / 17.5 / 30.5, 700 x 32000 15.3 / 17.1 / 20.5; few long ones more: 1 x 131072 20.2 / 16.2 / 14.9
     const int threads = vocab <= 4096 || (vocab <= 40000 && rows >= 512) ? 256 : vocab >= 65536 && rows <= 64 ? 1024 : 512;
-#define ODL_LPF(DT, THREADS) hipLaunchKernelGGL((token_logprobs_kernel<DT, THREADS>), grid, dim3(THREADS), 0, stream, a)
+#define ODL_LPF(DT, THREADS) hipLaunchKernelGGL((token_logprobs_kernel<DT, THREADS, false>), grid, dim3(THREADS), 0, stream, a)
 #define ODL_LPF_DT(THREADS) do { if (dtype == ODL_BF16) ODL_LPF(ODL_BF16, THREADS); else ODL_LPF(ODL_F32, THREADS); } while (0)
     if (threads == 256) ODL_LPF_DT(256);
     else if (threads == 512) ODL_LPF_DT(512);

@@ -106,6 +106,7 @@ EXPORTS = (
     "odl_fp8_mx_gemm_splitk",
     "odl_fp8_residual_norm",
     "odl_fp8_residual_norm_bwd",
+    "odl_fp8_token_logprobs_workspace",
     "odl_fp8_token_logprobs",
     "odl_fp8_token_logprobs_bwd",
     "odl_fp8_fp4_linear_runs",
@@ -220,7 +221,9 @@ def load() -> ctypes.CDLL:
         f32 = ctypes.c_float
         L.odl_fp8_residual_norm.argtypes = [vp, i32, vp, i32, vp, vp, vp, i64, i64, i64, f32, f32, f32, vp, vp, vp, vp, vp]
         L.odl_fp8_residual_norm_bwd.argtypes = [vp, vp, vp, i32, vp, i32, vp, vp, vp, i64, i64, i64, f32, vp, vp, vp, vp, vp, vp, vp, vp, vp]
-        L.odl_fp8_token_logprobs.argtypes = [vp, i32, i64, i64, i64, vp, i64, f32, i32, vp, vp, vp, vp, vp, vp]
+        L.odl_fp8_token_logprobs_workspace.argtypes = [i64, i64, i32]
+        L.odl_fp8_token_logprobs_workspace.restype = i64
+        L.odl_fp8_token_logprobs.argtypes = [vp, i32, i64, i64, i64, vp, i64, f32, i32, vp, vp, vp, vp, vp, vp, i64, vp]
         L.odl_fp8_token_logprobs_bwd.argtypes = [vp, i32, i64, i64, i64, i64, vp, i64, f32, i32, vp, vp, vp, vp, vp, vp, vp, vp, vp]
         L.odl_fp8_fp4_linear_runs.argtypes = [i64, i64, i64, i32]
         L.odl_fp8_fp4_linear_runs.restype = i32
@@ -1760,10 +1763,12 @@ def token_logprobs(logits: torch.Tensor, targets: torch.Tensor, n_vocab: int, to
         new = lambda *shape: torch.empty(shape, dtype=torch.float32, device=logits.device)
         out, stats = new(2, rows), new(2, rows) if keep_stats else None
         top, ids = (new(rows, top_k), torch.empty((rows, top_k), dtype=torch.int64, device=logits.device)) if top_k else (None, None)
+        floats = load().odl_fp8_token_logprobs_workspace(rows, n_vocab, top_k)
+        ws = new(floats) if floats else None
         p = lambda t: None if t is None else t.data_ptr()
         _check(load().odl_fp8_token_logprobs(p(logits), _src_dtype(logits), rows, logits.stride(0), n_vocab, p(targets), ignore_index,
                                              1.0 / temperature, top_k, out[0].data_ptr(), out[1].data_ptr(), p(stats), p(top), p(ids),
-                                             _stream()), "odl_fp8_token_logprobs")
+                                             p(ws), 4 * floats, _stream()), "odl_fp8_token_logprobs")
     return out[0], out[1], stats, top, ids
 
 

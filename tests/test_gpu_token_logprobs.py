@@ -307,3 +307,49 @@ def test_many_alternatives_wherever_the_logits_lie(dtype, cols):
         r = token_logprobs(l, t, top_k=top_k)
         assert torch.equal(r.top_ids, want[:, :top_k])
         assert bool((r.top_logprobs[:, 1:] <= r.top_logprobs[:, :-1]).all())
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("rows", [1, 3, 64, 127, 129])
+@pytest.mark.parametrize("cols", [98303, 98304, 131077, 151936])
+def test_rows_that_several_blocks_share(rows, cols, dtype):
+    l, t, grads = logits_of(rows, cols, dtype, seed=rows)
+    for top_k in (0, 1, 20, 64):
+        check(l, t, grads, top_k=top_k)
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+def test_what_parts_of_a_row_may_hold(dtype):
+    V = 131077                                              # eight parts of 16392, the last one shorter
+    l, t, _ = logits_of(10, V, dtype, seed=4)
+    l[0] = float("-inf")                                    # nothing
+    l[1, :100000] = float("-inf")                           # parts with nothing
+    l[2] = float("-inf")
+    l[2, [5, 40000, 131076]] = torch.tensor([1.0, 2.0, 1.0], device="cuda", dtype=dtype)
+    l[3, 70000] = float("nan")
+    l[4, 131076] = float("inf")
+    l[5] = 0.25                                             # all equal: thousands of candidates in each part
+    l[6] = torch.finfo(dtype).min
+    l[6, 100000:] = torch.randint(0, 5, (V - 100000,), device="cuda").to(dtype)        # ties within and across parts
+    l[7] = torch.randint(0, 3, (V,), device="cuda").to(dtype)
+    l[8] = torch.arange(V, device="cuda").to(dtype) / 1000  # all of the best in the last part
+    t[9] = -100
+    for top_k in (0, 5, 64):
+        live = l.clone().requires_grad_(True)
+        r = token_logprobs(live, t, top_k=top_k)
+        exact = l.double()
+        logp = torch.log_softmax(exact[[1, 2, 5, 6, 7, 8]], 1)
+        want = logp.gather(1, t[[1, 2, 5, 6, 7, 8], None]).squeeze(1)
+        got = r.logprobs[[1, 2, 5, 6, 7, 8]].double()
+        assert torch.equal(got == -math.inf, want == -math.inf)
+        ok = want > -1e30
+        assert bool(((got - want).abs()[ok] <= 2e-6 * (20 + want.abs()[ok])).all())
+        assert r.logprobs[0] == -math.inf and r.entropy[0] == 0 and r.logprobs[3].isnan() and r.logprobs[4].isnan() and r.logprobs[9] == 0 == r.entropy[9]
+        assert abs(r.entropy[5].item() - math.log(V)) < 1e-4 and r.entropy[[3, 4]].isnan().all()
+        if top_k:
+            order = l.float().sort(dim=1, descending=True, stable=True).indices[:, :top_k]
+            sound = [0, 1, 2, 5, 6, 7, 8]
+            assert torch.equal(r.top_ids[sound], order[sound]) and (r.top_ids[[3, 4, 9]] == -1).all()
+            assert r.top_logprobs[[3, 4]].isnan().all() and (r.top_logprobs[9] == 0).all() and (r.top_logprobs[0] == -math.inf).all()
+        (r.logprobs[[1, 5, 6, 7, 8, 9]].nan_to_num(neginf=0.0).sum() + r.entropy[[0, 1, 2, 5, 6, 7, 8, 9]].sum()).backward()
+        assert live.grad[[0, 9]].abs().max() == 0 and live.grad[[1, 2, 5, 6, 7, 8]].isfinite().all()

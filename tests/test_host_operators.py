@@ -34,10 +34,11 @@ def test_residual_norm_entry_refuses():
 
 @needs_library
 def test_token_logprobs_entry_refuses():
-    ok = dict(l=P, dt=0, rows=4, stride=100, vocab=100, t=P, ign=-100, it=1.0, k=5, lp=P, H=P, st=P, top=P, ids=P, stream=None)
+    ok = dict(l=P, dt=0, rows=4, stride=100, vocab=100, t=P, ign=-100, it=1.0, k=5, lp=P, H=P, st=P, top=P, ids=P, ws=None, wsb=0, stream=None)
     for change, word in ((dict(rows=-1), "negative"), (dict(dt=2), "dtype"), (dict(vocab=0), "columns"), (dict(vocab=(1 << 24) + 1), "columns"), (dict(rows=1 << 22), "rows"),
                          (dict(k=-1), "top_k"), (dict(k=65), "top_k"), (dict(vocab=4), "top_k"), (dict(it=0.0), "temperature"),
-                         (dict(it=float("nan")), "temperature"), (dict(it=float("inf")), "temperature"), (dict(l=None), "null"), (dict(ids=None), "null")):
+                         (dict(it=float("nan")), "temperature"), (dict(it=float("inf")), "temperature"), (dict(l=None), "null"), (dict(ids=None), "null"),
+                         (dict(vocab=1 << 20), "workspace"), (dict(vocab=1 << 20, ws=P, wsb=4), "workspace")):
         refused("odl_fp8_token_logprobs", tuple({**ok, **change}.values()), word)
     assert native.load().odl_fp8_token_logprobs(*{**ok, "rows": 0}.values()) == 0
     ok = dict(l=P, dt=1, rows=4, stride=100, vocab=90, padded=100, t=P, ign=-100, it=1.0, k=5, ids=P, st=P, H=P, a=P, b=P, c=P, dl=P, parts=P, stream=None)

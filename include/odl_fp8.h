@@ -751,7 +751,7 @@ int odl_fp8_token_logprobs_bwd(const void *logits, int dtype, int64_t rows, int6
  *   y[m, n] = bf16( sum_g scales[n, g] * sum_{k in group g} x[m, k] * e2m1(codes[n, k]) + bias[n] ), fp32 accumulation
  * codes [N, K / 2]: OCP E2M1 (sign, 2 bits of exponent, 1 of mantissa: 0, .5, 1, 1.5, 2, 3, 4, 6), two a byte, the even k in the low
  * nibble; scales bf16 [N, K / group]; group 32, 64 or 128, a divisor of K.  x bf16 [M, K], rows ldx elements apart (a multiple of 8);
- * bias bf16 or fp32 (bias_dtype), or NULL.  x and codes 16-byte aligned.  M up to 2^16, N up to 2^22, K and ldx up to 2^24.
+ * bias bf16 or fp32 (bias_dtype), or NULL.  x and codes 16-byte aligned.  M up to 2^20, N up to 2^22, K and ldx up to 2^24.
  * workspace: odl_fp8_fp4_linear_runs(M, N, K, group) * M * N floats, contents irrelevant; NULL where that is 0.
  */
 int odl_fp8_fp4_linear_runs(int64_t M, int64_t N, int64_t K, int group);

@@ -563,7 +563,7 @@ using namespace odl;
 
 // Partial results that a call writes: its workspace is as many times M * N floats; 0 needs none.
 extern "C" int odl_fp8_fp4_linear_runs(int64_t M, int64_t N, int64_t K, int group) {
-    if (M < 1 || N < 1 || K < 1 || M > (int64_t)1 << 16 || N > (int64_t)1 << 22 || K > (int64_t)1 << 24) return 0;
+    if (M < 1 || N < 1 || K < 1 || M > (int64_t)1 << 20 || N > (int64_t)1 << 22 || K > (int64_t)1 << 24) return 0;
     const int runs = plan_of(M, N, K, group).runs;
     return runs > 1 ? runs : 0;
 }
@@ -579,8 +579,8 @@ extern "C" int odl_fp8_fp4_linear(const void *x, int64_t ldx, const uint8_t *cod
     if (!x || !codes || !scales || !y) return set_error(ODL_ERR_ARG, "odl_fp8_fp4_linear: null pointer");
     if (ldx % 8 != 0 || (M > 1 && ldx < K) || ldx > (int64_t)1 << 24 || !aligned16(x) || !aligned16(codes))
         return set_error(ODL_ERR_SHAPE, "odl_fp8_fp4_linear: x and codes must be 16-byte aligned, rows of x too, at most 2^24 elements apart");
-    if (N > (int64_t)1 << 22 || M > (int64_t)1 << 16 || K > (int64_t)1 << 24)
-        return set_error(ODL_ERR_SHAPE, "odl_fp8_fp4_linear: up to 2^16 rows, 2^22 columns and 2^24 inputs");
+    if (N > (int64_t)1 << 22 || M > (int64_t)1 << 20 || K > (int64_t)1 << 24)
+        return set_error(ODL_ERR_SHAPE, "odl_fp8_fp4_linear: up to 2^20 rows, 2^22 columns and 2^24 inputs");
     const Fp4Plan how = plan_of(M, N, K, group);
     if (how.runs > 1 && (!workspace || workspace_bytes / 4 / M / N < how.runs))
         return set_error(ODL_ERR_ARG, "odl_fp8_fp4_linear: a workspace of %d * M * N floats is needed", how.runs);

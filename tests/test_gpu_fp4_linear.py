@@ -251,3 +251,10 @@ def test_captured_products_of_several_runs_on_two_streams():
         torch.cuda.synchronize()
         for (*_, want, y), e in zip(made, eager):
             assert torch.equal(y, want) and torch.equal(e, want)
+
+
+@pytest.mark.parametrize("rows,n,k,group", [(70001, 100, 64, 32), (66000, 770, 256, 64), (65537, 300, 1024, 128)])
+def test_rows_of_a_long_batch(rows, n, k, group):
+    codes, scales, g = weight_of(n, k, group)
+    x = torch.randn((rows, k), device="cuda", generator=g).bfloat16()
+    check(x, codes, scales, torch.randn(n, device="cuda", generator=g))

@@ -51,7 +51,7 @@ def test_fp4_entries_refuse():
     ok = dict(x=P, ldx=128, codes=P, scales=P, group=32, bias=None, bd=0, M=4, N=16, K=128, y=P, ws=None, wsb=0, stream=None)
     for change, word in ((dict(M=-1), "negative"), (dict(group=16), "group"), (dict(bias=P, bd=2), "bias_dtype"), (dict(K=100), "multiple"), (dict(K=0), "multiple"),
                          (dict(x=None), "null"), (dict(scales=None), "null"), (dict(ldx=132), "aligned"), (dict(ldx=64), "aligned"), (dict(codes=P + 8), "aligned"),
-                         (dict(x=P + 2), "aligned"), (dict(ldx=(1 << 24) + 8), "2^24"), (dict(N=(1 << 22) + 1), "2^22"), (dict(M=(1 << 16) + 1), "2^16"),
+                         (dict(x=P + 2), "aligned"), (dict(ldx=(1 << 24) + 8), "2^24"), (dict(N=(1 << 22) + 1), "2^22"), (dict(M=(1 << 20) + 1), "2^20"),
                          (dict(M=32, N=4096, K=14336, ldx=14336), "workspace"), (dict(M=32, N=4096, K=14336, ldx=14336, ws=P, wsb=1 << 20), "workspace")):
         refused("odl_fp8_fp4_linear", tuple({**ok, **change}.values()), word)
     runs = native.load().odl_fp8_fp4_linear_runs

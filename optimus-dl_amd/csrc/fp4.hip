@@ -496,26 +496,33 @@ __global__ __launch_bounds__(256) void fp4_quantise_kernel(const void *__restric
 bool aligned16(const void *p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 bool group_known(int group) { return group == 32 || group == 64 || group == 128; }
 
-// The thin kernel stages the scales of whole rows, which for a very long K do not fit.
-constexpr int64_t kThinLds = 64 * 1024;
+// The thin kernel stages the scales of whole rows, which for a very long K do not fit, and up to 16 rows of x where they fit beside them: 4 rows
+// 14336 -> 4096 13.6 -> 10.4 us, 16 rows 2048 -> 8192 9.5 -> 6.7.
+constexpr int64_t kThinLds = 64 * 1024, kThinX = 150 * 1024;
+
+template <int G>
+bool x_in_lds(int64_t M, int64_t K) {
+    const Fp4Tile t = fp4_tile<G>((int)K);
+    return M <= 16 && 2 * (16 * (int64_t)t.pitch + M * t.xpitch) <= kThinX;
+}
 
 // How a product is done: rows of a block of the wide kernel in 16s (0: the thin kernel), in how many parts its waves share a phase, and runs of K.
 struct Fp4Plan {
     int mt, shares, runs;
 };
 
-// Up to 4 rows the thin kernel, x in LDS: 4096 -> 14336 10 us (wide 17), 768 -> 2304 3.2 (10).  For more the cheapest by what a block was measured
-// to take: thin 0.39 + 0.058 a row, ns for each k; wide 3.1, 3.7, 5.0 and 9.2 for 16, 32, 64 and 128 rows, 15 for 128 rows by 256 columns, and 1.3 to
-// 4.6 us besides, with as many blocks at a time as there are compute units; a join 1.5 us and 0.86 ps for each number.  Over 182 products of 5 to 2048
-// rows, 768 -> 768 to 28672 -> 8192, what this takes is 1.5 % off the best of them all on average and 24 % at worst.  (By rows and size of the
-// weights alone: 20 % and 95 %.  Blocks of 16 rows were timed for up to 48.)
+// The cheapest by what a block was measured to take, ns for each k: thin 0.30 + 0.055 a row with x in LDS, 0.39 + 0.058 a row without; wide 3.1, 3.7, 5.0 and
+// 9.2 for 16, 32, 64 and 128 rows, 15 for 128 rows by 256 columns, and 1.3 to 4.6 us besides, with as many blocks at a time as there are compute
+// units; a join 1.5 us and 0.86 ps for each number.  Thin blocks of more than four for each unit do not begin together: one row 8192 -> 28672 35 us, wide 29.
+// Over 182 products of 5 to 2048 rows, 768 -> 768 to 28672 -> 8192, what this takes is 1.5 % off the best of them all on average and 24 % at worst, over
+// 176 of 1 to 16 rows 1 and 32 %.  (By rows and size of the weights alone: 20 % and 95 %.  Blocks of 16 rows were timed for up to 48.)
 template <int G>
 Fp4Plan plan(int64_t M, int64_t N, int64_t K) {
     const bool fits = 2 * 16 * (int64_t)fp4_tile<G>((int)K).pitch <= kThinLds;
-    if (fits && M <= 4) return {0, 1, 1};
-    const int64_t cus = device_cu_count(), thin = (N + 15) / 16 * (M <= 16 ? 1 : (M + 31) / 32);
+    const int64_t cus = device_cu_count(), thin = (N + 15) / 16 * (M <= 16 ? 1 : (M + 31) / 32), most = thin > cus ? thin : cus;
     Fp4Plan best = {0, 1, 1};
-    int64_t least = fits ? 4100000 + K * (390 + 58 * (M < 32 ? M : 32)) * (thin > cus ? thin : cus) / cus : INT64_MAX;      // ps
+    int64_t least = !fits ? INT64_MAX : x_in_lds<G>(M, K) ? 3400000 + K * (300 + 55 * M) * most / cus : 4100000 + K * (390 + 58 * (M < 32 ? M : 32)) * most / cus;      // ps
+    if (fits && thin > 4 * cus) least += least / 5 * 2;
     static constexpr struct { int mt, shares, phase, per_k, start; } kinds[] = {
         {1, 2, 1024, 3100, 1300000}, {2, 2, 1024, 3700, 1700000}, {4, 2, 512, 5000, 3000000}, {8, 2, 256, 9200, 4500000}, {8, 1, 256, 15000, 4600000}};
     for (const auto &kind : kinds) {
@@ -535,7 +542,7 @@ template <int G>
 void launch_linear(const Fp4Args &a, const Fp4Plan how, hipStream_t stream) {
     if (how.mt == 0) {
         const Fp4Tile t = fp4_tile<G>((int)a.K);
-        const bool lds = a.M <= 4 && 2 * (16 * (int64_t)t.pitch + a.M * t.xpitch) <= kThinLds, deep = t.whole >= 32;
+        const bool lds = x_in_lds<G>(a.M, a.K), deep = t.whole >= 32;
         // long rows: 16 waves share them (14336 -> 4096 11.5 -> 10.5, 4096 -> 14336 no faster)
         if (lds && deep) launch_thin<G, 1, 1, 16, 1, true>(a, stream);
         else if (lds) launch_thin<G, 1, 1, 8, 1, true>(a, stream);

@@ -523,6 +523,7 @@ Fp4Plan plan(int64_t M, int64_t N, int64_t K) {
     Fp4Plan best = {0, 1, 1};
     int64_t least = !fits ? INT64_MAX : x_in_lds<G>(M, K) ? 3400000 + K * (300 + 55 * M) * most / cus : 4100000 + K * (390 + 58 * (M < 32 ? M : 32)) * most / cus;      // ps
     if (fits && thin > 4 * cus) least += least / 5 * 2;
+    if (least < 6800000) return best;                        // (no wide one begins below)
     static constexpr struct { int mt, shares, phase, per_k, start; } kinds[] = {
         {1, 2, 1024, 3100, 1300000}, {2, 2, 1024, 3700, 1700000}, {4, 2, 512, 5000, 3000000}, {8, 2, 256, 9200, 4500000}, {8, 1, 256, 15000, 4600000}};
     for (const auto &kind : kinds) {

@@ -669,13 +669,12 @@ extern "C" int odl_fp8_token_logprobs(const void *logits, int dtype, int64_t row
     const dim3 grid((unsigned)rows);
     // Lanes of a row's block, us with 256 / 512 / 1024: 8192 x 50257 bf16 160 / 155 / 190, 2048 rows 44.8 / 42.5 / 46.4, 16 x 32000 (top 20) 10.1 / 9.4 / 10.6;
     // short rows, and rows of middle length where there are many, have less to do than a wide block to agree on: 2000 x 1000
-    // 11.4 / 17.5 / 30.5, 700 x 32000 15.3 / 17.1 / 20.5; few long ones more: 1 x 131072 20.2 / 16.2 / 14.9
-    const int threads = vocab <= 4096 || (vocab <= 40000 && rows >= 512) ? 256 : vocab >= 65536 && rows <= 64 ? 1024 : 512;
+    // 11.4 / 17.5 / 30.5, 700 x 32000 15.3 / 17.1 / 20.5; few long ones (top 20): 16 x 81920 - / 12.5 / 12.9
+    const int threads = vocab <= 4096 || (vocab <= 40000 && rows >= 512) ? 256 : 512;
 #define ODL_LPF(DT, THREADS) hipLaunchKernelGGL((token_logprobs_kernel<DT, THREADS, false>), grid, dim3(THREADS), 0, stream, a)
 #define ODL_LPF_DT(THREADS) do { if (dtype == ODL_BF16) ODL_LPF(ODL_BF16, THREADS); else ODL_LPF(ODL_F32, THREADS); } while (0)
     if (threads == 256) ODL_LPF_DT(256);
-    else if (threads == 512) ODL_LPF_DT(512);
-    else ODL_LPF_DT(1024);
+    else ODL_LPF_DT(512);
 #undef ODL_LPF_DT
 #undef ODL_LPF
     return check_launch("odl_fp8_token_logprobs");

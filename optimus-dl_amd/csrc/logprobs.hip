@@ -5,8 +5,8 @@
 // for gradients A of the logprob, B of the entropy, C_i of the top alternatives.
 //
 // The forward reads a row once, a block a row or a part of it, with a running maximum and the two sums of it per lane.  The top k cost no work in that
-// pass: the lanes' maxima are folded to 64, the k-th largest of those is a lower bound of the k-th largest logit, and only lanes whose
-// maximum reaches it can hold one; their share of the row is read again and what reaches the bound is ranked.
+// pass: the lanes' maxima are folded to 64 (or, for many alternatives, searched bit by bit), the k-th largest of those is a lower bound of the k-th
+// largest logit, and only lanes whose maximum reaches it can hold one; their share of the row is read again and what reaches the bound is ranked.
 // Rows are read and written with 16-byte accesses at any alignment (rows of an odd number of columns begin anywhere).
 // Bound by HBM for large calls (8 to 12 operations an element, one of them an exponential), by latency for a few rows.  8192 x 50257 bf16: forward
 // 155 to 165 us (5.0 to 5.3 TB/s), backward 340 us (4.8 TB/s read and written); 2048 rows with the top 5 47 us (4.3); 1004 rows of fp32 at odd addresses

@@ -53,10 +53,15 @@ class _NoGraph:
         pass
 
 
+def untransformed() -> bool:
+    """Whether nothing but a backward may look at what runs now: no forward-mode differentiation, no functorch transform, no tracer.  What these
+    see of a call into the native library is an autograd function in Python; the library's own calls, and nodes on the C++ side, they do not."""
+    return (_graph_state_known and _forward_ad._current_level < 0 and _functorch_stack() is None and _tracing_state() is None)
+
+
 def no_graph() -> bool:
     """Whether nothing records, transforms or traces what runs now."""
-    return not (not _graph_state_known or torch.is_grad_enabled() or _forward_ad._current_level >= 0 or _functorch_stack() is not None
-                or _tracing_state() is not None)
+    return not torch.is_grad_enabled() and untransformed()
 
 
 def apply(function: "type[torch.autograd.Function]", *args):

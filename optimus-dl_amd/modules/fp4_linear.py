@@ -13,7 +13,7 @@ import torch
 import torch.nn as nn
 
 from .. import native
-from .calls import untraced
+from .calls import untraced, untransformed
 
 GROUPS = native.FP4_GROUPS
 E2M1 = (0.0, 0.5, 1.0, 1.5, 2.0, 3.0, 4.0, 6.0)
@@ -47,6 +47,14 @@ def dequantise_fp4(codes: torch.Tensor, scales: torch.Tensor) -> torch.Tensor:
     return (table[nibbles.long()].unflatten(1, (-1, group)) * scales.float().unsqueeze(-1)).flatten(1)
 
 
+class _Fp4LinearFn(torch.autograd.Function):
+    """The product where something else than a backward looks at it: a tracer records it, what would differentiate or batch it is refused."""
+
+    @staticmethod
+    def forward(ctx, x: torch.Tensor, codes: torch.Tensor, scales: torch.Tensor, bias: torch.Tensor | None) -> torch.Tensor:
+        return native.fp4_linear(x, codes, scales, bias)
+
+
 @untraced
 def fp4_linear(x: torch.Tensor, codes: torch.Tensor, scales: torch.Tensor, bias: torch.Tensor | None = None) -> torch.Tensor:
     """``x @ weight.T + bias`` for x [..., in] in bf16 and weights as :func:`quantise_fp4` makes them; bias bf16 or fp32 [out] or None.  Accumulated in
@@ -63,7 +71,8 @@ def fp4_linear(x: torch.Tensor, codes: torch.Tensor, scales: torch.Tensor, bias:
     if not x.is_cuda:
         y = x.float() @ dequantise_fp4(codes, scales).t()
         return (y if bias is None else y + bias.float()).bfloat16()
-    y = native.fp4_linear(x if x.dim() == 2 else x.reshape(-1, x.shape[-1]), codes, scales, bias)
+    product = native.fp4_linear if untransformed() else _Fp4LinearFn.apply
+    y = product(x if x.dim() == 2 else x.reshape(-1, x.shape[-1]), codes, scales, bias)
     return y if x.dim() == 2 else y.reshape(*x.shape[:-1], y.shape[1])
 
 
@@ -83,6 +92,8 @@ class FP4Linear(nn.Module):
 
     @property
     def scales(self) -> torch.Tensor:
+        if torch.jit.is_tracing():                             # (the tracer has no operator for such a view and dies of it)
+            raise RuntimeError("an FP4Linear cannot be traced: trace fp4_linear with its codes and scales")
         return self.scale_bits.view(torch.bfloat16)
 
     @classmethod

@@ -22,7 +22,7 @@ import torch.nn.functional as F
 from .. import native
 from .amp import state as _state
 from .amp.fp8 import FP8Recipe
-from .calls import apply, no_graph, once_differentiable, untraced
+from .calls import apply, no_graph, once_differentiable, untraced, untransformed
 from .fp8_linear import (ROLE_G, ROLE_X, FP8Linear, _converted_input, _Fp8LinearFn, _Fp8LinearGroupFn, _MemberCtx, _product_jobs,
                          _quantise_delayed_for_all, _run_jobs, _wgrad_jobs)
 
@@ -442,7 +442,7 @@ def residual_norm(x: torch.Tensor, h: torch.Tensor, weight: torch.Tensor, eps: f
         return _residual_norm_plain(x, h, weight, eps, post_weight, post_eps, gate, residual_scale, out_dtype)
     if recipe is None and no_graph():
         return native.residual_norm(x, h, weight, eps, post_weight, post_eps, gate, residual_scale, keep=False)[:2]
-    if recipe is None and torch.is_grad_enabled():            # nobody to hand maxima to
+    if recipe is None and untransformed():                    # nobody to hand maxima to
         pair = native.residual_norm_node(x, h, weight, eps, post_weight, post_eps, gate, residual_scale)
         if pair is not None:
             return pair

@@ -14,7 +14,7 @@ import torch
 
 from .. import native
 from .amp import state as _state
-from .calls import no_graph, once_differentiable, untraced
+from .calls import no_graph, once_differentiable, untraced, untransformed
 from .fused import gradient_is_cast
 
 MAX_TOP = native.LOGPROBS_MAX_TOP
@@ -118,7 +118,7 @@ def token_logprobs(logits: torch.Tensor, targets: torch.Tensor, *, n_vocab: int 
         logprobs, entropy, _, top, ids = native.token_logprobs(logits.reshape(-1, columns), targets.reshape(-1), n_vocab, top_k, temperature, ignore_index)
         return TokenLogProbs(logprobs.view(lead), entropy.view(lead), *((None, None) if top is None else (t.view(*lead, top_k) for t in (top, ids))))
     recipe = _state.active_recipe()
-    if not gradient_is_cast(logits, recipe) and torch.is_grad_enabled():     # nobody to hand maxima to
+    if untransformed() and not gradient_is_cast(logits, recipe):             # nobody to hand maxima to
         r = native.token_logprobs_node(logits, targets, n_vocab, top_k, temperature, ignore_index)
         if r is not None:
             return TokenLogProbs(*r)

@@ -26,6 +26,7 @@ constexpr int kMaxParts = 16;                    // (their top k are ranked at o
 constexpr int kFolded = 32;                      // up to so many alternatives 64 folded maxima give a good bound
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 constexpr float kFar = 1e30f;                    // exponents are cut off here: finite times e^-far is 0, infinity times 0 is not
+constexpr float kGone = 256.0f;                  // and here in the backward: 2^-256 is 0 as well, and times a factor of up to 2^119 the exponent stays finite
 
 template <int DT> struct Elem;
 template <> struct Elem<ODL_BF16> { typedef uint16_t T; static constexpr int vecs = 1; };
@@ -496,8 +497,8 @@ __global__ __launch_bounds__(kBwdThreads) void token_logprobs_bwd_kernel(const B
         const float l2 = a.stats[a.rows + row];
         const Exponent x(a.stats[row], a.inv_t * kLog2e);
         const bool nothing = target == a.ignore_index || l2 == -INFINITY;
-        float sum = a.d_logprobs ? a.d_logprobs[row] : 0.0f;
-        const float given = sum * a.inv_t, b = a.d_entropy ? a.d_entropy[row] : 0.0f;
+        const float of_logprob = a.d_logprobs ? a.d_logprobs[row] : 0.0f, b = a.d_entropy ? a.d_entropy[row] : 0.0f, entropy = a.entropy[row];
+        float sum = of_logprob, reach = __builtin_fabsf(of_logprob) + __builtin_fabsf(b) * (kGone + entropy);
         if constexpr (TOP) {
             __syncthreads();                     // the item before has been read
             for (int i = tid; i < kMarks; i += kBwdThreads) marks[i] = 0;
@@ -509,16 +510,22 @@ __global__ __launch_bounds__(kBwdThreads) void token_logprobs_bwd_kernel(const B
                 if (id >= 0) atomicOr(&marks[(id / 8 / 32) % kMarks], 1u << (id / 8 % 32));
             }
             __syncthreads();
-            for (int i = 0; i < a.top_k; ++i) sum += top_d[i];
+            for (int i = 0; i < a.top_k; ++i) {
+                sum += top_d[i];
+                reach += __builtin_fabsf(top_d[i]);
+            }
         }
-        // gradient of an element = p * (k0 + k1 * log2 p)
-        float k0 = -a.inv_t * __fmaf_rn(b, a.entropy[row], sum);
-        const float k1 = -a.inv_t * b * kLn2;
+        // gradient of an element = p * (k0 + k1 * log2 p).  Factors that 1 / T would take out of range (0 times infinity is not 0) are left without
+        // it, and it is multiplied onto the products.
+        const bool late = !(reach * a.inv_t < 1e38f);
+        const float by = late ? 1.0f : a.inv_t, given = of_logprob * by;
+        float k0 = -by * __fmaf_rn(b, entropy, sum);
+        const float k1 = -by * b * kLn2;
         if (target < 0 || target >= a.vocab) k0 = __builtin_nanf("");          // no such token: its log probability is NaN too
         const int t_chunk = target >= 0 && target < a.vocab ? (int)target / 8 : -1;
         auto gradient = [&](float l) {
             const float y = x(l) - l2;
-            return __builtin_amdgcn_exp2f(y) * __fmaf_rn(fmaxf(y, -kFar), k1, k0);
+            return __builtin_amdgcn_exp2f(y) * __fmaf_rn(fmaxf(y, -kGone), k1, k0);
         };
         // gradients of a chunk in which the target or a top alternative may lie, or that ends behind the vocabulary
         auto special = [&](int chunk, float (&f)[8]) {
@@ -528,7 +535,7 @@ __global__ __launch_bounds__(kBwdThreads) void token_logprobs_bwd_kernel(const B
                 if (chunk == t_chunk && col == (int)target) f[e] += given;
                 if constexpr (TOP)
                     for (int i = 0; i < a.top_k; ++i)
-                        if (top_i[i] == col) f[e] = __fmaf_rn(top_d[i], a.inv_t, f[e]);
+                        if (top_i[i] == col) f[e] = __fmaf_rn(top_d[i], by, f[e]);
                 if (col >= a.vocab) f[e] = 0.0f;
             }
         };
@@ -573,6 +580,9 @@ __global__ __launch_bounds__(kBwdThreads) void token_logprobs_bwd_kernel(const B
                     bool look = edge || chunk == t_chunk;
                     if constexpr (TOP) look = look || (marks[(chunk / 32) % kMarks] >> (chunk % 32) & 1u);
                     if (look) special(chunk, f);
+                    if (late)
+#pragma unroll
+                        for (int e = 0; e < 8; ++e) f[e] *= a.inv_t;
                 }
                 store(chunk, f);
             }
@@ -586,7 +596,8 @@ __global__ __launch_bounds__(kBwdThreads) void token_logprobs_bwd_kernel(const B
                 if (col == (int)target && t_chunk >= 0) f += given;
                 if constexpr (TOP)
                     for (int i = 0; i < a.top_k; ++i)
-                        if (top_i[i] == col) f = __fmaf_rn(top_d[i], a.inv_t, f);
+                        if (top_i[i] == col) f = __fmaf_rn(top_d[i], by, f);
+                if (late) f *= a.inv_t;
             }
             if constexpr (DT == ODL_BF16) {
                 const uint32_t w = pack_bf16x2(f, 0.0f);

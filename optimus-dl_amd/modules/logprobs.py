@@ -65,7 +65,8 @@ def _plain(logits, targets, n_vocab, top_k, temperature, ignore_index) -> TokenL
     kept, known = targets != ignore_index, (targets >= 0) & (targets < n_vocab)
     empty = (x == float("-inf")).all(-1)
     dead = ~kept | empty
-    logp = torch.log_softmax(torch.where(dead.unsqueeze(-1), torch.zeros_like(x), x) / temperature, dim=-1)
+    d = torch.where(dead.unsqueeze(-1), torch.zeros_like(x), x)
+    logp = torch.log_softmax((d - d.detach().amax(-1, keepdim=True)) / temperature, dim=-1)      # (the quotient of the logits may be out of range)
     lp = logp.gather(-1, torch.where(known, targets, torch.zeros_like(targets)).unsqueeze(-1)).squeeze(-1)
     p = logp.exp()
     entropy = -(p * torch.where(p == 0, torch.zeros_like(p), logp)).sum(-1)

@@ -719,6 +719,8 @@ py::object token_logprobs_node(const Tensor &logits, const Tensor &targets, i64 
     if (logits.dim() < 1 || logits.numel() == 0 || !dense(targets) || targets.scalar_type() != at::kLong || targets.device() != logits.device()) return none();
     if (!(logits.dim() == 2 ? logits2d(logits) : dense(logits) && src_of(logits) >= 0)) return none();
     if (vocab < 1 || vocab > logits.size(-1) || top_k < 0 || top_k > ODL_FP8_LOGPROBS_MAX_TOP || top_k > vocab) return none();
+    // (what either direction of the kernels refuses is refused in front of the forward, by the wrapper)
+    if (logits.size(-1) > 1 << 24 || logits.numel() / logits.size(-1) >= 1 << 22) return none();
     variable_list out;
     {
         py::gil_scoped_release unlocked;

@@ -1752,7 +1752,7 @@ def token_logprobs(logits: torch.Tensor, targets: torch.Tensor, n_vocab: int, to
     """Log probabilities of targets [rows] from logits [rows, columns >= n_vocab] (bf16 or fp32, rows at any distance), with the entropy of
     each row and its top_k largest logits (``odl_fp8_token_logprobs`` says what ignored, empty and unsound rows answer).
     -> (logprobs, entropy, stats or None, top_logprobs or None, top_ids or None)."""
-    if _here(logits) and 1e-30 <= temperature <= 1e30 and top_k <= n_vocab:
+    if _here(logits) and 1e-30 <= temperature <= 1e30 and top_k <= n_vocab and not (keep_stats and logits.shape[-1] > 1 << 24):
         load()
         r = _host.token_logprobs(logits, targets, n_vocab, top_k, 1.0 / temperature, ignore_index, keep_stats, _stream())
         if r is not None:

@@ -11,13 +11,19 @@ import functools
 import torch
 import torch.autograd.forward_ad as _forward_ad
 
-# Whether a graph compiler, a functorch transform, forward-mode differentiation or a tracer is at work is known to private
-# parts of torch only.  Where a version of torch lacks one of them, every call takes the long way.
+# Whether a graph compiler, a functorch transform, forward-mode differentiation or a tracer is at work, or a hook of every module, is known to
+# private parts of torch only.  Where a version of torch lacks one of them, every call takes the long way.
 try:
     from torch._C._dynamo.eval_frame import get_eval_frame_callback as _compiler_callback
 except ImportError:
     def _compiler_callback():
         return False
+
+try:
+    from torch.nn.modules.module import _has_any_global_hook
+except ImportError:
+    def _has_any_global_hook():
+        return True
 
 _functorch_stack = getattr(getattr(torch._C, "_functorch", None), "peek_interpreter_stack", None)
 _tracing_state = getattr(torch._C, "_get_tracing_state", None)
@@ -62,6 +68,12 @@ def untransformed() -> bool:
 def no_graph() -> bool:
     """Whether nothing records, transforms or traces what runs now."""
     return not torch.is_grad_enabled() and untransformed()
+
+
+def called_as_it_is(module: torch.nn.Module) -> bool:
+    """Whether a call of the module is its class's forward and nothing else: no hook, no forward of its own."""
+    return not (module._forward_hooks or module._forward_pre_hooks or module._backward_hooks or module._backward_pre_hooks
+                or "forward" in module.__dict__ or _has_any_global_hook())
 
 
 def apply(function: "type[torch.autograd.Function]", *args):

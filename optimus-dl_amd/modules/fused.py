@@ -271,6 +271,12 @@ class _Reclassed:
         return _rebuild_fused, (mro[mro.index(_Reclassed) + 1], mro[1]), self.__dict__
 
 
+def plain_class(module: nn.Module) -> type:
+    """The class of a module, the one it had before where its forward was fused in place."""
+    mro = type(module).__mro__
+    return mro[mro.index(_Reclassed) + 1] if _Reclassed in mro else mro[0]
+
+
 class _FusedSwiGLUForward(_Reclassed):
     """Mixed into the class of an MLP with ``w1`` (gate), ``w2`` (up) and ``c_proj`` (down)."""
 

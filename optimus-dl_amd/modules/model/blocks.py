@@ -11,7 +11,8 @@ import torch
 import torch.nn as nn
 import torch.nn.functional as F
 
-from ..fused import residual_norm
+from ..calls import called_as_it_is
+from ..fused import plain_class, residual_norm
 
 
 class RMSNorm(nn.Module):
@@ -24,6 +25,12 @@ class RMSNorm(nn.Module):
         xf = x.float()
         y = xf * torch.rsqrt(xf.pow(2).mean(-1, keepdim=True) + self.eps)
         return (y * self.weight.float()).to(x.dtype)
+
+
+def _is_its_weight(norm: nn.Module) -> bool:
+    """Whether a call of the norm is the norm of its weight and nothing else, which a kernel may do in its place."""
+    cls = plain_class(norm)
+    return issubclass(cls, RMSNorm) and cls.forward is RMSNorm.forward and called_as_it_is(norm)
 
 
 def rope_tables(head_dim: int, seq_len: int, theta: float, device) -> tuple[torch.Tensor, torch.Tensor]:
@@ -111,7 +118,8 @@ class LlamaBlock(nn.Module):
     post_norms, layer_scale, residual_scale (not in the reference): a norm behind each half (``post_ln_1``, ``post_ln_2``), a learned gate for each
     channel of it that begins at ``layer_scale`` (``gate_1``, ``gate_2``) and a factor on the stream that it is added to.  With any of them a
     half ends in ``residual_norm``, one kernel that also is the norm in front of the next half: a model hands the block what the step before
-    made of ``ln_1`` (``z``) and the norm that comes behind it (``next_norm``), and gets the stream and that norm of it."""
+    made of ``ln_1`` (``z``) and the norm that comes behind it (``next_norm``), and gets the stream and that norm of it.  Norms that are more than their
+    weight (hooks, another class) are called."""
 
     def __init__(self, n_embd: int, n_head: int, n_kv_head: int | None, intermediate_size: int | None,
                  use_qk_norm: bool = False, head_dim: int | None = None, eps: float = 1e-5, rope_theta: float = 10000.0,
@@ -127,20 +135,27 @@ class LlamaBlock(nn.Module):
         self.post_ln_1, self.post_ln_2 = (RMSNorm(n_embd, eps) if post_norms else None for _ in range(2))
         self.gate_1, self.gate_2 = (None if layer_scale is None else nn.Parameter(torch.full((n_embd,), float(layer_scale))) for _ in range(2))
 
-    def _step(self, x: torch.Tensor, h: torch.Tensor, post: "RMSNorm | None", gate: torch.Tensor | None, norm: RMSNorm):
-        return residual_norm(x, h, norm.weight, norm.eps, post_weight=None if post is None else post.weight, post_eps=None if post is None else post.eps,
-                             gate=gate, residual_scale=self.residual_scale)
+    def takes_steps(self) -> bool:
+        """Whether what is in front of the block and behind it may hand each other norms of the stream.  Hooks of a block, and whatever stands in its
+        place, have the stream alone: what shards a block's weights while it does not run, say."""
+        return self.stepped and type(self).forward is LlamaBlock.forward and called_as_it_is(self)
+
+    def _end(self, x: torch.Tensor, h: torch.Tensor, post: "RMSNorm | None", gate: torch.Tensor | None, norm: RMSNorm | None):
+        """The stream behind a half that answered h, and the norm in front of the next half of it."""
+        if norm is not None and _is_its_weight(norm) and (post is None or _is_its_weight(post)):
+            return residual_norm(x, h, norm.weight, norm.eps, post_weight=None if post is None else post.weight,
+                                 post_eps=None if post is None else post.eps, gate=gate, residual_scale=self.residual_scale)
+        h = (h if post is None else post(h)).to(x.dtype)
+        x = self.residual_scale * x + (h if gate is None else (gate * h).to(x.dtype))
+        return x, None if norm is None else norm(x)
 
     def forward(self, x: torch.Tensor, z: torch.Tensor | None = None, next_norm: RMSNorm | None = None):
         if not self.stepped:
             x = x + self.attn(self.ln_1(x))
             return x + self.mlp(self.ln_2(x))
-        x, z = self._step(x, self.attn(self.ln_1(x) if z is None else z), self.post_ln_1, self.gate_1, self.ln_2)
-        h = self.mlp(z)
-        if next_norm is not None:
-            return self._step(x, h, self.post_ln_2, self.gate_2, next_norm)
-        h = (h if self.post_ln_2 is None else self.post_ln_2(h)).to(x.dtype)
-        return self.residual_scale * x + (h if self.gate_2 is None else (self.gate_2 * h).to(x.dtype))
+        x, z = self._end(x, self.attn(self.ln_1(x) if z is None else z), self.post_ln_1, self.gate_1, self.ln_2)
+        x, z = self._end(x, self.mlp(z), self.post_ln_2, self.gate_2, next_norm)
+        return x if next_norm is None else (x, z)
 
 
 class Qwen3Block(LlamaBlock):

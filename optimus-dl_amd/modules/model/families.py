@@ -81,7 +81,7 @@ class _DecoderLM(nn.Module):
     def forward(self, input_ids: torch.Tensor, **kwargs) -> dict:
         x, z = self.embed(input_ids), None
         blocks, ln_f = self.transformer.h, self.transformer.ln_f
-        stepped = [getattr(block, "stepped", False) for block in blocks]      # (a wrapper around a block has the stream alone)
+        stepped = [isinstance(block, LlamaBlock) and block.takes_steps() for block in blocks]      # (a wrapper around a block has the stream alone)
         for i, block in enumerate(blocks):
             if not stepped[i]:
                 x, z = block(x), None

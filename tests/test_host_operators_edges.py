@@ -21,3 +21,123 @@ def test_plain_log_probabilities_of_logits_of_any_size(dtype, temperature):
     assert r.top_ids.tolist() == [[0, 1], [0, 1], [0, 2]]
     (r.logprobs.sum() + r.entropy.sum()).backward()
     assert live.grad.isfinite().all() and not live.grad[1:].any()
+
+
+def stepped_llama():
+    from optimus_dl_amd.modules.model import Llama, LlamaConfig
+
+    torch.manual_seed(0)
+    return Llama(LlamaConfig(vocab_size=50, n_layer=3, n_embd=32, n_head=2, n_kv_head=2, intermediate_size=64, post_norms=True, layer_scale=0.5,
+                             residual_scale=0.9))
+
+
+IDS = torch.arange(14).reshape(2, 7)
+# the same fp32 operations, some in another order: a few roundings of values near one
+CLOSE = 64 * 2.0 ** -24
+
+
+def close(model, want, ids=IDS):
+    got = model(ids)["logits"]
+    torch.testing.assert_close(got, want, rtol=0, atol=CLOSE * float(want.abs().max()))
+
+
+@pytest.mark.parametrize("kind", ["forward", "forward_pre", "full_backward", "full_backward_pre", "global"])
+@pytest.mark.parametrize("name", ["transformer.h.0.ln_1", "transformer.h.1.ln_1", "transformer.h.1.ln_2", "transformer.h.2.post_ln_1", "transformer.h.0.post_ln_2",
+                                  "transformer.ln_f", "transformer.h.1"])
+def test_hooks_of_stepped_models_run(name, kind):
+    model = stepped_llama()
+    want, module, seen = model(IDS)["logits"].detach(), model.get_submodule(name), []
+    note = lambda m, *args: seen.append(args) if m is module else None
+    if kind == "global":
+        handle = torch.nn.modules.module.register_module_forward_hook(note)
+    else:
+        handle = getattr(module, f"register_{kind}_hook")(note)
+    try:
+        close(model, want)
+        model(IDS)["logits"].sum().backward()
+    finally:
+        handle.remove()
+    assert len(seen) == (1 if "backward" in kind else 2)
+    if kind in ("forward", "global"):
+        (inputs, output) = seen[0]
+        assert output.shape == (2, 7, 32) == inputs[0].shape and len(inputs) == 1      # the stream alone, as in a model of plain blocks
+
+
+def test_what_a_hook_answers_takes_effect():
+    model = stepped_llama()
+    x = model.embed(IDS)
+    for block in model.transformer.h:
+        x = 2 * block(x)
+    want = model.lm_head(model.transformer.ln_f(x)).detach()
+    for block in model.transformer.h:
+        block.register_forward_hook(lambda m, args, out: 2 * out)
+    close(model, want)
+
+
+def test_modules_in_the_place_of_norms_and_blocks_are_called():
+    from optimus_dl_amd.modules.model.blocks import LlamaBlock, RMSNorm
+
+    class Shifted(RMSNorm):
+        def forward(self, x):
+            return super().forward(x) + 1.0
+
+    class Doubled(LlamaBlock):
+        def forward(self, x):
+            return 2 * super().forward(x)
+
+    class Forwards(torch.nn.Module):                       # a wrapper that passes attributes on
+        def __init__(self, inner):
+            super().__init__()
+            self.inner = inner
+
+        def __getattr__(self, name):
+            try:
+                return super().__getattr__(name)
+            except AttributeError:
+                return getattr(self.inner, name)
+
+        def forward(self, x):
+            return self.inner(x)
+
+    def reference(model, after=1.0):
+        x = model.embed(IDS)
+        for block in model.transformer.h:
+            x = block(x)
+        return model.lm_head(model.transformer.ln_f(x)).detach()
+
+    for change in (lambda m: setattr(m.transformer, "ln_f", Shifted(32)), lambda m: setattr(m.transformer.h[1], "ln_1", Shifted(32)),
+                   lambda m: setattr(m.transformer.h[1], "ln_2", torch.nn.LayerNorm(32)), lambda m: setattr(m.transformer.h[0], "post_ln_2", Shifted(32)),
+                   lambda m: setattr(m.transformer.h[1], "__class__", Doubled), lambda m: setattr(m.transformer.h[2], "forward", lambda x: x + 1.0),
+                   lambda m: m.transformer.h.__setitem__(1, Forwards(m.transformer.h[1]))):
+        model = stepped_llama()
+        plain = reference(model)
+        change(model)
+        want = reference(model)
+        close(model, want)
+        if not isinstance(model.transformer.h[1], Forwards):
+            assert (want - plain).abs().max() > 0.01
+
+
+def test_blocks_sharded_in_place(tmp_path):
+    """A block that is sharded by itself has its weights whole while it runs, and nobody else then."""
+    import torch.distributed as dist
+    from torch.distributed.device_mesh import init_device_mesh
+    from torch.distributed.fsdp import fully_shard
+
+    model = stepped_llama()
+    want = model(IDS)["logits"].detach()
+    model(IDS)["logits"].square().sum().backward()
+    grads = {n: p.grad for n, p in model.named_parameters()}
+    dist.init_process_group("gloo", init_method=f"file://{tmp_path}/store", rank=0, world_size=1)
+    try:
+        mesh = init_device_mesh("cpu", (1,))
+        model = stepped_llama()
+        for block in model.transformer.h:
+            fully_shard(block, mesh=mesh)
+        fully_shard(model, mesh=mesh)
+        close(model, want)
+        model(IDS)["logits"].square().sum().backward()
+        for n, p in model.named_parameters():
+            torch.testing.assert_close(p.grad.full_tensor(), grads[n], rtol=1e-4, atol=1e-5 * float(grads[n].abs().max()))
+    finally:
+        dist.destroy_process_group()

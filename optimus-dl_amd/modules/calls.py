@@ -70,10 +70,15 @@ def no_graph() -> bool:
     return not torch.is_grad_enabled() and untransformed()
 
 
+def has_hooks(module: torch.nn.Module) -> bool:
+    """Whether a call of the module, by itself, is more than its class's forward: a hook, or a forward of its own."""
+    return bool(module._forward_hooks or module._forward_pre_hooks or module._backward_hooks or module._backward_pre_hooks
+                or "forward" in module.__dict__)
+
+
 def called_as_it_is(module: torch.nn.Module) -> bool:
-    """Whether a call of the module is its class's forward and nothing else: no hook, no forward of its own."""
-    return not (module._forward_hooks or module._forward_pre_hooks or module._backward_hooks or module._backward_pre_hooks
-                or "forward" in module.__dict__ or _has_any_global_hook())
+    """Whether a call of the module is its class's forward and nothing else."""
+    return not (has_hooks(module) or _has_any_global_hook())
 
 
 def apply(function: "type[torch.autograd.Function]", *args):

@@ -13,6 +13,7 @@ from typing import Any
 
 import torch.nn as nn
 
+from ..calls import has_hooks
 from ..fp4_linear import FP4Linear
 from . import register_model_transform
 from .base import BaseModelTransform
@@ -30,7 +31,8 @@ class Fp4LinearTransformConfig(ModelTransformConfig):
 
 @register_model_transform("fp4_linear", Fp4LinearTransformConfig)
 class Fp4LinearTransform(BaseModelTransform):
-    """nn.Linear -> FP4Linear over the whole module tree; Linears whose inputs are no whole groups stay as they are."""
+    """nn.Linear -> FP4Linear over the whole module tree; Linears whose inputs are no whole groups, and Linears with hooks (which may look at
+    the weight, or make it), stay as they are."""
 
     def apply(self, model: nn.Module, **kwargs: Any) -> nn.Module:
         self.replaced, self.left = 0, []
@@ -43,7 +45,7 @@ class Fp4LinearTransform(BaseModelTransform):
             for name, child in list(parent._modules.items()):
                 if type(child) is not nn.Linear or name in self.cfg.skip:
                     continue
-                if child.in_features % self.cfg.group_size:
+                if child.in_features % self.cfg.group_size or has_hooks(child):
                     self.left.append(f"{prefix}.{name}" if prefix else name)
                     continue
                 if id(child) not in made:

@@ -141,3 +141,33 @@ def test_blocks_sharded_in_place(tmp_path):
             torch.testing.assert_close(p.grad.full_tensor(), grads[n], rtol=1e-4, atol=1e-5 * float(grads[n].abs().max()))
     finally:
         dist.destroy_process_group()
+
+
+def fake_codes(monkeypatch):
+    """4-bit weights without a GPU."""
+    from optimus_dl_amd.modules import fp4_linear as F4
+
+    def quantise(w, group):
+        if w.dtype not in (torch.float32, torch.bfloat16):
+            raise F4.native.NativeError(f"weights of {w.dtype}")
+        return torch.zeros(w.shape[0], w.shape[1] // 2, dtype=torch.uint8), torch.zeros(w.shape[0], w.shape[1] // group, dtype=torch.bfloat16)
+
+    monkeypatch.setattr(F4.native, "fp4_quantise", quantise)
+    return F4.FP4Linear
+
+
+def test_linears_with_hooks_keep_them(monkeypatch):
+    from optimus_dl_amd.modules.model_transforms import build_model_transform
+
+    FP4Linear = fake_codes(monkeypatch)
+    net = torch.nn.Sequential(*(torch.nn.Linear(64, 64) for _ in range(5)))
+    seen = []
+    net[1].register_forward_hook(lambda m, args, out: seen.append(m))
+    net[2].register_forward_pre_hook(lambda m, args: seen.append(m))
+    net[3].forward = lambda x: seen.append(net[3]) or x
+    t = build_model_transform({"_name": "fp4_linear", "group_size": 32})
+    t.apply(net)
+    assert [isinstance(m, FP4Linear) for m in net] == [True, False, False, False, True] and t.left == ["1", "2", "3"] and t.replaced == 2
+    with torch.no_grad():
+        net(torch.zeros(1, 64))
+    assert seen == [net[1], net[2], net[3]]

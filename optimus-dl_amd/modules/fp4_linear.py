@@ -33,10 +33,16 @@ def _check_weight(codes: torch.Tensor, scales: torch.Tensor) -> int:
 def quantise_fp4(weight: torch.Tensor, group: int = 32) -> tuple[torch.Tensor, torch.Tensor]:
     """Weights [out, in], bf16 or fp32, finite, as codes and scales: a group's scale is the bf16 nearest to its largest magnitude / 6, a code the
     E2M1 nearest to weight / scale, ties to the even code.  On the GPU.  -> (codes uint8 [out, in / 2], scales bf16 [out, in / group])."""
+    check_castable(weight, group)
+    return native.fp4_quantise(weight.detach(), group)
+
+
+def check_castable(weight: torch.Tensor, group: int) -> None:
+    """Refuses what :func:`quantise_fp4` refuses."""
     w = weight.detach()
+    native.fp4_quantise(w[:0], group)                          # its device, type and shape: none of its rows are as all of them
     if not bool(torch.isfinite(w).all()):
         raise ValueError("quantise_fp4: the weights are not finite")
-    return native.fp4_quantise(w, group)
 
 
 def dequantise_fp4(codes: torch.Tensor, scales: torch.Tensor) -> torch.Tensor:

@@ -14,7 +14,7 @@ from typing import Any
 import torch.nn as nn
 
 from ..calls import has_hooks
-from ..fp4_linear import FP4Linear
+from ..fp4_linear import FP4Linear, check_castable
 from . import register_model_transform
 from .base import BaseModelTransform
 from .config import ModelTransformConfig
@@ -40,17 +40,22 @@ class Fp4LinearTransform(BaseModelTransform):
             return model
         if type(model) is nn.Linear:
             raise ValueError("the fp4_linear transform replaces the Linears inside of a model; this is one: FP4Linear.from_linear")
-        made: dict[int, FP4Linear] = {}                 # a module that is used in two places stays one
+        places: list[tuple[nn.Module, str, nn.Linear]] = []
         for prefix, parent in list(model.named_modules()):
-            for name, child in list(parent._modules.items()):
+            for name, child in parent._modules.items():
                 if type(child) is not nn.Linear or name in self.cfg.skip:
                     continue
                 if child.in_features % self.cfg.group_size or has_hooks(child):
                     self.left.append(f"{prefix}.{name}" if prefix else name)
                     continue
-                if id(child) not in made:
-                    made[id(child)] = FP4Linear.from_linear(child, self.cfg.group_size)
-                    self.replaced += 1
-                setattr(parent, name, made[id(child)])
+                places.append((parent, name, child))
+        for child in {id(child): child for *_, child in places}.values():      # a model is refused before anything of it is replaced
+            check_castable(child.weight, self.cfg.group_size)
+        made: dict[int, FP4Linear] = {}                 # a module that is used in two places stays one
+        for parent, name, child in places:
+            if id(child) not in made:
+                made[id(child)] = FP4Linear.from_linear(child, self.cfg.group_size)
+                self.replaced += 1
+            setattr(parent, name, made[id(child)])
         logger.info("Linears with 4-bit weights: %d%s", self.replaced, f"; left as they are: {', '.join(self.left)}" if self.left else "")
         return model

@@ -171,3 +171,34 @@ def test_linears_with_hooks_keep_them(monkeypatch):
     with torch.no_grad():
         net(torch.zeros(1, 64))
     assert seen == [net[1], net[2], net[3]]
+
+
+@pytest.mark.parametrize("bad", ["not finite", "type", "both"])
+def test_a_model_that_is_refused_is_left_whole(monkeypatch, bad):
+    from optimus_dl_amd import native
+    from optimus_dl_amd.modules.model_transforms import build_model_transform
+
+    fake_codes(monkeypatch)
+    net = torch.nn.Sequential(torch.nn.Linear(64, 64), torch.nn.Sequential(torch.nn.Linear(64, 64), torch.nn.Linear(64, 64)), torch.nn.Linear(64, 64))
+    if bad == "not finite":
+        net[1][1].weight.data[3, 5] = float("inf")
+    elif bad == "type":
+        net[1][1].half()
+    else:
+        net[1][1].weight.data[0, 0] = float("nan")
+        net[1][0].half()
+    before = list(net.modules())
+    with pytest.raises((ValueError, native.NativeError)):
+        build_model_transform({"_name": "fp4_linear"}).apply(net)
+    assert all(a is b for a, b in zip(before, net.modules())) and len(before) == len(list(net.modules()))
+
+
+def test_a_model_on_the_cpu_is_refused_whole():
+    from optimus_dl_amd import native
+    from optimus_dl_amd.modules.model_transforms import build_model_transform
+
+    net = torch.nn.Sequential(torch.nn.Linear(64, 64), torch.nn.Linear(64, 64))
+    if native.is_built():
+        with pytest.raises(native.NativeError, match="GPU"):
+            build_model_transform({"_name": "fp4_linear"}).apply(net)
+    assert type(net[0]) is type(net[1]) is torch.nn.Linear

@@ -202,3 +202,17 @@ def test_a_model_on_the_cpu_is_refused_whole():
         with pytest.raises(native.NativeError, match="GPU"):
             build_model_transform({"_name": "fp4_linear"}).apply(net)
     assert type(net[0]) is type(net[1]) is torch.nn.Linear
+
+
+def test_which_products_of_a_few_rows_are_cut_into_runs():
+    """What the comparisons of few rows of a long K rely on: one launch without partial results up to some 41 000 inputs of many columns, runs beyond."""
+    from optimus_dl_amd import native
+
+    if not native.is_built():
+        pytest.skip("library not built")
+    runs = native.load().odl_fp8_fp4_linear_runs
+    for rows, n, k, group in ((16, 1000, 5152, 32), (16, 4100, 5248, 128), (11, 4100, 7200, 32), (16, 100, 4128, 32), (7, 1030, 8256, 64), (4, 1030, 14464, 128),
+                              (1, 3001, 32800, 32), (1, 4099, 41024, 64)):
+        assert runs(rows, n, k, group) == 0, (rows, n, k, group)
+    for rows, n, k, group in ((1, 40, 65568, 32), (2, 300, 131392, 64), (5, 40, 262528, 128)):
+        assert runs(rows, n, k, group) > 8, (rows, n, k, group)

@@ -9,8 +9,8 @@
 // there times the group's scale, in fp32, onto the sums: nothing is rounded before the end.
 //
 // Two kernels.  Thin, for a few rows: a block has 16 columns, its waves share K in chunks of 256 and are added up through LDS in wave order;
-// 29 MB of codes for one token in 9.4 us (3.2 TB/s).  Wide, for more: a block has 128 columns and 16 to 128 rows, its waves share x in LDS, K is cut
-// into runs where there are few blocks.
+// 29 MB of codes for one token in 9.4 us (3.2 TB/s).  Wide, for more: a block has 128 columns and 16 to 128 rows, or 256 and 128, its waves share x in
+// LDS, K is cut into runs where there are few blocks.
 // In both a lane reads 16 bytes of a row of codes: 32 weights in order, of one group of 32 at most.  What the MFMA multiplies in one
 // instruction is 8 weights of each of the four lanes of a column, so for groups shorter than 128 the four lanes exchange their dwords first (four
 // swaps of half and quarter waves for 32 weights); with groups of 128 the order of k inside a group does not matter.
@@ -77,8 +77,9 @@ __host__ __device__ inline Fp4Tile fp4_tile(int K) {
 }
 
 // Up to 16 * MT rows a block.  Rows and columns past the end are read as the last ones are and not stored, so that nothing is masked on
-// the way; the K behind the last whole chunk is.  Codes of the next DEPTH chunks are on their way, x (from memory) of the next half chunk.
-template <int G, int MT, int NT, int WAVES, int DEPTH, bool XLDS>
+// the way; the K behind the last whole chunk is.  A wave asks for the codes of its next chunk behind the products of one, and for x (from memory) of the
+// next half chunk in front of those of one.
+template <int G, int MT, int WAVES, bool XLDS>
 __global__ __launch_bounds__(WAVES *kWave) void fp4_thin_kernel(const Fp4Args a) {
     constexpr int kGroups = kChunk / G;          // groups of a chunk
     constexpr int kSteps = G / 32;               // instructions of a group
@@ -86,31 +87,26 @@ __global__ __launch_bounds__(WAVES *kWave) void fp4_thin_kernel(const Fp4Args a)
     const int lane = threadIdx.x % kWave, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave), col = lane % 16, quarter = lane / 16;
     const int K = (int)a.K;
     const Fp4Tile tile = fp4_tile<G>(K);
-    const int64_t n0 = (int64_t)blockIdx.x * (16 * NT), m0 = (int64_t)blockIdx.y * (16 * MT);
+    const int64_t n0 = (int64_t)blockIdx.x * 16, m0 = (int64_t)blockIdx.y * (16 * MT);
     const uint8_t *cbase = a.codes + n0 * (a.K / 2);
     const uint16_t *sbase = a.scales + n0 * tile.groups, *xbase = a.x + m0 * a.ldx;
-    uint16_t *slds = reinterpret_cast<uint16_t *>(lds), *xlds = slds + 16 * NT * tile.pitch;
-    uint32_t coff[NT], xoff[MT];
-#pragma unroll
-    for (int j = 0; j < NT; ++j) coff[j] = (uint32_t)(min(n0 + 16 * j + col, a.N - 1) - n0) * (uint32_t)(K / 2) + quarter * 16;
+    uint16_t *slds = reinterpret_cast<uint16_t *>(lds), *xlds = slds + 16 * tile.pitch;
+    const uint32_t coff = (uint32_t)(min(n0 + col, a.N - 1) - n0) * (uint32_t)(K / 2) + quarter * 16;
+    uint32_t xoff[MT];
 #pragma unroll
     for (int i = 0; i < MT; ++i) {
         const uint32_t m = (uint32_t)(min(m0 + 16 * i + col, a.M - 1) - m0);
         xoff[i] = m * (uint32_t)(XLDS ? tile.xpitch : a.ldx) + quarter * (G < 128 ? 8 : 32);
     }
 
-    f32x4 acc[MT][NT];
+    f32x4 acc[MT];
 #pragma unroll
-    for (int i = 0; i < MT; ++i)
-#pragma unroll
-        for (int j = 0; j < NT; ++j) acc[i][j] = f32x4{0, 0, 0, 0};
+    for (int i = 0; i < MT; ++i) acc[i] = f32x4{0, 0, 0, 0};
 
-    u32x4 codes[DEPTH][NT][2], xv[XLDS ? 1 : 2][MT][4];
-    auto fetch = [&](int slot, int ch) {
+    u32x4 codes[2], xv[XLDS ? 1 : 2][MT][4];
+    auto fetch = [&](int ch) {
 #pragma unroll
-        for (int j = 0; j < NT; ++j)
-#pragma unroll
-            for (int t = 0; t < 2; ++t) codes[slot][j][t] = *reinterpret_cast<const u32x4 *>(cbase + (uint32_t)(ch * (kChunk / 2) + t * 64) + coff[j]);
+        for (int t = 0; t < 2; ++t) codes[t] = *reinterpret_cast<const u32x4 *>(cbase + (uint32_t)(ch * (kChunk / 2) + t * 64) + coff);
     };
     auto fetch_x = [&](int t, int ch) {
 #pragma unroll
@@ -122,39 +118,35 @@ __global__ __launch_bounds__(WAVES *kWave) void fp4_thin_kernel(const Fp4Args a)
                 else xv[t][i][s] = *reinterpret_cast<const u32x4 *>(xbase + k + xoff[i]);
             }
     };
-    auto multiply = [&](int slot, int t, int ch) {
+    auto multiply = [&](int t, int ch) {
+        const u32x4 w = G < 128 ? exchange(codes[t]) : codes[t];
+        const uint16_t *sc = slds + col * tile.pitch + ch * kGroups;
+        uint32_t pair = 0;
+        f32x4 p[MT];
 #pragma unroll
-        for (int j = 0; j < NT; ++j) {
-            const u32x4 w = G < 128 ? exchange(codes[slot][j][t]) : codes[slot][j][t];
-            const uint16_t *sc = slds + (16 * j + col) * tile.pitch + ch * kGroups;
-            uint32_t pair = 0;
-            f32x4 p[MT];
+        for (int s = 0; s < 4; ++s) {
+            const bf16x8 b = widen_codes(w[s]);
+            const int g = (t * 4 + s) / kSteps;
+            if (s == 0 || (s % kSteps == 0 && g % 2 == 0)) pair = *reinterpret_cast<const uint32_t *>(sc + g / 2 * 2);
+            const float scale = g % 2 ? bf16_hi(pair) : bf16_lo(pair);
 #pragma unroll
-            for (int s = 0; s < 4; ++s) {
-                const bf16x8 b = widen_codes(w[s]);
-                const int g = (t * 4 + s) / kSteps;
-                if (s == 0 || (s % kSteps == 0 && g % 2 == 0)) pair = *reinterpret_cast<const uint32_t *>(sc + g / 2 * 2);
-                const float scale = g % 2 ? bf16_hi(pair) : bf16_lo(pair);
+            for (int i = 0; i < MT; ++i) {
+                const f32x4 from = s % kSteps == 0 ? f32x4{0, 0, 0, 0} : p[i];
+                p[i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, xv[XLDS ? 0 : t][i][s]), b, from, 0, 0, 0);
+                if (s % kSteps == kSteps - 1)
 #pragma unroll
-                for (int i = 0; i < MT; ++i) {
-                    const f32x4 from = s % kSteps == 0 ? f32x4{0, 0, 0, 0} : p[i];
-                    p[i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, xv[XLDS ? 0 : t][i][s]), b, from, 0, 0, 0);
-                    if (s % kSteps == kSteps - 1)
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) acc[i][j][e] = __fmaf_rn(scale, p[i][e], acc[i][j][e]);
-                }
+                    for (int e = 0; e < 4; ++e) acc[i][e] = __fmaf_rn(scale, p[i][e], acc[i][e]);
             }
         }
     };
     const int first = wave, last = first < tile.whole ? first + (tile.whole - 1 - first) / WAVES * WAVES : 0;
     if (first < tile.whole) {
-#pragma unroll
-        for (int d = 0; d < DEPTH; ++d) fetch(d, min(first + d * WAVES, last));          // (chunks behind the last are that one, and not used)
+        fetch(first);
         if constexpr (!XLDS) fetch_x(0, first);
     }
     {                                            // rows of scales, eight at a time; groups and columns past the end are zero
-        const int per = (tile.pitch - 2) / 8, rows = 16 * NT, have = tile.groups;
-        for (int i = threadIdx.x; i < rows * per; i += WAVES * kWave) {
+        const int per = (tile.pitch - 2) / 8, have = tile.groups;
+        for (int i = threadIdx.x; i < 16 * per; i += WAVES * kWave) {
             const int r = i / per, g = i % per * 8;
             u32x4 v = {0, 0, 0, 0};
             const uint16_t *from = sbase + (uint32_t)(r * tile.groups + g);
@@ -178,28 +170,21 @@ __global__ __launch_bounds__(WAVES *kWave) void fp4_thin_kernel(const Fp4Args a)
         }
     }
     __syncthreads();
-    for (int ch0 = first; ch0 < tile.whole; ch0 += DEPTH * WAVES) {
-#pragma unroll
-        for (int d = 0; d < DEPTH; ++d) {
-            const int ch = ch0 + d * WAVES;
-            if (ch >= tile.whole) break;
-            if constexpr (XLDS) fetch_x(0, ch);
-            else fetch_x(1, ch);
-            multiply(d, 0, ch);
-            if constexpr (XLDS) fetch_x(1, ch);
-            else fetch_x(0, min(ch + WAVES, last));
-            multiply(d, 1, ch);
-            fetch(d, min(ch + DEPTH * WAVES, last));
-        }
+    for (int ch = first; ch < tile.whole; ch += WAVES) {
+        if constexpr (XLDS) fetch_x(0, ch);
+        else fetch_x(1, ch);
+        multiply(0, ch);
+        if constexpr (XLDS) fetch_x(1, ch);
+        else fetch_x(0, min(ch + WAVES, last));
+        multiply(1, ch);
+        fetch(min(ch + WAVES, last));            // (behind the last chunk that one, and not used)
     }
     if (K % kChunk && wave == tile.whole % WAVES) {      // the rest of K, shorter than a chunk
 #pragma unroll
-        for (int j = 0; j < NT; ++j)
-#pragma unroll
-            for (int t = 0; t < 2; ++t) {
-                const int k = tile.whole * kChunk + t * 128 + quarter * 32;
-                codes[0][j][t] = k < K ? *reinterpret_cast<const u32x4 *>(cbase + (uint32_t)(tile.whole * (kChunk / 2) + t * 64) + coff[j]) : u32x4{0, 0, 0, 0};
-            }
+        for (int t = 0; t < 2; ++t) {
+            const int k = tile.whole * kChunk + t * 128 + quarter * 32;
+            codes[t] = k < K ? *reinterpret_cast<const u32x4 *>(cbase + (uint32_t)(tile.whole * (kChunk / 2) + t * 64) + coff) : u32x4{0, 0, 0, 0};
+        }
 #pragma unroll
         for (int t = 0; t < 2; ++t) {
             if constexpr (XLDS) {
@@ -213,22 +198,20 @@ __global__ __launch_bounds__(WAVES *kWave) void fp4_thin_kernel(const Fp4Args a)
                         xv[t][i][s] = from < K ? *reinterpret_cast<const u32x4 *>(xbase + (uint32_t)k + xoff[i]) : u32x4{0, 0, 0, 0};
                     }
             }
-            multiply(0, t, tile.whole);
+            multiply(t, tile.whole);
         }
     }
     __syncthreads();                             // what was staged has been read
     f32x4 *part = reinterpret_cast<f32x4 *>(lds);
 #pragma unroll
-    for (int i = 0; i < MT; ++i)
-#pragma unroll
-        for (int j = 0; j < NT; ++j) part[(wave * MT * NT + i * NT + j) * kWave + lane] = acc[i][j];
+    for (int i = 0; i < MT; ++i) part[(wave * MT + i) * kWave + lane] = acc[i];
     __syncthreads();
-    for (int o = threadIdx.x; o < MT * NT * kWave; o += WAVES * kWave) {
+    for (int o = threadIdx.x; o < MT * kWave; o += WAVES * kWave) {
         const int t = o / kWave, l = o % kWave;
         f32x4 s = part[o];
 #pragma unroll
-        for (int w = 1; w < WAVES; ++w) s += part[w * MT * NT * kWave + o];
-        const int64_t n = n0 + 16 * (t % NT) + l % 16, m = m0 + 16 * (t / NT) + l / 16 * 4;
+        for (int w = 1; w < WAVES; ++w) s += part[w * MT * kWave + o];
+        const int64_t n = n0 + l % 16, m = m0 + 16 * t + l / 16 * 4;
         if (n >= a.N) continue;
         const float b = bias_of(a, n);
 #pragma unroll
@@ -237,12 +220,12 @@ __global__ __launch_bounds__(WAVES *kWave) void fp4_thin_kernel(const Fp4Args a)
     }
 }
 
-template <int G, int MT, int NT, int WAVES, int DEPTH, bool XLDS>
+template <int G, int MT, int WAVES, bool XLDS>
 void launch_thin(const Fp4Args &a, hipStream_t stream) {
     const Fp4Tile t = fp4_tile<G>((int)a.K);
     const int64_t rows = a.M < 16 * MT ? a.M : 16 * MT;
-    const int64_t staged = 2 * (16 * NT * (int64_t)t.pitch + (XLDS ? rows * t.xpitch : 0)), sums = (int64_t)WAVES * MT * NT * kWave * 16;
-    hipLaunchKernelGGL((fp4_thin_kernel<G, MT, NT, WAVES, DEPTH, XLDS>), dim3((unsigned)((a.N + 16 * NT - 1) / (16 * NT)), (unsigned)((a.M + 16 * MT - 1) / (16 * MT))),
+    const int64_t staged = 2 * (16 * (int64_t)t.pitch + (XLDS ? rows * t.xpitch : 0)), sums = (int64_t)WAVES * MT * kWave * 16;
+    hipLaunchKernelGGL((fp4_thin_kernel<G, MT, WAVES, XLDS>), dim3((unsigned)((a.N + 15) / 16), (unsigned)((a.M + 16 * MT - 1) / (16 * MT))),
                        dim3(WAVES * kWave), (size_t)(staged > sums ? staged : sums), stream, a);
 }
 
@@ -545,10 +528,10 @@ void launch_linear(const Fp4Args &a, const Fp4Plan how, hipStream_t stream) {
         const Fp4Tile t = fp4_tile<G>((int)a.K);
         const bool lds = x_in_lds<G>(a.M, a.K), deep = t.whole >= 32;
         // long rows: 16 waves share them (14336 -> 4096 11.5 -> 10.5, 4096 -> 14336 no faster)
-        if (lds && deep) launch_thin<G, 1, 1, 16, 1, true>(a, stream);
-        else if (lds) launch_thin<G, 1, 1, 8, 1, true>(a, stream);
-        else if (a.M <= 16) launch_thin<G, 1, 1, 8, 1, false>(a, stream);
-        else launch_thin<G, 2, 1, 4, 1, false>(a, stream);
+        if (lds && deep) launch_thin<G, 1, 16, true>(a, stream);
+        else if (lds) launch_thin<G, 1, 8, true>(a, stream);
+        else if (a.M <= 16) launch_thin<G, 1, 8, false>(a, stream);
+        else launch_thin<G, 2, 4, false>(a, stream);
         return;
     }
     int runs = how.runs;

@@ -96,13 +96,13 @@ template <int CTRL>
 __device__ __forceinline__ float max_dpp(float v) {
     return fmaxf(v, bits_to_float((uint32_t)__builtin_amdgcn_update_dpp(0, (int)float_to_bits(v), CTRL, 0xf, 0xf, false)));
 }
-// maxima over groups of 4, 8, 16 or 64 lanes
+// maxima over groups of 4, 8 or 64 lanes
 template <int LANES>
 __device__ __forceinline__ float group_max(float v) {
     v = max_dpp<0x4E>(max_dpp<0xB1>(v));
     if constexpr (LANES >= 8) v = max_dpp<0x141>(v);
-    if constexpr (LANES >= 16) v = max_dpp<0x140>(v);
     if constexpr (LANES >= 64) {
+        v = max_dpp<0x140>(v);
         const auto r = __builtin_amdgcn_permlane16_swap(float_to_bits(v), float_to_bits(v), false, false);
         v = fmaxf(bits_to_float(r[0]), bits_to_float(r[1]));
         const auto q = __builtin_amdgcn_permlane32_swap(float_to_bits(v), float_to_bits(v), false, false);

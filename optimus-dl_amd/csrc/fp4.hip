@@ -9,7 +9,7 @@
 // there times the group's scale, in fp32, onto the sums: nothing is rounded before the end.
 //
 // Two kernels.  Thin, for a few rows: a block has 16 columns, its waves share K in chunks of 256 and are added up through LDS in wave order;
-// 29 MB of codes for one token in 9.4 us (3.2 TB/s).  Wide, for more: a block has 128 columns and 16 to 128 rows, or 256 and 128, its waves share x in
+// 29 MB of codes for one token in 9.1 us (3.3 TB/s).  Wide, for more: a block has 128 columns and 16 to 128 rows, or 256 and 128, its waves share x in
 // LDS, K is cut into runs where there are few blocks.
 // In both a lane reads 16 bytes of a row of codes: 32 weights in order, of one group of 32 at most.  What the MFMA multiplies in one
 // instruction is 8 weights of each of the four lanes of a column, so for groups shorter than 128 the four lanes exchange their dwords first (four
@@ -231,11 +231,13 @@ void launch_thin(const Fp4Args &a, hipStream_t stream) {
 
 // Up to 16 * MT rows, many of them: x goes through LDS in phases of kPhase k, double-buffered, and the sixteen waves of a block share it, 16 columns each of
 // 16 * kSlots and one of SHARES parts of a phase.  Codes, scales and x of the next phase are on their way while the waves multiply.
-// Eight waves of 32 columns, which read x from LDS half as often, are slower: 32 rows 14336 -> 4096 18.0 us (15.9), 8192 -> 28672 38.7 (33.1), 120 rows 95 (90).
-// x through registers on its way to LDS: 120 rows 8192 -> 28672 94.8 (85.8).  128 rows by 256 columns bring x to LDS half as often as 128 by 128: 512
-// rows 4096 -> 14336 77 (90); for 120 rows of 8192 -> 28672 they are too few blocks, 129 (90), unless K is cut in two, 79 (81).
-// 120 rows 8192 -> 28672, groups of 64, 79 us: 710 TFLOP/s, a large bf16 product 1235.  Bound by the products (half of them left out: 24 us of 94 in a row of
-// twenty; scaling 11, bringing x to LDS 7, reading it there nothing); 32 rows 14336 -> 4096, 15.3 us, by the latency of two phases and of the join (4 us).
+// Forms that were tried on the way, us, each beside this one as it was then: eight waves of 32 columns, which read x from LDS half as often, 32 rows
+// 14336 -> 4096 18.0 (15.9), 8192 -> 28672 38.7 (33.1), 120 rows of that 95 (90); x through registers on its way to LDS, 120 rows 8192 -> 28672 94.8 (85.8).
+// 128 rows by 256 columns bring x to LDS half as often as 128 by 128, 512 rows 4096 -> 14336 77 (90); for 120 rows of 8192 -> 28672 they are too few
+// blocks, 129 (90), unless K is cut in two, 79 (81).
+// As it is: 120 rows 8192 -> 28672, groups of 64, 79 us a call with its join: 710 TFLOP/s, a large bf16 product 1235.  Twenty calls in a row take 77 each, without half
+// of the products 62, without three of four scalings 71, without bringing x to LDS 70; 512 rows 4096 -> 14336 72, 46, 72 and 70: bound by the products.  32 rows
+// 14336 -> 4096 15.3, 15.3, 14.5 and 14.2: by the latency of two phases, the second asked for behind the first one's arrival, and of the join.
 template <int G, int MT, int SHARES>
 struct Fp4Wide {
     static constexpr int kWaves = 16, kThreads = kWaves * kWave, kSlots = kWaves / SHARES, kColumns = 16 * kSlots;

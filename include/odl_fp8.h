@@ -46,7 +46,7 @@ enum odl_status {
 };
 
 /* ABI version of this header; bumped when a signature changes or an entry point is added. */
-#define ODL_FP8_ABI_VERSION 31
+#define ODL_FP8_ABI_VERSION 32
 int odl_fp8_abi_version(void);
 
 /*
@@ -764,6 +764,60 @@ int odl_fp8_fp4_linear(const void *x, int64_t ldx, const uint8_t *codes, const v
  */
 int odl_fp8_fp4_quantise(const void *w, int src_dtype, int64_t N, int64_t K, int group, uint8_t *codes, void *scales,
                          odl_stream_t stream);
+
+/*
+ * A cache of keys and values in pages, and the new tokens of a step (no counterpart in the reference, which runs whole sequences).
+ * Cache: keys and values [pages, kv_heads, page_size, head_dim], bf16 or OCP E4M3 codes (e4m3 != 0) that stand for code * scale[kv_head]; strides of
+ * page, head and token in elements (head_dim is dense), multiples of 16 bytes as the addresses are; page_size a power of two, head_dim a multiple of
+ * 16 up to 128.
+ * Batch: sequence s has its new tokens in rows offsets[s] to offsets[s + 1] of what is computed and, with them, lengths[s] tokens in the cache: row
+ * offsets[s] + j is at position lengths[s] - n + j, and position p in slot p % page_size of page table[s * table_stride + p / page_size].
+ * offsets rise from 0; rows from offsets[seqs] on belong to nobody.  A number in the table that is no page of the cache holds nothing: what would
+ * go there is not written, and takes no part in attention.  Positions outside of [0, width * page_size) likewise.  Entries behind a sequence's
+ * last page are not read.
+ */
+typedef struct odl_fp8_paged_cache {
+    void *keys, *values;
+    const float *key_scale, *value_scale;      /* [kv_heads] where e4m3, else NULL */
+    int64_t pages, kv_heads, page_size, head_dim;
+    int64_t key_strides[3], value_strides[3];
+    int32_t e4m3, reserved;
+} odl_fp8_paged_cache;
+typedef struct odl_fp8_paged_batch {
+    const int32_t *table, *offsets, *lengths;
+    int64_t seqs, rows, width, table_stride;
+} odl_fp8_paged_batch;
+
+/*
+ * New queries and keys normed and rotated, keys and values put into the cache.
+ *   n = x * r * w, r = 1 / sqrt(mean(x^2) + eps)   where q_weight / k_weight are not NULL (fp32 [head_dim]; r rounded to fp32 from 64 bits)
+ *   (a, b) -> (a * cos - b * sin, a * sin + b * cos)  for pairs of the first 2 * half elements of a head: (2 i, 2 i + 1) where interleaved, else
+ *             (i, half + i), angles of the token's position; half 0: none.  cos, sin fp32 [positions, half], positions >= width * page_size.
+ * Every step rounds to fp32, in this order, without fused multiply-adds; what is stored rounds once, to bf16 or, divided by the scale and clamped to
+ * +-448, to E4M3.
+ * q [rows, heads, head_dim], k and v [rows, kv_heads, head_dim] bf16, strides of row and head in elements, multiples of 8; addresses multiples
+ * of 16 bytes.  q_out bf16 [rows, heads, head_dim], zero in rows that belong to nobody.  half a multiple of 4 where interleaved, else of 8.
+ * No two rows may have the same slot.
+ */
+int odl_fp8_append_kv(const void *q, const int64_t *q_strides, const void *k, const int64_t *k_strides, const void *v, const int64_t *v_strides,
+                      int64_t heads, const odl_fp8_paged_cache *cache, const odl_fp8_paged_batch *batch, const float *cos, const float *sin,
+                      int64_t positions, int64_t half, int interleaved, const float *q_weight, const float *k_weight, double eps, void *q_out,
+                      odl_stream_t stream);
+
+/*
+ * Attention of the new tokens over the cache, which holds them.  Row at position p, of a head whose keys are those of head / (heads / kv_heads):
+ *   s_i = scale * q . key_i,  softcap > 0: s_i = softcap * tanh(s_i / softcap),  for max(0, p - window + 1) <= i <= p  (window 0: from 0)
+ *   out = sum_i e^(s_i - m) value_i / sum_i e^(s_i - m)
+ * Products of bf16 (E4M3 codes are widened exactly) with fp32 sums; weights round to bf16 in front of the second product.  Sums and maxima fp32.
+ * Keys and values that a row does not see do not reach it, NaN and infinities included.  A row that sees nothing, and rows that belong to
+ * nobody, answer 0.  q [rows, heads, head_dim] bf16 with strides as above; out bf16 [rows, heads, head_dim].
+ * most_new: the most new tokens of a sequence where the caller knows it, else `rows`: chooses kernels, results do not depend on its truth.
+ * The same call answers the same bits.  workspace: odl_fp8_paged_attention_workspace floats, contents irrelevant, of this call alone while it runs.
+ */
+int64_t odl_fp8_paged_attention_workspace(int64_t heads, int64_t most_new, const odl_fp8_paged_cache *cache, const odl_fp8_paged_batch *batch);
+int odl_fp8_paged_attention(const void *q, const int64_t *q_strides, int64_t heads, int64_t most_new, const odl_fp8_paged_cache *cache,
+                            const odl_fp8_paged_batch *batch, float scale, int64_t window, float softcap, void *out, float *workspace,
+                            int64_t workspace_floats, odl_stream_t stream);
 
 #ifdef __cplusplus
 }

@@ -23,7 +23,7 @@ LIB_PATH = os.path.join(HERE, LIB_NAME)
 HOST_NAME = "_host"
 HOST_PATH = os.path.join(HERE, HOST_NAME + ".so")
 SOURCES = ["api.hip", "quant.hip", "gemm_fp8.hip", "gemm_tiled.hip", "gemm_thin.hip", "gemm_deep.hip", "gemm_deep_many.hip", "gemm_pipe.hip", "gemm_stream.hip", "fused.hip", "mx.hip",
-           "residual_norm.hip", "logprobs.hip", "fp4.hip"]
+           "residual_norm.hip", "logprobs.hip", "fp4.hip", "append_kv.hip", "paged_attention.hip"]
 
 # Per-source additions.  The compiler-scheduled tiled GEMMs: left to its own choice the compiler computes in vector
 # registers but parks the accumulators in the accumulation registers between K steps, 64 copies out and 64 back per
@@ -34,6 +34,7 @@ EXTRA_FLAGS = {
     "gemm_tiled.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"],
     "gemm_thin.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"],
     "mx.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"],
+    "paged_attention.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"],
 }
 
 # -ffp-contract=off : the epilogues promise "multiply, round, add, round" (no FMA fusion)

@@ -1,0 +1,812 @@
+// Attention of a step's new tokens over a paged cache that holds them.  For a row (token, head) at position p, with the keys and values of its group:
+//   s_i = scale * q . k_i  (softcap * tanh(s_i / softcap)),  out = sum_i 2^(c s_i - m) v_i / sum_i 2^(c s_i - m),  c = log2 e, i the keys that the row sees
+// in one pass over the keys, with a running maximum m and sum.  Heads of a group share keys, so what a matrix instruction takes as its other operand
+// is the rows (token, head of the group) of one key head: S^T = K Q^T and O^T = V^T P^T by V_MFMA_F32_32X32X16_BF16.  In the result of the first a
+// lane holds one row's scores for 16 of 32 keys: sums and maxima of a row are a lane's own but for one exchange with lane ^ 32, and those registers are
+// the second operand of the second product as they are, when V^T's keys are taken in the same order (ds_read_b64_tr_b16 fetches them so).
+//
+// Two kernels.  Few rows a key head (32 at most: single tokens, drafts): the cache is read once and that bounds it; the four waves of a block take
+// every fourth tile of 32 keys, each on its own, and are joined in LDS.  Many (prompts, chunks): MFMA and the exponentials bound it; eight waves of 32
+// rows share tiles of 64 keys.  In both tiles go to LDS without passing registers, one ahead, and where there are fewer tiles of rows than
+// compute units the keys are cut into splits, whose sums a third kernel joins in order.  Every block works out from the lengths which part is its own
+// (`find`): lengths never pass the host.
+#include "paged.h"
+
+#pragma clang fp contract(off)
+
+namespace odl {
+namespace {
+
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+typedef __attribute__((address_space(3))) uint8_t lds_u8;
+
+constexpr int kFewRows = 32, kFewKeys = 32, kFewWaves = 4;
+constexpr int kManyRows = 256, kManyKeys = 64, kManyWaves = 8;
+constexpr int kFewTarget = 512, kManyTarget = 256;             // blocks that splits are made for
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kSlack = 8.0f;                                 // how far, in powers of two, a running maximum may lag behind
+
+// What lanes read that have no key: a row of zeros.
+__device__ const uint32_t g_zeros[64] __attribute__((aligned(256))) = {};
+
+struct Attend {
+    Paged p;
+    const uint16_t *q;
+    int64_t q_row, q_head;
+    int heads, group, window;                                  // group: heads of a key head; window: INT_MAX for none
+    int least_rows, most_rows;                                 // rows a key head of the sequences that this launch is for
+    float scale, softcap;
+    uint16_t *out;
+    float *partial;                                            // [slots][rows of a tile][D] sums, then [slots][rows of a tile][2] maxima and sums
+    int64_t slots;
+};
+
+// ---------------------------------------------------------------------------------------------------------------- whose work a block does
+// A sequence's share: `tiles` of rows, each cut into `splits` of its keys.
+struct Share {
+    Run run;
+    int length;                                                // tokens in the cache, within the table's reach
+    uint32_t tiles, units, splits;
+};
+
+template <int ROWS, int KEYS>
+__device__ __forceinline__ Share share_of(const Attend &a, int s) {
+    Share h = {{0, 0}, 0, 0, 0, 0};
+    if (s >= a.p.seqs) return h;
+    h.run = run_of(a.p, s);
+    h.length = a.p.lengths[s];
+    const int rows = h.run.n * a.group, held = min(max(h.length, 0), a.p.reach);
+    if (rows <= a.least_rows || rows > a.most_rows) return h;
+    h.tiles = (uint32_t)(rows + ROWS - 1) / ROWS;
+    const int64_t seen = min((int64_t)held, (int64_t)a.window + ROWS / a.group + KEYS);
+    h.units = max(1u, (uint32_t)((seen + KEYS - 1) / KEYS));
+    return h;
+}
+
+template <class T>
+__device__ __forceinline__ T wave_add(T v) {
+#pragma unroll
+    for (int off = kWave / 2; off > 0; off >>= 1) v += __shfl_xor(v, off, kWave);
+    return v;
+}
+
+struct Item {
+    Run run;
+    int seq, length, tile, split, splits;
+    int64_t slot;                                              // of its first split, among those of tiles that are cut
+};
+
+// The index-th part (CUT: the index-th tile that is cut) of the batch, in the order sequence, tile, split, the tiles with most keys first.  Tiles are cut so
+// that a split has at least 1 / target of all the work: no more than `target` splits begin anew, whatever the lengths are, so that grids
+// and workspaces are known on the host.
+template <int ROWS, int KEYS, bool CUT>
+__device__ bool find(const Attend &a, uint32_t index, uint32_t target, Item &it) {
+    const int lane = threadIdx.x % kWave;
+    Share mine = share_of<ROWS, KEYS>(a, lane);
+    int64_t work = (int64_t)mine.tiles * mine.units;
+    for (int s0 = kWave; s0 < a.p.seqs; s0 += kWave) {
+        const Share h = share_of<ROWS, KEYS>(a, s0 + lane);
+        work += (int64_t)h.tiles * h.units;
+    }
+    const int64_t per64 = (wave_add(work) * a.p.kv_heads + target - 1) / target;
+    const uint32_t per = (uint32_t)min(max(per64, (int64_t)1), (int64_t)INT32_MAX);
+    uint32_t parts0 = 0;
+    int64_t slots0 = 0;
+    for (int s0 = 0; s0 < a.p.seqs; s0 += kWave) {
+        if (s0) mine = share_of<ROWS, KEYS>(a, s0 + lane);
+        mine.splits = (mine.units + per - 1) / per;
+        const uint32_t all = mine.tiles * mine.splits;
+        const uint32_t slots = mine.splits > 1 ? all : 0, parts = CUT ? (mine.splits > 1 ? mine.tiles : 0) : all;
+        uint32_t sum_parts = parts, sum_slots = slots;
+#pragma unroll
+        for (int off = 1; off < kWave; off <<= 1) {
+            const uint32_t u = __shfl_up(sum_parts, off, kWave), v = __shfl_up(sum_slots, off, kWave);
+            if (lane >= off) { sum_parts += u; sum_slots += v; }
+        }
+        const uint32_t first = parts0 + sum_parts - parts;
+        const uint64_t hit = __ballot(parts && index >= first && index - first < parts);
+        if (hit) {
+            const int from = __builtin_ctzll(hit);
+            auto of = [&](uint32_t v) { return (uint32_t)__builtin_amdgcn_readlane((int)v, from); };
+            const uint32_t rest = index - of(first), splits = of(mine.splits), tile = CUT ? rest : rest / splits;
+            it.run = {(int)of(mine.run.first), (int)of(mine.run.n)};
+            it.seq = s0 + from;
+            it.length = (int)of(mine.length);
+            it.splits = (int)splits;
+            it.split = CUT ? 0 : (int)(rest - tile * splits);
+            it.tile = (int)(of(mine.tiles) - 1 - tile);
+            it.slot = slots0 + of(sum_slots - slots) + (int64_t)tile * splits;
+            return true;
+        }
+        parts0 += __builtin_amdgcn_readlane((int)sum_parts, kWave - 1);
+        slots0 += (uint32_t)__builtin_amdgcn_readlane((int)sum_slots, kWave - 1);
+    }
+    return false;
+}
+
+// Rows that belong to nobody answer 0; the blocks of a launch share them.
+__device__ void clear_rest(const Attend &a, int64_t block, int64_t blocks, int threads) {
+    const int used = a.p.seqs ? min(max(a.p.offsets[a.p.seqs], 0), a.p.rows) : 0;
+    const int64_t row = (int64_t)a.heads * a.p.dim / 8, end = (int64_t)a.p.rows * row;
+    for (int64_t i = used * row + block * threads + threadIdx.x; i < end; i += blocks * threads) reinterpret_cast<u32x4 *>(a.out)[i] = u32x4{0, 0, 0, 0};
+}
+
+// ---------------------------------------------------------------------------------------------------------------- tiles in LDS
+// A tile is [keys][D] bf16, its rows cut into pieces of 16 bytes that stand at piece ^ swizzle(row): for K so that the 16 rows that are read at a time,
+// one piece each, lie in different banks; for V so that four rows, four pieces each, do.
+template <int D>
+__device__ __forceinline__ int swizzle_k(int row) { return D == 128 ? row & 15 : (row >> 1) & 7; }
+template <int D>
+__device__ __forceinline__ int swizzle_v(int row) { return D == 128 ? (row & 3) << 2 : ((row >> 1) & 1) << 2; }
+
+// 16 bytes of each lane's to LDS at `to` + 16 * lane, without passing registers
+__device__ __forceinline__ void to_lds(uint32_t to, const uint8_t *from) {
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(to), "v"(from) : "memory");
+}
+__device__ __forceinline__ void all_loads_done() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
+
+__device__ __forceinline__ const uint8_t *shuffled(const uint8_t *p, int lane) {
+    const uint64_t v = reinterpret_cast<uint64_t>(p);
+    const uint32_t lo = __shfl((int)(uint32_t)v, lane, kWave), hi = __shfl((int)(uint32_t)(v >> 32), lane, kWave);
+    return reinterpret_cast<const uint8_t *>((uint64_t)hi << 32 | lo);
+}
+
+// sixteen codes -> sixteen bf16 (exact: E4M3 has 3 bits of mantissa)
+__device__ __forceinline__ void widen16(u32x4 codes, u32x4 &lo, u32x4 &hi) {
+    uint32_t o[8];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const auto a = __builtin_amdgcn_cvt_pk_f32_fp8((int)codes[i], false), b = __builtin_amdgcn_cvt_pk_f32_fp8((int)codes[i], true);
+        o[2 * i] = __builtin_amdgcn_perm(float_to_bits(a[1]), float_to_bits(a[0]), 0x07060302u);
+        o[2 * i + 1] = __builtin_amdgcn_perm(float_to_bits(b[1]), float_to_bits(b[0]), 0x07060302u);
+    }
+    lo = u32x4{o[0], o[1], o[2], o[3]};
+    hi = u32x4{o[4], o[5], o[6], o[7]};
+}
+
+// Where the token at a position lies; rows of zeros where there is none.
+struct Place {
+    const uint8_t *key, *value;
+    bool held;
+};
+__device__ __forceinline__ Place place_of(const Paged &p, int page, int pos, int head) {
+    const uint8_t *zeros = reinterpret_cast<const uint8_t *>(g_zeros);
+    Place w = {zeros, zeros, page >= 0 && page < p.pages};
+    if (w.held) {
+        const int at = pos & ((1 << p.shift) - 1);
+        w.key = p.keys + page * p.k_page + head * p.k_head + at * p.k_tok;
+        w.value = p.values + page * p.v_page + head * p.v_head + at * p.v_tok;
+    }
+    return w;
+}
+
+// ---------------------------------------------------------------------------------------------------------------- the attention of 32 rows
+enum Mode { kPlain, kMasked, kCareful };
+
+// exchange with lane ^ 32
+__device__ __forceinline__ float other_half(float v) {
+    const auto r = __builtin_amdgcn_permlane32_swap(float_to_bits(v), float_to_bits(v), false, false);
+    return bits_to_float(threadIdx.x % kWave < 32 ? r[1] : r[0]);
+}
+
+// A lane's 32 rows by 16 of 32 keys (element i is key 8 (i / 4) + 4 (lane / 32) + i % 4), NB such blocks of keys a tile.
+template <int D, int NB>
+struct Rows32 {
+    bf16x8 q[D / 16];
+    f32x16 o[D / 32];
+    float m, l;                                                // running maximum in powers of two, the sum of this lane's keys against it
+
+    __device__ __forceinline__ void start() {
+        m = -INFINITY;
+        l = 0.0f;
+#pragma unroll
+        for (int d = 0; d < D / 32; ++d) o[d] = f32x16{};
+    }
+
+    // rows first_row + lane % 32 of a tile's: q of a token's head, zeros where there is no such row
+    __device__ __forceinline__ void load_q(const Attend &a, const Run &run, int row, int kv_head) {
+        const int lane = threadIdx.x % kWave, token = row / a.group, head = kv_head * a.group + row % a.group;
+        const bool live = token < run.n;
+        const uint16_t *from = a.q + (int64_t)(run.first + (live ? token : 0)) * a.q_row + head * a.q_head;
+#pragma unroll
+        for (int s = 0; s < D / 16; ++s) {
+            const int c = 16 * s + 8 * (lane / 32);
+            u32x4 v = {0, 0, 0, 0};
+            if (live && c < a.p.dim) v = *reinterpret_cast<const u32x4 *>(from + c);
+            q[s] = __builtin_bit_cast(bf16x8, v);
+        }
+    }
+
+    // One tile of keys and values at LDS addresses kt and vt.  c: powers of two a unit of a score; where softcap > 0 scores are capped first and in powers
+    // of two then.  kMasked: of seen, bit e says whether the lane's row sees key e + 4 (lane / 32), for e % 8 < 4.  kCareful: infinities and NaN among the
+    // values reach only the rows that see them, row_sees says which (0 * NaN would reach all).
+    template <int MODE>
+    __device__ __forceinline__ void tile(uint32_t kt, uint32_t vt, float c, float cap_in, float cap_out, uint64_t seen, uint64_t row_sees) {
+        constexpr int kPitch = 2 * D;
+        const int lane = threadIdx.x % kWave, h = lane / 32, r = lane % 32;
+        f32x16 s[NB];
+        {
+            const uint32_t at = kt + r * kPitch + 16 * (h ^ swizzle_k<D>(r));
+#pragma unroll
+            for (int b = 0; b < NB; ++b) s[b] = f32x16{};
+#pragma unroll
+            for (int d = 0; d < D / 16; ++d) {
+                const lds_u8 *from = (const lds_u8 *)(uintptr_t)(at ^ (32 * d));
+#pragma unroll
+                for (int b = 0; b < NB; ++b)
+                    s[b] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(*(const __attribute__((address_space(3))) bf16x8 *)(from + b * 32 * kPitch), q[d], s[b], 0, 0, 0);
+            }
+        }
+        if (cap_in > 0.0f) {                                   // tanh(x) = 1 - 2 / (e^2x + 1)
+#pragma unroll
+            for (int b = 0; b < NB; ++b)
+#pragma unroll
+                for (int i = 0; i < 16; ++i)
+                    s[b][i] = cap_out * (1.0f - 2.0f * __builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(s[b][i] * cap_in) + 1.0f));
+        }
+        if constexpr (MODE != kPlain) {
+#pragma unroll
+            for (int b = 0; b < NB; ++b)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) s[b][i] = (seen >> (32 * b + 8 * (i / 4) + i % 4)) & 1 ? s[b][i] : -INFINITY;
+        }
+        float top = -INFINITY;
+#pragma unroll
+        for (int b = 0; b < NB; ++b)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) top = fmaxf(top, s[b][i]);
+        top = fmaxf(top, other_half(top)) * c;
+        // The maximum may lag by 2^8: weights are then up to 2^8, in types that hold that as well, and most tiles leave sums as they are.
+        if (__any(top > m + kSlack)) {
+            const float to = fmaxf(m, top), by = to == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(m - to);
+            m = to;
+            l *= by;
+#pragma unroll
+            for (int d = 0; d < D / 32; ++d)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) o[d][i] *= by;
+        }
+        const float against = m == -INFINITY ? 0.0f : m;
+#pragma unroll
+        for (int b = 0; b < NB; ++b)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+                s[b][i] = __builtin_amdgcn_exp2f(__fmaf_rn(s[b][i], c, -against));
+                l += s[b][i];
+            }
+        bf16x8 w[2 * NB];
+#pragma unroll
+        for (int k = 0; k < 2 * NB; ++k) {
+            uint32_t v[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) v[i] = pack_bf16x2(s[k / 2][8 * (k % 2) + 2 * i], s[k / 2][8 * (k % 2) + 2 * i + 1]);
+            w[k] = __builtin_bit_cast(bf16x8, u32x4{v[0], v[1], v[2], v[3]});
+        }
+        const uint32_t at = value_address(vt);
+#pragma unroll
+        for (int k = 0; k < 2 * NB; ++k)
+#pragma unroll
+            for (int d = 0; d < D / 32; ++d) {
+                u32x4 v = values(at, d, k);
+                if constexpr (MODE == kCareful) {
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        if ((v[i] & 0x7f80u) == 0x7f80u) v[i] &= 0xffff0000u;
+                        if ((v[i] & 0x7f800000u) == 0x7f800000u) v[i] &= 0xffffu;
+                    }
+                }
+                o[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, v), w[k], o[d], 0, 0, 0);
+            }
+        if constexpr (MODE == kCareful) add_odd(vt, row_sees);
+    }
+
+    // Lane i of 16 reads 4 of 16 columns of key i / 4, and gets 4 keys of column i.
+    static __device__ __forceinline__ uint32_t value_address(uint32_t vt) {
+        const int lane = threadIdx.x % kWave, i = lane % 16, key = 4 * (lane / 32) + i / 4;
+        const int piece = (2 * ((lane / 16) % 2) + (i % 4) / 2) ^ swizzle_v<D>(key);
+        return vt + key * 2 * D + piece * 16 + (i % 2) * 8;
+    }
+    // V^T of columns 32 d to 32 d + 31, keys 16 k + {0 to 3, 8 to 11} + 4 (lane / 32)
+    static __device__ __forceinline__ u32x4 values(uint32_t at, int d, int k) {
+        const uint32_t from = (at ^ (64 * d)) + k * 16 * 2 * D;
+        const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4 *)(uintptr_t)from);
+        const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4 *)(uintptr_t)(from + 8 * 2 * D));
+        const u32x2 a = __builtin_bit_cast(u32x2, lo), b = __builtin_bit_cast(u32x2, hi);
+        return u32x4{a[0], a[1], b[0], b[1]};
+    }
+
+    // Infinities and NaN among a tile's values, for the rows that see them: weights are above 0, so they come through as they are.
+    __device__ __forceinline__ void add_odd(uint32_t vt, uint64_t row_sees) {
+        const int h = threadIdx.x % kWave / 32;
+#pragma unroll 1
+        for (int key = 0; key < 32 * NB; ++key) {
+#pragma unroll
+            for (int d = 0; d < D / 32; ++d)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {    // columns 32 d + 8 i + 4 h to + 3
+                    const u32x2 v = *(const __attribute__((address_space(3))) u32x2 *)(uintptr_t)(vt + key * 2 * D + 16 * ((4 * d + i) ^ swizzle_v<D>(key)) + 8 * h);
+#pragma unroll
+                    for (int z = 0; z < 4; ++z) {
+                        const float f = z % 2 ? bf16_hi(v[z / 2]) : bf16_lo(v[z / 2]);
+                        if ((row_sees >> key & 1) && !(__builtin_fabsf(f) < INFINITY)) o[d][4 * i + z] += f;
+                    }
+                }
+        }
+    }
+
+    // Whether a sum of this lane's rows is not finite.
+    __device__ __forceinline__ bool odd() const {
+        float most = 0.0f;
+#pragma unroll
+        for (int d = 0; d < D / 32; ++d)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) most = fmaxf(most, o[d][i] != o[d][i] ? INFINITY : __builtin_fabsf(o[d][i]));
+        return !(most < INFINITY);
+    }
+};
+
+// Which keys of the tile from `base` on a row at position pos sees.  held: which there are.
+__device__ __forceinline__ uint64_t seen_of(int pos, int base, int window, uint64_t held) {
+    const int last = pos - base;
+    const int64_t first = (int64_t)last - window + 1;
+    uint64_t seen = last < 0 ? 0 : last >= 63 ? ~0ull : (2ull << last) - 1;
+    if (first > 0) seen = first > 63 ? 0 : seen & (~0ull << first);
+    return seen & held;
+}
+
+// The keys that a tile of rows sees, in units of KEYS: from `first` (aligned) to `end`.
+struct Range {
+    int first, end;
+};
+template <int ROWS, int KEYS>
+__device__ __forceinline__ Range range_of(const Attend &a, const Item &it) {
+    const int tokens = it.run.n, t0 = it.tile * ROWS / a.group, t1 = min((it.tile * ROWS + ROWS - 1) / a.group, tokens - 1);
+    const int pos0 = it.length - tokens + t0, pos1 = it.length - tokens + t1;
+    const int held = min(max(it.length, 0), a.p.reach);
+    const int64_t from = (int64_t)pos0 - a.window + 1;
+    Range r;
+    r.first = from > 0 ? (int)(from / KEYS * KEYS) : 0;
+    r.end = min(held, pos1 + 1);
+    const int units = max(0, (r.end - r.first + KEYS - 1) / KEYS), each = (units + it.splits - 1) / it.splits;
+    const int first = r.first + min(it.split * each, units) * KEYS;
+    r.end = min(r.end, r.first + min((it.split + 1) * each, units) * KEYS);
+    r.first = first;
+    return r;
+}
+
+__device__ __forceinline__ void store_row(const Attend &a, const Run &run, int row, int kv_head, int d, f32x4 v) {
+    const int token = row / a.group, head = kv_head * a.group + row % a.group;
+    *reinterpret_cast<u32x2 *>(a.out + ((int64_t)(run.first + token) * a.heads + head) * a.p.dim + d) = u32x2{pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3])};
+}
+
+// What a sum against maximum m counts where `top` is the maximum of all.  A part that sees nothing has maximum -inf and sums 0, one that sees only NaN
+// -inf and NaN.
+__device__ __forceinline__ float weight_of(float m, float top) { return m == top ? 1.0f : __builtin_amdgcn_exp2f(m - top); }
+// By what a row's sums are multiplied in the end; a row that sees nothing answers 0.
+__device__ __forceinline__ float quotient_of(const Attend &a, int kv_head, float l) {
+    return l == 0.0f ? 0.0f : (a.p.value_scale ? a.p.value_scale[kv_head] : 1.0f) / l;
+}
+
+struct Caps {
+    float c, in, out;
+};
+__device__ __forceinline__ Caps caps_of(const Attend &a, int kv_head) {
+    const float scale = a.p.key_scale ? a.scale * a.p.key_scale[kv_head] : a.scale;
+    if (a.softcap > 0.0f) return {1.0f, 2.0f * kLog2e * scale / a.softcap, a.softcap * kLog2e};
+    return {scale * kLog2e, 0.0f, 0.0f};
+}
+
+// ---------------------------------------------------------------------------------------------------------------- keys and values on their way to LDS
+// A wave's KEYS keys of a tile, from their places (lane i has that of key i) to LDS tiles at kt and vt, which begin with the wave's first key `first`.
+// bf16 goes there directly; codes pass registers, where they are widened.
+template <int D, int KEYS, bool E4M3>
+struct Stager;
+
+template <int D, int KEYS>
+struct Stager<D, KEYS, false> {
+    static constexpr int kPieces = D / 8, kEach = kWave / kPieces, kLoads = KEYS / kEach;      // pieces of a row, rows a load
+    static __device__ __forceinline__ void send(const Place &place, int first, int dim, uint32_t kt, uint32_t vt) {
+        const int lane = threadIdx.x % kWave, piece = lane % kPieces;
+        const uint8_t *zeros = reinterpret_cast<const uint8_t *>(g_zeros);
+#pragma unroll
+        for (int i = 0; i < kLoads; ++i) {
+            const int row = first + i * kEach + lane / kPieces, ck = piece ^ swizzle_k<D>(row), cv = piece ^ swizzle_v<D>(row);
+            const uint8_t *k = shuffled(place.key, row), *v = shuffled(place.value, row);
+            to_lds(kt + (first + i * kEach) * 2 * D, (ck * 8 < dim ? k : zeros) + ck * 16);
+            to_lds(vt + (first + i * kEach) * 2 * D, (cv * 8 < dim ? v : zeros) + cv * 16);
+        }
+    }
+};
+
+template <int D, int KEYS>
+struct Stager<D, KEYS, true> {
+    static constexpr int kPieces = D / 16, kEach = kWave / kPieces < KEYS ? kWave / kPieces : KEYS, kLoads = KEYS / kEach;
+    u32x4 k[kLoads], v[kLoads];
+    __device__ __forceinline__ void fetch(const Place &place, int first, int dim) {
+        const int lane = threadIdx.x % kWave, piece = lane % kPieces;
+        const uint8_t *zeros = reinterpret_cast<const uint8_t *>(g_zeros);
+#pragma unroll
+        for (int i = 0; i < kLoads; ++i) {
+            const int row = first + i * kEach + lane / kPieces % kEach;
+            const uint8_t *pk = shuffled(place.key, row), *pv = shuffled(place.value, row);
+            k[i] = *reinterpret_cast<const u32x4 *>((piece * 16 < dim ? pk : zeros) + piece * 16);
+            v[i] = *reinterpret_cast<const u32x4 *>((piece * 16 < dim ? pv : zeros) + piece * 16);
+        }
+    }
+    __device__ __forceinline__ void put(int first, uint32_t kt, uint32_t vt) const {
+        const int lane = threadIdx.x % kWave, piece = lane % kPieces;
+        if (lane / kPieces >= kEach) return;
+#pragma unroll
+        for (int i = 0; i < kLoads; ++i) {
+            const int row = first + i * kEach + lane / kPieces;
+            auto write = [&](u32x4 codes, uint32_t tile, int swizzle) {
+                u32x4 lo, hi;
+                widen16(codes, lo, hi);
+                *(__attribute__((address_space(3))) u32x4 *)(uintptr_t)(tile + row * 2 * D + 16 * ((2 * piece) ^ swizzle)) = lo;
+                *(__attribute__((address_space(3))) u32x4 *)(uintptr_t)(tile + row * 2 * D + 16 * ((2 * piece + 1) ^ swizzle)) = hi;
+            };
+            write(k[i], kt, swizzle_k<D>(row));
+            write(v[i], vt, swizzle_v<D>(row));
+        }
+    }
+};
+
+__device__ __forceinline__ uint32_t lds_base(uint8_t *lds) { return (uint32_t)(uintptr_t)(lds_u8 *)lds; }
+
+// ---------------------------------------------------------------------------------------------------------------- few rows
+constexpr int few_lds(int D, bool e4m3) {
+    const int tiles = kFewWaves * (e4m3 ? 1 : 2) * 2 * kFewKeys * 2 * D, joined = kFewWaves * 32 * (D + 4) * 4 + kFewWaves * 32 * 8;
+    return tiles > joined ? tiles : joined;
+}
+
+template <int D, bool E4M3>
+__global__ __launch_bounds__(kFewWaves *kWave) void attend_few_kernel(Attend a) {
+    extern __shared__ __attribute__((aligned(1024))) uint8_t lds[];
+    constexpr int kTile = kFewKeys * 2 * D, kStages = E4M3 ? 1 : 2, kStep = kFewKeys * kFewWaves;
+    const int head = blockIdx.x % a.p.kv_heads, lane = threadIdx.x % kWave;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+    clear_rest(a, blockIdx.x, gridDim.x, kFewWaves * kWave);
+    Item it;
+    if (!find<kFewRows, kStep, false>(a, blockIdx.x / a.p.kv_heads, kFewTarget, it)) return;
+    const Range range = range_of<kFewRows, kStep>(a, it);
+    const int rows = it.run.n * a.group, row0 = it.tile * kFewRows, row = row0 + lane % 32, before = it.length - it.run.n;
+    const int pos = before + row / a.group, pos0 = before + row0 / a.group, pos1 = before + min(row0 + kFewRows - 1, rows - 1) / a.group;
+    const Caps caps = caps_of(a, head);
+    const int32_t *table = a.p.table + it.seq * a.p.table_stride;
+    Rows32<D, 1> w;
+    w.load_q(a, it.run, row, head);
+
+    const int h4 = 4 * (lane / 32);
+    bool careful = false;
+    const uint32_t mine = lds_base(lds) + wave * kStages * 2 * kTile;
+    auto page_of = [&](int base) { return base + lane % 32 < range.end ? table[(base + lane % 32) >> a.p.shift] : -1; };
+    auto attend = [&](int base, uint32_t held, uint32_t kt) {
+        const uint64_t seen = seen_of(pos, base, a.window, held);
+        if (careful) w.template tile<kCareful>(kt, kt + kTile, caps.c, caps.in, caps.out, seen >> h4, seen);
+        else if (held != ~0u || base + kFewKeys - 1 > pos0 || base <= pos1 - a.window)
+            w.template tile<kMasked>(kt, kt + kTile, caps.c, caps.in, caps.out, seen >> h4, seen);
+        else
+            w.template tile<kPlain>(kt, kt + kTile, caps.c, caps.in, caps.out, 0, 0);
+    };
+    for (;;) {                                   // once, or again where the sums say that there are infinities or NaN
+        w.start();
+        int base = range.first + wave * kFewKeys;
+        int page = page_of(base);
+        if constexpr (E4M3) {
+            Stager<D, kFewKeys, true> stager;
+            Place place = place_of(a.p, page, base + lane % 32, head);
+            uint32_t held = (uint32_t)__ballot(place.held);
+            stager.fetch(place, 0, a.p.dim);
+            page = page_of(base + kStep);
+            for (; base < range.end; base += kStep) {
+                const uint32_t now = held;
+                stager.put(0, mine, mine + kTile);
+                place = place_of(a.p, page, base + kStep + lane % 32, head);      // (behind the end: rows of zeros)
+                held = (uint32_t)__ballot(place.held);
+                stager.fetch(place, 0, a.p.dim);
+                page = page_of(base + 2 * kStep);
+                attend(base, now, mine);
+            }
+        } else {
+            uint32_t stage = 0, held = 0;
+            if (base < range.end) {
+                const Place place = place_of(a.p, page, base + lane % 32, head);
+                held = (uint32_t)__ballot(place.held);
+                Stager<D, kFewKeys, false>::send(place, 0, a.p.dim, mine, mine + kTile);
+                page = page_of(base + kStep);
+            }
+            for (; base < range.end; base += kStep) {
+                all_loads_done();
+                const uint32_t now = held, kt = mine + stage;
+                stage ^= 2 * kTile;
+                if (base + kStep < range.end) {
+                    const Place place = place_of(a.p, page, base + kStep + lane % 32, head);
+                    held = (uint32_t)__ballot(place.held);
+                    Stager<D, kFewKeys, false>::send(place, 0, a.p.dim, mine + stage, mine + stage + kTile);
+                    page = page_of(base + 2 * kStep);
+                }
+                attend(base, now, kt);
+            }
+        }
+        if (careful || !__any(w.odd())) break;
+        careful = true;
+    }
+    w.l += other_half(w.l);
+
+    // the four waves' sums as one
+    __syncthreads();
+    constexpr int kRow = D + 4;                  // floats: rows begin in other banks
+    float *sums = reinterpret_cast<float *>(lds), *ml = sums + kFewWaves * 32 * kRow;
+    const int r = lane % 32, used = min(rows - row0, 32);
+    if (lane < 32) {
+        ml[(wave * 32 + r) * 2] = w.m;
+        ml[(wave * 32 + r) * 2 + 1] = w.l;
+    }
+    __syncthreads();
+    float top = ml[r * 2];
+#pragma unroll
+    for (int v = 1; v < kFewWaves; ++v) top = fmaxf(top, ml[(v * 32 + r) * 2]);
+    const float part = weight_of(w.m, top);
+    if (r < used) {
+#pragma unroll
+        for (int d = 0; d < D / 32; ++d)
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                *reinterpret_cast<f32x4 *>(sums + (wave * 32 + r) * kRow + 32 * d + 8 * i + 4 * (lane / 32)) =
+                    f32x4{w.o[d][4 * i] * part, w.o[d][4 * i + 1] * part, w.o[d][4 * i + 2] * part, w.o[d][4 * i + 3] * part};
+    }
+    __syncthreads();
+    const int64_t slot = (it.slot + it.split) * a.p.kv_heads + head;
+    for (int e = threadIdx.x; e < used * (D / 4); e += kFewWaves * kWave) {
+        const int rr = e / (D / 4), d = e % (D / 4) * 4;
+        float m = ml[rr * 2];
+#pragma unroll
+        for (int v = 1; v < kFewWaves; ++v) m = fmaxf(m, ml[(v * 32 + rr) * 2]);
+        f32x4 o = {0.0f, 0.0f, 0.0f, 0.0f};
+        float l = 0.0f;
+#pragma unroll
+        for (int v = 0; v < kFewWaves; ++v) {
+            o += *reinterpret_cast<const f32x4 *>(sums + (v * 32 + rr) * kRow + d);
+            l = __fmaf_rn(ml[(v * 32 + rr) * 2 + 1], weight_of(ml[(v * 32 + rr) * 2], m), l);
+        }
+        if (it.splits == 1) {
+            if (d < a.p.dim) store_row(a, it.run, row0 + rr, head, d, o * quotient_of(a, head, l));
+        } else if (slot < a.slots) {
+            *reinterpret_cast<f32x4 *>(a.partial + (slot * kFewRows + rr) * D + d) = o;
+            if (d == 0) {
+                float *to = a.partial + a.slots * kFewRows * D + (slot * kFewRows + rr) * 2;
+                to[0] = m;
+                to[1] = l;
+            }
+        }
+    }
+}
+
+// ---------------------------------------------------------------------------------------------------------------- many rows
+constexpr int many_lds(int D) { return 2 * 2 * kManyKeys * 2 * D; }
+
+template <int D, bool E4M3>
+__global__ __launch_bounds__(kManyWaves *kWave) void attend_many_kernel(Attend a, int clear) {
+    extern __shared__ __attribute__((aligned(1024))) uint8_t lds[];
+    constexpr int kTile = kManyKeys * 2 * D, kMine = kManyKeys / kManyWaves;
+    const int head = blockIdx.x % a.p.kv_heads, lane = threadIdx.x % kWave;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+    if (clear) clear_rest(a, blockIdx.x, gridDim.x, kManyWaves * kWave);
+    Item it;
+    if (!find<kManyRows, kManyKeys, false>(a, blockIdx.x / a.p.kv_heads, kManyTarget, it)) return;
+    const Range range = range_of<kManyRows, kManyKeys>(a, it);
+    const int rows = it.run.n * a.group, row0 = it.tile * kManyRows + 32 * wave, row = row0 + lane % 32, before = it.length - it.run.n;
+    const int pos = before + row / a.group, pos0 = before + row0 / a.group, pos1 = before + min(row0 + 31, rows - 1) / a.group;
+    const Caps caps = caps_of(a, head);
+    const int32_t *table = a.p.table + it.seq * a.p.table_stride;
+    Rows32<D, 2> w;
+    w.load_q(a, it.run, row, head);
+
+    const int h4 = 4 * (lane / 32);
+    bool careful = false;
+    const uint32_t tiles = lds_base(lds);
+    auto page_of = [&](int base) { return base + lane < range.end ? table[(base + lane) >> a.p.shift] : -1; };
+    auto attend = [&](int base, uint64_t held, uint32_t kt) {
+        if (row0 >= rows || base > pos1 || base + kManyKeys - 1 <= pos0 - a.window) return;
+        const uint64_t seen = seen_of(pos, base, a.window, held);
+        if (careful) w.template tile<kCareful>(kt, kt + kTile, caps.c, caps.in, caps.out, seen >> h4, seen);
+        else if (held != ~0ull || base + kManyKeys - 1 > pos0 || base <= pos1 - a.window)
+            w.template tile<kMasked>(kt, kt + kTile, caps.c, caps.in, caps.out, seen >> h4, seen);
+        else
+            w.template tile<kPlain>(kt, kt + kTile, caps.c, caps.in, caps.out, 0, 0);
+    };
+    for (;;) {                                   // (again: the whole block)
+        w.start();
+        int base = range.first;
+        uint32_t stage = 0;
+        int page = page_of(base);
+        Place place = place_of(a.p, page, base + lane, head);
+        uint64_t held = __ballot(place.held);
+        if constexpr (E4M3) {
+            Stager<D, kMine, true> stager;
+            stager.fetch(place, wave * kMine, a.p.dim);
+            stager.put(wave * kMine, tiles, tiles + kTile);
+            page = page_of(base + kManyKeys);
+            place = place_of(a.p, page, base + kManyKeys + lane, head);
+            uint64_t next = __ballot(place.held);
+            stager.fetch(place, wave * kMine, a.p.dim);
+            page = page_of(base + 2 * kManyKeys);
+            for (; base < range.end; base += kManyKeys) {
+                __syncthreads();
+                attend(base, held, tiles + stage);
+                stage ^= 2 * kTile;
+                held = next;
+                if (base + kManyKeys < range.end) {
+                    stager.put(wave * kMine, tiles + stage, tiles + stage + kTile);
+                    place = place_of(a.p, page, base + 2 * kManyKeys + lane, head);
+                    next = __ballot(place.held);
+                    stager.fetch(place, wave * kMine, a.p.dim);
+                    page = page_of(base + 3 * kManyKeys);
+                }
+            }
+        } else {
+            if (base < range.end) {
+                Stager<D, kMine, false>::send(place, wave * kMine, a.p.dim, tiles, tiles + kTile);
+                page = page_of(base + kManyKeys);
+            }
+            for (; base < range.end; base += kManyKeys) {
+                all_loads_done();
+                __builtin_amdgcn_s_barrier();
+                asm volatile("" ::: "memory");
+                const uint64_t now = held;
+                const uint32_t kt = tiles + stage;
+                stage ^= 2 * kTile;
+                if (base + kManyKeys < range.end) {
+                    place = place_of(a.p, page, base + kManyKeys + lane, head);
+                    held = __ballot(place.held);
+                    Stager<D, kMine, false>::send(place, wave * kMine, a.p.dim, tiles + stage, tiles + stage + kTile);
+                    page = page_of(base + 2 * kManyKeys);
+                }
+                attend(base, now, kt);
+            }
+        }
+        if (careful || !__syncthreads_or(w.odd())) break;
+        careful = true;
+    }
+    w.l += other_half(w.l);
+    if (row >= rows) return;
+    const int64_t slot = (it.slot + it.split) * a.p.kv_heads + head;
+    const float by = quotient_of(a, head, w.l);
+#pragma unroll
+    for (int d = 0; d < D / 32; ++d)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int at = 32 * d + 8 * i + 4 * (lane / 32);
+            const f32x4 o = {w.o[d][4 * i], w.o[d][4 * i + 1], w.o[d][4 * i + 2], w.o[d][4 * i + 3]};
+            if (it.splits == 1) {
+                if (at < a.p.dim) store_row(a, it.run, row, head, at, o * by);
+            } else if (slot < a.slots) {
+                *reinterpret_cast<f32x4 *>(a.partial + (slot * kManyRows + row - it.tile * kManyRows) * D + at) = o;
+            }
+        }
+    if (it.splits > 1 && slot < a.slots && lane < 32) {
+        float *to = a.partial + a.slots * kManyRows * D + (slot * kManyRows + row - it.tile * kManyRows) * 2;
+        to[0] = w.m;
+        to[1] = w.l;
+    }
+}
+
+// ---------------------------------------------------------------------------------------------------------------- splits as one
+// A block has 32 rows of a tile that was cut; splits in order.
+template <int D, int ROWS, int KEYS>
+__global__ __launch_bounds__(256) void attend_join_kernel(Attend a, uint32_t target) {
+    const int head = blockIdx.x % a.p.kv_heads;
+    Item it;
+    if (!find<ROWS, KEYS, true>(a, blockIdx.x / a.p.kv_heads, target, it)) return;
+    const int row0 = it.tile * ROWS + blockIdx.y * 32, used = min(it.run.n * a.group - row0, 32);
+    if (((it.slot + it.splits - 1) * a.p.kv_heads + head) >= a.slots) return;
+    const float *ml = a.partial + a.slots * ROWS * D;
+    for (int e = threadIdx.x; e < used * (D / 4); e += 256) {
+        const int r = e / (D / 4), d = e % (D / 4) * 4;
+        auto place = [&](int s) { return ((it.slot + s) * a.p.kv_heads + head) * ROWS + blockIdx.y * 32 + r; };
+        float m = -INFINITY;
+        for (int s = 0; s < it.splits; ++s) m = fmaxf(m, ml[place(s) * 2]);
+        f32x4 o = {0.0f, 0.0f, 0.0f, 0.0f};
+        float l = 0.0f;
+        for (int s = 0; s < it.splits; ++s) {
+            const float ls = ml[place(s) * 2 + 1], by = weight_of(ml[place(s) * 2], m);
+            const f32x4 v = *reinterpret_cast<const f32x4 *>(a.partial + place(s) * D + d);
+            o += v * by;
+            l = __fmaf_rn(ls, by, l);
+        }
+        if (d < a.p.dim) store_row(a, it.run, row0 + r, head, d, o * quotient_of(a, head, l));
+    }
+}
+
+// ---------------------------------------------------------------------------------------------------------------- host
+// What a call launches: which sequences go to which kernel, and what they need.
+struct Plan {
+    bool few, many;
+    int least;                                   // rows a key head from which on (exclusive) the kernel for many has them
+};
+Plan plan_of(int64_t group, int64_t rows, int64_t seqs, int64_t most_new) {
+    if (most_new * group <= kFewRows) return {true, false, 0};
+    if (seqs <= 1) return {false, true, 0};
+    return {true, true, kFewRows};
+}
+int64_t slots_of(int target) { return 2 * target; }
+int64_t floats_of(int rows, int target, int D) { return slots_of(target) * rows * (D + 2); }
+
+}  // namespace
+}  // namespace odl
+
+using namespace odl;
+
+namespace {
+
+int check(const char *who, int64_t heads, int64_t most_new, const odl_fp8_paged_cache *cache, const odl_fp8_paged_batch *batch, Paged &p) {
+    if (const int rc = take_paged(who, cache, batch, p)) return rc;
+    if (heads < 1 || heads > 1024 || heads % p.kv_heads) return set_error(ODL_ERR_SHAPE, "%s: %lld heads for %d of keys (a multiple, up to 1024)", who, (long long)heads, p.kv_heads);
+    if (batch->rows * heads >= INT32_MAX) return set_error(ODL_ERR_SHAPE, "%s: more than 2^31 rows of heads", who);
+    if (most_new < 0) return set_error(ODL_ERR_ARG, "%s: most_new is negative", who);
+    return ODL_OK;
+}
+
+template <int D>
+int launch(Attend &a, const Plan &plan, float *workspace, hipStream_t stream) {
+    const int64_t kv = a.p.kv_heads, rows = (int64_t)a.p.rows * a.group, seqs = a.p.seqs < a.p.rows ? a.p.seqs : a.p.rows;
+    auto blocks = [&](int tile, int target) { return (unsigned)((target / kv + 1 + seqs + rows / tile) * kv); };
+    auto joins = [&](int target) { return (unsigned)((target / kv + 1) * kv); };
+    if (plan.many) {
+        a.least_rows = plan.least, a.most_rows = INT32_MAX;
+        a.partial = workspace, a.slots = slots_of(kManyTarget);
+        const int clear = !plan.few;
+        if (a.p.e4m3) hipLaunchKernelGGL((attend_many_kernel<D, true>), dim3(blocks(kManyRows, kManyTarget)), dim3(kManyWaves * kWave), many_lds(D), stream, a, clear);
+        else hipLaunchKernelGGL((attend_many_kernel<D, false>), dim3(blocks(kManyRows, kManyTarget)), dim3(kManyWaves * kWave), many_lds(D), stream, a, clear);
+        if (a.p.reach > kManyKeys)
+            hipLaunchKernelGGL((attend_join_kernel<D, kManyRows, kManyKeys>), dim3(joins(kManyTarget), kManyRows / 32), dim3(256), 0, stream, a, (uint32_t)kManyTarget);
+        workspace += floats_of(kManyRows, kManyTarget, D);
+    }
+    if (plan.few) {
+        a.least_rows = 0, a.most_rows = plan.many ? plan.least : INT32_MAX;
+        a.partial = workspace, a.slots = slots_of(kFewTarget);
+        if (a.p.e4m3) hipLaunchKernelGGL((attend_few_kernel<D, true>), dim3(blocks(kFewRows, kFewTarget)), dim3(kFewWaves * kWave), few_lds(D, true), stream, a);
+        else hipLaunchKernelGGL((attend_few_kernel<D, false>), dim3(blocks(kFewRows, kFewTarget)), dim3(kFewWaves * kWave), few_lds(D, false), stream, a);
+        if (a.p.reach > kFewKeys * kFewWaves)
+            hipLaunchKernelGGL((attend_join_kernel<D, kFewRows, kFewKeys * kFewWaves>), dim3(joins(kFewTarget)), dim3(256), 0, stream, a, (uint32_t)kFewTarget);
+    }
+    return check_launch("odl_fp8_paged_attention");
+}
+
+int64_t workspace_of(const Plan &plan, int dim) {
+    const int D = dim > 64 ? 128 : 64;
+    return (plan.many ? floats_of(kManyRows, kManyTarget, D) : 0) + (plan.few ? floats_of(kFewRows, kFewTarget, D) : 0);
+}
+
+}  // namespace
+
+extern "C" int64_t odl_fp8_paged_attention_workspace(int64_t heads, int64_t most_new, const odl_fp8_paged_cache *cache, const odl_fp8_paged_batch *batch) {
+    Paged p;
+    if (check("odl_fp8_paged_attention_workspace", heads, most_new, cache, batch, p)) return -1;
+    return workspace_of(plan_of(heads / p.kv_heads, p.rows, p.seqs, most_new < p.rows ? most_new : p.rows), p.dim);
+}
+
+extern "C" int odl_fp8_paged_attention(const void *q, const int64_t *q_strides, int64_t heads, int64_t most_new, const odl_fp8_paged_cache *cache,
+                                       const odl_fp8_paged_batch *batch, float scale, int64_t window, float softcap, void *out, float *workspace,
+                                       int64_t workspace_floats, odl_stream_t stream_) {
+    static const char who[] = "odl_fp8_paged_attention";
+    Attend a;
+    if (const int rc = check(who, heads, most_new, cache, batch, a.p)) return rc;
+    if (const int rc = check_strides(who, "q", q, q_strides, a.p.rows)) return rc;
+    if (!(scale > 0.0f) || scale > 1e30f) return set_error(ODL_ERR_ARG, "%s: scale %g (above 0, up to 1e30)", who, (double)scale);
+    if (!(softcap == 0.0f || (softcap >= 1e-3f && softcap <= 1e6f))) return set_error(ODL_ERR_ARG, "%s: softcap %g (0, or 1e-3 to 1e6)", who, (double)softcap);
+    if (window < 0) return set_error(ODL_ERR_ARG, "%s: window %lld", who, (long long)window);
+    if (a.p.rows == 0) return ODL_OK;
+    if (!out || (reinterpret_cast<uintptr_t>(out) & 15)) return set_error(ODL_ERR_ARG, "%s: out must be a 16-byte aligned address", who);
+    a.q = static_cast<const uint16_t *>(q), a.q_row = q_strides[0], a.q_head = q_strides[1];
+    a.heads = (int)heads, a.group = (int)(heads / a.p.kv_heads), a.window = window == 0 || window > INT32_MAX / 2 ? INT32_MAX / 2 : (int)window;
+    a.scale = scale, a.softcap = softcap, a.out = static_cast<uint16_t *>(out);
+    const Plan plan = plan_of(a.group, a.p.rows, a.p.seqs, most_new < a.p.rows ? most_new : a.p.rows);
+    if (!workspace || workspace_floats < workspace_of(plan, a.p.dim) || (reinterpret_cast<uintptr_t>(workspace) & 15))
+        return set_error(ODL_ERR_ARG, "%s: a workspace of %lld floats, 16-byte aligned", who, (long long)workspace_of(plan, a.p.dim));
+    hipStream_t stream = reinterpret_cast<hipStream_t>(stream_);
+    return a.p.dim > 64 ? launch<128>(a, plan, workspace, stream) : launch<64>(a, plan, workspace, stream);
+}

@@ -1,0 +1,179 @@
+"""A cache of keys and values in pages, and the two steps of a decoder that work on it: what goes into it, and attention over it.
+
+A sequence's tokens lie in pages of a fixed number of tokens, anywhere in the cache; a table says which.  A step brings some new tokens of each of
+several sequences, one behind the other: single tokens of a decode step, drafted tokens that are to be verified, chunks of prompts, or all of
+them at once.  The reference runs whole sequences through PyTorch's attention and keeps nothing (optimus_dl/modules/model/blocks/attention.py:128-170).
+
+For inference: inputs that want gradients are refused.
+"""
+
+from __future__ import annotations
+
+
+import torch
+
+from .. import native
+from .calls import untraced
+
+E4M3_MAX = 448.0
+
+
+def _refuse_gradients(what: str, *tensors: "torch.Tensor | None") -> None:
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
+        raise ValueError(f"{what} is for inference; an input wants a gradient (torch.no_grad() around the call, or detach it)")
+
+
+def _check(what: str, q, keys, values, pages, offsets, lengths, key_scale, value_scale) -> None:
+    if keys.dim() != 4 or values.shape != keys.shape or values.dtype != keys.dtype:
+        raise ValueError(f"{what}: keys {keys.dtype} {tuple(keys.shape)} and values {values.dtype} {tuple(values.shape)}, expected [pages, kv heads, page size, "
+                         "head_dim] of one type")
+    if q.dim() != 3 or q.shape[2] != keys.shape[3] or q.shape[1] % keys.shape[1]:
+        raise ValueError(f"{what}: q {tuple(q.shape)} for a cache of {keys.shape[1]} heads of {keys.shape[3]}, expected [rows, a multiple of the heads, head_dim]")
+    if any(t.dtype != torch.int32 for t in (pages, offsets, lengths)) or pages.dim() != 2 or lengths.shape != pages.shape[:1] or offsets.shape != (lengths.numel() + 1,):
+        raise ValueError(f"{what}: pages {pages.dtype} {tuple(pages.shape)}, offsets {offsets.dtype} {tuple(offsets.shape)} and lengths {lengths.dtype} "
+                         f"{tuple(lengths.shape)}, expected int32 [sequences, width], [sequences + 1], [sequences]")
+    if keys.shape[2] < 1 or keys.shape[2] & (keys.shape[2] - 1):
+        raise ValueError(f"{what}: pages of {keys.shape[2]} tokens (a power of two)")
+    for scale in (key_scale, value_scale):
+        if (keys.dtype == torch.float8_e4m3fn) != (scale is not None) or (scale is not None and scale.shape != (keys.shape[1],)):
+            raise ValueError(f"{what}: a float8_e4m3fn cache has a scale for each of {keys.shape[1]} heads of keys and of values, others have none")
+
+
+def _sequences(offsets, lengths, rows: int):
+    """(first row, new tokens, position of the first) of every sequence, on the CPU."""
+    at = offsets.tolist()
+    for s, length in enumerate(lengths.tolist()):
+        first = min(max(at[s], 0), rows)
+        n = max(min(at[s + 1], rows) - first, 0)
+        yield s, first, n, length - n
+
+
+def _slots(pages_row, position, n_pages: int, page_size: int):
+    """Page and place in it of every position; which of them there are."""
+    inside = (position >= 0) & (position < pages_row.numel() * page_size)
+    at = torch.where(inside, position, torch.zeros_like(position))
+    page = pages_row.long()[at // page_size] if pages_row.numel() else torch.full_like(at, -1)
+    held = inside & (page >= 0) & (page < n_pages)
+    return torch.where(held, page, torch.zeros_like(page)), at % page_size, held
+
+
+def _append_plain(q, k, v, keys, values, pages, offsets, lengths, cos, sin, interleaved, q_weight, k_weight, eps, key_scale, value_scale):
+    wide = torch.promote_types(q.dtype, torch.float32)
+    out = torch.zeros(q.shape, dtype=q.dtype)
+
+    def turned(x, weight, position):
+        x = x.to(wide)
+        if weight is not None:
+            x = x * (1.0 / (x.double().square().mean(-1, keepdim=True) + eps).sqrt()).to(wide) * weight.to(wide)
+        if cos is None:
+            return x
+        c, s = cos[position].to(wide).unsqueeze(1), sin[position].to(wide).unsqueeze(1)
+        half = c.shape[-1]
+        a, b = (x[..., 0:2 * half:2], x[..., 1:2 * half:2]) if interleaved else (x[..., :half], x[..., half:2 * half])
+        a, b = a * c - b * s, a * s + b * c
+        return torch.cat((torch.stack((a, b), -1).flatten(-2) if interleaved else torch.cat((a, b), -1), x[..., 2 * half:]), -1)
+
+    for s, first, n, before in _sequences(offsets, lengths, q.shape[0]):
+        position = torch.arange(before, before + n)
+        inside = (position >= 0) & (position < pages.shape[1] * keys.shape[2])
+        rows, position = torch.arange(first, first + n)[inside], position[inside]
+        page, slot, held = _slots(pages[s], position, keys.shape[0], keys.shape[2])
+        out[rows] = turned(q[rows], q_weight, position).to(q.dtype)
+        for cache, x, scale in ((keys, turned(k[rows], k_weight, position), key_scale), (values, v[rows].to(wide), value_scale)):
+            if scale is not None:
+                x = (x / scale.view(1, -1, 1)).clamp(-E4M3_MAX, E4M3_MAX)
+            x = x.to(cache.dtype)
+            bits = {1: torch.uint8, 2: torch.int16, 4: torch.int32, 8: torch.int64}[cache.element_size()]
+            cache.view(bits)[page[held], :, slot[held]] = x.view(bits)[held]
+    return out
+
+
+def _attention_plain(q, keys, values, pages, offsets, lengths, scale, window, softcap, key_scale, value_scale):
+    wide = torch.promote_types(q.dtype, torch.float32)
+    out = torch.zeros(q.shape, dtype=q.dtype)
+    group, size = q.shape[1] // keys.shape[1], keys.shape[2]
+    for s, first, n, before in _sequences(offsets, lengths, q.shape[0]):
+        if n == 0:
+            continue
+        place = torch.arange(min(max(before + n, 0), pages.shape[1] * size))
+        page, slot, held = _slots(pages[s], place, keys.shape[0], size)
+
+        def read(cache, scale):
+            x = cache.to(wide)[page, :, slot]                                # [positions, kv heads, head_dim]
+            x = x if scale is None else x * scale.to(wide).view(1, -1, 1)
+            return x.repeat_interleave(group, dim=1).transpose(0, 1)
+
+        score = torch.matmul(q[first:first + n].to(wide).transpose(0, 1), read(keys, key_scale).transpose(1, 2)) * scale
+        if softcap:
+            score = softcap * torch.tanh(score / softcap)
+        position = torch.arange(before, before + n).unsqueeze(1)
+        seen = (place <= position) & held
+        if window:
+            seen = seen & (place > position - window)
+        score = score.masked_fill(~seen, float("-inf"))
+        weight = torch.where(seen.any(-1, keepdim=True), torch.softmax(score, -1), torch.zeros_like(score))
+        v = read(values, value_scale).unsqueeze(1)                           # (an unseen value does not reach a row, not even a NaN)
+        odd = ~v.isfinite()
+        y = torch.matmul(weight.unsqueeze(2), torch.where(odd, torch.zeros_like(v), v)).squeeze(2)
+        if odd.any():
+            y = y + torch.where(odd & seen.view(1, *seen.shape, 1), v, torch.zeros_like(v)).sum(2)
+        out[first:first + n] = y.transpose(0, 1).to(q.dtype)
+    return out
+
+
+@untraced
+def append_kv(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, keys: torch.Tensor, values: torch.Tensor, pages: torch.Tensor, offsets: torch.Tensor,
+              lengths: torch.Tensor, *, cos: torch.Tensor | None = None, sin: torch.Tensor | None = None, interleaved: bool = True,
+              q_weight: torch.Tensor | None = None, k_weight: torch.Tensor | None = None, eps: float = 1e-6, key_scale: torch.Tensor | None = None,
+              value_scale: torch.Tensor | None = None) -> torch.Tensor:
+    """Puts the keys and values of new tokens into a paged cache, with the norm and the rotation of queries and keys on the way.  -> the queries.
+
+    q [rows, heads, head_dim], k and v [rows, kv heads, head_dim]: the new tokens of sequence s are rows ``offsets[s]`` to ``offsets[s + 1]``.  keys, values
+    [pages, kv heads, page size, head_dim]: the cache, bf16, or float8_e4m3fn with ``key_scale`` and ``value_scale`` [kv heads] (fp32; a code stands for
+    code * scale, larger values are clamped).  lengths: tokens of each sequence in the cache, with the new ones; position p of sequence s is in slot
+    ``p % page size`` of page ``pages[s, p // page size]``.  pages, offsets, lengths int32.
+
+    cos, sin: fp32 [positions, pairs], of every position that the table reaches; the first 2 * pairs elements of a head are rotated, as pairs (2 i, 2 i + 1)
+    where ``interleaved``, else (i, pairs + i).  q_weight, k_weight [head_dim]: norms by root mean square in front of the rotation.
+    Rows behind the last sequence are not read: their queries are 0.  Tokens whose page is none of the cache are not written, those behind the
+    table's reach neither, and their queries are 0.  Two rows of a call must not share a slot.
+
+    bf16 on the GPU, one kernel, in head dimensions of 16 to 128 (a multiple of 16).  CPU tensors run as torch operations, in any floating type."""
+    _check("append_kv", q, keys, values, pages, offsets, lengths, key_scale, value_scale)
+    if k.shape != v.shape or k.shape != (q.shape[0], keys.shape[1], keys.shape[3]) or k.dtype != q.dtype or v.dtype != q.dtype:
+        raise ValueError(f"append_kv: k {k.dtype} {tuple(k.shape)} and v {v.dtype} {tuple(v.shape)} beside q {q.dtype} {tuple(q.shape)}, expected "
+                         f"[{q.shape[0]}, {keys.shape[1]}, {keys.shape[3]}]")
+    if (cos is None) != (sin is None) or (cos is not None and (cos.dim() != 2 or cos.shape != sin.shape or 2 * cos.shape[1] > q.shape[2]
+                                                              or cos.shape[0] < pages.shape[1] * keys.shape[2])):
+        raise ValueError(f"append_kv: cos and sin of {pages.shape[1] * keys.shape[2]} positions, [positions, up to {q.shape[2] // 2}] of both")
+    for weight in (q_weight, k_weight):
+        if weight is not None and weight.shape != q.shape[2:]:
+            raise ValueError(f"append_kv: norms of heads have {q.shape[2]} weights")
+    _refuse_gradients("append_kv", q, k, v, keys, values, q_weight, k_weight, cos, sin)
+    if not q.is_cuda:
+        return _append_plain(q, k, v, keys, values, pages, offsets, lengths, cos, sin, interleaved, q_weight, k_weight, eps, key_scale, value_scale)
+    return native.append_kv(q, k, v, keys, values, pages, offsets, lengths, cos, sin, interleaved, q_weight, k_weight, eps, key_scale, value_scale)
+
+
+@untraced
+def paged_attention(q: torch.Tensor, keys: torch.Tensor, values: torch.Tensor, pages: torch.Tensor, offsets: torch.Tensor, lengths: torch.Tensor, *,
+                    max_new: int | None = None, scale: float | None = None, window: int = 0, softcap: float = 0.0,
+                    key_scale: torch.Tensor | None = None, value_scale: torch.Tensor | None = None) -> torch.Tensor:
+    """Attention of new tokens over a paged cache that holds them (see :func:`append_kv` for both).  -> [rows, heads, head_dim].
+
+    A token at position p sees positions ``max(0, p - window + 1)`` to p (window 0: from 0).  Scores are ``scale * q . key`` (1 / sqrt(head_dim) by
+    default), and ``softcap * tanh(score / softcap)`` where softcap is not 0.  Heads in groups share a head of the cache.
+    max_new: the most new tokens of a sequence, where the program knows it: it chooses kernels, results hold without.
+    Keys and values that a token does not see do not reach it, NaN and infinities included.  A token that sees nothing, and rows behind
+    the last sequence, answer 0.
+
+    bf16 on the GPU: one kernel for up to 32 rows (tokens times heads of a group) a sequence, another for more, and one that joins parts; sums and maxima
+    in fp32, weights rounded to bf16.  The same call answers the same bits.  CPU tensors run as torch operations, in any floating type."""
+    _check("paged_attention", q, keys, values, pages, offsets, lengths, key_scale, value_scale)
+    scale = q.shape[2] ** -0.5 if scale is None else scale
+    if not 0.0 < scale <= 1e30 or window < 0 or not (softcap == 0.0 or 1e-3 <= softcap <= 1e6) or (max_new is not None and max_new < 0):
+        raise ValueError(f"paged_attention: scale {scale} (above 0, up to 1e30), window {window} (0 or more), softcap {softcap} (0, or 1e-3 to 1e6), max_new {max_new}")
+    _refuse_gradients("paged_attention", q, keys, values)
+    if not q.is_cuda:
+        return _attention_plain(q, keys, values, pages, offsets, lengths, scale, window, softcap, key_scale, value_scale)
+    return native.paged_attention(q, keys, values, pages, offsets, lengths, max_new, scale, window, softcap, key_scale, value_scale)

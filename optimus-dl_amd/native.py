@@ -26,7 +26,7 @@ DT_BF16, DT_F32 = 0, 1
 AMAX_MAX, AMAX_MOST_RECENT = 0, 1
 FP8_MAX = {E4M3: 448.0, E5M2: 57344.0}
 TORCH_FP8 = {E4M3: torch.float8_e4m3fn, E5M2: torch.float8_e5m2}
-ABI_VERSION = 31
+ABI_VERSION = 32
 _OUT_DTYPES = {torch.bfloat16: DT_BF16, torch.float32: DT_F32}
 AMAX_PARTS = 512                       # ODL_FP8_AMAX_PARTS
 
@@ -112,6 +112,9 @@ EXPORTS = (
     "odl_fp8_fp4_linear_runs",
     "odl_fp8_fp4_linear",
     "odl_fp8_fp4_quantise",
+    "odl_fp8_append_kv",
+    "odl_fp8_paged_attention_workspace",
+    "odl_fp8_paged_attention",
 )
 
 logger = logging.getLogger(__name__)
@@ -221,6 +224,10 @@ def load() -> ctypes.CDLL:
         f32 = ctypes.c_float
         L.odl_fp8_residual_norm.argtypes = [vp, i32, vp, i32, vp, vp, vp, i64, i64, i64, f32, f32, f32, vp, vp, vp, vp, vp]
         L.odl_fp8_residual_norm_bwd.argtypes = [vp, vp, vp, i32, vp, i32, vp, vp, vp, i64, i64, i64, f32, vp, vp, vp, vp, vp, vp, vp, vp, vp]
+        L.odl_fp8_append_kv.argtypes = [vp, vp, vp, vp, vp, vp, i64, vp, vp, vp, vp, i64, i64, i32, vp, vp, ctypes.c_double, vp, vp]
+        L.odl_fp8_paged_attention_workspace.argtypes = [i64, i64, vp, vp]
+        L.odl_fp8_paged_attention_workspace.restype = i64
+        L.odl_fp8_paged_attention.argtypes = [vp, vp, i64, i64, vp, vp, f32, i64, f32, vp, vp, i64, vp]
         L.odl_fp8_token_logprobs_workspace.argtypes = [i64, i64, i32]
         L.odl_fp8_token_logprobs_workspace.restype = i64
         L.odl_fp8_token_logprobs.argtypes = [vp, i32, i64, i64, i64, vp, i64, f32, i32, vp, vp, vp, vp, vp, vp, i64, vp]
@@ -1859,3 +1866,107 @@ def fp4_quantise(w: torch.Tensor, group: int):
         scales = torch.empty((N, K // group), dtype=torch.bfloat16, device=w.device)
         _check(load().odl_fp8_fp4_quantise(w.data_ptr(), src, N, K, group, codes.data_ptr(), scales.data_ptr(), _stream()), "odl_fp8_fp4_quantise")
     return codes, scales
+
+
+class _PagedCache(ctypes.Structure):
+    """odl_fp8_paged_cache"""
+
+    _fields_ = [("keys", ctypes.c_void_p), ("values", ctypes.c_void_p), ("key_scale", ctypes.c_void_p), ("value_scale", ctypes.c_void_p),
+                ("pages", ctypes.c_int64), ("kv_heads", ctypes.c_int64), ("page_size", ctypes.c_int64), ("head_dim", ctypes.c_int64),
+                ("key_strides", ctypes.c_int64 * 3), ("value_strides", ctypes.c_int64 * 3), ("e4m3", ctypes.c_int32), ("reserved", ctypes.c_int32)]
+
+
+class _PagedBatch(ctypes.Structure):
+    """odl_fp8_paged_batch"""
+
+    _fields_ = [("table", ctypes.c_void_p), ("offsets", ctypes.c_void_p), ("lengths", ctypes.c_void_p), ("seqs", ctypes.c_int64),
+                ("rows", ctypes.c_int64), ("width", ctypes.c_int64), ("table_stride", ctypes.c_int64)]
+
+
+_CACHE_TYPES = (torch.bfloat16, torch.float8_e4m3fn)
+
+
+def _paged_cache(keys, values, key_scale, value_scale) -> _PagedCache:
+    if keys.dtype not in _CACHE_TYPES or values.dtype != keys.dtype or keys.dim() != 4 or values.shape != keys.shape:
+        raise NativeError(f"paged cache: keys are {keys.dtype} {tuple(keys.shape)} and values {values.dtype} {tuple(values.shape)}, "
+                          "expected bf16 or float8_e4m3fn [pages, kv heads, page size, head_dim] of both")
+    if keys.stride(3) != 1 or values.stride(3) != 1:
+        raise NativeError("paged cache: a token's keys and values of a head have to be dense")
+    e4m3, heads = keys.dtype == torch.float8_e4m3fn, keys.shape[1]
+    for scale, name in ((key_scale, "key_scale"), (value_scale, "value_scale")):
+        if e4m3 != (scale is not None):
+            raise NativeError(f"paged cache: {name} belongs to a float8_e4m3fn cache, and it to that")
+        if scale is not None:
+            _f32_dev(scale, heads, "paged cache " + name)
+    c = _PagedCache(keys.data_ptr(), values.data_ptr(), None if key_scale is None else key_scale.data_ptr(),
+                    None if value_scale is None else value_scale.data_ptr(), *keys.shape)
+    c.key_strides[:], c.value_strides[:] = keys.stride()[:3], values.stride()[:3]
+    c.e4m3 = int(e4m3)
+    return c
+
+
+def _paged_batch(pages, offsets, lengths, rows: int) -> _PagedBatch:
+    seqs = lengths.numel()
+    if any(t.dtype != torch.int32 for t in (pages, offsets, lengths)) or pages.dim() != 2 or pages.shape[0] != seqs or lengths.dim() != 1 or offsets.shape != (seqs + 1,):
+        raise NativeError(f"paged batch: pages {pages.dtype} {tuple(pages.shape)}, offsets {offsets.dtype} {tuple(offsets.shape)}, lengths {lengths.dtype} "
+                          f"{tuple(lengths.shape)}, expected int32 [sequences, width], [sequences + 1] and [sequences]")
+    if not (offsets.is_contiguous() and lengths.is_contiguous()) or (pages.numel() and pages.stride(1) != 1):
+        raise NativeError("paged batch: rows of pages, offsets and lengths have to be dense")
+    return _PagedBatch(pages.data_ptr(), offsets.data_ptr(), lengths.data_ptr(), seqs, rows, pages.shape[1], pages.stride(0))
+
+
+def _new_rows(t: torch.Tensor, heads: int | None, dim: int, what: str) -> torch.Tensor:
+    """Rows of heads as the kernels read them; a copy where rows or heads lie at odd distances."""
+    if t.dtype != torch.bfloat16 or t.dim() != 3 or t.shape[2] != dim or (heads is not None and t.shape[1] != heads):
+        raise NativeError(f"{what} is {t.dtype} {tuple(t.shape)}, expected bf16 [rows, {'heads' if heads is None else heads}, {dim}]")
+    if t.numel() and (t.stride(2) != 1 or t.stride(0) % 8 or t.stride(1) % 8 or t.data_ptr() % 16):
+        t = _dense_16(t)
+    return t
+
+
+def _strides(t: torch.Tensor):
+    return (ctypes.c_int64 * 2)(*t.stride()[:2])
+
+
+def append_kv(q, k, v, keys, values, pages, offsets, lengths, cos=None, sin=None, interleaved: bool = True, q_weight=None, k_weight=None,
+              eps: float = 1e-6, key_scale=None, value_scale=None) -> torch.Tensor:
+    """New queries and keys [rows, heads, head_dim] normed and rotated, keys and values put into the cache (``odl_fp8_append_kv``).  -> q, dense."""
+    with _Elsewhere(q, k, v, keys, values, pages, offsets, lengths, cos, sin, q_weight, k_weight, key_scale, value_scale):
+        cache = _paged_cache(keys, values, key_scale, value_scale)
+        kv, dim = cache.kv_heads, cache.head_dim
+        q, k, v = _new_rows(q, None, dim, "append_kv: q"), _new_rows(k, kv, dim, "append_kv: k"), _new_rows(v, kv, dim, "append_kv: v")
+        if not q.shape[0] == k.shape[0] == v.shape[0]:
+            raise NativeError(f"append_kv: {q.shape[0]}, {k.shape[0]} and {v.shape[0]} rows of q, k and v")
+        batch = _paged_batch(pages, offsets, lengths, q.shape[0])
+        half, positions = 0, 0
+        if (cos is None) != (sin is None):
+            raise NativeError("append_kv: cos and sin come together")
+        if cos is not None:
+            if cos.dim() != 2 or sin.shape != cos.shape:
+                raise NativeError(f"append_kv: angles {tuple(cos.shape)} and {tuple(sin.shape)}, expected [positions, pairs] of both")
+            cos, sin = (_f32_dev(t, t.numel(), "append_kv angles") for t in (cos, sin))
+            positions, half = cos.shape
+        q_weight, k_weight = (_f32_vector(w, dim, q.device, "append_kv " + n) for w, n in ((q_weight, "q_weight"), (k_weight, "k_weight")))
+        out = torch.empty(q.shape, dtype=torch.bfloat16, device=q.device)
+        p = lambda t: None if t is None else t.data_ptr()
+        _check(load().odl_fp8_append_kv(p(q), _strides(q), p(k), _strides(k), p(v), _strides(v), q.shape[1], ctypes.byref(cache), ctypes.byref(batch),
+                                        p(cos), p(sin), positions, half, int(interleaved), p(q_weight), p(k_weight), float(eps), p(out), _stream()),
+               "odl_fp8_append_kv")
+    return out
+
+
+def paged_attention(q, keys, values, pages, offsets, lengths, most_new: int | None = None, scale: float = 1.0, window: int = 0, softcap: float = 0.0,
+                    key_scale=None, value_scale=None) -> torch.Tensor:
+    """Attention of new queries [rows, heads, head_dim] over the cache (``odl_fp8_paged_attention``).  -> bf16 [rows, heads, head_dim]."""
+    with _Elsewhere(q, keys, values, pages, offsets, lengths, key_scale, value_scale):
+        cache = _paged_cache(keys, values, key_scale, value_scale)
+        q = _new_rows(q, None, cache.head_dim, "paged_attention: q")
+        rows, heads = q.shape[:2]
+        batch = _paged_batch(pages, offsets, lengths, rows)
+        most_new = rows if most_new is None else most_new
+        out = torch.empty(q.shape, dtype=torch.bfloat16, device=q.device)
+        floats = load().odl_fp8_paged_attention_workspace(heads, most_new, ctypes.byref(cache), ctypes.byref(batch))
+        ws = torch.empty(max(floats, 0), dtype=torch.float32, device=q.device)
+        _check(load().odl_fp8_paged_attention(q.data_ptr(), _strides(q), heads, most_new, ctypes.byref(cache), ctypes.byref(batch), float(scale), int(window),
+                                              float(softcap), out.data_ptr(), ws.data_ptr(), ws.numel(), _stream()), "odl_fp8_paged_attention")
+    return out

@@ -819,6 +819,25 @@ int odl_fp8_paged_attention(const void *q, const int64_t *q_strides, int64_t hea
                             const odl_fp8_paged_batch *batch, float scale, int64_t window, float softcap, void *out, float *workspace,
                             int64_t workspace_floats, odl_stream_t stream);
 
+/*
+ * Verification of drafted tokens (no counterpart in the reference).  Sequence s fed its rows offsets[s] to offsets[s + 1] to the model: tokens[first], the
+ * last one that is sure, and behind it the drafts.  Row r's logits speak of the token behind it.  With p = softmax(logits[r, :vocab] / temperature), q the
+ * same of draft_logits (NULL: q is all on the drafted token) and u = uniforms, a draft d = tokens[r + 1] is accepted where u[r] * q(d) < p(d).
+ * At the first that is not, the token is the least i with sum_{k <= i} w_k > u[last] * sum_k w_k, w = max(p - q, 0) (p where that is nothing but 0);
+ * behind the last draft, w = p.  last: the sequence's last row, whose number nothing else uses.
+ * temperature 0: p is all on the largest logit (the lowest of them), draft_logits and uniforms are not read.
+ *   accepted[s]: how many drafts; out_tokens[r]: the token behind row r, -1 behind the row that stopped; logprobs[r]: log p of it (of
+ *   temperature 1 where that is 0), 0 where there is none.  Rows behind the last sequence: -1 and 0.
+ * A draft that is no token is refused.  A row with NaN or +inf, or of -inf only, stops: token -1, logprob NaN.  Where the drafter's row is such, w = p.
+ * logits bf16 or fp32 (dtype, both), rows `stride` elements apart, at any alignment.  Exponentials and sums in 64 bits; the order of the sums of
+ * parts is fixed.  Up to 65535 rows and sequences, a vocabulary of up to 2^24.  draft_logits of a sequence's last row are not read.
+ * workspace: odl_fp8_verify_drafts_workspace floats, contents irrelevant, of this call alone while it runs.
+ */
+int64_t odl_fp8_verify_drafts_workspace(int64_t rows, int64_t seqs, int64_t vocab);
+int odl_fp8_verify_drafts(const void *logits, int64_t stride, const void *draft_logits, int64_t draft_stride, int dtype, int64_t rows, int64_t vocab,
+                          const int64_t *tokens, const int32_t *offsets, int64_t seqs, const float *uniforms, double temperature, int32_t *accepted,
+                          int64_t *out_tokens, float *logprobs, float *workspace, int64_t workspace_floats, odl_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

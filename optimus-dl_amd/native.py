@@ -115,6 +115,8 @@ EXPORTS = (
     "odl_fp8_append_kv",
     "odl_fp8_paged_attention_workspace",
     "odl_fp8_paged_attention",
+    "odl_fp8_verify_drafts_workspace",
+    "odl_fp8_verify_drafts",
 )
 
 logger = logging.getLogger(__name__)
@@ -228,6 +230,9 @@ def load() -> ctypes.CDLL:
         L.odl_fp8_paged_attention_workspace.argtypes = [i64, i64, vp, vp]
         L.odl_fp8_paged_attention_workspace.restype = i64
         L.odl_fp8_paged_attention.argtypes = [vp, vp, i64, i64, vp, vp, f32, i64, f32, vp, vp, i64, vp]
+        L.odl_fp8_verify_drafts_workspace.argtypes = [i64, i64, i64]
+        L.odl_fp8_verify_drafts_workspace.restype = i64
+        L.odl_fp8_verify_drafts.argtypes = [vp, i64, vp, i64, i32, i64, i64, vp, vp, i64, vp, ctypes.c_double, vp, vp, vp, vp, i64, vp]
         L.odl_fp8_token_logprobs_workspace.argtypes = [i64, i64, i32]
         L.odl_fp8_token_logprobs_workspace.restype = i64
         L.odl_fp8_token_logprobs.argtypes = [vp, i32, i64, i64, i64, vp, i64, f32, i32, vp, vp, vp, vp, vp, vp, i64, vp]
@@ -1970,3 +1975,38 @@ def paged_attention(q, keys, values, pages, offsets, lengths, most_new: int | No
         _check(load().odl_fp8_paged_attention(q.data_ptr(), _strides(q), heads, most_new, ctypes.byref(cache), ctypes.byref(batch), float(scale), int(window),
                                               float(softcap), out.data_ptr(), ws.data_ptr(), ws.numel(), _stream()), "odl_fp8_paged_attention")
     return out
+
+
+def _logits_rows(logits, what: str) -> torch.Tensor:
+    if logits.dtype not in _OUT_DTYPES or logits.dim() != 2:
+        raise NativeError(f"verify_drafts: {what} are {logits.dtype} {tuple(logits.shape)}, expected bf16 or fp32 [rows, columns]")
+    return logits if (logits.stride(1) == 1 or logits.shape[1] == 1) and logits.stride(0) >= 0 else logits.contiguous()
+
+
+def verify_drafts(logits, tokens, offsets, uniforms, draft_logits=None, temperature: float = 1.0, n_vocab: int | None = None):
+    """How many drafted tokens the logits accept and what follows them (``odl_fp8_verify_drafts``).  -> (accepted int32 [sequences], tokens int64 [rows],
+    logprobs fp32 [rows])."""
+    with _Elsewhere(logits, tokens, offsets, uniforms, draft_logits):
+        logits = _logits_rows(logits, "logits")
+        rows, n_vocab = logits.shape[0], logits.shape[1] if n_vocab is None else n_vocab
+        if draft_logits is not None:
+            draft_logits = _logits_rows(draft_logits, "draft_logits")
+            if draft_logits.dtype != logits.dtype or draft_logits.shape[0] != rows or draft_logits.shape[1] < n_vocab:
+                raise NativeError(f"verify_drafts: draft_logits are {draft_logits.dtype} {tuple(draft_logits.shape)} beside logits {logits.dtype} {tuple(logits.shape)}")
+        if not 1 <= n_vocab <= logits.shape[1]:
+            raise NativeError(f"verify_drafts: n_vocab {n_vocab} of {logits.shape[1]} columns")
+        if tokens.dtype != torch.int64 or tokens.shape != (rows,) or offsets.dtype != torch.int32 or offsets.dim() != 1 or offsets.numel() < 1:
+            raise NativeError(f"verify_drafts: tokens {tokens.dtype} {tuple(tokens.shape)} and offsets {offsets.dtype} {tuple(offsets.shape)}, expected int64 [{rows}] and "
+                              "int32 [sequences + 1]")
+        tokens, offsets, seqs = tokens.contiguous(), offsets.contiguous(), offsets.numel() - 1
+        uniforms = _f32_dev(uniforms.contiguous(), rows, "verify_drafts uniforms")
+        accepted = torch.empty(seqs, dtype=torch.int32, device=logits.device)
+        out = torch.empty(rows, dtype=torch.int64, device=logits.device)
+        logprobs = torch.empty(rows, dtype=torch.float32, device=logits.device)
+        floats = load().odl_fp8_verify_drafts_workspace(rows, seqs, n_vocab)
+        ws = torch.empty(max(floats, 0), dtype=torch.float32, device=logits.device)
+        _check(load().odl_fp8_verify_drafts(logits.data_ptr(), logits.stride(0), None if draft_logits is None else draft_logits.data_ptr(),
+                                            0 if draft_logits is None else draft_logits.stride(0), _src_dtype(logits), rows, n_vocab, tokens.data_ptr(), offsets.data_ptr(),
+                                            seqs, uniforms.data_ptr(), float(temperature), accepted.data_ptr(), out.data_ptr(), logprobs.data_ptr(), ws.data_ptr(),
+                                            ws.numel(), _stream()), "odl_fp8_verify_drafts")
+    return accepted, out, logprobs

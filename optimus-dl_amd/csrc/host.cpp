@@ -61,6 +61,11 @@ decltype(&odl_fp8_token_logprobs) logprobs_c;
 decltype(&odl_fp8_token_logprobs_bwd) logprobs_bwd_c;
 decltype(&odl_fp8_fp4_linear_runs) fp4_runs_c;
 decltype(&odl_fp8_fp4_linear) fp4_linear_c;
+decltype(&odl_fp8_append_kv) append_kv_c;
+decltype(&odl_fp8_paged_attention_workspace) paged_workspace_c;
+decltype(&odl_fp8_paged_attention) paged_attention_c;
+decltype(&odl_fp8_verify_drafts_workspace) verify_workspace_c;
+decltype(&odl_fp8_verify_drafts) verify_drafts_c;
 
 template <class F>
 void take(F &f, const py::dict &d, const char *name) { f = reinterpret_cast<F>(py::cast<uintptr_t>(d[name])); }
@@ -105,6 +110,11 @@ void bind(const py::dict &d) {
     take(logprobs_bwd_c, d, "odl_fp8_token_logprobs_bwd");
     take(fp4_runs_c, d, "odl_fp8_fp4_linear_runs");
     take(fp4_linear_c, d, "odl_fp8_fp4_linear");
+    take(append_kv_c, d, "odl_fp8_append_kv");
+    take(paged_workspace_c, d, "odl_fp8_paged_attention_workspace");
+    take(paged_attention_c, d, "odl_fp8_paged_attention");
+    take(verify_workspace_c, d, "odl_fp8_verify_drafts_workspace");
+    take(verify_drafts_c, d, "odl_fp8_verify_drafts");
 }
 
 // as ctypes does: other Python threads run while a launch waits for room in its queue
@@ -576,6 +586,89 @@ py::object fp4_linear(const Tensor &x, const Tensor &codes, const Tensor &scales
     return rc ? status(rc) : py::cast(y);
 }
 
+// A step's new tokens over a paged cache.  Everything that does not fit is left to the long way, what the entries refuse as well.
+bool wants_gradient(const Tensor &t) { return t.requires_grad() && at::GradMode::is_enabled(); }
+bool wants_gradient(const OptTensor &t) { return t && wants_gradient(*t); }
+
+bool paged_operands(const Tensor &q, const Tensor &keys, const Tensor &values, const Tensor &pages, const Tensor &offsets, const Tensor &lengths,
+                    const OptTensor &ks, const OptTensor &vs, odl_fp8_paged_cache &c, odl_fp8_paged_batch &b) {
+    const auto device = q.device();
+    const bool e4m3 = keys.scalar_type() == at::kFloat8_e4m3fn;
+    if (!q.is_cuda() || (!e4m3 && keys.scalar_type() != at::kBFloat16) || values.scalar_type() != keys.scalar_type() || keys.dim() != 4 ||
+        values.sizes() != keys.sizes() || keys.device() != device || values.device() != device || keys.stride(3) != 1 || values.stride(3) != 1)
+        return false;
+    if (q.dim() != 3 || q.scalar_type() != at::kBFloat16 || keys.size(1) < 1 || q.size(2) != keys.size(3) || q.size(1) % keys.size(1) || q.numel() == 0) return false;
+    const i64 seqs = lengths.numel(), kv = keys.size(1);
+    for (const Tensor *t : {&pages, &offsets, &lengths})
+        if (t->scalar_type() != at::kInt || t->device() != device || !t->is_non_overlapping_and_dense()) return false;
+    if (pages.dim() != 2 || lengths.dim() != 1 || offsets.dim() != 1 || pages.size(0) != seqs || offsets.numel() != seqs + 1 || !pages.is_contiguous()) return false;
+    if (e4m3 != ks.has_value() || e4m3 != vs.has_value()) return false;
+    if (e4m3 && (!floats(*ks, kv) || !floats(*vs, kv) || ks->device() != device || vs->device() != device || ks->dim() != 1 || vs->dim() != 1)) return false;
+    if (wants_gradient(q) || wants_gradient(keys) || wants_gradient(values)) return false;
+    c = {keys.data_ptr(), values.data_ptr(), ptr(ks), ptr(vs), keys.size(0), kv, keys.size(2), keys.size(3), {keys.stride(0), keys.stride(1), keys.stride(2)},
+         {values.stride(0), values.stride(1), values.stride(2)}, e4m3, 0};
+    b = {ptr(pages), ptr(offsets), ptr(lengths), seqs, q.size(0), pages.size(1), pages.size(1)};
+    return true;
+}
+// rows of heads as the kernels read them
+bool new_rows(const Tensor &t, const Tensor &q, i64 heads) {
+    return t.dim() == 3 && t.scalar_type() == at::kBFloat16 && t.device() == q.device() && t.size(0) == q.size(0) && t.size(1) == heads && t.size(2) == q.size(2) &&
+           t.stride(2) == 1 && t.stride(0) % 8 == 0 && t.stride(1) % 8 == 0 && aligned(t) && !wants_gradient(t);
+}
+
+py::object append_kv(const Tensor &q, const Tensor &k, const Tensor &v, const Tensor &keys, const Tensor &values, const Tensor &pages, const Tensor &offsets,
+                     const Tensor &lengths, const OptTensor &cos, const OptTensor &sin, bool interleaved, const OptTensor &qw, const OptTensor &kw, double eps,
+                     const OptTensor &ks, const OptTensor &vs, i64 stream) {
+    odl_fp8_paged_cache c;
+    odl_fp8_paged_batch b;
+    if (!paged_operands(q, keys, values, pages, offsets, lengths, ks, vs, c, b)) return none();
+    if (!new_rows(q, q, q.size(1)) || !new_rows(k, q, c.kv_heads) || !new_rows(v, q, c.kv_heads) || cos.has_value() != sin.has_value()) return none();
+    i64 half = 0, positions = 0;
+    if (cos) {
+        if (cos->dim() != 2 || cos->sizes() != sin->sizes() || wants_gradient(cos) || wants_gradient(sin)) return none();
+        positions = cos->size(0), half = cos->size(1);
+        if (!floats(*cos, positions * half) || !floats(*sin, positions * half) || cos->device() != q.device() || sin->device() != q.device()) return none();
+    }
+    for (const OptTensor *w : {&qw, &kw})
+        if (*w && (!floats(**w, c.head_dim) || (*w)->dim() != 1 || (*w)->device() != q.device() || wants_gradient(*w))) return none();
+    Tensor out = at::empty({q.size(0), q.size(1), q.size(2)}, q.options());
+    const int rc = call(append_kv_c, ptr(q), q.strides().data(), ptr(k), k.strides().data(), ptr(v), v.strides().data(), q.size(1), &c, &b, ptr(cos), ptr(sin),
+                        positions, half, (int)interleaved, ptr(qw), ptr(kw), eps, ptr(out), str(stream));
+    return rc ? none() : py::cast(out);
+}
+
+py::object paged_attention(const Tensor &q, const Tensor &keys, const Tensor &values, const Tensor &pages, const Tensor &offsets, const Tensor &lengths,
+                           const std::optional<i64> &most, double scale, i64 window, double softcap, const OptTensor &ks, const OptTensor &vs, i64 stream) {
+    odl_fp8_paged_cache c;
+    odl_fp8_paged_batch b;
+    if (!paged_operands(q, keys, values, pages, offsets, lengths, ks, vs, c, b) || !new_rows(q, q, q.size(1))) return none();
+    const i64 most_new = most.value_or(q.size(0)), need = paged_workspace_c(q.size(1), most_new, &c, &b);
+    if (need < 0) return none();
+    Tensor out = at::empty({q.size(0), q.size(1), q.size(2)}, q.options()), ws = f32(q, {need});
+    const int rc = call(paged_attention_c, ptr(q), q.strides().data(), q.size(1), most_new, &c, &b, (float)scale, window, (float)softcap, ptr(out), ptr(ws), need,
+                        str(stream));
+    return rc ? none() : py::cast(out);
+}
+
+py::object verify_drafts(const Tensor &l, const Tensor &tokens, const Tensor &offsets, const Tensor &u, const OptTensor &drafts, double temperature,
+                         const std::optional<i64> &n_vocab, i64 stream) {
+    if (!logits2d(l) || wants_gradient(l) || wants_gradient(drafts)) return none();
+    const i64 rows = l.size(0), vocab = n_vocab.value_or(l.size(1)), seqs = offsets.numel() - 1;
+    if (vocab < 1 || vocab > l.size(1) || !dense(tokens) || tokens.scalar_type() != at::kLong || tokens.dim() != 1 || tokens.numel() != rows || !floats(u, rows) ||
+        u.dim() != 1 || !dense(offsets) || offsets.scalar_type() != at::kInt || offsets.dim() != 1 || seqs < 0)
+        return none();
+    if (tokens.device() != l.device() || u.device() != l.device() || offsets.device() != l.device()) return none();
+    if (drafts && (!logits2d(*drafts) || drafts->scalar_type() != l.scalar_type() || drafts->size(0) != rows || drafts->size(1) < vocab || drafts->device() != l.device()))
+        return none();
+    const i64 need = verify_workspace_c(rows, seqs, vocab);
+    if (need < 0) return none();
+    Tensor accepted = at::empty({seqs}, offsets.options()), out = at::empty({rows}, tokens.options()), lp = f32(l, {rows}), ws = f32(l, {need});
+    const int rc = call(verify_drafts_c, ptr(l), l.stride(0), ptr(drafts), drafts ? drafts->stride(0) : 0, src_of(l), rows, vocab, tokens.data_ptr<i64>(),
+                        offsets.data_ptr<int32_t>(), seqs, u.data_ptr<float>(), temperature, accepted.data_ptr<int32_t>(), out.data_ptr<i64>(), lp.data_ptr<float>(),
+                        ws.data_ptr<float>(), need, str(stream));
+    return rc ? none() : py::make_tuple(accepted, out, lp);
+}
+
 // ---- The same two as autograd nodes, for graphs without a recipe (which would be handed maxima, in Python).  Python's part of a
 // node is 60 to 100 us of a step that computes for 20; these take 25.
 using torch::autograd::AutogradContext;
@@ -769,6 +862,9 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
     m.def("token_logprobs", &token_logprobs);
     m.def("token_logprobs_bwd", &token_logprobs_bwd);
     m.def("fp4_linear", &fp4_linear);
+    m.def("append_kv", &append_kv);
+    m.def("paged_attention", &paged_attention);
+    m.def("verify_drafts", &verify_drafts);
     m.def("residual_norm_node", &residual_norm_node);
     m.def("token_logprobs_node", &token_logprobs_node);
 }

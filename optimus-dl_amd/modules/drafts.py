@@ -11,7 +11,8 @@ from typing import NamedTuple
 import torch
 
 from .. import native
-from .calls import untraced
+from .calls import untraced, untransformed
+from .paged import refuse_transforms
 
 
 class VerifiedDrafts(NamedTuple):
@@ -91,6 +92,10 @@ def verify_drafts(logits: torch.Tensor, tokens: torch.Tensor, offsets: torch.Ten
     NaN.  Rows behind the last sequence answer -1 and 0.
 
     bf16 and fp32 logits on the GPU (rows at any distance and alignment): two kernels, sums in 64 bits, so that tokens do not depend on how a row is cut."""
+    if logits.is_cuda and untransformed():
+        r = native.plain_verify_drafts(logits, tokens, offsets, uniforms, draft_logits, temperature, n_vocab)
+        if r is not None:
+            return VerifiedDrafts(*r)
     if logits.dim() != 2 or not logits.is_floating_point():
         raise ValueError(f"verify_drafts: logits are {logits.dtype} {tuple(logits.shape)}, expected [rows, columns]")
     rows, columns = logits.shape
@@ -109,4 +114,5 @@ def verify_drafts(logits: torch.Tensor, tokens: torch.Tensor, offsets: torch.Ten
         raise ValueError("verify_drafts is for inference; logits want a gradient (torch.no_grad() around the call, or detach them)")
     if not logits.is_cuda:
         return _plain(logits, tokens, offsets, uniforms, draft_logits, float(temperature), n_vocab)
+    refuse_transforms("verify_drafts")
     return VerifiedDrafts(*native.verify_drafts(logits, tokens, offsets, uniforms, draft_logits, float(temperature), n_vocab))

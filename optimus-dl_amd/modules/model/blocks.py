@@ -13,6 +13,7 @@ import torch.nn.functional as F
 
 from ..calls import called_as_it_is
 from ..fused import plain_class, residual_norm
+from ..paged import PagedLayer, append_kv, paged_attention
 
 
 class RMSNorm(nn.Module):
@@ -67,7 +68,28 @@ class CausalSelfAttention(nn.Module):
             self.q_norm = RMSNorm(self.head_dim, eps=rmsnorm_eps)
             self.k_norm = RMSNorm(self.head_dim, eps=rmsnorm_eps)
 
-    def forward(self, x: torch.Tensor) -> torch.Tensor:
+    def step(self, x: torch.Tensor, layer: PagedLayer) -> torch.Tensor:
+        """New tokens [rows, n_embd] of the sequences of a batch, over a cache of those in front of them that they are put into."""
+        q, k, v = (w(x).unflatten(-1, (-1, self.head_dim)) for w in (self.wq, self.wk, self.wv))
+        norms = {}
+        if self.use_qk_norm:
+            if _is_its_weight(self.q_norm) and _is_its_weight(self.k_norm) and self.q_norm.eps == self.k_norm.eps:
+                norms = {"q_weight": self.q_norm.weight, "k_weight": self.k_norm.weight, "eps": self.q_norm.eps}
+            else:
+                q, k = self.q_norm(q), self.k_norm(k)
+        dtype = q.dtype
+        if x.is_cuda:                                  # (what the kernels and the cache hold)
+            q, k, v = q.bfloat16(), k.bfloat16(), v.bfloat16()
+        cos, sin = layer.cache.angles(rope_tables, self.head_dim, self.rope_theta) if self.rope else (None, None)
+        pages, offsets, lengths, max_new = layer.batch
+        scales = {"key_scale": layer.key_scale, "value_scale": layer.value_scale}
+        q = append_kv(q, k, v, layer.keys, layer.values, pages, offsets, lengths, cos=cos, sin=sin, **norms, **scales)
+        y = paged_attention(q, layer.keys, layer.values, pages, offsets, lengths, max_new=max_new, **scales)
+        return self.wo(y.to(dtype).flatten(1))
+
+    def forward(self, x: torch.Tensor, layer: PagedLayer | None = None) -> torch.Tensor:
+        if layer is not None:
+            return self.step(x, layer)
         B, T_, _ = x.shape
         q = self.wq(x).view(B, T_, self.n_head, self.head_dim).transpose(1, 2)
         k = self.wk(x).view(B, T_, self.n_kv_head, self.head_dim).transpose(1, 2)
@@ -149,11 +171,12 @@ class LlamaBlock(nn.Module):
         x = self.residual_scale * x + (h if gate is None else (gate * h).to(x.dtype))
         return x, None if norm is None else norm(x)
 
-    def forward(self, x: torch.Tensor, z: torch.Tensor | None = None, next_norm: RMSNorm | None = None):
+    def forward(self, x: torch.Tensor, z: torch.Tensor | None = None, next_norm: RMSNorm | None = None, layer: PagedLayer | None = None):
+        over = () if layer is None else (layer,)
         if not self.stepped:
-            x = x + self.attn(self.ln_1(x))
+            x = x + self.attn(self.ln_1(x), *over)
             return x + self.mlp(self.ln_2(x))
-        x, z = self._end(x, self.attn(self.ln_1(x) if z is None else z), self.post_ln_1, self.gate_1, self.ln_2)
+        x, z = self._end(x, self.attn(self.ln_1(x) if z is None else z, *over), self.post_ln_1, self.gate_1, self.ln_2)
         x, z = self._end(x, self.mlp(z), self.post_ln_2, self.gate_2, next_norm)
         return x if next_norm is None else (x, z)
 
@@ -173,6 +196,6 @@ class GPT2Block(nn.Module):
         self.ln_2 = nn.LayerNorm(n_embd, bias=bias)
         self.mlp = GELUMLP(n_embd, bias=bias)
 
-    def forward(self, x: torch.Tensor) -> torch.Tensor:
-        x = x + self.attn(self.ln_1(x))
+    def forward(self, x: torch.Tensor, layer: PagedLayer | None = None) -> torch.Tensor:
+        x = x + self.attn(self.ln_1(x), *(() if layer is None else (layer,)))
         return x + self.mlp(self.ln_2(x))

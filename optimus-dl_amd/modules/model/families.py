@@ -2,7 +2,8 @@
 as in optimus_dl/modules/model/{llama2,qwen3,gpt2}.py), random-initialised with
 the reference's standard deviations (gpt2.py:167-180: 0.02, and 0.02/sqrt(2*n_layer)
 for the residual projections ``c_proj`` / ``wo``).  Not in the reference: norms behind the blocks, gates and a scaled stream
-(``post_norms``, ``layer_scale``, ``residual_scale``), and ``score``, the log probabilities that a model gives to tokens."""
+(``post_norms``, ``layer_scale``, ``residual_scale``), ``score``, the log probabilities that a model gives to tokens, and ``step`` and ``verify_step``, new tokens
+over a paged cache of those in front of them."""
 
 from __future__ import annotations
 
@@ -12,7 +13,9 @@ from dataclasses import dataclass
 import torch
 import torch.nn as nn
 
+from ..drafts import VerifiedDrafts, verify_drafts
 from ..logprobs import TokenLogProbs, token_logprobs
+from ..paged import PagedBatch, PagedKVCache
 from .blocks import GPT2Block, LlamaBlock, Qwen3Block, RMSNorm
 
 
@@ -75,21 +78,50 @@ class _DecoderLM(nn.Module):
             self.transformer.wte.weight = self.lm_head.weight
         _init_weights(self, cfg.n_layer)
 
-    def embed(self, input_ids: torch.Tensor) -> torch.Tensor:
+    def embed(self, input_ids: torch.Tensor, batch: PagedBatch | None = None) -> torch.Tensor:
         return self.transformer.wte(input_ids)
 
     def forward(self, input_ids: torch.Tensor, **kwargs) -> dict:
-        x, z = self.embed(input_ids), None
+        return {"logits": self.lm_head(self._hidden(input_ids))}
+
+    def _hidden(self, input_ids: torch.Tensor, cache: PagedKVCache | None = None, batch: PagedBatch | None = None) -> torch.Tensor:
+        x, z = self.embed(input_ids) if cache is None else self.embed(input_ids, batch), None
         blocks, ln_f = self.transformer.h, self.transformer.ln_f
         stepped = [isinstance(block, LlamaBlock) and block.takes_steps() for block in blocks]      # (a wrapper around a block has the stream alone)
         for i, block in enumerate(blocks):
+            over = {} if cache is None else {"layer": cache.layer(i, batch)}
             if not stepped[i]:
-                x, z = block(x), None
+                x, z = block(x, **over), None
             elif i + 1 == len(blocks) or stepped[i + 1]:                      # the end of a block and the norm in front of the next in one
-                x, z = block(x, z, ln_f if i + 1 == len(blocks) else blocks[i + 1].ln_1)
+                x, z = block(x, z, ln_f if i + 1 == len(blocks) else blocks[i + 1].ln_1, **over)
             else:
-                x, z = block(x, z), None
-        return {"logits": self.lm_head(ln_f(x) if z is None else z)}
+                x, z = block(x, z, **over), None
+        return ln_f(x) if z is None else z
+
+    def new_cache(self, pages: int, page_size: int = 64, max_tokens: int | None = None, dtype: torch.dtype | None = None, **scales: float) -> PagedKVCache:
+        """An empty cache for :meth:`step`, on the model's device.  Sequences of up to ``max_tokens``, by default the configuration's ``block_size``.
+        dtype: bf16 by default (on the CPU the weights' own), or float8_e4m3fn, with ``key_scale`` and ``value_scale``."""
+        attn, weight = self.transformer.h[0].attn, self.lm_head.weight
+        dtype = (torch.bfloat16 if weight.is_cuda else weight.dtype) if dtype is None else dtype
+        return PagedKVCache(len(self.transformer.h), attn.n_kv_head, attn.head_dim, pages=pages, page_size=page_size,
+                            max_tokens=self.config.block_size if max_tokens is None else max_tokens, dtype=dtype, device=weight.device, **scales)
+
+    @torch.no_grad()
+    def step(self, input_ids: torch.Tensor, cache: PagedKVCache, batch: PagedBatch, last_only: bool = False) -> dict:
+        """Logits of new tokens [rows] (the sequences of the batch one behind the other), which are put into the cache: single tokens, drafts,
+        chunks of prompts.  ``last_only``: of each sequence's last new token alone."""
+        z = self._hidden(input_ids, cache, batch)
+        if last_only:
+            z = z[(batch.offsets[1:].long() - 1).clamp(min=0)]
+        return {"logits": self.lm_head(z)}
+
+    @torch.no_grad()
+    def verify_step(self, input_ids: torch.Tensor, cache: PagedKVCache, batch: PagedBatch, uniforms: torch.Tensor, draft_logits: torch.Tensor | None = None,
+                    temperature: float = 1.0) -> VerifiedDrafts:
+        """A step over drafts: of each sequence the last token that is sure and what was drafted behind it.  How many drafts hold, and the token behind
+        them (see ``verify_drafts``); ``cache.shorten`` takes the others out again."""
+        logits = self.step(input_ids, cache, batch)["logits"]
+        return verify_drafts(logits, input_ids, batch.offsets, uniforms, draft_logits=draft_logits, temperature=temperature, n_vocab=self.config.vocab_size)
 
     def score(self, input_ids: torch.Tensor, targets: torch.Tensor | None = None, top_k: int = 0, temperature: float = 1.0,
               ignore_index: int = -100) -> TokenLogProbs:
@@ -141,6 +173,6 @@ class GPT2(_DecoderLM):
         })
         self._finish(config)
 
-    def embed(self, input_ids: torch.Tensor) -> torch.Tensor:
-        pos = torch.arange(input_ids.shape[1], device=input_ids.device)
+    def embed(self, input_ids: torch.Tensor, batch: PagedBatch | None = None) -> torch.Tensor:
+        pos = torch.arange(input_ids.shape[1], device=input_ids.device) if batch is None else batch.positions(input_ids.shape[0])
         return self.transformer.wte(input_ids) + self.transformer.wpe(pos)

@@ -10,10 +10,12 @@ For inference: inputs that want gradients are refused.
 from __future__ import annotations
 
 
+from typing import NamedTuple
+
 import torch
 
 from .. import native
-from .calls import untraced
+from .calls import untraced, untransformed
 
 E4M3_MAX = 448.0
 
@@ -21,6 +23,11 @@ E4M3_MAX = 448.0
 def _refuse_gradients(what: str, *tensors: "torch.Tensor | None") -> None:
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
         raise ValueError(f"{what} is for inference; an input wants a gradient (torch.no_grad() around the call, or detach it)")
+
+
+def refuse_transforms(what: str) -> None:
+    if not untransformed():
+        raise native.NativeError(f"{what} on the GPU is a call that torch does not see into: no forward-mode derivative, functorch rule or trace of it")
 
 
 def _check(what: str, q, keys, values, pages, offsets, lengths, key_scale, value_scale) -> None:
@@ -139,6 +146,10 @@ def append_kv(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, keys: torch.Ten
     table's reach neither, and their queries are 0.  Two rows of a call must not share a slot.
 
     bf16 on the GPU, one kernel, in head dimensions of 16 to 128 (a multiple of 16).  CPU tensors run as torch operations, in any floating type."""
+    if q.is_cuda and untransformed():
+        out = native.plain_append_kv(q, k, v, keys, values, pages, offsets, lengths, cos, sin, interleaved, q_weight, k_weight, eps, key_scale, value_scale)
+        if out is not None:
+            return out
     _check("append_kv", q, keys, values, pages, offsets, lengths, key_scale, value_scale)
     if k.shape != v.shape or k.shape != (q.shape[0], keys.shape[1], keys.shape[3]) or k.dtype != q.dtype or v.dtype != q.dtype:
         raise ValueError(f"append_kv: k {k.dtype} {tuple(k.shape)} and v {v.dtype} {tuple(v.shape)} beside q {q.dtype} {tuple(q.shape)}, expected "
@@ -152,6 +163,7 @@ def append_kv(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, keys: torch.Ten
     _refuse_gradients("append_kv", q, k, v, keys, values, q_weight, k_weight, cos, sin)
     if not q.is_cuda:
         return _append_plain(q, k, v, keys, values, pages, offsets, lengths, cos, sin, interleaved, q_weight, k_weight, eps, key_scale, value_scale)
+    refuse_transforms("append_kv")
     return native.append_kv(q, k, v, keys, values, pages, offsets, lengths, cos, sin, interleaved, q_weight, k_weight, eps, key_scale, value_scale)
 
 
@@ -169,11 +181,134 @@ def paged_attention(q: torch.Tensor, keys: torch.Tensor, values: torch.Tensor, p
 
     bf16 on the GPU: one kernel for up to 32 rows (tokens times heads of a group) a sequence, another for more, and one that joins parts; sums and maxima
     in fp32, weights rounded to bf16.  The same call answers the same bits.  CPU tensors run as torch operations, in any floating type."""
+    scale = q.shape[-1] ** -0.5 if scale is None and q.dim() and q.shape[-1] else scale
+    if q.is_cuda and untransformed() and scale is not None:
+        out = native.plain_paged_attention(q, keys, values, pages, offsets, lengths, max_new, scale, window, softcap, key_scale, value_scale)
+        if out is not None:
+            return out
     _check("paged_attention", q, keys, values, pages, offsets, lengths, key_scale, value_scale)
-    scale = q.shape[2] ** -0.5 if scale is None else scale
     if not 0.0 < scale <= 1e30 or window < 0 or not (softcap == 0.0 or 1e-3 <= softcap <= 1e6) or (max_new is not None and max_new < 0):
         raise ValueError(f"paged_attention: scale {scale} (above 0, up to 1e30), window {window} (0 or more), softcap {softcap} (0, or 1e-3 to 1e6), max_new {max_new}")
     _refuse_gradients("paged_attention", q, keys, values)
     if not q.is_cuda:
         return _attention_plain(q, keys, values, pages, offsets, lengths, scale, window, softcap, key_scale, value_scale)
+    refuse_transforms("paged_attention")
     return native.paged_attention(q, keys, values, pages, offsets, lengths, max_new, scale, window, softcap, key_scale, value_scale)
+
+
+class PagedBatch(NamedTuple):
+    """The new tokens of a step: what :func:`append_kv` and :func:`paged_attention` are told of them.  ``max_new``: the most of a sequence, None where the
+    program does not know (a captured step whose tensors change)."""
+
+    pages: torch.Tensor
+    offsets: torch.Tensor
+    lengths: torch.Tensor
+    max_new: int | None = None
+
+    def positions(self, rows: int) -> torch.Tensor:
+        """The position of every row's token, 0 for rows behind the last sequence."""
+        row, offsets = torch.arange(rows, device=self.offsets.device), self.offsets.long()
+        if offsets.numel() == 1:
+            return torch.zeros_like(row)
+        seq = torch.searchsorted(offsets[1:], row, right=True)
+        live, seq = seq < offsets.numel() - 1, seq.clamp(max=offsets.numel() - 2)
+        position = self.lengths.long()[seq] - offsets[seq + 1] + row
+        return torch.where(live, position.clamp(min=0), torch.zeros_like(row))
+
+
+class PagedLayer(NamedTuple):
+    """One layer's part of a cache, and a batch."""
+
+    keys: torch.Tensor
+    values: torch.Tensor
+    key_scale: torch.Tensor | None
+    value_scale: torch.Tensor | None
+    batch: PagedBatch
+    cache: "PagedKVCache"
+
+
+class PagedKVCache:
+    """Keys and values of all layers of a decoder in pages, and which sequence has which of them.
+
+    ``max_tokens`` bounds a sequence: tables have room for that many.  dtype: bf16 or float8_e4m3fn on the GPU; a code of the latter stands for code *
+    ``key_scale`` (``value_scale``), by default 1 / 16, at which values of up to 28 are kept and a normal one has three bits behind its leading one down to
+    2^-10.  The book-keeping is the host's; pages are handed out when a batch is made of new tokens."""
+
+    def __init__(self, n_layer: int, kv_heads: int, head_dim: int, *, pages: int, page_size: int = 64, max_tokens: int | None = None,
+                 dtype: torch.dtype = torch.bfloat16, device: "torch.device | str" = "cuda", key_scale: float = 1 / 16, value_scale: float = 1 / 16):
+        if page_size < 1 or page_size & (page_size - 1):
+            raise ValueError(f"pages of {page_size} tokens (a power of two)")
+        if n_layer < 1 or kv_heads < 1 or head_dim < 1 or pages < 1:
+            raise ValueError(f"a cache of {n_layer} layers, {kv_heads} heads of {head_dim} and {pages} pages")
+        self.page_size, self.device = page_size, torch.device(device)
+        self.max_tokens = pages * page_size if max_tokens is None else max_tokens
+        self.width = -(-self.max_tokens // page_size)
+        shape = (n_layer, pages, kv_heads, page_size, head_dim)
+        self.keys, self.values = (torch.zeros(shape, dtype=dtype, device=self.device) for _ in range(2))
+        scales = dtype == torch.float8_e4m3fn
+        self.key_scale = torch.full((n_layer, kv_heads), key_scale, dtype=torch.float32, device=self.device) if scales else None
+        self.value_scale = torch.full((n_layer, kv_heads), value_scale, dtype=torch.float32, device=self.device) if scales else None
+        self._free = list(range(pages - 1, -1, -1))
+        self._pages: dict[int, list[int]] = {}
+        self._length: dict[int, int] = {}
+        self._next = 0
+        self._angles: dict[tuple, tuple] = {}
+
+    def add(self) -> int:
+        """A new sequence without tokens."""
+        s, self._next = self._next, self._next + 1
+        self._pages[s], self._length[s] = [], 0
+        return s
+
+    def length(self, sequence: int) -> int:
+        return self._length[sequence]
+
+    @property
+    def free_pages(self) -> int:
+        return len(self._free)
+
+    def shorten(self, sequence: int, length: int) -> None:
+        """The sequence's first ``length`` tokens are kept (drafts that were refused go, say); pages that hold none of them are free again."""
+        if not 0 <= length <= self._length[sequence]:
+            raise ValueError(f"sequence {sequence} has {self._length[sequence]} tokens, not {length}")
+        self._length[sequence] = length
+        kept = -(-length // self.page_size)
+        while len(self._pages[sequence]) > kept:
+            self._free.append(self._pages[sequence].pop())
+
+    def remove(self, sequence: int) -> None:
+        self.shorten(sequence, 0)
+        del self._pages[sequence], self._length[sequence]
+
+    def batch(self, sequences: "list[int]", new: "list[int]") -> PagedBatch:
+        """Room for ``new`` more tokens of each of ``sequences``, and the batch of them in this order.  Refused as a whole where pages run out."""
+        if len(sequences) != len(new) or len(set(sequences)) != len(sequences) or any(n < 0 for n in new):
+            raise ValueError(f"{len(sequences)} sequences, each once, and {len(new)} numbers of new tokens")
+        need = []
+        for s, n in zip(sequences, new):
+            if self._length[s] + n > self.max_tokens:
+                raise ValueError(f"sequence {s}: {self._length[s]} tokens and {n} new ones, of {self.max_tokens}")
+            need.append(-(-(self._length[s] + n) // self.page_size) - len(self._pages[s]))
+        if sum(need) > len(self._free):
+            raise RuntimeError(f"{sum(need)} pages wanted, {len(self._free)} are free")
+        table = torch.zeros((len(sequences), self.width), dtype=torch.int32)
+        offsets, lengths = [0], []
+        for i, (s, n, k) in enumerate(zip(sequences, new, need)):
+            self._pages[s] += [self._free.pop() for _ in range(k)]
+            self._length[s] += n
+            table[i, :len(self._pages[s])] = torch.tensor(self._pages[s], dtype=torch.int32)
+            offsets.append(offsets[-1] + n)
+            lengths.append(self._length[s])
+        ints = lambda v: torch.tensor(v, dtype=torch.int32).to(self.device)
+        return PagedBatch(table.to(self.device), ints(offsets), ints(lengths), max(new, default=0))
+
+    def layer(self, i: int, batch: PagedBatch) -> PagedLayer:
+        scale = lambda t: None if t is None else t[i]
+        return PagedLayer(self.keys[i], self.values[i], scale(self.key_scale), scale(self.value_scale), batch, self)
+
+    def angles(self, tables, head_dim: int, theta: float) -> tuple[torch.Tensor, torch.Tensor]:
+        """``tables(head_dim, positions, theta, device)`` for every position that the tables reach, made once."""
+        key = (head_dim, theta)
+        if key not in self._angles:
+            self._angles[key] = tables(head_dim, self.width * self.page_size, theta, self.device)
+        return self._angles[key]

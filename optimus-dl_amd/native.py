@@ -1933,6 +1933,30 @@ def _strides(t: torch.Tensor):
     return (ctypes.c_int64 * 2)(*t.stride()[:2])
 
 
+def plain_append_kv(*args):
+    """:func:`append_kv` of the C++ side; None where the call is not a plain one, or refused."""
+    if not _here(args[0]):
+        return None
+    load()
+    return _host.append_kv(*args, _stream())
+
+
+def plain_paged_attention(*args):
+    """:func:`paged_attention` of the C++ side; None where the call is not a plain one, or refused."""
+    if not _here(args[0]):
+        return None
+    load()
+    return _host.paged_attention(*args, _stream())
+
+
+def plain_verify_drafts(*args):
+    """:func:`verify_drafts` of the C++ side; None where the call is not a plain one, or refused."""
+    if not _here(args[0]):
+        return None
+    load()
+    return _host.verify_drafts(*args, _stream())
+
+
 def append_kv(q, k, v, keys, values, pages, offsets, lengths, cos=None, sin=None, interleaved: bool = True, q_weight=None, k_weight=None,
               eps: float = 1e-6, key_scale=None, value_scale=None) -> torch.Tensor:
     """New queries and keys [rows, heads, head_dim] normed and rotated, keys and values put into the cache (``odl_fp8_append_kv``).  -> q, dense."""

@@ -6,9 +6,10 @@
 // would differ.  In fp32 that is one in a hundred for 10^5 tokens; so exponentials and sums are held in 64 bits (2^r by its series to the
 // eleventh power, 6e-15), which the vector units do at the rate that memory delivers: some 20 operations an element.
 //
-// Two launches.  The first reads every row once, in parts, and leaves a maximum and a sum of each.  In the second every sequence has a block for each part of a
-// row: each works out for itself which draft is the first to be refused, sums what is left of its part of that row (again from memory: one row
-// of each sequence), and the last to arrive finds the part and the token in it.  T = 0: p is all on the largest logit, the lowest of them.
+// Three launches.  The first reads every row once, in parts, and leaves a maximum and a sum of each.  In the second every sequence has a block for each
+// part of a row: each works out for itself which draft is the first to be refused and sums what is left of its part of that row (again from
+// memory: one row of each sequence).  In the third a block a sequence finds the part that holds the number drawn and the token in it.
+// T = 0: p is all on the largest logit, the lowest of them, and the second launch ends it.
 #include "common.h"
 
 #pragma clang fp contract(off)
@@ -38,7 +39,7 @@ struct Verify {
     float *logprobs;
     Part *part;                                  // [2][rows][parts]
     double *left;                                // [seqs][parts]
-    uint32_t *arrived;                           // [seqs]
+    struct Stop *stop;                           // [seqs]
 };
 
 // 2^t
@@ -88,22 +89,55 @@ __device__ __forceinline__ const void *row_at(const void *base, int64_t row, int
     return static_cast<const uint8_t *>(base) + row * stride * (DT == ODL_BF16 ? 2 : 4);
 }
 
-// One of two parts as one.
-__device__ __forceinline__ void join(Part &a, double s, float m, int at, double c) {
-    const float top = fmaxf(a.m, m);
-    if (top == -INFINITY) { a.s += s; return; }                 // (sums of NaN rows stay NaN)
-    a.at = a.m == m ? min(a.at, at) : a.m > m ? a.at : at;
-    a.s = (a.m == top ? a.s : a.s * weight(a.m, top, c)) + (m == top ? s : s * weight(m, top, c));
-    a.m = top;
-}
-__device__ __forceinline__ void wave_join(Part &a, double c) {
+// A value of another lane of a row of 16 (a DPP control word), and over the wave what F makes of all lanes' values, in every lane.
+template <int CTRL, class T>
+__device__ __forceinline__ T from_dpp(T v) {
+    uint32_t w[sizeof(T) / 4];
+    __builtin_memcpy(w, &v, sizeof(T));
 #pragma unroll
-    for (int off = kWave / 2; off > 0; off >>= 1) {
-        const double s = __shfl_xor(a.s, off, kWave);
-        const float m = __shfl_xor(a.m, off, kWave);
-        const int at = __shfl_xor(a.at, off, kWave);
-        join(a, s, m, at, c);
+    for (int i = 0; i < (int)(sizeof(T) / 4); ++i) w[i] = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)w[i], CTRL, 0xf, 0xf, false);
+    __builtin_memcpy(&v, w, sizeof(T));
+    return v;
+}
+template <class T, class F>
+__device__ __forceinline__ T over_wave(T v, F f) {
+    v = f(v, from_dpp<0xB1>(v));                 // lane ^ 1, ^ 2, the other quad of 8, the other half of 16
+    v = f(v, from_dpp<0x4E>(v));
+    v = f(v, from_dpp<0x141>(v));
+    v = f(v, from_dpp<0x140>(v));
+    uint32_t w[sizeof(T) / 4], a[sizeof(T) / 4], b[sizeof(T) / 4];
+    T x, y;
+    __builtin_memcpy(w, &v, sizeof(T));
+#pragma unroll
+    for (int i = 0; i < (int)(sizeof(T) / 4); ++i) {
+        const auto r = __builtin_amdgcn_permlane16_swap(w[i], w[i], false, false);
+        a[i] = r[0], b[i] = r[1];
     }
+    __builtin_memcpy(&x, a, sizeof(T));
+    __builtin_memcpy(&y, b, sizeof(T));
+    v = f(x, y);
+    __builtin_memcpy(w, &v, sizeof(T));
+#pragma unroll
+    for (int i = 0; i < (int)(sizeof(T) / 4); ++i) {
+        const auto r = __builtin_amdgcn_permlane32_swap(w[i], w[i], false, false);
+        a[i] = r[0], b[i] = r[1];
+    }
+    __builtin_memcpy(&x, a, sizeof(T));
+    __builtin_memcpy(&y, b, sizeof(T));
+    return f(x, y);
+}
+__device__ __forceinline__ double wave_sum(double v) { return over_wave(v, [](double a, double b) { return a + b; }); }
+__device__ __forceinline__ float wave_max(float v) { return over_wave(v, [](float a, float b) { return fmaxf(a, b); }); }
+__device__ __forceinline__ int wave_min(int v) { return over_wave(v, [](int a, int b) { return min(a, b); }); }
+
+// The parts of a wave's lanes as one, in every lane.  (Sums of NaN rows stay NaN.)
+template <bool GREEDY>
+__device__ __forceinline__ Part wave_join(const Part &a, double c) {
+    Part r = {a.s, wave_max(a.m), INT32_MAX};
+    if (r.m != -INFINITY) r.s = a.m == r.m ? a.s : a.s * weight(a.m, r.m, c);
+    r.s = wave_sum(r.s);
+    if (GREEDY) r.at = wave_min(a.m == r.m ? a.at : INT32_MAX);
+    return r;
 }
 
 // The sequence of a row: how many of them end at or in front of it.
@@ -118,9 +152,9 @@ template <int DT, bool GREEDY>
 __global__ __launch_bounds__(kThreads) void draft_sums_kernel(Verify a) {
     __shared__ Part waves[kThreads / kWave];
     const int row = blockIdx.y, part = blockIdx.x, side = blockIdx.z, tid = threadIdx.x;
-    if (side == 0 && part == 0) {
-        if (tid == 0) { a.out[row] = -1; a.logprobs[row] = 0.0f; }
-        for (int s = row * kThreads + tid; s < a.seqs; s += a.rows * kThreads) a.arrived[s] = 0;
+    if (side == 0 && part == 0 && tid == 0) {
+        a.out[row] = -1;
+        a.logprobs[row] = 0.0f;
     }
     const int s = sequence_of(a.offsets, a.seqs, row);
     if (s >= a.seqs || (side == 1 && a.offsets[s + 1] == row + 1)) return;               // (nobody reads the drafter's answer to the last token)
@@ -163,174 +197,203 @@ __global__ __launch_bounds__(kThreads) void draft_sums_kernel(Verify a) {
             }
     }
     if (odd) mine.s = __builtin_nan("");
-    wave_join(mine, a.c);
+    mine = wave_join<GREEDY>(mine, a.c);
     if (tid % kWave == 0) waves[tid / kWave] = mine;
     __syncthreads();
-    if (tid) return;
-    for (int w = 1; w < kThreads / kWave; ++w) join(mine, waves[w].s, waves[w].m, waves[w].at, a.c);
-    a.part[((int64_t)side * a.rows + row) * a.parts + part] = mine;
+    if (tid >= kWave) return;
+    mine = {0.0, -INFINITY, INT32_MAX};
+    if (tid < kThreads / kWave) mine = waves[tid];
+    mine = wave_join<GREEDY>(mine, a.c);
+    if (tid == 0) a.part[((int64_t)side * a.rows + row) * a.parts + part] = mine;
 }
 
-// A row's parts as one, in every lane of a wave.
-__device__ __forceinline__ Part whole(const Verify &a, int side, int row) {
-    const Part *p = a.part + ((int64_t)side * a.rows + row) * a.parts;
-    const int lane = threadIdx.x % kWave;
-    Part r = {0.0, -INFINITY, INT32_MAX};
-    for (int i = lane; i < a.parts; i += kWave) join(r, p[i].s, p[i].m, p[i].at, a.c);
-    wave_join(r, a.c);
-    return r;
-}
+// A row's parts as one, in every lane of a wave: the loads, and what they make.
+struct Parts {
+    Part p[kMaxParts / kWave];
+    __device__ __forceinline__ void load(const Verify &a, int side, int row) {
+        const Part *from = a.part + ((int64_t)side * a.rows + row) * a.parts;
+        const int lane = threadIdx.x % kWave;
+#pragma unroll
+        for (int i = 0; i < kMaxParts / kWave; ++i) {
+            p[i] = {0.0, -INFINITY, INT32_MAX};
+            if (lane + i * kWave < a.parts) p[i] = from[lane + i * kWave];
+        }
+    }
+    template <bool GREEDY>
+    __device__ __forceinline__ Part whole(const Verify &a) const {
+        Part r = p[0];
+#pragma unroll
+        for (int i = 1; i < kMaxParts / kWave; ++i)
+            if (a.parts > i * kWave) {
+                const float top = fmaxf(r.m, p[i].m);
+                if (top != -INFINITY) r.s = (r.m == top ? r.s : r.s * weight(r.m, top, a.c)) + (p[i].m == top ? p[i].s : p[i].s * weight(p[i].m, top, a.c));
+                else r.s += p[i].s;
+                if (GREEDY) r.at = r.m == p[i].m ? min(r.at, p[i].at) : r.m > p[i].m ? r.at : p[i].at;
+                r.m = top;
+            }
+        return wave_join<GREEDY>(r, a.c);
+    }
+};
+
+__device__ __forceinline__ bool sound(const Part &p) { return p.s > 0.0 && p.s < INFINITY; }
 
 struct Row {                                     // a distribution: the maximum of its logits, and 1 / sum
     float m;
     double by;
 };
 struct Stop {                                    // where a sequence stops and what is drawn from there
-    int row, draft;                              // draft: what the drafter had there, -1 where there is none to take off
     Row p, q;
-    int residual;                                // 0: p, 1: p without the draft, 2: max(p - q, 0)
+    int row, draft;                              // draft: what is to be taken off p as a whole, -1 where nothing is
+    int residual, number;                        // residual: max(p - q, 0) and not p; number: the row whose number draws, -1: the answer is there
 };
 
-__device__ __forceinline__ bool sound(const Part &p) { return p.s > 0.0 && p.s < INFINITY; }
-
-// What is left of eight elements.
-template <int DT>
-__device__ __forceinline__ void left8(const Verify &a, const Stop &st, int residual, int i, int end, double (&r)[8]) {
-    float x[8], y[8];
-    load8<DT>(row_at<DT>(a.logits, st.row, a.stride), i, end, x);
-    if (residual == 2) load8<DT>(row_at<DT>(a.drafts, st.row, a.draft_stride), i, end, y);
+// What is left of a lane's eight elements of each of four pieces from column `base` on (32 columns a lane in all, loaded at once): f(piece, element, it).
+template <int DT, class F>
+__device__ __forceinline__ void left32(const Verify &a, const Stop &st, int base, int end, F f) {
+    const void *p = row_at<DT>(a.logits, st.row, a.stride), *q = row_at<DT>(a.drafts, st.row, a.draft_stride);
+    float x[4][8], y[4][8];
 #pragma unroll
-    for (int k = 0; k < 8; ++k) {
-        r[k] = i + k < end ? weight(x[k], st.p.m, a.c) * st.p.by : 0.0;
-        if (residual == 2) r[k] = i + k < end ? fmax(r[k] - weight(y[k], st.q.m, a.c) * st.q.by, 0.0) : 0.0;
-        if (residual == 1 && i + k == st.draft) r[k] = 0.0;
+    for (int k = 0; k < 4; ++k) load8<DT>(p, base + k * kPiece + threadIdx.x * 8, end, x[k]);
+    if (st.residual)
+#pragma unroll
+        for (int k = 0; k < 4; ++k) load8<DT>(q, base + k * kPiece + threadIdx.x * 8, end, y[k]);
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+        const int at = base + k * kPiece;
+        if (at >= end) break;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            double r = weight(x[k][i], st.p.m, a.c) * st.p.by;
+            if (st.residual) r = fmax(r - weight(y[k][i], st.q.m, a.c) * st.q.by, 0.0);
+            if (at + (int)threadIdx.x * 8 + i == st.draft) r = 0.0;
+            f(k, i, r);
+        }
     }
 }
 
-__device__ __forceinline__ double block_sum(double v, double *lds) {
-#pragma unroll
-    for (int off = kWave / 2; off > 0; off >>= 1) v += __shfl_xor(v, off, kWave);
-    __syncthreads();
-    if (threadIdx.x % kWave == 0) lds[threadIdx.x / kWave] = v;
-    __syncthreads();
-    double s = lds[0];
-#pragma unroll
-    for (int w = 1; w < kThreads / kWave; ++w) s += lds[w];
-    return s;
-}
-
+// How far a sequence's drafts hold, and what is left of a part of the row behind which it stops.
 template <int DT, bool GREEDY>
-__global__ __launch_bounds__(kThreads) void draft_verify_kernel(Verify a) {
+__global__ __launch_bounds__(kThreads) void draft_stop_kernel(Verify a) {
+    constexpr int kWaves = kThreads / kWave, kBoth = 2;        // rows a wave looks at at a time
     __shared__ Stop stop;
-    __shared__ int best, agreed[kThreads / kWave], chosen, last_one;
-    __shared__ Part found[kThreads / kWave][2];
-    __shared__ double sums[kThreads / kWave], lefts[kMaxParts];
+    __shared__ bool agreed[kBoth * kWaves];
+    __shared__ Part found[kBoth * kWaves][2];
+    __shared__ double sums[kWaves];
     const int s = blockIdx.y, part = blockIdx.x, tid = threadIdx.x, wave = tid / kWave, lane = tid % kWave;
     const int first = min(max(a.offsets[s], 0), a.rows), n = min(a.offsets[s + 1], a.rows) - first;
     if (n <= 0) {
-        if (part == 0 && tid == 0) a.accepted[s] = 0;
+        if (part == 0 && tid == 0) {
+            a.accepted[s] = 0;
+            a.stop[s].number = -1;
+        }
         return;
     }
-    // how far the drafts are accepted: a wave a row
-    int at = 0;
-    for (;; at += kThreads / kWave) {
-        const int j = at + wave, row = first + j;
-        bool yes = false;
-        int64_t draft = -1;
-        float logprob = 0.0f;
-        if (j < n) {
-            const Part p = whole(a, 0, row);
-            Part q = {0.0, 0.0f, 0};
-            if (j < n - 1) {
-                const int64_t d = a.tokens[row + 1];
-                const bool known = d >= 0 && d < a.vocab;
-                if (GREEDY) {
-                    yes = sound(p) && d == p.at;
-                } else {
-                    const float x = known ? element<DT>(row_at<DT>(a.logits, row, a.stride), d) : -INFINITY;
-                    const double of_p = known ? weight(x, p.m, a.c) / p.s : 0.0;
-                    double of_q = 1.0;
-                    if (a.drafts) {
-                        q = whole(a, 1, row);
-                        of_q = known ? weight(element<DT>(row_at<DT>(a.drafts, row, a.draft_stride), d), q.m, a.c) / q.s : 1.0;
-                    }
-                    yes = sound(p) && (double)a.uniforms[row] * of_q < of_p;
-                }
-                if (yes && part == 0) {
-                    draft = d;
-                    logprob = (float)(((double)element<DT>(row_at<DT>(a.logits, row, a.stride), d) - (double)p.m) * a.c * 0.69314718055994530942 - log(p.s));
-                }
-            }
-            if (lane == 0) found[wave][0] = p, found[wave][1] = q;
+    for (int at = 0;; at += kBoth * kWaves) {
+        Parts of_row[kBoth], of_draft[kBoth];
+        int64_t draft[kBoth];
+        float x[kBoth], y[kBoth], logprob[kBoth];
+#pragma unroll
+        for (int b = 0; b < kBoth; ++b) {
+            const int j = at + b * kWaves + wave, row = first + j;
+            draft[b] = j < n - 1 ? a.tokens[row + 1] : -1;
+            if (j < n) of_row[b].load(a, 0, row);
+            if (!GREEDY && a.drafts && j < n - 1) of_draft[b].load(a, 1, row);
+            if (draft[b] >= a.vocab) draft[b] = -1;
         }
-        if (lane == 0) agreed[wave] = yes;
+#pragma unroll
+        for (int b = 0; b < kBoth; ++b) {
+            const int row = first + at + b * kWaves + wave;
+            if (draft[b] < 0) continue;
+            x[b] = element<DT>(row_at<DT>(a.logits, row, a.stride), draft[b]);
+            if (!GREEDY && a.drafts) y[b] = element<DT>(row_at<DT>(a.drafts, row, a.draft_stride), draft[b]);
+        }
+#pragma unroll
+        for (int b = 0; b < kBoth; ++b) {
+            const int j = at + b * kWaves + wave, row = first + j;
+            bool yes = false;
+            if (j < n) {
+                const Part p = of_row[b].template whole<GREEDY>(a);
+                Part q = {0.0, 0.0f, 0};
+                if (!GREEDY && a.drafts && j < n - 1) q = of_draft[b].template whole<GREEDY>(a);
+                if (draft[b] >= 0 && sound(p)) {
+                    if (GREEDY) yes = draft[b] == p.at;
+                    else yes = (double)a.uniforms[row] * (a.drafts ? weight(y[b], q.m, a.c) / q.s : 1.0) < weight(x[b], p.m, a.c) / p.s;
+                    if (yes && part == 0) logprob[b] = (float)(((double)x[b] - (double)p.m) * a.c * 0.69314718055994530942 - log(p.s));
+                }
+                if (lane == 0) found[b * kWaves + wave][0] = p, found[b * kWaves + wave][1] = q;
+            }
+            if (lane == 0) agreed[b * kWaves + wave] = yes;
+        }
         __syncthreads();
         int w = 0;
-        while (w < kThreads / kWave && agreed[w]) ++w;
-        if (part == 0 && lane == 0 && wave < w) {
-            a.out[row] = draft;
-            a.logprobs[row] = logprob;
-        }
-        if (w < kThreads / kWave) {
-            at += w;
+        while (w < kBoth * kWaves && agreed[w]) ++w;
+#pragma unroll
+        for (int b = 0; b < kBoth; ++b)
+            if (part == 0 && lane == 0 && b * kWaves + wave < w) {
+                const int row = first + at + b * kWaves + wave;
+                a.out[row] = draft[b];
+                a.logprobs[row] = logprob[b];
+            }
+        if (w < kBoth * kWaves) {
             if (tid == 0) {
                 const Part p = found[w][0], q = found[w][1];
-                const int row = first + at;
-                const int64_t d = at < n - 1 ? a.tokens[row + 1] : -1;
+                const int j = at + w, row = first + j;
+                const int64_t d = j < n - 1 ? a.tokens[row + 1] : -1;
                 stop.row = row;
-                stop.draft = d >= 0 && d < a.vocab ? (int)d : -1;
+                stop.draft = d >= 0 && d < a.vocab && !a.drafts ? (int)d : -1;
                 stop.p = {p.m, 1.0 / p.s};
                 stop.q = {q.m, 1.0 / q.s};
-                stop.residual = at == n - 1 ? 0 : !a.drafts ? 1 : sound(q) ? 2 : 0;
-                best = sound(p) ? p.at : -1;
-                if (!sound(p)) stop.residual = -1;
+                stop.residual = j < n - 1 && a.drafts && sound(q);
+                stop.number = GREEDY || !sound(p) ? -1 : first + n - 1;
+                if (part == 0) {
+                    a.accepted[s] = j;
+                    if (GREEDY || !sound(p)) {
+                        a.out[row] = sound(p) ? p.at : -1;
+                        a.logprobs[row] = sound(p) ? (float)-log(p.s) : __builtin_nanf("");
+                    }
+                    a.stop[s] = stop;
+                }
             }
             break;
         }
         __syncthreads();
     }
     __syncthreads();
+    if (GREEDY || stop.number < 0) return;
     const Stop st = stop;
-    const double *mine = a.left + (int64_t)s * a.parts;
-    if (GREEDY || st.residual < 0) {
-        if (part == 0 && tid == 0) {
-            a.accepted[s] = at;
-            a.out[st.row] = best;
-            a.logprobs[st.row] = best < 0 ? __builtin_nanf("") : (float)log(st.p.by);
+    double sum = 0.0;
+    if (!st.residual && st.draft < 0) {          // p as it is: summed already
+        if (tid == 0) {
+            const Part p = a.part[(int64_t)st.row * a.parts + part];
+            a.left[(int64_t)s * a.parts + part] = p.m == -INFINITY ? 0.0 : p.s * weight(p.m, st.p.m, a.c) * st.p.by;
         }
         return;
     }
-    // what is left of this part of the row
     const int begin = part * a.span, end = min(begin + a.span, a.vocab);
-    double sum = 0.0;
-    if (st.residual == 0) {
-        const Part p = a.part[(int64_t)st.row * a.parts + part];
-        sum = p.m == -INFINITY ? 0.0 : p.s * weight(p.m, st.p.m, a.c) * st.p.by;
-    } else {
-        for (int i = begin + tid * 8; i < end; i += kPiece) {
-            double r[8];
-            left8<DT>(a, st, st.residual, i, end, r);
-#pragma unroll
-            for (int k = 0; k < 8; ++k) sum += r[k];
-        }
-        sum = block_sum(sum, sums);
-    }
-    if (tid == 0) {
-        a.left[(int64_t)s * a.parts + part] = sum;
-        __threadfence();
-        last_one = atomicAdd(a.arrived + s, 1u) == (uint32_t)a.parts - 1;
-        __threadfence();
-    }
+    for (int base = begin; base < end; base += 4 * kPiece) left32<DT>(a, st, base, end, [&](int, int, double r) { sum += r; });
+    sum = wave_sum(sum);
+    if (lane == 0) sums[wave] = sum;
     __syncthreads();
-    if (!last_one) return;
-    // the last block of the sequence: the part that holds the number drawn, and the token in it
-    for (int i = tid; i < a.parts; i += kThreads) lefts[i] = __hip_atomic_load(mine + i, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    if (tid == 0) a.left[(int64_t)s * a.parts + part] = (sums[0] + sums[1]) + (sums[2] + sums[3]);
+}
+
+// The part that holds the number drawn, and the token in it.
+template <int DT>
+__global__ __launch_bounds__(kThreads) void draft_pick_kernel(Verify a) {
+    constexpr int kWaves = kThreads / kWave;
+    __shared__ double sums[kWaves][4], lefts[kMaxParts];
+    __shared__ int hits[kWaves];
+    const int s = blockIdx.x, tid = threadIdx.x, wave = tid / kWave, lane = tid % kWave;
+    Stop st = a.stop[s];
+    for (int i = tid; i < a.parts; i += kThreads) lefts[i] = a.left[(int64_t)s * a.parts + i];
+    if (st.number < 0) return;                   // (what else the workspace holds of this sequence is of no call)
+    const double u = a.uniforms[st.number];
     __syncthreads();
-    int residual = st.residual;
     double total = 0.0;
     for (int i = 0; i < a.parts; ++i) total += lefts[i];
     if (!(total > 0.0)) {                        // nothing is left (p and q are the same): p itself
-        residual = 0;
+        st.residual = 0;
+        st.draft = -1;
         __syncthreads();
         for (int i = tid; i < a.parts; i += kThreads) {
             const Part p = a.part[(int64_t)st.row * a.parts + i];
@@ -340,7 +403,7 @@ __global__ __launch_bounds__(kThreads) void draft_verify_kernel(Verify a) {
         total = 0.0;
         for (int i = 0; i < a.parts; ++i) total += lefts[i];
     }
-    const double want = (double)a.uniforms[first + n - 1] * total;
+    const double want = u * total;
     double before = 0.0;
     int in = -1, some = 0;
     for (int i = 0; i < a.parts && in < 0; ++i) {
@@ -353,67 +416,65 @@ __global__ __launch_bounds__(kThreads) void draft_verify_kernel(Verify a) {
         before -= lefts[some];
     }
     const int from = in * a.span, to = min(from + a.span, a.vocab);
-    if (tid == 0) chosen = -1;
-    int tail = -1;                               // the last token of this lane's that has any weight
-    for (int base = from; base < to; base += kPiece) {
-        double r[8], local = 0.0;
-        const int i0 = base + tid * 8;
-        left8<DT>(a, st, residual, i0, to, r);
+    int hit = INT32_MAX, tail = -1;              // the token, and the last that has any weight
+    for (int base = from; base < to && hit == INT32_MAX; base += 4 * kPiece) {
+        double r[4][8], local[4] = {0.0, 0.0, 0.0, 0.0}, upto[4];
 #pragma unroll
-        for (int k = 0; k < 8; ++k) {
-            local += r[k];
-            if (r[k] > 0.0) tail = i0 + k;
-        }
-        double upto = local;
+        for (int k = 0; k < 4; ++k)
 #pragma unroll
-        for (int off = 1; off < kWave; off <<= 1) {
-            const double v = __shfl_up(upto, off, kWave);
-            if (lane >= off) upto += v;
+            for (int i = 0; i < 8; ++i) r[k][i] = 0.0;
+        left32<DT>(a, st, base, to, [&](int k, int i, double v) {
+            r[k][i] = v;
+            local[k] += v;
+            if (v > 0.0) tail = base + k * kPiece + tid * 8 + i;
+        });
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            upto[k] = local[k];
+#pragma unroll
+            for (int off = 1; off < kWave; off <<= 1) {
+                const double v = __shfl_up(upto[k], off, kWave);
+                if (lane >= off) upto[k] += v;
+            }
         }
         __syncthreads();
-        if (lane == kWave - 1) sums[wave] = upto;
-        __syncthreads();
-        double behind = before;
-        for (int w = 0; w < wave; ++w) behind += sums[w];
-        const double all = before + ((sums[0] + sums[1]) + (sums[2] + sums[3]));
-        double c = behind + (upto - local);
-        int hit = INT32_MAX;
+        if (lane == kWave - 1)
 #pragma unroll
-        for (int k = 0; k < 8; ++k) {
-            c += r[k];
-            if (hit == INT32_MAX && c > want && r[k] > 0.0) hit = i0 + k;
-        }
-#pragma unroll
-        for (int off = kWave / 2; off > 0; off >>= 1) hit = min(hit, __shfl_xor(hit, off, kWave));
-        if (lane == 0) agreed[wave] = hit;
+            for (int k = 0; k < 4; ++k) sums[wave][k] = upto[k];
         __syncthreads();
-        hit = min(min(agreed[0], agreed[1]), min(agreed[2], agreed[3]));
-        if (hit != INT32_MAX) {
-            if (tid == 0) chosen = hit;
-            break;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            double c = before + (upto[k] - local[k]);
+            for (int w = 0; w < wave; ++w) c += sums[w][k];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                c += r[k][i];
+                if (c > want && r[k][i] > 0.0) hit = min(hit, base + k * kPiece + tid * 8 + i);
+            }
+            before += (sums[0][k] + sums[1][k]) + (sums[2][k] + sums[3][k]);
         }
-        before = all;
+        hit = wave_min(hit);
+        if (lane == 0) hits[wave] = hit;
+        __syncthreads();
+        hit = min(min(hits[0], hits[1]), min(hits[2], hits[3]));
     }
-    __syncthreads();
-    if (chosen < 0) {                            // (uniform)
-#pragma unroll
-        for (int off = kWave / 2; off > 0; off >>= 1) tail = max(tail, __shfl_xor(tail, off, kWave));
-        if (lane == 0) agreed[wave] = tail;
+    if (hit == INT32_MAX) {                      // (uniform)
+        tail = -wave_min(-tail);
         __syncthreads();
-        if (tid == 0) chosen = max(max(agreed[0], agreed[1]), max(agreed[2], agreed[3]));
+        if (lane == 0) hits[wave] = tail;
+        __syncthreads();
+        hit = max(max(hits[0], hits[1]), max(hits[2], hits[3]));
     }
     if (tid == 0) {
-        a.accepted[s] = at;
-        a.out[st.row] = chosen;
-        const float x = element<DT>(row_at<DT>(a.logits, st.row, a.stride), max(chosen, 0));
+        a.out[st.row] = hit;
+        const float x = element<DT>(row_at<DT>(a.logits, st.row, a.stride), max(hit, 0));
         a.logprobs[st.row] = (float)(((double)x - (double)st.p.m) * a.c * 0.69314718055994530942 + log(st.p.by));
     }
 }
 
-// Parts of a row: so that a call has about four blocks a compute unit, of 2048 columns at least and 8192 where there are enough.
+// Parts of a row: of 8192 columns where that makes two blocks a compute unit, else of 2048.
 int parts_of(int64_t rows, int64_t vocab, int &span) {
-    const int64_t blocks = 4 * (int64_t)device_cu_count();
-    span = rows * ((vocab + 4 * kPiece - 1) / (4 * kPiece)) >= blocks ? 4 * kPiece : kPiece;
+    span = rows * ((vocab + 4 * kPiece - 1) / (4 * kPiece)) >= 2 * (int64_t)device_cu_count() ? 4 * kPiece : kPiece;
     if ((vocab + span - 1) / span > kMaxParts) span = (int)(((vocab + kMaxParts - 1) / kMaxParts + kPiece - 1) / kPiece * kPiece);
     return (int)((vocab + span - 1) / span);
 }
@@ -434,7 +495,7 @@ extern "C" int64_t odl_fp8_verify_drafts_workspace(int64_t rows, int64_t seqs, i
     if (check("odl_fp8_verify_drafts_workspace", rows, seqs, vocab)) return -1;
     int span;
     const int64_t parts = parts_of(rows, vocab, span);
-    return rows * 2 * parts * 4 + seqs * parts * 2 + seqs;
+    return (rows * 2 * parts * (int64_t)sizeof(Part) + seqs * (int64_t)(sizeof(Stop) + parts * sizeof(double))) / 4;
 }
 
 extern "C" int odl_fp8_verify_drafts(const void *logits, int64_t stride, const void *draft_logits, int64_t draft_stride, int dtype, int64_t rows, int64_t vocab,
@@ -458,8 +519,8 @@ extern "C" int odl_fp8_verify_drafts(const void *logits, int64_t stride, const v
     a.c = 1.4426950408889634074 / (greedy ? 1.0 : temperature);
     a.accepted = accepted, a.out = out_tokens, a.logprobs = logprobs;
     a.part = reinterpret_cast<Part *>(workspace);
-    a.left = reinterpret_cast<double *>(a.part + 2 * rows * a.parts);
-    a.arrived = reinterpret_cast<uint32_t *>(a.left + seqs * a.parts);
+    a.stop = reinterpret_cast<Stop *>(a.part + 2 * rows * a.parts);
+    a.left = reinterpret_cast<double *>(a.stop + seqs);
     hipStream_t stream = reinterpret_cast<hipStream_t>(stream_);
 #define ODL_VERIFY(KERNEL, GRID)                                                                                              \
     do {                                                                                                                      \
@@ -469,7 +530,11 @@ extern "C" int odl_fp8_verify_drafts(const void *logits, int64_t stride, const v
         else hipLaunchKernelGGL((KERNEL<ODL_F32, false>), GRID, dim3(kThreads), 0, stream, a);                                \
     } while (0)
     if (rows > 0) ODL_VERIFY(draft_sums_kernel, dim3((unsigned)a.parts, (unsigned)rows, a.drafts ? 2u : 1u));
-    if (seqs > 0) ODL_VERIFY(draft_verify_kernel, dim3(greedy ? 1u : (unsigned)a.parts, (unsigned)seqs));
+    if (seqs > 0) ODL_VERIFY(draft_stop_kernel, dim3(greedy || rows == 0 ? 1u : (unsigned)a.parts, (unsigned)seqs));
 #undef ODL_VERIFY
+    if (seqs > 0 && rows > 0 && !greedy) {
+        if (dtype == ODL_BF16) hipLaunchKernelGGL((draft_pick_kernel<ODL_BF16>), dim3((unsigned)seqs), dim3(kThreads), 0, stream, a);
+        else hipLaunchKernelGGL((draft_pick_kernel<ODL_F32>), dim3((unsigned)seqs), dim3(kThreads), 0, stream, a);
+    }
     return check_launch(who);
 }

@@ -146,6 +146,10 @@ __device__ __forceinline__ int swizzle_v(int row) { return D == 128 ? (row & 3) 
 __device__ __forceinline__ void to_lds(uint32_t to, const uint8_t *from) {
     asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(to), "v"(from) : "memory");
 }
+// and from an address of the wave's at a distance of the lane's
+__device__ __forceinline__ void to_lds(uint32_t to, const uint8_t *from, uint32_t at) {
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(to), "v"(at), "s"(from) : "memory");
+}
 __device__ __forceinline__ void all_loads_done() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
 
 __device__ __forceinline__ const uint8_t *shuffled(const uint8_t *p, int lane) {
@@ -184,7 +188,9 @@ __device__ __forceinline__ Place place_of(const Paged &p, int page, int pos, int
 }
 
 // ---------------------------------------------------------------------------------------------------------------- the attention of 32 rows
-enum Mode { kPlain, kMasked, kCareful };
+// A block goes over its keys once; where the sums then say that there are infinities or NaN, which 0 * NaN may have brought to rows that do not see them,
+// it goes over them again with zeros in their places, and once more to add them where they are seen.
+enum Pass { kOnce, kFinite, kOdd };
 
 // exchange with lane ^ 32
 __device__ __forceinline__ float other_half(float v) {
@@ -197,6 +203,8 @@ template <int D, int NB>
 struct Rows32 {
     bf16x8 q[D / 16];
     f32x16 o[D / 32];
+    f32x16 s[NB];                                              // of a tile: scores, weights as fp32
+    bf16x8 w[2 * NB];                                          // and as bf16
     float m, l;                                                // running maximum in powers of two, the sum of this lane's keys against it
 
     __device__ __forceinline__ void start() {
@@ -220,39 +228,39 @@ struct Rows32 {
         }
     }
 
-    // One tile of keys and values at LDS addresses kt and vt.  c: powers of two a unit of a score; where softcap > 0 scores are capped first and in powers
-    // of two then.  kMasked: of seen, bit e says whether the lane's row sees key e + 4 (lane / 32), for e % 8 < 4.  kCareful: infinities and NaN among the
-    // values reach only the rows that see them, row_sees says which (0 * NaN would reach all).
-    template <int MODE>
-    __device__ __forceinline__ void tile(uint32_t kt, uint32_t vt, float c, float cap_in, float cap_out, uint64_t seen, uint64_t row_sees) {
-        constexpr int kPitch = 2 * D;
+    // One tile in three steps.  Scores of the keys at LDS address kt:
+    __device__ __forceinline__ void scores(uint32_t kt) {
         const int lane = threadIdx.x % kWave, h = lane / 32, r = lane % 32;
-        f32x16 s[NB];
-        {
-            const uint32_t at = kt + r * kPitch + 16 * (h ^ swizzle_k<D>(r));
+        const uint32_t at = kt + r * 2 * D + 16 * (h ^ swizzle_k<D>(r));
 #pragma unroll
-            for (int b = 0; b < NB; ++b) s[b] = f32x16{};
+        for (int b = 0; b < NB; ++b) s[b] = f32x16{};
 #pragma unroll
-            for (int d = 0; d < D / 16; ++d) {
-                const lds_u8 *from = (const lds_u8 *)(uintptr_t)(at ^ (32 * d));
-#pragma unroll
-                for (int b = 0; b < NB; ++b)
-                    s[b] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(*(const __attribute__((address_space(3))) bf16x8 *)(from + b * 32 * kPitch), q[d], s[b], 0, 0, 0);
-            }
-        }
-        if (cap_in > 0.0f) {                                   // tanh(x) = 1 - 2 / (e^2x + 1)
+        for (int d = 0; d < D / 16; ++d) {
+            const lds_u8 *from = (const lds_u8 *)(uintptr_t)(at ^ (32 * d));
 #pragma unroll
             for (int b = 0; b < NB; ++b)
-#pragma unroll
-                for (int i = 0; i < 16; ++i)
-                    s[b][i] = cap_out * (1.0f - 2.0f * __builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(s[b][i] * cap_in) + 1.0f));
+                s[b] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(*(const __attribute__((address_space(3))) bf16x8 *)(from + b * 32 * 2 * D), q[d], s[b], 0, 0, 0);
         }
-        if constexpr (MODE != kPlain) {
+    }
+
+    // Scores capped, and then in powers of two: tanh(x) = 1 - 2 / (e^2x + 1).
+    __device__ __forceinline__ void cap(float in, float out) {
 #pragma unroll
-            for (int b = 0; b < NB; ++b)
+        for (int b = 0; b < NB; ++b)
 #pragma unroll
-                for (int i = 0; i < 16; ++i) s[b][i] = (seen >> (32 * b + 8 * (i / 4) + i % 4)) & 1 ? s[b][i] : -INFINITY;
-        }
+            for (int i = 0; i < 16; ++i) s[b][i] = out * (1.0f - 2.0f * __builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(s[b][i] * in) + 1.0f));
+    }
+
+    // Scores of keys that the lane's row does not see go: of seen, bit e is key e + 4 (lane / 32), for e % 8 < 4.
+    __device__ __forceinline__ void hide(uint64_t seen) {
+#pragma unroll
+        for (int b = 0; b < NB; ++b)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) s[b][i] = (uint32_t)(seen >> 32 * b) & 1u << (8 * (i / 4) + i % 4) ? s[b][i] : -INFINITY;
+    }
+
+    // Weights from scores.  c: powers of two a unit of a score.
+    __device__ __forceinline__ void weights(float c) {
         float top = -INFINITY;
 #pragma unroll
         for (int b = 0; b < NB; ++b)
@@ -277,30 +285,61 @@ struct Rows32 {
                 s[b][i] = __builtin_amdgcn_exp2f(__fmaf_rn(s[b][i], c, -against));
                 l += s[b][i];
             }
-        bf16x8 w[2 * NB];
 #pragma unroll
         for (int k = 0; k < 2 * NB; ++k) {
             uint32_t v[4];
 #pragma unroll
             for (int i = 0; i < 4; ++i) v[i] = pack_bf16x2(s[k / 2][8 * (k % 2) + 2 * i], s[k / 2][8 * (k % 2) + 2 * i + 1]);
-            w[k] = __builtin_bit_cast(bf16x8, u32x4{v[0], v[1], v[2], v[3]});
+            u32x4 packed = {v[0], v[1], v[2], v[3]};
+            asm volatile("" : "+v"(packed));                   // (here, and not where they are used first: that is the other half's turn)
+            w[k] = __builtin_bit_cast(bf16x8, packed);
         }
+    }
+
+    // The weighted values at LDS address vt.
+    __device__ __forceinline__ void sums(uint32_t vt) {
         const uint32_t at = value_address(vt);
 #pragma unroll
         for (int k = 0; k < 2 * NB; ++k)
 #pragma unroll
-            for (int d = 0; d < D / 32; ++d) {
-                u32x4 v = values(at, d, k);
-                if constexpr (MODE == kCareful) {
+            for (int d = 0; d < D / 32; ++d)
+                o[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, values(at, d, k)), w[k], o[d], 0, 0, 0);
+    }
+
+    // The weighted values of one tile and the scores of another, both steps' operands four at a time and two groups ahead (left to itself the compiler reads each
+    // where it is used, and waits: 2350 cycles, of which 1024 multiply).
+    __device__ __forceinline__ void sums_and_scores(uint32_t vt, uint32_t kt) {
+        constexpr int kColumns = D / 32, kSums = 2 * NB * kColumns, kGroups = (kSums + D / 16 * NB) / 4, kAhead = 2;
+        static_assert(kSums % 4 == 0 && D / 16 * NB % 4 == 0, "groups");
+        const int lane = threadIdx.x % kWave, h = lane / 32, r = lane % 32;
+        const uint32_t v_at = value_address(vt), k_at = kt + r * 2 * D + 16 * (h ^ swizzle_k<D>(r));
+        u32x4 f[kAhead + 1][4];
+        auto read = [&](int g) {
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        if ((v[i] & 0x7f80u) == 0x7f80u) v[i] &= 0xffff0000u;
-                        if ((v[i] & 0x7f800000u) == 0x7f800000u) v[i] &= 0xffffu;
-                    }
-                }
-                o[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, v), w[k], o[d], 0, 0, 0);
+            for (int i = 0; i < 4; ++i) {
+                const int n = 4 * g + i, m = n - kSums;
+                f[g % (kAhead + 1)][i] = n < kSums ? values(v_at, n % kColumns, n / kColumns)
+                                                   : *(const __attribute__((address_space(3))) u32x4 *)(uintptr_t)((k_at ^ (32 * (m / NB))) + m % NB * 32 * 2 * D);
             }
-        if constexpr (MODE == kCareful) add_odd(vt, row_sees);
+        };
+        auto multiply = [&](int g) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const int n = 4 * g + i, m = n - kSums;
+                const bf16x8 x = __builtin_bit_cast(bf16x8, f[g % (kAhead + 1)][i]);
+                if (n < kSums) o[n % kColumns] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(x, w[n / kColumns], o[n % kColumns], 0, 0, 0);
+                else s[m % NB] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(x, q[m / NB], m < NB ? f32x16{} : s[m % NB], 0, 0, 0);
+            }
+        };
+#pragma unroll
+        for (int g = 0; g < kAhead; ++g) read(g);
+#pragma unroll
+        for (int g = 0; g < kGroups; ++g) {
+            if (g + kAhead < kGroups) read(g + kAhead);
+            __builtin_amdgcn_sched_barrier(0);
+            multiply(g);
+            __builtin_amdgcn_sched_barrier(0);
+        }
     }
 
     // Lane i of 16 reads 4 of 16 columns of key i / 4, and gets 4 keys of column i.
@@ -318,8 +357,8 @@ struct Rows32 {
         return u32x4{a[0], a[1], b[0], b[1]};
     }
 
-    // Infinities and NaN among a tile's values, for the rows that see them: weights are above 0, so they come through as they are.
-    __device__ __forceinline__ void add_odd(uint32_t vt, uint64_t row_sees) {
+    // Infinities and NaN among a tile's values, for the rows that see them (bit k: key k): weights are above 0, so they come through as they are.
+    __device__ __forceinline__ void add_odd(uint32_t vt, uint64_t seen) {
         const int h = threadIdx.x % kWave / 32;
 #pragma unroll 1
         for (int key = 0; key < 32 * NB; ++key) {
@@ -331,7 +370,7 @@ struct Rows32 {
 #pragma unroll
                     for (int z = 0; z < 4; ++z) {
                         const float f = z % 2 ? bf16_hi(v[z / 2]) : bf16_lo(v[z / 2]);
-                        if ((row_sees >> key & 1) && !(__builtin_fabsf(f) < INFINITY)) o[d][4 * i + z] += f;
+                        if ((seen >> key & 1) && !(__builtin_fabsf(f) < INFINITY)) o[d][4 * i + z] += f;
                     }
                 }
         }
@@ -400,59 +439,79 @@ __device__ __forceinline__ Caps caps_of(const Attend &a, int kv_head) {
 }
 
 // ---------------------------------------------------------------------------------------------------------------- keys and values on their way to LDS
-// A wave's KEYS keys of a tile, from their places (lane i has that of key i) to LDS tiles at kt and vt, which begin with the wave's first key `first`.
+// A wave's KEYS rows of a tile of keys or values, `first` to first + KEYS, from their places (lane i has that of the tile's row i) to LDS at `tile`.
 // bf16 goes there directly; codes pass registers, where they are widened.
-template <int D, int KEYS, bool E4M3>
+template <int D, int KEYS, bool E4M3, bool VALUES>
 struct Stager;
 
-template <int D, int KEYS>
-struct Stager<D, KEYS, false> {
+template <int D, bool VALUES>
+__device__ __forceinline__ int swizzle(int row) { return VALUES ? swizzle_v<D>(row) : swizzle_k<D>(row); }
+
+template <int D, int KEYS, bool VALUES>
+struct Stager<D, KEYS, false, VALUES> {
     static constexpr int kPieces = D / 8, kEach = kWave / kPieces, kLoads = KEYS / kEach;      // pieces of a row, rows a load
-    static __device__ __forceinline__ void send(const Place &place, int first, int dim, uint32_t kt, uint32_t vt) {
+    __device__ __forceinline__ void fetch(const uint8_t *place, int first, int dim, uint32_t tile) const {
         const int lane = threadIdx.x % kWave, piece = lane % kPieces;
         const uint8_t *zeros = reinterpret_cast<const uint8_t *>(g_zeros);
 #pragma unroll
         for (int i = 0; i < kLoads; ++i) {
-            const int row = first + i * kEach + lane / kPieces, ck = piece ^ swizzle_k<D>(row), cv = piece ^ swizzle_v<D>(row);
-            const uint8_t *k = shuffled(place.key, row), *v = shuffled(place.value, row);
-            to_lds(kt + (first + i * kEach) * 2 * D, (ck * 8 < dim ? k : zeros) + ck * 16);
-            to_lds(vt + (first + i * kEach) * 2 * D, (cv * 8 < dim ? v : zeros) + cv * 16);
+            const int row = first + i * kEach + lane / kPieces, c = piece ^ swizzle<D, VALUES>(row);
+            const uint8_t *from = shuffled(place, row);
+            to_lds(tile + (first + i * kEach) * 2 * D, (c * 8 < dim ? from : zeros) + c * 16);
         }
     }
+    // the i-th load from one page
+    __device__ __forceinline__ void one(int i, const uint8_t *page, uint32_t at, bool in, int first, uint32_t tile) const {
+        if (in) to_lds(tile + (first + i * kEach) * 2 * D, page, at);
+    }
+    __device__ __forceinline__ void put(int, uint32_t) const { all_loads_done(); }
 };
 
-template <int D, int KEYS>
-struct Stager<D, KEYS, true> {
+template <int D, int KEYS, bool VALUES>
+struct Stager<D, KEYS, true, VALUES> {
     static constexpr int kPieces = D / 16, kEach = kWave / kPieces < KEYS ? kWave / kPieces : KEYS, kLoads = KEYS / kEach;
-    u32x4 k[kLoads], v[kLoads];
-    __device__ __forceinline__ void fetch(const Place &place, int first, int dim) {
+    u32x4 codes[kLoads];
+    __device__ __forceinline__ void fetch(const uint8_t *place, int first, int dim, uint32_t) {
         const int lane = threadIdx.x % kWave, piece = lane % kPieces;
         const uint8_t *zeros = reinterpret_cast<const uint8_t *>(g_zeros);
 #pragma unroll
         for (int i = 0; i < kLoads; ++i) {
-            const int row = first + i * kEach + lane / kPieces % kEach;
-            const uint8_t *pk = shuffled(place.key, row), *pv = shuffled(place.value, row);
-            k[i] = *reinterpret_cast<const u32x4 *>((piece * 16 < dim ? pk : zeros) + piece * 16);
-            v[i] = *reinterpret_cast<const u32x4 *>((piece * 16 < dim ? pv : zeros) + piece * 16);
+            const uint8_t *from = shuffled(place, first + i * kEach + lane / kPieces % kEach);
+            codes[i] = *reinterpret_cast<const u32x4 *>((piece * 16 < dim ? from : zeros) + piece * 16);
         }
     }
-    __device__ __forceinline__ void put(int first, uint32_t kt, uint32_t vt) const {
+    __device__ __forceinline__ void one(int i, const uint8_t *page, uint32_t at, bool in, int, uint32_t) {
+        codes[i] = u32x4{0, 0, 0, 0};
+        if (in) codes[i] = *reinterpret_cast<const u32x4 *>(page + at);
+    }
+    __device__ __forceinline__ void put(int first, uint32_t tile) const {
         const int lane = threadIdx.x % kWave, piece = lane % kPieces;
         if (lane / kPieces >= kEach) return;
 #pragma unroll
         for (int i = 0; i < kLoads; ++i) {
-            const int row = first + i * kEach + lane / kPieces;
-            auto write = [&](u32x4 codes, uint32_t tile, int swizzle) {
-                u32x4 lo, hi;
-                widen16(codes, lo, hi);
-                *(__attribute__((address_space(3))) u32x4 *)(uintptr_t)(tile + row * 2 * D + 16 * ((2 * piece) ^ swizzle)) = lo;
-                *(__attribute__((address_space(3))) u32x4 *)(uintptr_t)(tile + row * 2 * D + 16 * ((2 * piece + 1) ^ swizzle)) = hi;
-            };
-            write(k[i], kt, swizzle_k<D>(row));
-            write(v[i], vt, swizzle_v<D>(row));
+            const int row = first + i * kEach + lane / kPieces, z = swizzle<D, VALUES>(row);
+            u32x4 lo, hi;
+            widen16(codes[i], lo, hi);
+            *(__attribute__((address_space(3))) u32x4 *)(uintptr_t)(tile + row * 2 * D + 16 * ((2 * piece) ^ z)) = lo;
+            *(__attribute__((address_space(3))) u32x4 *)(uintptr_t)(tile + row * 2 * D + 16 * ((2 * piece + 1) ^ z)) = hi;
         }
     }
 };
+
+// Zeros in the place of infinities and NaN, in 16-byte pieces first, first + step, .. of a tile of values.
+__device__ __forceinline__ void make_finite(uint32_t vt, int first, int step, int pieces) {
+#pragma unroll 1
+    for (int i = first; i < pieces; i += step) {
+        auto at = (__attribute__((address_space(3))) u32x4 *)(uintptr_t)(vt + 16 * i);
+        u32x4 v = *at;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            if ((v[k] & 0x7f80u) == 0x7f80u) v[k] &= 0xffff0000u;
+            if ((v[k] & 0x7f800000u) == 0x7f800000u) v[k] &= 0xffffu;
+        }
+        *at = v;
+    }
+}
 
 __device__ __forceinline__ uint32_t lds_base(uint8_t *lds) { return (uint32_t)(uintptr_t)(lds_u8 *)lds; }
 
@@ -480,59 +539,47 @@ __global__ __launch_bounds__(kFewWaves *kWave) void attend_few_kernel(Attend a) 
     w.load_q(a, it.run, row, head);
 
     const int h4 = 4 * (lane / 32);
-    bool careful = false;
+    Pass pass = kOnce;
     const uint32_t mine = lds_base(lds) + wave * kStages * 2 * kTile;
     auto page_of = [&](int base) { return base + lane % 32 < range.end ? table[(base + lane % 32) >> a.p.shift] : -1; };
     auto attend = [&](int base, uint32_t held, uint32_t kt) {
         const uint64_t seen = seen_of(pos, base, a.window, held);
-        if (careful) w.template tile<kCareful>(kt, kt + kTile, caps.c, caps.in, caps.out, seen >> h4, seen);
-        else if (held != ~0u || base + kFewKeys - 1 > pos0 || base <= pos1 - a.window)
-            w.template tile<kMasked>(kt, kt + kTile, caps.c, caps.in, caps.out, seen >> h4, seen);
-        else
-            w.template tile<kPlain>(kt, kt + kTile, caps.c, caps.in, caps.out, 0, 0);
+        if (pass == kOdd) {
+            w.add_odd(kt + kTile, seen);
+            return;
+        }
+        if (pass == kFinite) make_finite(kt + kTile, lane, kWave, kTile / 16);
+        w.scores(kt);
+        if (caps.in > 0.0f) w.cap(caps.in, caps.out);
+        if (held != ~0u || base + kFewKeys - 1 > pos0 || base <= pos1 - a.window) w.hide(seen >> h4);
+        w.weights(caps.c);
+        w.sums(kt + kTile);
     };
-    for (;;) {                                   // once, or again where the sums say that there are infinities or NaN
-        w.start();
+    for (;;) {
+        if (pass != kOdd) w.start();
         int base = range.first + wave * kFewKeys;
         int page = page_of(base);
-        if constexpr (E4M3) {
-            Stager<D, kFewKeys, true> stager;
-            Place place = place_of(a.p, page, base + lane % 32, head);
-            uint32_t held = (uint32_t)__ballot(place.held);
-            stager.fetch(place, 0, a.p.dim);
-            page = page_of(base + kStep);
-            for (; base < range.end; base += kStep) {
-                const uint32_t now = held;
-                stager.put(0, mine, mine + kTile);
-                place = place_of(a.p, page, base + kStep + lane % 32, head);      // (behind the end: rows of zeros)
-                held = (uint32_t)__ballot(place.held);
-                stager.fetch(place, 0, a.p.dim);
-                page = page_of(base + 2 * kStep);
-                attend(base, now, mine);
-            }
-        } else {
-            uint32_t stage = 0, held = 0;
-            if (base < range.end) {
-                const Place place = place_of(a.p, page, base + lane % 32, head);
-                held = (uint32_t)__ballot(place.held);
-                Stager<D, kFewKeys, false>::send(place, 0, a.p.dim, mine, mine + kTile);
-                page = page_of(base + kStep);
-            }
-            for (; base < range.end; base += kStep) {
-                all_loads_done();
-                const uint32_t now = held, kt = mine + stage;
-                stage ^= 2 * kTile;
-                if (base + kStep < range.end) {
-                    const Place place = place_of(a.p, page, base + kStep + lane % 32, head);
-                    held = (uint32_t)__ballot(place.held);
-                    Stager<D, kFewKeys, false>::send(place, 0, a.p.dim, mine + stage, mine + stage + kTile);
-                    page = page_of(base + 2 * kStep);
-                }
-                attend(base, now, kt);
-            }
+        uint32_t held = 0, stage = 0;
+        Stager<D, kFewKeys, E4M3, false> keys;
+        Stager<D, kFewKeys, E4M3, true> values;
+        auto fetch = [&](int at) {               // the tile at `at`, whose pages are known; then the pages of the next
+            const Place place = place_of(a.p, page, at + lane % 32, head);
+            held = (uint32_t)__ballot(place.held);
+            keys.fetch(place.key, 0, a.p.dim, mine + stage);
+            values.fetch(place.value, 0, a.p.dim, mine + stage + kTile);
+            page = page_of(at + kStep);
+        };
+        if (base < range.end) fetch(base);
+        for (; base < range.end; base += kStep) {
+            const uint32_t now = held, kt = mine + stage;
+            keys.put(0, kt);
+            values.put(0, kt + kTile);
+            if (!E4M3) stage ^= 2 * kTile;
+            if (base + kStep < range.end) fetch(base + kStep);
+            attend(base, now, kt);
         }
-        if (careful || !__any(w.odd())) break;
-        careful = true;
+        if (pass == kOdd || (pass == kOnce && !__any(w.odd()))) break;
+        pass = pass == kOnce ? kFinite : kOdd;
     }
     w.l += other_half(w.l);
 
@@ -586,7 +633,49 @@ __global__ __launch_bounds__(kFewWaves *kWave) void attend_few_kernel(Attend a) 
 }
 
 // ---------------------------------------------------------------------------------------------------------------- many rows
-constexpr int many_lds(int D) { return 2 * 2 * kManyKeys * 2 * D; }
+// Whether a wave is the second (fourth, ..) of its block on its SIMD.  lds: room for a number of each wave, which nothing else uses yet.
+template <int WAVES>
+__device__ __forceinline__ bool second_of_simd(uint8_t *lds, int wave) {
+    constexpr int kHwId = 4, kOffset = 4, kBits = 2;           // of the register that says where a wave runs, its SIMD
+    const int simd = __builtin_amdgcn_s_getreg(kHwId | kOffset << 6 | (kBits - 1) << 11);
+    int *at = reinterpret_cast<int *>(lds);
+    if (threadIdx.x % kWave == 0) at[wave] = simd;
+    __syncthreads();
+    int before = 0;
+#pragma unroll
+    for (int w = 0; w < WAVES; ++w) before += w < wave && at[w] == simd;
+    __syncthreads();
+    return __builtin_amdgcn_readfirstlane(before & 1);
+}
+
+// The eight waves in two halves, each with a wave on every SIMD: while one half multiplies, the other makes weights, and a barrier turns them.  In the
+// half's turn at the matrix units a wave adds up the values of tile t - 1 and makes the scores of tile t.
+//   step          0        1        2        3        4
+//   first half    s0       w0       o0 s1    w1       o1 s2    ..         K(t) and V(t - 1) are read in steps 2 t and 2 t + 1; three tiles of each are in
+//   second half            s0       w0       o0 s1    w1       ..         LDS, so that those of t + 2 can be asked for while the half makes weights of t
+constexpr int many_lds(int D) { return 3 * 2 * kManyKeys * 2 * D; }
+
+// A wave's eight rows of a tile in one page: one address for the wave and each lane's distance from it, worked out once.  Pieces behind head_dim are
+// neither read nor written.
+template <int D, bool E4M3>
+struct Eight {
+    static constexpr int kPieces = E4M3 ? D / 16 : D / 8, kEach = kWave / kPieces < 8 ? kWave / kPieces : 8, kLoads = 8 / kEach;
+    uint32_t k_at[kLoads], v_at[kLoads];
+    bool k_in[kLoads], v_in[kLoads], paged;
+    __device__ __forceinline__ void start(const Paged &p, int first) {
+        const int lane = threadIdx.x % kWave, piece = lane % kPieces;
+        paged = p.shift >= 3 && p.k_tok < 1 << 24 && p.v_tok < 1 << 24;
+#pragma unroll
+        for (int i = 0; i < kLoads; ++i) {
+            const int r = i * kEach + lane / kPieces;
+            const int ck = E4M3 ? piece : piece ^ swizzle_k<D>(first + r), cv = E4M3 ? piece : piece ^ swizzle_v<D>(first + r);
+            k_at[i] = r * (uint32_t)p.k_tok + ck * 16;
+            v_at[i] = r * (uint32_t)p.v_tok + cv * 16;
+            k_in[i] = ck * (E4M3 ? 16 : 8) < p.dim && r < 8;
+            v_in[i] = cv * (E4M3 ? 16 : 8) < p.dim && r < 8;
+        }
+    }
+};
 
 template <int D, bool E4M3>
 __global__ __launch_bounds__(kManyWaves *kWave) void attend_many_kernel(Attend a, int clear) {
@@ -594,6 +683,7 @@ __global__ __launch_bounds__(kManyWaves *kWave) void attend_many_kernel(Attend a
     constexpr int kTile = kManyKeys * 2 * D, kMine = kManyKeys / kManyWaves;
     const int head = blockIdx.x % a.p.kv_heads, lane = threadIdx.x % kWave;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+    const bool second = second_of_simd<kManyWaves>(lds, wave);
     if (clear) clear_rest(a, blockIdx.x, gridDim.x, kManyWaves * kWave);
     Item it;
     if (!find<kManyRows, kManyKeys, false>(a, blockIdx.x / a.p.kv_heads, kManyTarget, it)) return;
@@ -602,75 +692,118 @@ __global__ __launch_bounds__(kManyWaves *kWave) void attend_many_kernel(Attend a
     const int pos = before + row / a.group, pos0 = before + row0 / a.group, pos1 = before + min(row0 + 31, rows - 1) / a.group;
     const Caps caps = caps_of(a, head);
     const int32_t *table = a.p.table + it.seq * a.p.table_stride;
+    const int tiles = (range.end - range.first + kManyKeys - 1) / kManyKeys;
     Rows32<D, 2> w;
     w.load_q(a, it.run, row, head);
 
+    const uint32_t keys = lds_base(lds), values = keys + 3 * kTile;
     const int h4 = 4 * (lane / 32);
-    bool careful = false;
-    const uint32_t tiles = lds_base(lds);
-    auto page_of = [&](int base) { return base + lane < range.end ? table[(base + lane) >> a.p.shift] : -1; };
-    auto attend = [&](int base, uint64_t held, uint32_t kt) {
-        if (row0 >= rows || base > pos1 || base + kManyKeys - 1 <= pos0 - a.window) return;
-        const uint64_t seen = seen_of(pos, base, a.window, held);
-        if (careful) w.template tile<kCareful>(kt, kt + kTile, caps.c, caps.in, caps.out, seen >> h4, seen);
-        else if (held != ~0ull || base + kManyKeys - 1 > pos0 || base <= pos1 - a.window)
-            w.template tile<kMasked>(kt, kt + kTile, caps.c, caps.in, caps.out, seen >> h4, seen);
-        else
-            w.template tile<kPlain>(kt, kt + kTile, caps.c, caps.in, caps.out, 0, 0);
-    };
-    for (;;) {                                   // (again: the whole block)
-        w.start();
-        int base = range.first;
-        uint32_t stage = 0;
-        int page = page_of(base);
-        Place place = place_of(a.p, page, base + lane, head);
-        uint64_t held = __ballot(place.held);
-        if constexpr (E4M3) {
-            Stager<D, kMine, true> stager;
-            stager.fetch(place, wave * kMine, a.p.dim);
-            stager.put(wave * kMine, tiles, tiles + kTile);
-            page = page_of(base + kManyKeys);
-            place = place_of(a.p, page, base + kManyKeys + lane, head);
-            uint64_t next = __ballot(place.held);
-            stager.fetch(place, wave * kMine, a.p.dim);
-            page = page_of(base + 2 * kManyKeys);
-            for (; base < range.end; base += kManyKeys) {
-                __syncthreads();
-                attend(base, held, tiles + stage);
-                stage ^= 2 * kTile;
-                held = next;
-                if (base + kManyKeys < range.end) {
-                    stager.put(wave * kMine, tiles + stage, tiles + stage + kTile);
-                    place = place_of(a.p, page, base + 2 * kManyKeys + lane, head);
-                    next = __ballot(place.held);
-                    stager.fetch(place, wave * kMine, a.p.dim);
-                    page = page_of(base + 3 * kManyKeys);
-                }
-            }
-        } else {
-            if (base < range.end) {
-                Stager<D, kMine, false>::send(place, wave * kMine, a.p.dim, tiles, tiles + kTile);
-                page = page_of(base + kManyKeys);
-            }
-            for (; base < range.end; base += kManyKeys) {
-                all_loads_done();
-                __builtin_amdgcn_s_barrier();
-                asm volatile("" ::: "memory");
-                const uint64_t now = held;
-                const uint32_t kt = tiles + stage;
-                stage ^= 2 * kTile;
-                if (base + kManyKeys < range.end) {
-                    place = place_of(a.p, page, base + kManyKeys + lane, head);
-                    held = __ballot(place.held);
-                    Stager<D, kMine, false>::send(place, wave * kMine, a.p.dim, tiles + stage, tiles + stage + kTile);
-                    page = page_of(base + 2 * kManyKeys);
-                }
-                attend(base, now, kt);
+    bool finite = false;
+    Stager<D, kMine, E4M3, false> key_stager;
+    Stager<D, kMine, E4M3, true> value_stager;
+    const int mine = wave * kMine;
+    static_assert(kMine == 8, "rows of a wave");
+    Eight<D, E4M3> eight;
+    eight.start(a.p, mine);
+    if (!E4M3 && a.p.dim < D) {                  // (what no load writes)
+        for (int i = threadIdx.x; i < many_lds(D) / 16; i += kManyWaves * kWave) reinterpret_cast<u32x4 *>(lds)[i] = u32x4{0, 0, 0, 0};
+        __syncthreads();
+    }
+    auto base_of = [&](int t) { return range.first + t * kManyKeys; };
+    auto page_of = [&](int t) { return base_of(t) + lane < range.end ? table[(base_of(t) + lane) >> a.p.shift] : -1; };
+    // Pages of the tile whose keys are asked for next, a lane a key, where its wave's values lie, and which keys there are of the last tile asked for, of the
+    // one in front of it and of the one in front of that (2, 1, 0).
+    int page;
+    struct {
+        const uint8_t *at;                       // the wave's first row, null where every lane has its own place
+        const uint8_t *place;
+    } value = {nullptr, nullptr};
+    uint64_t held[3];
+    const bool whole = a.p.dim == D && Eight<D, E4M3>::kEach * Eight<D, E4M3>::kPieces == kWave;
+    auto fetch = [&](int t, uint32_t kt, uint32_t vt) {        // keys of tile t, values of the one in front of it
+        held[0] = held[1], held[1] = held[2];
+        // (what takes `page` waits for it, and so for all loads in front of that: before any of these are sent)
+        const int base = base_of(t), pos = base + mine, id = __builtin_amdgcn_readlane(page, mine);
+        held[2] = __ballot(base + lane < range.end && (uint32_t)page < (uint32_t)a.p.pages);
+        if (t > 0 && t <= tiles) {
+            if (value.at) {
+#pragma unroll
+                for (int i = 0; i < Eight<D, E4M3>::kLoads; ++i) value_stager.one(i, value.at, eight.v_at[i], whole || eight.v_in[i], mine, vt);
+            } else {
+                value_stager.fetch(value.place, mine, a.p.dim, vt);
             }
         }
-        if (careful || !__syncthreads_or(w.odd())) break;
-        careful = true;
+        if (t >= tiles) return;
+        if (eight.paged && pos + kMine <= range.end && (uint32_t)id < (uint32_t)a.p.pages) {
+            const int at = pos & ((1 << a.p.shift) - 1);
+            const uint8_t *key = a.p.keys + id * a.p.k_page + head * a.p.k_head + at * a.p.k_tok;
+            value.at = a.p.values + id * a.p.v_page + head * a.p.v_head + at * a.p.v_tok;
+#pragma unroll
+            for (int i = 0; i < Eight<D, E4M3>::kLoads; ++i) key_stager.one(i, key, eight.k_at[i], whole || eight.k_in[i], mine, kt);
+        } else {
+            const Place place = place_of(a.p, page, base + lane, head);
+            key_stager.fetch(place.key, mine, a.p.dim, kt);
+            value = {nullptr, place.value};
+        }
+        page = page_of(t + 1);
+    };
+    auto arrived = [&](int t, uint32_t kt, uint32_t vt) {
+        if (t < tiles) key_stager.put(mine, kt);
+        if (t > 0 && t <= tiles) {
+            value_stager.put(mine, vt);
+            if (finite) make_finite(vt + mine * 2 * D, lane, kWave, kMine * 2 * D / 16);
+        }
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    };
+    auto turn = [&]() {
+        __builtin_amdgcn_sched_barrier(0);
+        __builtin_amdgcn_s_barrier();
+        __builtin_amdgcn_sched_barrier(0);
+        asm volatile("" ::: "memory");
+    };
+    for (;;) {
+        w.start();
+        uint32_t b0 = 0, b1 = kTile, b2 = 2 * kTile;           // where tiles t, t + 1 and t + 2 lie
+        page = page_of(0);
+        fetch(0, keys + b0, 0);
+        arrived(0, keys + b0, 0);
+        fetch(1, keys + b1, values + b0);
+        turn();
+        if (second) turn();
+        w.scores(keys + b0);
+        if (second) arrived(1, keys + b1, values + b0);
+        turn();
+        for (int t = 0; t < tiles; ++t) {
+            if (second) fetch(t + 2, keys + b2, values + b1);
+            const int base = base_of(t);
+            const uint64_t now = second ? held[0] : held[1];
+            if (caps.in > 0.0f) w.cap(caps.in, caps.out);
+            if (now != ~0ull || base + kManyKeys - 1 > pos0 || base <= pos1 - a.window) w.hide(seen_of(pos, base, a.window, now) >> h4);
+            w.weights(caps.c);
+            if (!second) {
+                arrived(t + 1, keys + b1, values + b0);
+                fetch(t + 2, keys + b2, values + b1);
+            }
+            turn();
+            w.sums_and_scores(values + b0, keys + b1);          // (scores behind the last tile: of what was there, for nobody)
+            if (second) arrived(t + 2, keys + b2, values + b1);
+            turn();
+            const uint32_t b = b0;
+            b0 = b1, b1 = b2, b2 = b;
+        }
+        if (!second) turn();
+        if (!__syncthreads_or(w.odd()) || finite) break;
+        finite = true;
     }
+    if (finite)
+        for (int t = 0; t < tiles; ++t) {
+            const Place place = place_of(a.p, page_of(t), base_of(t) + lane, head);
+            value_stager.fetch(place.value, mine, a.p.dim, values);
+            value_stager.put(mine, values);
+            __syncthreads();
+            w.add_odd(values, seen_of(pos, base_of(t), a.window, __ballot(place.held)));
+            __syncthreads();
+        }
     w.l += other_half(w.l);
     if (row >= rows) return;
     const int64_t slot = (it.slot + it.split) * a.p.kv_heads + head;

@@ -148,7 +148,9 @@ __device__ __forceinline__ void to_lds(uint32_t to, const uint8_t *from) {
 }
 // and from an address of the wave's at a distance of the lane's
 __device__ __forceinline__ void to_lds(uint32_t to, const uint8_t *from, uint32_t at) {
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(to), "v"(at), "s"(from) : "memory");
+    const uint64_t v = reinterpret_cast<uint64_t>(from);       // (the same in all lanes, which the compiler does not always see)
+    const uint64_t base = (uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)(v >> 32)) << 32 | (uint32_t)__builtin_amdgcn_readfirstlane((int)v);
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 4\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(to), "v"(at), "s"(base) : "memory");
 }
 __device__ __forceinline__ void all_loads_done() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
 
@@ -522,7 +524,7 @@ constexpr int few_lds(int D, bool e4m3) {
 }
 
 template <int D, bool E4M3>
-__global__ __launch_bounds__(kFewWaves *kWave) void attend_few_kernel(Attend a) {
+__global__ __launch_bounds__(kFewWaves *kWave, E4M3 ? 2 : 1) void attend_few_kernel(Attend a) {
     extern __shared__ __attribute__((aligned(1024))) uint8_t lds[];
     constexpr int kTile = kFewKeys * 2 * D, kStages = E4M3 ? 1 : 2, kStep = kFewKeys * kFewWaves;
     const int head = blockIdx.x % a.p.kv_heads, lane = threadIdx.x % kWave;
@@ -711,41 +713,59 @@ __global__ __launch_bounds__(kManyWaves *kWave) void attend_many_kernel(Attend a
     }
     auto base_of = [&](int t) { return range.first + t * kManyKeys; };
     auto page_of = [&](int t) { return base_of(t) + lane < range.end ? table[(base_of(t) + lane) >> a.p.shift] : -1; };
-    // Pages of the tile whose keys are asked for next, a lane a key, where its wave's values lie, and which keys there are of the last tile asked for, of the
-    // one in front of it and of the one in front of that (2, 1, 0).
-    int page;
-    struct {
+    // Where this wave's rows of 64 tiles to come lie, a lane a tile (0: every lane has its own place), and which keys of the tile there are.
+    using E = Eight<D, E4M3>;
+    uint64_t key_of = 0, value_of = 0, held_of = 0;
+    auto look_ahead = [&](int t0) {
+        const int base = base_of(t0 + lane);
+        uint64_t keys_held = 0;
+        int id = -1;
+#pragma unroll
+        for (int g = 0; g < kManyWaves; ++g) {
+            const int pos = base + 8 * g, page = pos < range.end ? table[pos >> a.p.shift] : -1;
+            if ((uint32_t)page < (uint32_t)a.p.pages) keys_held |= 0xffull << 8 * g;
+            if (g == wave) id = page;
+        }
+        const int pos = base + mine, at = pos & ((1 << a.p.shift) - 1), left = range.end - base;
+        held_of = left >= kManyKeys ? keys_held : left <= 0 ? 0 : keys_held & ~(~0ull << left);
+        const bool together = eight.paged && pos + kMine <= range.end && (uint32_t)id < (uint32_t)a.p.pages;
+        key_of = together ? reinterpret_cast<uint64_t>(a.p.keys + id * a.p.k_page + head * a.p.k_head + at * a.p.k_tok) : 0;
+        value_of = together ? reinterpret_cast<uint64_t>(a.p.values + id * a.p.v_page + head * a.p.v_head + at * a.p.v_tok) : 0;
+    };
+    auto of_lane = [](uint64_t v, int lane) {
+        return (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(v >> 32), lane) << 32 | (uint32_t)__builtin_amdgcn_readlane((int)v, lane);
+    };
+    struct Where {
         const uint8_t *at;                       // the wave's first row, null where every lane has its own place
         const uint8_t *place;
-    } value = {nullptr, nullptr};
-    uint64_t held[3];
-    const bool whole = a.p.dim == D && Eight<D, E4M3>::kEach * Eight<D, E4M3>::kPieces == kWave;
+    } key = {a.p.keys, a.p.keys}, value = {a.p.values, a.p.values};
+    uint64_t held[2];                            // of the last tile asked for and of the one in front of it (1, 0)
+    const bool whole = a.p.dim == D && E::kEach * E::kPieces == kWave;
     auto fetch = [&](int t, uint32_t kt, uint32_t vt) {        // keys of tile t, values of the one in front of it
-        held[0] = held[1], held[1] = held[2];
-        // (what takes `page` waits for it, and so for all loads in front of that: before any of these are sent)
-        const int base = base_of(t), pos = base + mine, id = __builtin_amdgcn_readlane(page, mine);
-        held[2] = __ballot(base + lane < range.end && (uint32_t)page < (uint32_t)a.p.pages);
+        if (t % kWave == 0) look_ahead(t);
+        held[0] = held[1];
+        held[1] = of_lane(held_of, t % kWave);
         if (t > 0 && t <= tiles) {
             if (value.at) {
 #pragma unroll
-                for (int i = 0; i < Eight<D, E4M3>::kLoads; ++i) value_stager.one(i, value.at, eight.v_at[i], whole || eight.v_in[i], mine, vt);
+                for (int i = 0; i < E::kLoads; ++i) value_stager.one(i, value.at, eight.v_at[i], whole || eight.v_in[i], mine, vt);
             } else {
                 value_stager.fetch(value.place, mine, a.p.dim, vt);
             }
         }
         if (t >= tiles) return;
-        if (eight.paged && pos + kMine <= range.end && (uint32_t)id < (uint32_t)a.p.pages) {
-            const int at = pos & ((1 << a.p.shift) - 1);
-            const uint8_t *key = a.p.keys + id * a.p.k_page + head * a.p.k_head + at * a.p.k_tok;
-            value.at = a.p.values + id * a.p.v_page + head * a.p.v_head + at * a.p.v_tok;
+        key.at = reinterpret_cast<const uint8_t *>(of_lane(key_of, t % kWave));
+        value.at = reinterpret_cast<const uint8_t *>(of_lane(value_of, t % kWave));
+        if (key.at) {
 #pragma unroll
-            for (int i = 0; i < Eight<D, E4M3>::kLoads; ++i) key_stager.one(i, key, eight.k_at[i], whole || eight.k_in[i], mine, kt);
+            for (int i = 0; i < E::kLoads; ++i) key_stager.one(i, key.at, eight.k_at[i], whole || eight.k_in[i], mine, kt);
         } else {
-            const Place place = place_of(a.p, page, base + lane, head);
+            const int at = base_of(t) + lane;
+            const Place place = place_of(a.p, at < range.end ? table[at >> a.p.shift] : -1, at, head);
+            held[1] = __ballot(place.held);
             key_stager.fetch(place.key, mine, a.p.dim, kt);
-            value = {nullptr, place.value};
+            value.place = place.value;
         }
-        page = page_of(t + 1);
     };
     auto arrived = [&](int t, uint32_t kt, uint32_t vt) {
         if (t < tiles) key_stager.put(mine, kt);
@@ -764,29 +784,23 @@ __global__ __launch_bounds__(kManyWaves *kWave) void attend_many_kernel(Attend a
     for (;;) {
         w.start();
         uint32_t b0 = 0, b1 = kTile, b2 = 2 * kTile;           // where tiles t, t + 1 and t + 2 lie
-        page = page_of(0);
         fetch(0, keys + b0, 0);
         arrived(0, keys + b0, 0);
         fetch(1, keys + b1, values + b0);
         turn();
         if (second) turn();
         w.scores(keys + b0);
-        if (second) arrived(1, keys + b1, values + b0);
+        arrived(1, keys + b1, values + b0);
         turn();
         for (int t = 0; t < tiles; ++t) {
-            if (second) fetch(t + 2, keys + b2, values + b1);
             const int base = base_of(t);
-            const uint64_t now = second ? held[0] : held[1];
             if (caps.in > 0.0f) w.cap(caps.in, caps.out);
-            if (now != ~0ull || base + kManyKeys - 1 > pos0 || base <= pos1 - a.window) w.hide(seen_of(pos, base, a.window, now) >> h4);
+            if (held[0] != ~0ull || base + kManyKeys - 1 > pos0 || base <= pos1 - a.window) w.hide(seen_of(pos, base, a.window, held[0]) >> h4);
             w.weights(caps.c);
-            if (!second) {
-                arrived(t + 1, keys + b1, values + b0);
-                fetch(t + 2, keys + b2, values + b1);
-            }
+            fetch(t + 2, keys + b2, values + b1);
             turn();
             w.sums_and_scores(values + b0, keys + b1);          // (scores behind the last tile: of what was there, for nobody)
-            if (second) arrived(t + 2, keys + b2, values + b1);
+            arrived(t + 2, keys + b2, values + b1);
             turn();
             const uint32_t b = b0;
             b0 = b1, b1 = b2, b2 = b;
@@ -828,29 +842,66 @@ __global__ __launch_bounds__(kManyWaves *kWave) void attend_many_kernel(Attend a
 }
 
 // ---------------------------------------------------------------------------------------------------------------- splits as one
-// A block has 32 rows of a tile that was cut; splits in order.
-template <int D, int ROWS, int KEYS>
+// A block has some rows of a tile that was cut.  First the weights of their splits, a lane a row and split, then the sums: the block's lanes in groups that
+// share the splits, each in order, and are added up in order.
+constexpr int kJoinFew = 4, kJoinMany = 32;                   // rows of a block
+
+template <int D, int ROWS, int KEYS, int MINE>
 __global__ __launch_bounds__(256) void attend_join_kernel(Attend a, uint32_t target) {
+    constexpr int kColumns = D / 4, kItems = MINE * kColumns, kGroups = kItems < 256 ? 256 / kItems : 1, kSplits = 2048 / MINE;
+    __shared__ float weight[MINE][kSplits], tops[MINE], totals[MINE];
+    __shared__ f32x4 part[kGroups > 1 ? 256 : 1];
     const int head = blockIdx.x % a.p.kv_heads;
     Item it;
     if (!find<ROWS, KEYS, true>(a, blockIdx.x / a.p.kv_heads, target, it)) return;
-    const int row0 = it.tile * ROWS + blockIdx.y * 32, used = min(it.run.n * a.group - row0, 32);
-    if (((it.slot + it.splits - 1) * a.p.kv_heads + head) >= a.slots) return;
+    if ((it.slot + it.splits - 1) * a.p.kv_heads + head >= a.slots) return;
     const float *ml = a.partial + a.slots * ROWS * D;
-    for (int e = threadIdx.x; e < used * (D / 4); e += 256) {
-        const int r = e / (D / 4), d = e % (D / 4) * 4;
-        auto place = [&](int s) { return ((it.slot + s) * a.p.kv_heads + head) * ROWS + blockIdx.y * 32 + r; };
-        float m = -INFINITY;
-        for (int s = 0; s < it.splits; ++s) m = fmaxf(m, ml[place(s) * 2]);
-        f32x4 o = {0.0f, 0.0f, 0.0f, 0.0f};
-        float l = 0.0f;
-        for (int s = 0; s < it.splits; ++s) {
-            const float ls = ml[place(s) * 2 + 1], by = weight_of(ml[place(s) * 2], m);
-            const f32x4 v = *reinterpret_cast<const f32x4 *>(a.partial + place(s) * D + d);
-            o += v * by;
-            l = __fmaf_rn(ls, by, l);
+    const int wave = threadIdx.x / kWave, lane = threadIdx.x % kWave, group = threadIdx.x / kItems % kGroups;
+    const int rows = min(it.run.n * a.group - it.tile * ROWS, ROWS);
+    for (int first = blockIdx.y * MINE; first < rows; first += gridDim.y * MINE) {
+        const int row0 = it.tile * ROWS + first, used = min(rows - first, MINE);
+        auto place = [&](int s, int r) { return ((it.slot + s) * a.p.kv_heads + head) * ROWS + first + r; };
+        f32x4 o[(kItems + 255) / 256];
+#pragma unroll
+        for (int k = 0; k < (kItems + 255) / 256; ++k) o[k] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+        __syncthreads();                         // (what the rows in front of these have left)
+        // maxima and sums of rows: a wave a row
+        for (int r = wave; r < used; r += 4) {
+            float m = -INFINITY, l = 0.0f;
+            for (int s = lane; s < it.splits; s += kWave) m = fmaxf(m, ml[place(s, r) * 2]);
+#pragma unroll
+            for (int off = kWave / 2; off > 0; off >>= 1) m = fmaxf(m, __shfl_xor(m, off, kWave));
+            for (int s = lane; s < it.splits; s += kWave) l = __fmaf_rn(ml[place(s, r) * 2 + 1], weight_of(ml[place(s, r) * 2], m), l);
+            l = wave_add(l);
+            if (lane == 0) tops[r] = m, totals[r] = l;
         }
-        if (d < a.p.dim) store_row(a, it.run, row0 + r, head, d, o * quotient_of(a, head, l));
+        for (int s0 = 0; s0 < it.splits; s0 += kSplits) {
+            const int count = min(kSplits, it.splits - s0);
+            __syncthreads();
+            for (int e = threadIdx.x; e < used * count; e += 256) weight[e / count][e % count] = weight_of(ml[place(s0 + e % count, e / count) * 2], tops[e / count]);
+            __syncthreads();
+#pragma unroll
+            for (int k = 0; k < (kItems + 255) / 256; ++k) {
+                const int e = kGroups > 1 ? threadIdx.x % kItems : threadIdx.x + k * 256, r = e / kColumns, d = e % kColumns * 4;
+                if (r >= used) continue;
+                const float *from = a.partial + place(s0, r) * D + d;
+                const int64_t step = (int64_t)a.p.kv_heads * ROWS * D;
+#pragma unroll 4
+                for (int s = group; s < count; s += kGroups) o[k] += *reinterpret_cast<const f32x4 *>(from + s * step) * weight[r][s];
+            }
+        }
+        if constexpr (kGroups > 1) {
+            part[threadIdx.x] = o[0];
+            __syncthreads();
+#pragma unroll
+            for (int g = 1; g < kGroups; ++g)
+                if (!group) o[0] += part[threadIdx.x + g * kItems];
+        }
+#pragma unroll
+        for (int k = 0; k < (kItems + 255) / 256; ++k) {
+            const int e = threadIdx.x + k * 256, r = e / kColumns, d = e % kColumns * 4;
+            if (r < used && d < a.p.dim && (kGroups == 1 || !group)) store_row(a, it.run, row0 + r, head, d, o[k] * quotient_of(a, head, totals[r]));
+        }
     }
 }
 
@@ -884,27 +935,31 @@ int check(const char *who, int64_t heads, int64_t most_new, const odl_fp8_paged_
 }
 
 template <int D>
-int launch(Attend &a, const Plan &plan, float *workspace, hipStream_t stream) {
+int launch(Attend &a, const Plan &plan, int64_t most_rows, float *workspace, hipStream_t stream) {
     const int64_t kv = a.p.kv_heads, rows = (int64_t)a.p.rows * a.group, seqs = a.p.seqs < a.p.rows ? a.p.seqs : a.p.rows;
-    auto blocks = [&](int tile, int target) { return (unsigned)((target / kv + 1 + seqs + rows / tile) * kv); };
+    // no more tiles than sequences (those that fill no tile) and rows / tile; splits that begin anew: see `find`
+    auto blocks = [&](int64_t tiles, int target) { return (unsigned)((target / kv + 1 + tiles) * kv); };
     auto joins = [&](int target) { return (unsigned)((target / kv + 1) * kv); };
     if (plan.many) {
         a.least_rows = plan.least, a.most_rows = INT32_MAX;
         a.partial = workspace, a.slots = slots_of(kManyTarget);
         const int clear = !plan.few;
-        if (a.p.e4m3) hipLaunchKernelGGL((attend_many_kernel<D, true>), dim3(blocks(kManyRows, kManyTarget)), dim3(kManyWaves * kWave), many_lds(D), stream, a, clear);
-        else hipLaunchKernelGGL((attend_many_kernel<D, false>), dim3(blocks(kManyRows, kManyTarget)), dim3(kManyWaves * kWave), many_lds(D), stream, a, clear);
+        const dim3 grid(blocks(seqs + rows / kManyRows, kManyTarget));
+        if (a.p.e4m3) hipLaunchKernelGGL((attend_many_kernel<D, true>), grid, dim3(kManyWaves * kWave), many_lds(D), stream, a, clear);
+        else hipLaunchKernelGGL((attend_many_kernel<D, false>), grid, dim3(kManyWaves * kWave), many_lds(D), stream, a, clear);
         if (a.p.reach > kManyKeys)
-            hipLaunchKernelGGL((attend_join_kernel<D, kManyRows, kManyKeys>), dim3(joins(kManyTarget), kManyRows / 32), dim3(256), 0, stream, a, (uint32_t)kManyTarget);
+            hipLaunchKernelGGL((attend_join_kernel<D, kManyRows, kManyKeys, kJoinMany>), dim3(joins(kManyTarget), kManyRows / kJoinMany), dim3(256), 0, stream, a, (uint32_t)kManyTarget);
         workspace += floats_of(kManyRows, kManyTarget, D);
     }
     if (plan.few) {
         a.least_rows = 0, a.most_rows = plan.many ? plan.least : INT32_MAX;
         a.partial = workspace, a.slots = slots_of(kFewTarget);
-        if (a.p.e4m3) hipLaunchKernelGGL((attend_few_kernel<D, true>), dim3(blocks(kFewRows, kFewTarget)), dim3(kFewWaves * kWave), few_lds(D, true), stream, a);
-        else hipLaunchKernelGGL((attend_few_kernel<D, false>), dim3(blocks(kFewRows, kFewTarget)), dim3(kFewWaves * kWave), few_lds(D, false), stream, a);
+        const dim3 grid(blocks(plan.many ? seqs : seqs + rows / kFewRows, kFewTarget));         // (beside the other kernel: a tile a sequence)
+        if (a.p.e4m3) hipLaunchKernelGGL((attend_few_kernel<D, true>), grid, dim3(kFewWaves * kWave), few_lds(D, true), stream, a);
+        else hipLaunchKernelGGL((attend_few_kernel<D, false>), grid, dim3(kFewWaves * kWave), few_lds(D, false), stream, a);
         if (a.p.reach > kFewKeys * kFewWaves)
-            hipLaunchKernelGGL((attend_join_kernel<D, kFewRows, kFewKeys * kFewWaves>), dim3(joins(kFewTarget)), dim3(256), 0, stream, a, (uint32_t)kFewTarget);
+            hipLaunchKernelGGL((attend_join_kernel<D, kFewRows, kFewKeys * kFewWaves, kJoinFew>), dim3(joins(kFewTarget), (unsigned)(((most_rows < kFewRows ? most_rows : kFewRows) + kJoinFew - 1) / kJoinFew)), dim3(256), 0, stream, a,
+                               (uint32_t)kFewTarget);
     }
     return check_launch("odl_fp8_paged_attention");
 }
@@ -941,5 +996,6 @@ extern "C" int odl_fp8_paged_attention(const void *q, const int64_t *q_strides, 
     if (!workspace || workspace_floats < workspace_of(plan, a.p.dim) || (reinterpret_cast<uintptr_t>(workspace) & 15))
         return set_error(ODL_ERR_ARG, "%s: a workspace of %lld floats, 16-byte aligned", who, (long long)workspace_of(plan, a.p.dim));
     hipStream_t stream = reinterpret_cast<hipStream_t>(stream_);
-    return a.p.dim > 64 ? launch<128>(a, plan, workspace, stream) : launch<64>(a, plan, workspace, stream);
+    const int64_t most_rows = (most_new < 1 ? 1 : most_new < a.p.rows ? most_new : a.p.rows) * a.group;
+    return a.p.dim > 64 ? launch<128>(a, plan, most_rows, workspace, stream) : launch<64>(a, plan, most_rows, workspace, stream);
 }

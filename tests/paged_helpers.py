@@ -18,7 +18,7 @@ class Case:
         self.pages = torch.full((len(need), self.width), -7, dtype=torch.int32)
         at = 0
         for s, n in enumerate(need):
-            self.pages[s, :n] = ids[at:at + n]
+            self.pages[s, :n] = ids[at:at + n][:self.width]
             at += n
         self.offsets = torch.tensor([sum(new[:i]) for i in range(len(need) + 1)], dtype=torch.int32)
         self.lengths = torch.tensor(self.length, dtype=torch.int32)

@@ -913,7 +913,7 @@ struct Plan {
 };
 Plan plan_of(int64_t group, int64_t rows, int64_t seqs, int64_t most_new) {
     if (most_new * group <= kFewRows) return {true, false, 0};
-    if (seqs <= 1) return {false, true, 0};
+    if (seqs <= 1 || rows >= seqs * most_new) return {false, true, 0};        // (all of them alike: none has few)
     return {true, true, kFewRows};
 }
 int64_t slots_of(int target) { return 2 * target; }

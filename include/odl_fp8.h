@@ -809,7 +809,7 @@ int odl_fp8_append_kv(const void *q, const int64_t *q_strides, const void *k, co
  *   s_i = scale * q . key_i,  softcap > 0: s_i = softcap * tanh(s_i / softcap),  for max(0, p - window + 1) <= i <= p  (window 0: from 0)
  *   out = sum_i e^(s_i - m) value_i / sum_i e^(s_i - m)
  * Products of bf16 (E4M3 codes are widened exactly) with fp32 sums; weights round to bf16 in front of the second product.  Sums and maxima fp32.
- * Keys and values that a row does not see do not reach it, NaN and infinities included.  A row that sees nothing, and rows that belong to
+ * Keys and values that a row does not see do not reach it, NaN and infinities included.  A row that sees nothing, or no score above -inf, and rows that belong to
  * nobody, answer 0.  q [rows, heads, head_dim] bf16 with strides as above; out bf16 [rows, heads, head_dim].
  * most_new: the most new tokens of a sequence where the caller knows it, else `rows`: chooses kernels, results do not depend on its truth.
  * The same call answers the same bits.  workspace: odl_fp8_paged_attention_workspace floats, contents irrelevant, of this call alone while it runs.

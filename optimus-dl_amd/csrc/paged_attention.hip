@@ -426,7 +426,7 @@ __device__ __forceinline__ void store_row(const Attend &a, const Run &run, int r
 // What a sum against maximum m counts where `top` is the maximum of all.  A part that sees nothing has maximum -inf and sums 0, one that sees only NaN
 // -inf and NaN.
 __device__ __forceinline__ float weight_of(float m, float top) { return m == top ? 1.0f : __builtin_amdgcn_exp2f(m - top); }
-// By what a row's sums are multiplied in the end; a row that sees nothing answers 0.
+// By what a row's sums are multiplied in the end; a row that sees nothing, or no score above -inf, answers 0.
 __device__ __forceinline__ float quotient_of(const Attend &a, int kv_head, float l) {
     return l == 0.0f ? 0.0f : (a.p.value_scale ? a.p.value_scale[kv_head] : 1.0f) / l;
 }

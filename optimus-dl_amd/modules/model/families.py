@@ -109,10 +109,15 @@ class _DecoderLM(nn.Module):
     @torch.no_grad()
     def step(self, input_ids: torch.Tensor, cache: PagedKVCache, batch: PagedBatch, last_only: bool = False) -> dict:
         """Logits of new tokens [rows] (the sequences of the batch one behind the other), which are put into the cache: single tokens, drafts,
-        chunks of prompts.  ``last_only``: of each sequence's last new token alone."""
+        chunks of prompts.  ``last_only``: of each sequence's last new token alone (of no particular one where it has none)."""
+        places = self.transformer["wpe"].num_embeddings if "wpe" in self.transformer else None
+        if places is not None and cache.max_tokens > places:
+            raise ValueError(f"a cache for sequences of {cache.max_tokens} tokens, and embeddings of {places} positions")
+        if last_only and input_ids.shape[0] == 0:
+            raise ValueError("a step without tokens has no last one")
         z = self._hidden(input_ids, cache, batch)
         if last_only:
-            z = z[(batch.offsets[1:].long() - 1).clamp(min=0)]
+            z = z[(batch.offsets[1:].long() - 1).clamp(min=0, max=z.shape[0] - 1)]
         return {"logits": self.lm_head(z)}
 
     @torch.no_grad()
@@ -174,5 +179,5 @@ class GPT2(_DecoderLM):
         self._finish(config)
 
     def embed(self, input_ids: torch.Tensor, batch: PagedBatch | None = None) -> torch.Tensor:
-        pos = torch.arange(input_ids.shape[1], device=input_ids.device) if batch is None else batch.positions(input_ids.shape[0])
+        pos = torch.arange(input_ids.shape[1], device=input_ids.device) if batch is None else batch.positions(input_ids.shape[0]).clamp(max=self.config.block_size - 1)
         return self.transformer.wte(input_ids) + self.transformer.wpe(pos)

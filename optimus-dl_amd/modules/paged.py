@@ -118,7 +118,8 @@ def _attention_plain(q, keys, values, pages, offsets, lengths, scale, window, so
         if window:
             seen = seen & (place > position - window)
         score = score.masked_fill(~seen, float("-inf"))
-        weight = torch.where(seen.any(-1, keepdim=True), torch.softmax(score, -1), torch.zeros_like(score))
+        some = (score != float("-inf")).any(-1, keepdim=True)
+        weight = torch.where(some, torch.softmax(score, -1), torch.zeros_like(score))
         v = read(values, value_scale).unsqueeze(1)                           # (an unseen value does not reach a row, not even a NaN)
         odd = ~v.isfinite()
         y = torch.matmul(weight.unsqueeze(2), torch.where(odd, torch.zeros_like(v), v)).squeeze(2)
@@ -176,8 +177,8 @@ def paged_attention(q: torch.Tensor, keys: torch.Tensor, values: torch.Tensor, p
     A token at position p sees positions ``max(0, p - window + 1)`` to p (window 0: from 0).  Scores are ``scale * q . key`` (1 / sqrt(head_dim) by
     default), and ``softcap * tanh(score / softcap)`` where softcap is not 0.  Heads in groups share a head of the cache.
     max_new: the most new tokens of a sequence, where the program knows it: it chooses kernels, results hold without.
-    Keys and values that a token does not see do not reach it, NaN and infinities included.  A token that sees nothing, and rows behind
-    the last sequence, answer 0.
+    Keys and values that a token does not see do not reach it, NaN and infinities included.  A token that sees nothing, or
+    no score above -inf, and rows behind the last sequence answer 0.
 
     bf16 on the GPU: one kernel for up to 32 rows (tokens times heads of a group) a sequence, another for more, and one that joins parts; sums and maxima
     in fp32, weights rounded to bf16.  The same call answers the same bits.  CPU tensors run as torch operations, in any floating type."""
@@ -310,5 +311,10 @@ class PagedKVCache:
         """``tables(head_dim, positions, theta, device)`` for every position that the tables reach, made once."""
         key = (head_dim, theta)
         if key not in self._angles:
+            on_gpu = self.device.type == "cuda"
+            if on_gpu and torch.cuda.is_current_stream_capturing():
+                raise RuntimeError("a cache makes its angles in its first step: run one before a step is captured")
             self._angles[key] = tables(head_dim, self.width * self.page_size, theta, self.device)
+            if on_gpu:                                 # (steps on other streams use them too)
+                torch.cuda.current_stream(self.device).synchronize()
         return self._angles[key]

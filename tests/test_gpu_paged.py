@@ -305,3 +305,13 @@ def test_refusals_on_the_gpu():
 
         with fwd.dual_level():
             paged_attention(fwd.make_dual(c.q, torch.ones_like(c.q)), *args)
+
+
+@pytest.mark.parametrize("rows", [2, 40])
+def test_a_row_of_scores_of_minus_infinity_answers_0(rows):
+    q = torch.ones(rows, 1, 16, dtype=BF16, device="cuda")
+    keys = torch.zeros(1, 1, 64, 16, dtype=BF16, device="cuda")
+    keys[0, 0, 0, 3] = -torch.inf
+    args = (torch.tensor(v, dtype=torch.int32, device="cuda") for v in ([[0]], [0, rows], [rows]))
+    y = paged_attention(q, keys, torch.ones_like(keys), *args)
+    assert (y[0] == 0).all() and (y[1:] == 1).all()            # (the first token sees that key alone)

@@ -148,6 +148,36 @@ def test_verify_on_the_cpu():
         verify_drafts(x.requires_grad_(True), tokens, offsets, torch.rand(3))
 
 
+def test_a_row_of_scores_of_minus_infinity_answers_0():
+    q, keys = torch.ones(2, 1, 16), torch.zeros(1, 1, 4, 16)
+    keys[0, 0, 0, 3] = -torch.inf
+    args = torch.zeros(1, 1, dtype=torch.int32), torch.tensor([0, 2], dtype=torch.int32), torch.tensor([2], dtype=torch.int32)
+    y = paged_attention(q, keys, torch.ones_like(keys), *args)
+    assert (y[0] == 0).all() and (y[1] == 1).all()             # (the first token sees that key alone)
+
+
+def test_steps_that_a_model_has_no_place_for():
+    model = GPT2(GPT2Config(vocab_size=32, n_embd=32, n_head=2, n_layer=1, block_size=16))
+    cache = model.new_cache(pages=4, page_size=8)
+    s = cache.add()
+    with pytest.raises(ValueError, match="no last one"):
+        model.step(torch.zeros(0, dtype=torch.int64), cache, cache.batch([s], [0]), last_only=True)
+    batch = cache.batch([s], [1])                              # rows behind the last sequence, and an offset behind the rows
+    late = batch._replace(offsets=torch.tensor([0, 9], dtype=torch.int32))
+    assert model.step(torch.zeros(3, dtype=torch.int64), cache, late, last_only=True)["logits"].shape == (1, 32)
+    wide = model.new_cache(pages=4, page_size=8, max_tokens=17)
+    with pytest.raises(ValueError, match="embeddings of 16"):
+        model.step(torch.zeros(1, dtype=torch.int64), wide, wide.batch([wide.add()], [1]))
+
+
+def test_angles_are_not_made_in_a_capture(monkeypatch):
+    cache = PagedKVCache(1, 1, 16, pages=1, page_size=8, device="cpu")
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: True)
+    cache.device = torch.device("cuda")
+    with pytest.raises(RuntimeError, match="before a step is captured"):
+        cache.angles(lambda *args: args, 16, 1e4)
+
+
 def test_refusals_of_arguments():
     c = Case([1, 2], [5, 9], 4, 2, 16, 4, seed=4)
     args = (c.keys, c.values, *c.batch())

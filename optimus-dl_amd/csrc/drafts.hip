@@ -10,6 +10,10 @@
 // part of a row: each works out for itself which draft is the first to be refused and sums what is left of its part of that row (again from
 // memory: one row of each sequence).  In the third a block a sequence finds the part that holds the number drawn and the token in it.
 // T = 0: p is all on the largest logit, the lowest of them, and the second launch ends it.
+//
+// One launch for both of the first two would need the blocks of a row to wait for each other; tickets for the last block of a row to go on took longer than the launch
+// that they save.  Measured (calls in a row): 17 us for one sequence of 3 rows, 37 for 24 of 108 rows in all (50257 columns of bf16), which is the three launches' latency
+// (their bytes take 4), 149 for 64 of 6 rows (151936 of fp32), of which 84 are bytes: the first launch runs at 4.2 TB/s, the second reads one row of each side again.
 #include "common.h"
 
 #pragma clang fp contract(off)

@@ -7,9 +7,17 @@
 //
 // Two kernels.  Few rows a key head (32 at most: single tokens, drafts): the cache is read once and that bounds it; the four waves of a block take
 // every fourth tile of 32 keys, each on its own, and are joined in LDS.  Many (prompts, chunks): MFMA and the exponentials bound it; eight waves of 32
-// rows share tiles of 64 keys.  In both tiles go to LDS without passing registers, one ahead, and where there are fewer tiles of rows than
-// compute units the keys are cut into splits, whose sums a third kernel joins in order.  Every block works out from the lengths which part is its own
-// (`find`): lengths never pass the host.
+// rows share tiles of 64 keys, three in LDS.  In both tiles of bf16 go to LDS without passing registers, one or two ahead, and where there are fewer
+// tiles of rows than compute units the keys are cut into splits, whose sums a third kernel joins in order.  Every block works out from the lengths which
+// part is its own (`find`): lengths never pass the host.
+//
+// Measured (calls in a row, host included; a large copy moves 5.1 TB/s on this card, a large product in bf16 makes 1206 TFLOP/s):
+//   few   64 sequences of up to 8192 tokens, 32 heads on 8 of 128, bf16               311 us   5.1 TB/s
+//         1 sequence of 131072 tokens, the same heads                                 115 us   4.7 TB/s  (of which the join 5 to 15)
+//         32 sequences of 4099, 5 new tokens of each, E4M3                             72 us   3.8 TB/s  (codes pass registers; the join 10)
+//   many  2048 new tokens behind 14336, 32 heads on 8 of 128                          500 us   1030 TFLOP/s  (the card runs at some 2.0 GHz meanwhile)
+//         12 prompts of up to 1000 tokens behind up to 3000, 16 heads on 4 of 96, capped, a window of 1500: 188 us  (288 tiles on 256 compute units: two rounds)
+// A sequence with up to 32 rows a key head fills one tile of the first kernel; from there on that would read the cache again for every 32 rows.
 #include "paged.h"
 
 #pragma clang fp contract(off)
@@ -25,7 +33,9 @@ typedef __attribute__((address_space(3))) uint8_t lds_u8;
 
 constexpr int kFewRows = 32, kFewKeys = 32, kFewWaves = 4;
 constexpr int kManyRows = 256, kManyKeys = 64, kManyWaves = 8;
-constexpr int kFewTarget = 512, kManyTarget = 256;             // blocks that splits are made for
+// Blocks that splits are made for.  Of the small ones two run on a compute unit: with 256 / 512 / 1024 the decode step above takes 304 / 316 / 301 us, drafts on codes
+// 84 / 77 / 90, the long sequence 111 / 117 / 135.  Of the large ones one: with 256 / 512 the chunk takes 524 / 556, the prompts 206 / 231.
+constexpr int kFewTarget = 512, kManyTarget = 256;
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kSlack = 8.0f;                                 // how far, in powers of two, a running maximum may lag behind
 
@@ -200,11 +210,12 @@ __device__ __forceinline__ float other_half(float v) {
     return bits_to_float(threadIdx.x % kWave < 32 ? r[1] : r[0]);
 }
 
-// A lane's 32 rows by 16 of 32 keys (element i is key 8 (i / 4) + 4 (lane / 32) + i % 4), NB such blocks of keys a tile.
-template <int D, int NB>
+// A lane's 32 rows by 16 of 32 keys (element i is key 8 (i / 4) + 4 (lane / 32) + i % 4), NB such blocks of keys a tile.  C of the D
+// columns that tiles have room for are multiplied.
+template <int D, int NB, int C = D>
 struct Rows32 {
-    bf16x8 q[D / 16];
-    f32x16 o[D / 32];
+    bf16x8 q[C / 16];
+    f32x16 o[C / 32];
     f32x16 s[NB];                                              // of a tile: scores, weights as fp32
     bf16x8 w[2 * NB];                                          // and as bf16
     float m, l;                                                // running maximum in powers of two, the sum of this lane's keys against it
@@ -213,7 +224,7 @@ struct Rows32 {
         m = -INFINITY;
         l = 0.0f;
 #pragma unroll
-        for (int d = 0; d < D / 32; ++d) o[d] = f32x16{};
+        for (int d = 0; d < C / 32; ++d) o[d] = f32x16{};
     }
 
     // rows first_row + lane % 32 of a tile's: q of a token's head, zeros where there is no such row
@@ -222,7 +233,7 @@ struct Rows32 {
         const bool live = token < run.n;
         const uint16_t *from = a.q + (int64_t)(run.first + (live ? token : 0)) * a.q_row + head * a.q_head;
 #pragma unroll
-        for (int s = 0; s < D / 16; ++s) {
+        for (int s = 0; s < C / 16; ++s) {
             const int c = 16 * s + 8 * (lane / 32);
             u32x4 v = {0, 0, 0, 0};
             if (live && c < a.p.dim) v = *reinterpret_cast<const u32x4 *>(from + c);
@@ -237,7 +248,7 @@ struct Rows32 {
 #pragma unroll
         for (int b = 0; b < NB; ++b) s[b] = f32x16{};
 #pragma unroll
-        for (int d = 0; d < D / 16; ++d) {
+        for (int d = 0; d < C / 16; ++d) {
             const lds_u8 *from = (const lds_u8 *)(uintptr_t)(at ^ (32 * d));
 #pragma unroll
             for (int b = 0; b < NB; ++b)
@@ -275,7 +286,7 @@ struct Rows32 {
             m = to;
             l *= by;
 #pragma unroll
-            for (int d = 0; d < D / 32; ++d)
+            for (int d = 0; d < C / 32; ++d)
 #pragma unroll
                 for (int i = 0; i < 16; ++i) o[d][i] *= by;
         }
@@ -304,15 +315,16 @@ struct Rows32 {
 #pragma unroll
         for (int k = 0; k < 2 * NB; ++k)
 #pragma unroll
-            for (int d = 0; d < D / 32; ++d)
+            for (int d = 0; d < C / 32; ++d)
                 o[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, values(at, d, k)), w[k], o[d], 0, 0, 0);
     }
 
-    // The weighted values of one tile and the scores of another, both steps' operands four at a time and two groups ahead (left to itself the compiler reads each
-    // where it is used, and waits: 2350 cycles, of which 1024 multiply).
+    // The weighted values of one tile and the scores of another, both steps' operands four at a time and a group ahead (left to itself the compiler reads each
+    // where it is used, and waits: 2350 cycles, of which 1024 multiply; two groups ahead keep 16 registers more in scratch memory: a chunk of 2048 tokens behind
+    // 14336 takes 526 us and not 500).
     __device__ __forceinline__ void sums_and_scores(uint32_t vt, uint32_t kt) {
-        constexpr int kColumns = D / 32, kSums = 2 * NB * kColumns, kGroups = (kSums + D / 16 * NB) / 4, kAhead = 2;
-        static_assert(kSums % 4 == 0 && D / 16 * NB % 4 == 0, "groups");
+        constexpr int kColumns = C / 32, kSums = 2 * NB * kColumns, kGroups = (kSums + C / 16 * NB) / 4, kAhead = 1;
+        static_assert(kSums % 4 == 0 && C / 16 * NB % 4 == 0, "groups");
         const int lane = threadIdx.x % kWave, h = lane / 32, r = lane % 32;
         const uint32_t v_at = value_address(vt), k_at = kt + r * 2 * D + 16 * (h ^ swizzle_k<D>(r));
         u32x4 f[kAhead + 1][4];
@@ -365,7 +377,7 @@ struct Rows32 {
 #pragma unroll 1
         for (int key = 0; key < 32 * NB; ++key) {
 #pragma unroll
-            for (int d = 0; d < D / 32; ++d)
+            for (int d = 0; d < C / 32; ++d)
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {    // columns 32 d + 8 i + 4 h to + 3
                     const u32x2 v = *(const __attribute__((address_space(3))) u32x2 *)(uintptr_t)(vt + key * 2 * D + 16 * ((4 * d + i) ^ swizzle_v<D>(key)) + 8 * h);
@@ -382,7 +394,7 @@ struct Rows32 {
     __device__ __forceinline__ bool odd() const {
         float most = 0.0f;
 #pragma unroll
-        for (int d = 0; d < D / 32; ++d)
+        for (int d = 0; d < C / 32; ++d)
 #pragma unroll
             for (int i = 0; i < 16; ++i) most = fmaxf(most, o[d][i] != o[d][i] ? INFINITY : __builtin_fabsf(o[d][i]));
         return !(most < INFINITY);
@@ -679,7 +691,7 @@ struct Eight {
     }
 };
 
-template <int D, bool E4M3>
+template <int D, int C, bool E4M3>
 __global__ __launch_bounds__(kManyWaves *kWave) void attend_many_kernel(Attend a, int clear) {
     extern __shared__ __attribute__((aligned(1024))) uint8_t lds[];
     constexpr int kTile = kManyKeys * 2 * D, kMine = kManyKeys / kManyWaves;
@@ -695,7 +707,7 @@ __global__ __launch_bounds__(kManyWaves *kWave) void attend_many_kernel(Attend a
     const Caps caps = caps_of(a, head);
     const int32_t *table = a.p.table + it.seq * a.p.table_stride;
     const int tiles = (range.end - range.first + kManyKeys - 1) / kManyKeys;
-    Rows32<D, 2> w;
+    Rows32<D, 2, C> w;
     w.load_q(a, it.run, row, head);
 
     const uint32_t keys = lds_base(lds), values = keys + 3 * kTile;
@@ -823,7 +835,7 @@ __global__ __launch_bounds__(kManyWaves *kWave) void attend_many_kernel(Attend a
     const int64_t slot = (it.slot + it.split) * a.p.kv_heads + head;
     const float by = quotient_of(a, head, w.l);
 #pragma unroll
-    for (int d = 0; d < D / 32; ++d)
+    for (int d = 0; d < C / 32; ++d)
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
             const int at = 32 * d + 8 * i + 4 * (lane / 32);
@@ -934,7 +946,7 @@ int check(const char *who, int64_t heads, int64_t most_new, const odl_fp8_paged_
     return ODL_OK;
 }
 
-template <int D>
+template <int D, int C>
 int launch(Attend &a, const Plan &plan, int64_t most_rows, float *workspace, hipStream_t stream) {
     const int64_t kv = a.p.kv_heads, rows = (int64_t)a.p.rows * a.group, seqs = a.p.seqs < a.p.rows ? a.p.seqs : a.p.rows;
     // no more tiles than sequences (those that fill no tile) and rows / tile; splits that begin anew: see `find`
@@ -945,8 +957,8 @@ int launch(Attend &a, const Plan &plan, int64_t most_rows, float *workspace, hip
         a.partial = workspace, a.slots = slots_of(kManyTarget);
         const int clear = !plan.few;
         const dim3 grid(blocks(seqs + rows / kManyRows, kManyTarget));
-        if (a.p.e4m3) hipLaunchKernelGGL((attend_many_kernel<D, true>), grid, dim3(kManyWaves * kWave), many_lds(D), stream, a, clear);
-        else hipLaunchKernelGGL((attend_many_kernel<D, false>), grid, dim3(kManyWaves * kWave), many_lds(D), stream, a, clear);
+        if (a.p.e4m3) hipLaunchKernelGGL((attend_many_kernel<D, C, true>), grid, dim3(kManyWaves * kWave), many_lds(D), stream, a, clear);
+        else hipLaunchKernelGGL((attend_many_kernel<D, C, false>), grid, dim3(kManyWaves * kWave), many_lds(D), stream, a, clear);
         if (a.p.reach > kManyKeys)
             hipLaunchKernelGGL((attend_join_kernel<D, kManyRows, kManyKeys, kJoinMany>), dim3(joins(kManyTarget), kManyRows / kJoinMany), dim3(256), 0, stream, a, (uint32_t)kManyTarget);
         workspace += floats_of(kManyRows, kManyTarget, D);
@@ -997,5 +1009,8 @@ extern "C" int odl_fp8_paged_attention(const void *q, const int64_t *q_strides, 
         return set_error(ODL_ERR_ARG, "%s: a workspace of %lld floats, 16-byte aligned", who, (long long)workspace_of(plan, a.p.dim));
     hipStream_t stream = reinterpret_cast<hipStream_t>(stream_);
     const int64_t most_rows = (most_new < 1 ? 1 : most_new < a.p.rows ? most_new : a.p.rows) * a.group;
-    return a.p.dim > 64 ? launch<128>(a, plan, most_rows, workspace, stream) : launch<64>(a, plan, most_rows, workspace, stream);
+    // heads of up to 96: a quarter of the products of 128 less (the prompts above 206 -> 192 us; the kernel for few rows waits for memory, and has one form)
+    if (a.p.dim > 96) return launch<128, 128>(a, plan, most_rows, workspace, stream);
+    if (a.p.dim > 64) return launch<128, 96>(a, plan, most_rows, workspace, stream);
+    return launch<64, 64>(a, plan, most_rows, workspace, stream);
 }

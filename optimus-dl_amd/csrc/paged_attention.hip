@@ -36,6 +36,11 @@ constexpr int kManyRows = 256, kManyKeys = 64, kManyWaves = 8;
 // Blocks that splits are made for.  Of the small ones two run on a compute unit: with 256 / 512 / 1024 the decode step above takes 304 / 316 / 301 us, drafts on codes
 // 84 / 77 / 90, the long sequence 111 / 117 / 135.  Of the large ones one: with 256 / 512 the chunk takes 524 / 556, the prompts 206 / 231.
 constexpr int kFewTarget = 512, kManyTarget = 256;
+// Steps of 128 keys that a split of the small ones has at least.  A table of up to four is not cut, which saves the join: one token behind 200 / 500 / 1000, 12 heads of 64 (a
+// captured step, us): 7.8 / 9.9 / 14.5 with four, 7.8 / 12.3 / 12.3 with two, 11.2 / 11.4 / 11.7 with one; 8 sequences, 32 heads on 8 of 128: 9.8 / 13.2 / 18.9, 9.8 / 14.3 / 18.5
+// and 12.4 / 15.4 / 23.1.
+constexpr int kUncut = 4;
+__host__ __device__ constexpr int few_least(int reach) { return reach <= kUncut * kFewKeys * kFewWaves ? kUncut : 2; }
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kSlack = 8.0f;                                 // how far, in powers of two, a running maximum may lag behind
 
@@ -102,7 +107,7 @@ __device__ bool find(const Attend &a, uint32_t index, uint32_t target, Item &it)
         work += (int64_t)h.tiles * h.units;
     }
     const int64_t per64 = (wave_add(work) * a.p.kv_heads + target - 1) / target;
-    const uint32_t per = (uint32_t)min(max(per64, (int64_t)1), (int64_t)INT32_MAX);
+    const uint32_t per = (uint32_t)min(max(per64, (int64_t)(KEYS == kFewKeys * kFewWaves ? few_least(a.p.reach) : 1)), (int64_t)INT32_MAX);
     uint32_t parts0 = 0;
     int64_t slots0 = 0;
     for (int s0 = 0; s0 < a.p.seqs; s0 += kWave) {
@@ -969,7 +974,7 @@ int launch(Attend &a, const Plan &plan, int64_t most_rows, float *workspace, hip
         const dim3 grid(blocks(plan.many ? seqs : seqs + rows / kFewRows, kFewTarget));         // (beside the other kernel: a tile a sequence)
         if (a.p.e4m3) hipLaunchKernelGGL((attend_few_kernel<D, true>), grid, dim3(kFewWaves * kWave), few_lds(D, true), stream, a);
         else hipLaunchKernelGGL((attend_few_kernel<D, false>), grid, dim3(kFewWaves * kWave), few_lds(D, false), stream, a);
-        if (a.p.reach > kFewKeys * kFewWaves)
+        if (a.p.reach > kFewKeys * kFewWaves * few_least(a.p.reach))
             hipLaunchKernelGGL((attend_join_kernel<D, kFewRows, kFewKeys * kFewWaves, kJoinFew>), dim3(joins(kFewTarget), (unsigned)(((most_rows < kFewRows ? most_rows : kFewRows) + kJoinFew - 1) / kJoinFew)), dim3(256), 0, stream, a,
                                (uint32_t)kFewTarget);
     }

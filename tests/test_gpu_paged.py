@@ -315,3 +315,18 @@ def test_a_row_of_scores_of_minus_infinity_answers_0(rows):
     args = (torch.tensor(v, dtype=torch.int32, device="cuda") for v in ([[0]], [0, rows], [rows]))
     y = paged_attention(q, keys, torch.ones_like(keys), *args)
     assert (y[0] == 0).all() and (y[1:] == 1).all()            # (the first token sees that key alone)
+
+
+@pytest.mark.parametrize("length", [1, 129, 257, 511, 512])
+@pytest.mark.parametrize("cache", [BF16, E4M3])
+def test_wider_tables_answer_the_same(length, cache):
+    """A table of 512 tokens is not cut, wider ones are: a rounding of the weights and one of the result each, of at most half a step, relative to the largest value."""
+    g = torch.Generator(device="cuda").manual_seed(length)
+    q = torch.randn(1, 8, 64, generator=g, device="cuda").to(BF16)
+    keys, values = (torch.randn(32, 2, 16, 64, generator=g, device="cuda").to(cache) for _ in range(2))
+    scales = {k: torch.ones(2, device="cuda") for k in ("key_scale", "value_scale")} if cache == E4M3 else {}
+    ints = lambda v: torch.tensor(v, dtype=torch.int32, device="cuda")
+    outs = [paged_attention(q, keys, values, ints([list(range(32)) + [-1] * more]), ints([0, 1]), ints([length]), max_new=1, **scales).double() for more in (0, 1, 40)]
+    most = values.double().abs().max()
+    for y in outs[1:]:
+        assert (y - outs[0]).abs().max() <= 4 * (torch.finfo(BF16).eps / 2 + 2.0 ** -16) * most

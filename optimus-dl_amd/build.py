@@ -130,6 +130,34 @@ def check_saturating_conversions(asm_text: str, name: str = "") -> list[str]:
     return problems
 
 
+def check_masked_spills(asm_text: str, name: str = "") -> list[str]:
+    """Finds spills and reloads of vector registers in front of the instruction with which a block switches lanes on again.
+
+    Where paths of a branch that lanes take differently meet, the block begins with ``s_or_b64 exec, exec, ..``.  What register allocation puts in front of it
+    is done for the lanes of one path alone, though all lanes go on with it: the others read back what was never stored.  The compiler has been seen to do so
+    (with a copy of a scalar register at the start of such a block), so the generated code is checked after every build."""
+    problems, func, pending = [], "", None
+    for i, raw in enumerate(asm_text.split("\n")):
+        m = re.match(r"^(_Z\w+):", raw)
+        if m:
+            func, pending = m.group(1), None
+            continue
+        if re.match(r"^(\.LBB\d+_\d+:|; %bb\.\d+:)", raw):
+            pending = []
+            continue
+        text = raw.strip()
+        if pending is None or not text or text[0] in ";.":
+            continue
+        if text.startswith("s_or_b64 exec, exec"):
+            problems += [f"{name}:{n}: '{t}' in {func} in front of '{text}'" for n, t in pending]
+            pending = None
+        elif text.startswith(("s_cbranch", "s_branch")) or "exec" in text.split(";")[0]:
+            pending = None
+        elif "Folded Spill" in text or "Folded Reload" in text:
+            pending.append((i + 1, text))
+    return problems
+
+
 def host_command() -> list[str]:
     """The command that compiles csrc/host.cpp against the installed torch."""
     import torch
@@ -172,6 +200,7 @@ def build(verbose: bool = False, keep_asm: bool = False) -> str:
             text = fh.read()
         problems += check_asm_hazards(text, os.path.basename(asm))
         problems += check_saturating_conversions(text, os.path.basename(asm))
+        problems += check_masked_spills(text, os.path.basename(asm))
     if problems:
         raise RuntimeError("hazards in the generated code:\n" + "\n".join(problems))
     if not keep_asm:

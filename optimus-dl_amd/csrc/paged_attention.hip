@@ -232,7 +232,8 @@ struct Rows32 {
         for (int d = 0; d < C / 32; ++d) o[d] = f32x16{};
     }
 
-    // rows first_row + lane % 32 of a tile's: q of a token's head, zeros where there is no such row
+    // rows first_row + lane % 32 of a tile's: q of a token's head, zeros where there is no such row.  Every lane reads, the sequence's first token where it has no row: around
+    // masked loads the compiler may spill what all lanes need, for the lanes that are on alone.
     __device__ __forceinline__ void load_q(const Attend &a, const Run &run, int row, int kv_head) {
         const int lane = threadIdx.x % kWave, token = row / a.group, head = kv_head * a.group + row % a.group;
         const bool live = token < run.n;
@@ -240,8 +241,9 @@ struct Rows32 {
 #pragma unroll
         for (int s = 0; s < C / 16; ++s) {
             const int c = 16 * s + 8 * (lane / 32);
-            u32x4 v = {0, 0, 0, 0};
-            if (live && c < a.p.dim) v = *reinterpret_cast<const u32x4 *>(from + c);
+            u32x4 v = *reinterpret_cast<const u32x4 *>(from + (c < a.p.dim ? c : 0));
+#pragma unroll
+            for (int i = 0; i < 4; ++i) v[i] = live && c < a.p.dim ? v[i] : 0u;
             q[s] = __builtin_bit_cast(bf16x8, v);
         }
     }

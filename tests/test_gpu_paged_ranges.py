@@ -1,0 +1,42 @@
+"""Attention over a paged cache where numbers are large, odd or 0: caps over their whole range."""
+
+import pytest
+import torch
+
+from optimus_dl_amd.modules.paged import paged_attention
+from tests.paged_helpers import BF16, E4M3, Case, assert_near
+from tests.paged_oracle import attention_rows
+
+pytestmark = pytest.mark.gpu
+CUDA = torch.device("cuda")
+
+
+def attend(c, rows=None, scale=None, **kwargs):
+    """Against the definition, in the given rows (all)."""
+    scale, rows = c.dim ** -0.5 if scale is None else scale, list(range(c.rows)) if rows is None else rows
+    want, far = attention_rows(c, rows, scale, kwargs.get("window", 0), kwargs.get("softcap", 0.0))
+    c.to(CUDA)
+    got = paged_attention(c.q, c.keys, c.values, *c.batch(), scale=scale, **kwargs, **c.scales())
+    assert_near(got[rows], want, far)
+    return got
+
+
+FEW, MANY = ([1, 4], [300, 70]), ([70, 2], [200, 33])
+
+
+@pytest.mark.parametrize("cap", [0.5, 3.0, 30.0, 256.0, 257.0, 1e3, 1e4, 1e5, 1e6])
+@pytest.mark.parametrize("cache", [BF16, E4M3])
+@pytest.mark.parametrize("new,lengths", [FEW, MANY])
+def test_caps_of_every_size(cap, cache, new, lengths):
+    attend(Case(new, lengths, 4, 2, 64, 16, cache, seed=1), softcap=cap)
+    attend(Case(new, lengths, 4, 2, 96, 16, cache, seed=2, q_scale=6.0), softcap=cap)
+
+
+@pytest.mark.parametrize("cap", [1e3, 1e6])
+@pytest.mark.parametrize("new,lengths", [FEW, MANY])
+def test_scores_near_a_large_cap_beside_small_ones(cap, new, lengths):
+    """Heads whose scores reach the cap in the same tile as heads whose scores are of size 1."""
+    c = Case(new, lengths, 4, 1, 64, 16, seed=3)
+    c.q[:, 1] *= cap / 10
+    c.q[:, 3] *= cap / 200
+    attend(c, softcap=cap)

@@ -238,12 +238,13 @@ struct Rows32 {
         const int lane = threadIdx.x % kWave, token = row / a.group, head = kv_head * a.group + row % a.group;
         const bool live = token < run.n;
         const uint16_t *from = a.q + (int64_t)(run.first + (live ? token : 0)) * a.q_row + head * a.q_head;
+        const uint32_t sign = a.p.key_scale && a.p.key_scale[kv_head] < 0.0f ? 0x80008000u : 0u;             // (see caps_of)
 #pragma unroll
         for (int s = 0; s < C / 16; ++s) {
             const int c = 16 * s + 8 * (lane / 32);
             u32x4 v = *reinterpret_cast<const u32x4 *>(from + (c < a.p.dim ? c : 0));
 #pragma unroll
-            for (int i = 0; i < 4; ++i) v[i] = live && c < a.p.dim ? v[i] : 0u;
+            for (int i = 0; i < 4; ++i) v[i] = live && c < a.p.dim ? v[i] ^ sign : 0u;
             q[s] = __builtin_bit_cast(bf16x8, v);
         }
     }
@@ -288,7 +289,7 @@ struct Rows32 {
         for (int b = 0; b < NB; ++b)
 #pragma unroll
             for (int i = 0; i < 16; ++i) most = fmaxf(most, __builtin_fabsf(s[b][i]));
-        if (!__any(most * __builtin_fabsf(by) > 0.5f)) return all(near);
+        if (!__any(most * by > 0.5f)) return all(near);
         all([&](float v) { return __builtin_fabsf(v * by) > 0.5f ? far(v) : near(v); });
     }
 
@@ -471,13 +472,16 @@ __device__ __forceinline__ float quotient_of(const Attend &a, int kv_head, float
     return l == 0.0f ? 0.0f : (a.p.value_scale ? a.p.value_scale[kv_head] : 1.0f) / l;
 }
 
+// Scores from products: c powers of two a unit, or a cap's in and out.  A sign of the keys' scale is in q, so that larger products are larger scores; with a scale of 0 all
+// scores are 0, which the least c above 0 makes of them too, and hidden ones stay -inf.
 struct Caps {
     float c, in, out;
 };
 __device__ __forceinline__ Caps caps_of(const Attend &a, int kv_head) {
-    const float scale = a.p.key_scale ? a.scale * a.p.key_scale[kv_head] : a.scale;
+    const float scale = a.p.key_scale ? a.scale * __builtin_fabsf(a.p.key_scale[kv_head]) : a.scale;
     if (a.softcap > 0.0f) return {1.0f, 2.0f * kLog2e * scale / a.softcap, a.softcap * kLog2e};
-    return {scale * kLog2e, 0.0f, 0.0f};
+    const float c = scale * kLog2e;
+    return {c == 0.0f ? __FLT_DENORM_MIN__ : c, 0.0f, 0.0f};
 }
 
 // ---------------------------------------------------------------------------------------------------------------- keys and values on their way to LDS
@@ -592,7 +596,7 @@ __global__ __launch_bounds__(kFewWaves *kWave, E4M3 ? 2 : 1) void attend_few_ker
         }
         if (pass == kFinite) make_finite(kt + kTile, lane, kWave, kTile / 16);
         w.scores(kt);
-        if (caps.in > 0.0f) w.cap(caps.in, caps.out);
+        if (a.softcap > 0.0f) w.cap(caps.in, caps.out);
         if (held != ~0u || base + kFewKeys - 1 > pos0 || base <= pos1 - a.window) w.hide(seen >> h4);
         w.weights(caps.c);
         w.sums(kt + kTile);
@@ -834,7 +838,7 @@ __global__ __launch_bounds__(kManyWaves *kWave) void attend_many_kernel(Attend a
         turn();
         for (int t = 0; t < tiles; ++t) {
             const int base = base_of(t);
-            if (caps.in > 0.0f) w.cap(caps.in, caps.out);
+            if (a.softcap > 0.0f) w.cap(caps.in, caps.out);
             if (held[0] != ~0ull || base + kManyKeys - 1 > pos0 || base <= pos1 - a.window) w.hide(seen_of(pos, base, a.window, held[0]) >> h4);
             w.weights(caps.c);
             fetch(t + 2, keys + b2, values + b1);

@@ -1,4 +1,5 @@
-"""Attention over a paged cache where numbers are large, odd or 0: caps over their whole range."""
+"""Attention over a paged cache where numbers are large, odd or 0: caps and scales over their whole range."""
+import math
 
 import pytest
 import torch
@@ -40,3 +41,26 @@ def test_scores_near_a_large_cap_beside_small_ones(cap, new, lengths):
     c.q[:, 1] *= cap / 10
     c.q[:, 3] *= cap / 200
     attend(c, softcap=cap)
+
+
+@pytest.mark.parametrize("softcap", [0.0, 30.0])
+@pytest.mark.parametrize("new,lengths", [FEW, MANY])
+def test_scales_of_0_and_below(softcap, new, lengths):
+    """A code stands for code * scale, whatever the scale: keys of 0 answer the mean of the values that are seen."""
+    c = Case(new, lengths, 6, 3, 64, 16, E4M3, seed=4)
+    c.key_scale[0], c.key_scale[1], c.value_scale[2] = 0.0, -c.key_scale[1], -c.value_scale[2]
+    attend(c, softcap=softcap)
+    c = Case(new, lengths, 4, 2, 128, 16, E4M3, seed=5)
+    c.key_scale[1], c.value_scale[0] = 0.0, 0.0
+    got = attend(c, softcap=softcap, window=50)
+    assert (got[:, :2] == 0).all()
+
+
+@pytest.mark.parametrize("new,lengths", [FEW, MANY])
+def test_scales_that_are_none(new, lengths):
+    """A scale of NaN is that head's answer, and that head's alone."""
+    c = Case(new, lengths, 4, 2, 64, 16, E4M3, seed=6)
+    c.key_scale[0] = math.nan
+    c.to(CUDA)
+    got = paged_attention(c.q, c.keys, c.values, *c.batch(), **c.scales())
+    assert got[:, :2].isnan().all() and got[:, 2:].isfinite().all()

@@ -794,7 +794,7 @@ typedef struct odl_fp8_paged_batch {
  *   (a, b) -> (a * cos - b * sin, a * sin + b * cos)  for pairs of the first 2 * half elements of a head: (2 i, 2 i + 1) where interleaved, else
  *             (i, half + i), angles of the token's position; half 0: none.  cos, sin fp32 [positions, half], positions >= width * page_size.
  * Every step rounds to fp32, in this order, without fused multiply-adds; what is stored rounds once, to bf16 or, divided by the scale and clamped to
- * +-448, to E4M3.
+ * +-448, to E4M3; where the scale is 0 that is code 0, NaN for a NaN.
  * q [rows, heads, head_dim], k and v [rows, kv_heads, head_dim] bf16, strides of row and head in elements, multiples of 8; addresses multiples
  * of 16 bytes.  q_out bf16 [rows, heads, head_dim], zero in rows that belong to nobody.  half a multiple of 4 where interleaved, else of 8.
  * No two rows may have the same slot.

@@ -153,7 +153,7 @@ __global__ __launch_bounds__(256) void append_kv_kernel(Append a) {
     if (p.e4m3) {
         const float scale = (is_v ? p.value_scale : p.key_scale)[head];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) x[i] = __fdiv_rn(x[i], scale);
+        for (int i = 0; i < 8; ++i) x[i] = scale != 0.0f ? __fdiv_rn(x[i], scale) : x[i] != x[i] ? x[i] : 0.0f;           // (every code stands for 0; 0 / 0 would be none)
         *reinterpret_cast<u32x2 *>(to + c * 8) = u32x2{quantise4<ODL_FP8_E4M3>(x[0], x[1], x[2], x[3], 1.0f, 1.0f, 1.0f, 1.0f),
                                                         quantise4<ODL_FP8_E4M3>(x[4], x[5], x[6], x[7], 1.0f, 1.0f, 1.0f, 1.0f)};
     } else {

@@ -88,7 +88,8 @@ def _append_plain(q, k, v, keys, values, pages, offsets, lengths, cos, sin, inte
         out[rows] = turned(q[rows], q_weight, position).to(q.dtype)
         for cache, x, scale in ((keys, turned(k[rows], k_weight, position), key_scale), (values, v[rows].to(wide), value_scale)):
             if scale is not None:
-                x = (x / scale.view(1, -1, 1)).clamp(-E4M3_MAX, E4M3_MAX)
+                scale = scale.view(1, -1, 1)
+                x = torch.where(scale == 0, torch.where(x.isnan(), x, torch.zeros_like(x)), (x / scale).clamp(-E4M3_MAX, E4M3_MAX))
             x = x.to(cache.dtype)
             bits = {1: torch.uint8, 2: torch.int16, 4: torch.int32, 8: torch.int64}[cache.element_size()]
             cache.view(bits)[page[held], :, slot[held]] = x.view(bits)[held]
@@ -138,7 +139,7 @@ def append_kv(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, keys: torch.Ten
 
     q [rows, heads, head_dim], k and v [rows, kv heads, head_dim]: the new tokens of sequence s are rows ``offsets[s]`` to ``offsets[s + 1]``.  keys, values
     [pages, kv heads, page size, head_dim]: the cache, bf16, or float8_e4m3fn with ``key_scale`` and ``value_scale`` [kv heads] (fp32; a code stands for
-    code * scale, larger values are clamped).  lengths: tokens of each sequence in the cache, with the new ones; position p of sequence s is in slot
+    code * scale, larger values are clamped, and all are 0 where the scale is).  lengths: tokens of each sequence in the cache, with the new ones; position p of sequence s is in slot
     ``p % page size`` of page ``pages[s, p // page size]``.  pages, offsets, lengths int32.
 
     cos, sin: fp32 [positions, pairs], of every position that the table reaches; the first 2 * pairs elements of a head are rotated, as pairs (2 i, 2 i + 1)

@@ -4,8 +4,8 @@ import math
 import pytest
 import torch
 
-from optimus_dl_amd.modules.paged import paged_attention
-from tests.paged_helpers import BF16, E4M3, Case, assert_near
+from optimus_dl_amd.modules.paged import append_kv, paged_attention
+from tests.paged_helpers import BF16, E4M3, Case, assert_near, bits
 from tests.paged_oracle import attention_rows
 
 pytestmark = pytest.mark.gpu
@@ -64,3 +64,20 @@ def test_scales_that_are_none(new, lengths):
     c.to(CUDA)
     got = paged_attention(c.q, c.keys, c.values, *c.batch(), **c.scales())
     assert got[:, :2].isnan().all() and got[:, 2:].isfinite().all()
+
+
+def test_nothing_is_kept_of_a_head_whose_scale_is_0():
+    """Every code stands for 0 there; 0 / 0 is no code."""
+    c = Case([3, 1], [20, 9], 4, 2, 64, 16, E4M3, seed=14)
+    c.key_scale[0], c.value_scale[1] = 0.0, 0.0
+    c.k[1, 0], c.v[2, 1] = 0.0, 0.0
+    c.to(CUDA)
+    q = append_kv(c.q, c.k, c.v, c.keys, c.values, *c.batch(), **c.scales())
+    for t, dead in ((c.keys, 0), (c.values, 1)):
+        for s, p in ((0, 17), (0, 18), (0, 19), (1, 8)):
+            page = int(c.pages[s, p // 16])
+            assert (bits(t)[page, dead, p % 16] == 0).all() and (bits(t)[page, 1 - dead, p % 16] != 0).any()
+    assert paged_attention(q, c.keys, c.values, *c.batch(), **c.scales()).isfinite().all()
+    c.k[0, 0, 3], c.k[0, 0, 5] = math.nan, math.inf
+    append_kv(c.q, c.k, c.v, c.keys, c.values, *c.batch(), **c.scales())
+    assert c.keys[int(c.pages[0, 1]), 0, 1].float().isnan().tolist() == [i == 3 for i in range(64)]

@@ -467,6 +467,12 @@ __device__ __forceinline__ void store_row(const Attend &a, const Run &run, int r
 // What a sum against maximum m counts where `top` is the maximum of all.  A part that sees nothing has maximum -inf and sums 0, one that sees only NaN
 // -inf and NaN.
 __device__ __forceinline__ float weight_of(float m, float top) { return m == top ? 1.0f : __builtin_amdgcn_exp2f(m - top); }
+// A part's sum among others: an infinity that a row sees counts whatever its part weighs, though the weight of a part far below the others is 0 here.
+__device__ __forceinline__ f32x4 weighed(f32x4 o, float weight) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) o[i] *= __builtin_fabsf(o[i]) < INFINITY ? weight : 1.0f;
+    return o;
+}
 // By what a row's sums are multiplied in the end; a row that sees nothing, or no score above -inf, answers 0.
 __device__ __forceinline__ float quotient_of(const Attend &a, int kv_head, float l) {
     return l == 0.0f ? 0.0f : (a.p.value_scale ? a.p.value_scale[kv_head] : 1.0f) / l;
@@ -649,7 +655,7 @@ __global__ __launch_bounds__(kFewWaves *kWave, E4M3 ? 2 : 1) void attend_few_ker
 #pragma unroll
             for (int i = 0; i < 4; ++i)
                 *reinterpret_cast<f32x4 *>(sums + (wave * 32 + r) * kRow + 32 * d + 8 * i + 4 * (lane / 32)) =
-                    f32x4{w.o[d][4 * i] * part, w.o[d][4 * i + 1] * part, w.o[d][4 * i + 2] * part, w.o[d][4 * i + 3] * part};
+                    weighed(f32x4{w.o[d][4 * i], w.o[d][4 * i + 1], w.o[d][4 * i + 2], w.o[d][4 * i + 3]}, part);
     }
     __syncthreads();
     const int64_t slot = (it.slot + it.split) * a.p.kv_heads + head;
@@ -931,7 +937,7 @@ __global__ __launch_bounds__(256) void attend_join_kernel(Attend a, uint32_t tar
                 const float *from = a.partial + place(s0, r) * D + d;
                 const int64_t step = (int64_t)a.p.kv_heads * ROWS * D;
 #pragma unroll 4
-                for (int s = group; s < count; s += kGroups) o[k] += *reinterpret_cast<const f32x4 *>(from + s * step) * weight[r][s];
+                for (int s = group; s < count; s += kGroups) o[k] += weighed(*reinterpret_cast<const f32x4 *>(from + s * step), weight[r][s]);
             }
         }
         if constexpr (kGroups > 1) {

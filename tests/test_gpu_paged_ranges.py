@@ -1,4 +1,4 @@
-"""Attention over a paged cache where numbers are large, odd or 0: caps and scales over their whole range."""
+"""Attention over a paged cache where numbers are large, odd or 0: caps and scales over their whole range, infinities in work that is cut into splits."""
 import math
 
 import pytest
@@ -81,3 +81,23 @@ def test_nothing_is_kept_of_a_head_whose_scale_is_0():
     c.k[0, 0, 3], c.k[0, 0, 5] = math.nan, math.inf
     append_kv(c.q, c.k, c.v, c.keys, c.values, *c.batch(), **c.scales())
     assert c.keys[int(c.pages[0, 1]), 0, 1].float().isnan().tolist() == [i == 3 for i in range(64)]
+
+
+# Contexts that are cut into splits: (new tokens, tokens, heads, key heads)
+CUT = [([1, 1], [3000, 40], 4, 1), ([40, 1], [5000, 70], 2, 1)]
+
+
+@pytest.mark.parametrize("new,lengths,heads,kv", CUT)
+def test_infinities_of_little_weight_in_a_split(new, lengths, heads, kv):
+    """A seen infinity comes through whatever its weight, some e^-160 here, in whichever split or wave it lies."""
+    for place in (5, 700, lengths[0] - new[0] - 60):
+        c = Case(new, lengths, heads, kv, 64, 16, seed=7)
+        c.q.fill_(1.0)
+        c.keys.mul_(0.01)
+        last = lengths[0] - new[0] - 10            # keys from here on score 20 * 64 / 8 more
+        for p in range(last, lengths[0]):
+            c.keys[int(c.pages[0, p // 16]), :, p % 16] += 20.0
+        at = int(c.pages[0, place // 16]), 0, place % 16
+        c.values[at + (3,)], c.values[at + (4,)], c.values[at + (5,)] = math.inf, -math.inf, math.nan
+        got = attend(c, rows=list(range(sum(new))))[0]
+        assert (got[:, 3] == math.inf).all() and (got[:, 4] == -math.inf).all() and got[:, 5].isnan().all() and got[:, 6:].isfinite().all()

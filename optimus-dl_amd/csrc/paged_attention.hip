@@ -473,10 +473,9 @@ __device__ __forceinline__ f32x4 weighed(f32x4 o, float weight) {
     for (int i = 0; i < 4; ++i) o[i] *= __builtin_fabsf(o[i]) < INFINITY ? weight : 1.0f;
     return o;
 }
-// By what a row's sums are multiplied in the end; a row that sees nothing, or no score above -inf, answers 0.
-__device__ __forceinline__ float quotient_of(const Attend &a, int kv_head, float l) {
-    return l == 0.0f ? 0.0f : (a.p.value_scale ? a.p.value_scale[kv_head] : 1.0f) / l;
-}
+// A row's answer from its sums; a row that sees nothing, or no score above -inf, answers 0, infinities and NaN among its values or not.
+__device__ __forceinline__ float quotient_of(const Attend &a, int kv_head, float l) { return (a.p.value_scale ? a.p.value_scale[kv_head] : 1.0f) / l; }
+__device__ __forceinline__ f32x4 answer_of(f32x4 o, float l, float quotient) { return l == 0.0f ? f32x4{0.0f, 0.0f, 0.0f, 0.0f} : o * quotient; }
 
 // Scores from products: c powers of two a unit, or a cap's in and out.  A sign of the keys' scale is in q, so that larger products are larger scores; with a scale of 0 all
 // scores are 0, which the least c above 0 makes of them too, and hidden ones stay -inf.
@@ -672,7 +671,7 @@ __global__ __launch_bounds__(kFewWaves *kWave, E4M3 ? 2 : 1) void attend_few_ker
             l = __fmaf_rn(ml[(v * 32 + rr) * 2 + 1], weight_of(ml[(v * 32 + rr) * 2], m), l);
         }
         if (it.splits == 1) {
-            if (d < a.p.dim) store_row(a, it.run, row0 + rr, head, d, o * quotient_of(a, head, l));
+            if (d < a.p.dim) store_row(a, it.run, row0 + rr, head, d, answer_of(o, l, quotient_of(a, head, l)));
         } else if (slot < a.slots) {
             *reinterpret_cast<f32x4 *>(a.partial + (slot * kFewRows + rr) * D + d) = o;
             if (d == 0) {
@@ -879,7 +878,7 @@ __global__ __launch_bounds__(kManyWaves *kWave) void attend_many_kernel(Attend a
             const int at = 32 * d + 8 * i + 4 * (lane / 32);
             const f32x4 o = {w.o[d][4 * i], w.o[d][4 * i + 1], w.o[d][4 * i + 2], w.o[d][4 * i + 3]};
             if (it.splits == 1) {
-                if (at < a.p.dim) store_row(a, it.run, row, head, at, o * by);
+                if (at < a.p.dim) store_row(a, it.run, row, head, at, answer_of(o, w.l, by));
             } else if (slot < a.slots) {
                 *reinterpret_cast<f32x4 *>(a.partial + (slot * kManyRows + row - it.tile * kManyRows) * D + at) = o;
             }
@@ -950,7 +949,7 @@ __global__ __launch_bounds__(256) void attend_join_kernel(Attend a, uint32_t tar
 #pragma unroll
         for (int k = 0; k < (kItems + 255) / 256; ++k) {
             const int e = threadIdx.x + k * 256, r = e / kColumns, d = e % kColumns * 4;
-            if (r < used && d < a.p.dim && (kGroups == 1 || !group)) store_row(a, it.run, row0 + r, head, d, o[k] * quotient_of(a, head, totals[r]));
+            if (r < used && d < a.p.dim && (kGroups == 1 || !group)) store_row(a, it.run, row0 + r, head, d, answer_of(o[k], totals[r], quotient_of(a, head, totals[r])));
         }
     }
 }

@@ -125,7 +125,7 @@ def _attention_plain(q, keys, values, pages, offsets, lengths, scale, window, so
         odd = ~v.isfinite()
         y = torch.matmul(weight.unsqueeze(2), torch.where(odd, torch.zeros_like(v), v)).squeeze(2)
         if odd.any():
-            y = y + torch.where(odd & seen.view(1, *seen.shape, 1), v, torch.zeros_like(v)).sum(2)
+            y = y + torch.where(odd & seen.view(1, *seen.shape, 1) & some.unsqueeze(2), v, torch.zeros_like(v)).sum(2)
         out[first:first + n] = y.transpose(0, 1).to(q.dtype)
     return out
 

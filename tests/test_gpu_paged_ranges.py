@@ -101,3 +101,13 @@ def test_infinities_of_little_weight_in_a_split(new, lengths, heads, kv):
         c.values[at + (3,)], c.values[at + (4,)], c.values[at + (5,)] = math.inf, -math.inf, math.nan
         got = attend(c, rows=list(range(sum(new))))[0]
         assert (got[:, 3] == math.inf).all() and (got[:, 4] == -math.inf).all() and got[:, 5].isnan().all() and got[:, 6:].isfinite().all()
+
+
+@pytest.mark.parametrize("new,lengths", [([2], [40]), ([60], [200]), ([1], [3000])])
+def test_rows_without_a_score_above_minus_infinity_answer_0_beside_odd_values(new, lengths):
+    c = Case(new, lengths, 2, 1, 64, 16, seed=8)
+    c.q.fill_(1.0)
+    c.keys[..., 7] = -math.inf
+    c.values[..., 3], c.values[..., 4] = math.inf, math.nan
+    c.to(CUDA)
+    assert (paged_attention(c.q, c.keys, c.values, *c.batch()) == 0).all()

@@ -19,3 +19,13 @@ def test_nothing_is_kept_of_a_head_whose_scale_is_0():
     c.k[0, 0, 3] = float("nan")
     append_kv(c.q, c.k, c.v, c.keys, c.values, *c.batch(), **c.scales())
     assert c.keys[int(c.pages[0, 4]), 0, 1].float().isnan().tolist() == [i == 3 for i in range(16)]
+
+
+def test_rows_without_a_score_above_minus_infinity_answer_0_beside_odd_values():
+    c = Case([2, 1], [30, 5], 4, 2, 16, 4, seed=2)
+    c.q.fill_(1.0)
+    c.values[..., 3], c.values[..., 4] = float("inf"), float("nan")
+    c.keys[..., 7] = -torch.inf
+    c.keys[int(c.pages[1, 1])] = 0.0             # the second sequence's last token
+    y = paged_attention(c.q, c.keys, c.values, *c.batch())
+    assert (y[:2] == 0).all() and (y[2, :, 3] == torch.inf).all() and y[2, :, 4].isnan().all() and y[2, :, 5:].isfinite().all()

@@ -772,7 +772,7 @@ int odl_fp8_fp4_quantise(const void *w, int src_dtype, int64_t N, int64_t K, int
  * 16 up to 128.
  * Batch: sequence s has its new tokens in rows offsets[s] to offsets[s + 1] of what is computed and, with them, lengths[s] tokens in the cache: row
  * offsets[s] + j is at position lengths[s] - n + j, and position p in slot p % page_size of page table[s * table_stride + p / page_size].
- * offsets rise from 0; rows from offsets[seqs] on belong to nobody.  A number in the table that is no page of the cache holds nothing: what would
+ * offsets rise; rows in front of offsets[0] and from offsets[seqs] on belong to nobody.  A number in the table that is no page of the cache holds nothing: what would
  * go there is not written, and takes no part in attention.  Positions outside of [0, width * page_size) likewise.  Entries behind a sequence's
  * last page are not read.
  */

@@ -142,11 +142,11 @@ __device__ bool find(const Attend &a, uint32_t index, uint32_t target, Item &it)
     return false;
 }
 
-// Rows that belong to nobody answer 0; the blocks of a launch share them.
+// Rows that belong to nobody, in front of the first sequence and behind the last, answer 0; the blocks of a launch share them.
 __device__ void clear_rest(const Attend &a, int64_t block, int64_t blocks, int threads) {
-    const int used = a.p.seqs ? min(max(a.p.offsets[a.p.seqs], 0), a.p.rows) : 0;
-    const int64_t row = (int64_t)a.heads * a.p.dim / 8, end = (int64_t)a.p.rows * row;
-    for (int64_t i = used * row + block * threads + threadIdx.x; i < end; i += blocks * threads) reinterpret_cast<u32x4 *>(a.out)[i] = u32x4{0, 0, 0, 0};
+    const int first = a.p.seqs ? min(max(a.p.offsets[0], 0), a.p.rows) : 0, used = a.p.seqs ? min(max(a.p.offsets[a.p.seqs], 0), a.p.rows) : 0;
+    const int64_t row = (int64_t)a.heads * a.p.dim / 8, front = first * row, end = front + (a.p.rows - used) * row;
+    for (int64_t i = block * threads + threadIdx.x; i < end; i += blocks * threads) reinterpret_cast<u32x4 *>(a.out)[i < front ? i : i - front + used * row] = u32x4{0, 0, 0, 0};
 }
 
 // ---------------------------------------------------------------------------------------------------------------- tiles in LDS

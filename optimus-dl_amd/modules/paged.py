@@ -144,7 +144,7 @@ def append_kv(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, keys: torch.Ten
 
     cos, sin: fp32 [positions, pairs], of every position that the table reaches; the first 2 * pairs elements of a head are rotated, as pairs (2 i, 2 i + 1)
     where ``interleaved``, else (i, pairs + i).  q_weight, k_weight [head_dim]: norms by root mean square in front of the rotation.
-    Rows behind the last sequence are not read: their queries are 0.  Tokens whose page is none of the cache are not written, those behind the
+    Rows of no sequence, in front of the first or behind the last, are not read: their queries are 0.  Tokens whose page is none of the cache are not written, those behind the
     table's reach neither, and their queries are 0.  Two rows of a call must not share a slot.
 
     bf16 on the GPU, one kernel, in head dimensions of 16 to 128 (a multiple of 16).  CPU tensors run as torch operations, in any floating type."""
@@ -179,7 +179,7 @@ def paged_attention(q: torch.Tensor, keys: torch.Tensor, values: torch.Tensor, p
     default), and ``softcap * tanh(score / softcap)`` where softcap is not 0.  Heads in groups share a head of the cache.
     max_new: the most new tokens of a sequence, where the program knows it: it chooses kernels, results hold without.
     Keys and values that a token does not see do not reach it, NaN and infinities included.  A token that sees nothing, or
-    no score above -inf, and rows behind the last sequence answer 0.
+    no score above -inf, and rows of no sequence answer 0.
 
     bf16 on the GPU: one kernel for up to 32 rows (tokens times heads of a group) a sequence, another for more, and one that joins parts; sums and maxima
     in fp32, weights rounded to bf16.  The same call answers the same bits.  CPU tensors run as torch operations, in any floating type."""

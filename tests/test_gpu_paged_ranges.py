@@ -111,3 +111,18 @@ def test_rows_without_a_score_above_minus_infinity_answer_0_beside_odd_values(ne
     c.values[..., 3], c.values[..., 4] = math.inf, math.nan
     c.to(CUDA)
     assert (paged_attention(c.q, c.keys, c.values, *c.batch()) == 0).all()
+
+
+@pytest.mark.parametrize("new,lengths", [FEW, MANY])
+def test_rows_in_front_of_the_first_sequence_answer_0(new, lengths):
+    """Offsets that begin behind row 0: those rows belong to nobody, as those behind the last sequence do."""
+    c = Case(new, lengths, 4, 2, 64, 16, pad=3, seed=9)
+    c.offsets = c.offsets + 2
+    want, far = attention_rows(c, list(range(c.rows)), 0.125)
+    c.to(CUDA)
+    for _ in range(3):                             # (memory that the answer is likely to get)
+        torch.full_like(c.q, math.nan)
+        got = paged_attention(c.q, c.keys, c.values, *c.batch())
+        assert (got[:2] == 0).all() and (got[-1:] == 0).all()
+        assert_near(got, want, far)
+    assert (append_kv(c.q, c.k, c.v, c.keys, c.values, *c.batch())[:2] == 0).all()

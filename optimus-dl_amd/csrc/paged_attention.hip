@@ -232,13 +232,14 @@ struct Rows32 {
         for (int d = 0; d < C / 32; ++d) o[d] = f32x16{};
     }
 
-    // rows first_row + lane % 32 of a tile's: q of a token's head, zeros where there is no such row.  Every lane reads, the sequence's first token where it has no row: around
-    // masked loads the compiler may spill what all lanes need, for the lanes that are on alone.
-    __device__ __forceinline__ void load_q(const Attend &a, const Run &run, int row, int kv_head) {
+    // Rows first_row + lane % 32 of a tile's: q of a token's head, zeros where there is no such row; the other sign where `negative` (see caps_of).  Every lane reads, those without a
+    // row the sequence's first token and pieces behind head_dim the first one: around masked loads the compiler may spill what all lanes need, for the lanes that are on
+    // alone.  (One token behind 200, heads of 128: 0.3 of 10 us.)
+    __device__ __forceinline__ void load_q(const Attend &a, const Run &run, int row, int kv_head, bool negative) {
         const int lane = threadIdx.x % kWave, token = row / a.group, head = kv_head * a.group + row % a.group;
         const bool live = token < run.n;
         const uint16_t *from = a.q + (int64_t)(run.first + (live ? token : 0)) * a.q_row + head * a.q_head;
-        const uint32_t sign = a.p.key_scale && a.p.key_scale[kv_head] < 0.0f ? 0x80008000u : 0u;             // (see caps_of)
+        const uint32_t sign = negative ? 0x80008000u : 0u;
 #pragma unroll
         for (int s = 0; s < C / 16; ++s) {
             const int c = 16 * s + 8 * (lane / 32);
@@ -465,28 +466,23 @@ __device__ __forceinline__ void store_row(const Attend &a, const Run &run, int r
 }
 
 // What a sum against maximum m counts where `top` is the maximum of all.  A part that sees nothing has maximum -inf and sums 0, one that sees only NaN
-// -inf and NaN.
-__device__ __forceinline__ float weight_of(float m, float top) { return m == top ? 1.0f : __builtin_amdgcn_exp2f(m - top); }
-// A part's sum among others: an infinity that a row sees counts whatever its part weighs, though the weight of a part far below the others is 0 here.
-__device__ __forceinline__ f32x4 weighed(f32x4 o, float weight) {
-#pragma unroll
-    for (int i = 0; i < 4; ++i) o[i] *= __builtin_fabsf(o[i]) < INFINITY ? weight : 1.0f;
-    return o;
-}
+// -inf and NaN.  No part counts nothing: an infinity that a row sees is its answer whatever its part weighs, and 2^-149 of any finite sum is none to be seen.
+__device__ __forceinline__ float weight_of(float m, float top) { return m == top ? 1.0f : fmaxf(__builtin_amdgcn_exp2f(m - top), __FLT_DENORM_MIN__); }
 // A row's answer from its sums; a row that sees nothing, or no score above -inf, answers 0, infinities and NaN among its values or not.
 __device__ __forceinline__ float quotient_of(const Attend &a, int kv_head, float l) { return (a.p.value_scale ? a.p.value_scale[kv_head] : 1.0f) / l; }
 __device__ __forceinline__ f32x4 answer_of(f32x4 o, float l, float quotient) { return l == 0.0f ? f32x4{0.0f, 0.0f, 0.0f, 0.0f} : o * quotient; }
 
-// Scores from products: c powers of two a unit, or a cap's in and out.  A sign of the keys' scale is in q, so that larger products are larger scores; with a scale of 0 all
+// Scores from products: c powers of two a unit, or a cap's in and out.  A sign of the keys' scale goes into q, so that larger products are larger scores; with a scale of 0 all
 // scores are 0, which the least c above 0 makes of them too, and hidden ones stay -inf.
 struct Caps {
     float c, in, out;
+    bool negative;
 };
 __device__ __forceinline__ Caps caps_of(const Attend &a, int kv_head) {
-    const float scale = a.p.key_scale ? a.scale * __builtin_fabsf(a.p.key_scale[kv_head]) : a.scale;
-    if (a.softcap > 0.0f) return {1.0f, 2.0f * kLog2e * scale / a.softcap, a.softcap * kLog2e};
+    const float of_keys = a.p.key_scale ? a.p.key_scale[kv_head] : 1.0f, scale = a.scale * __builtin_fabsf(of_keys);
+    if (a.softcap > 0.0f) return {1.0f, 2.0f * kLog2e * scale / a.softcap, a.softcap * kLog2e, of_keys < 0.0f};
     const float c = scale * kLog2e;
-    return {c == 0.0f ? __FLT_DENORM_MIN__ : c, 0.0f, 0.0f};
+    return {c == 0.0f ? __FLT_DENORM_MIN__ : c, 0.0f, 0.0f, of_keys < 0.0f};
 }
 
 // ---------------------------------------------------------------------------------------------------------------- keys and values on their way to LDS
@@ -587,7 +583,7 @@ __global__ __launch_bounds__(kFewWaves *kWave, E4M3 ? 2 : 1) void attend_few_ker
     const Caps caps = caps_of(a, head);
     const int32_t *table = a.p.table + it.seq * a.p.table_stride;
     Rows32<D, 1> w;
-    w.load_q(a, it.run, row, head);
+    w.load_q(a, it.run, row, head, E4M3 && caps.negative);
 
     const int h4 = 4 * (lane / 32);
     Pass pass = kOnce;
@@ -654,7 +650,7 @@ __global__ __launch_bounds__(kFewWaves *kWave, E4M3 ? 2 : 1) void attend_few_ker
 #pragma unroll
             for (int i = 0; i < 4; ++i)
                 *reinterpret_cast<f32x4 *>(sums + (wave * 32 + r) * kRow + 32 * d + 8 * i + 4 * (lane / 32)) =
-                    weighed(f32x4{w.o[d][4 * i], w.o[d][4 * i + 1], w.o[d][4 * i + 2], w.o[d][4 * i + 3]}, part);
+                    f32x4{w.o[d][4 * i] * part, w.o[d][4 * i + 1] * part, w.o[d][4 * i + 2] * part, w.o[d][4 * i + 3] * part};
     }
     __syncthreads();
     const int64_t slot = (it.slot + it.split) * a.p.kv_heads + head;
@@ -745,7 +741,7 @@ __global__ __launch_bounds__(kManyWaves *kWave) void attend_many_kernel(Attend a
     const int32_t *table = a.p.table + it.seq * a.p.table_stride;
     const int tiles = (range.end - range.first + kManyKeys - 1) / kManyKeys;
     Rows32<D, 2, C> w;
-    w.load_q(a, it.run, row, head);
+    w.load_q(a, it.run, row, head, E4M3 && caps.negative);
 
     const uint32_t keys = lds_base(lds), values = keys + 3 * kTile;
     const int h4 = 4 * (lane / 32);
@@ -936,7 +932,7 @@ __global__ __launch_bounds__(256) void attend_join_kernel(Attend a, uint32_t tar
                 const float *from = a.partial + place(s0, r) * D + d;
                 const int64_t step = (int64_t)a.p.kv_heads * ROWS * D;
 #pragma unroll 4
-                for (int s = group; s < count; s += kGroups) o[k] += weighed(*reinterpret_cast<const f32x4 *>(from + s * step), weight[r][s]);
+                for (int s = group; s < count; s += kGroups) o[k] += *reinterpret_cast<const f32x4 *>(from + s * step) * weight[r][s];
             }
         }
         if constexpr (kGroups > 1) {

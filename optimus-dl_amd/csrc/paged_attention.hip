@@ -167,7 +167,8 @@ __device__ __forceinline__ void to_lds(uint32_t to, const uint8_t *from, uint32_
     const uint64_t base = (uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)(v >> 32)) << 32 | (uint32_t)__builtin_amdgcn_readfirstlane((int)v);
     asm volatile("s_mov_b32 m0, %0\n\ts_nop 4\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(to), "v"(at), "s"(base) : "memory");
 }
-__device__ __forceinline__ void all_loads_done() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
+// Everything asked for is in LDS, and everything read from there in registers: what is asked for next may take its place.
+__device__ __forceinline__ void all_loads_done() { asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory"); }
 
 __device__ __forceinline__ const uint8_t *shuffled(const uint8_t *p, int lane) {
     const uint64_t v = reinterpret_cast<uint64_t>(p);

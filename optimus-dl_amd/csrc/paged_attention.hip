@@ -33,14 +33,20 @@ typedef __attribute__((address_space(3))) uint8_t lds_u8;
 
 constexpr int kFewRows = 32, kFewKeys = 32, kFewWaves = 4;
 constexpr int kManyRows = 256, kManyKeys = 64, kManyWaves = 8;
-// Blocks that splits are made for.  Of the small ones two run on a compute unit: with 256 / 512 / 1024 the decode step above takes 304 / 316 / 301 us, drafts on codes
-// 84 / 77 / 90, the long sequence 111 / 117 / 135.  Of the large ones one: with 256 / 512 the chunk takes 524 / 556, the prompts 206 / 231.
-constexpr int kFewTarget = 512, kManyTarget = 256;
-// Steps of 128 keys that a split of the small ones has at least.  A table of up to four is not cut, which saves the join: one token behind 200 / 500 / 1000, 12 heads of 64 (a
-// captured step, us): 7.8 / 9.9 / 14.5 with four, 7.8 / 12.3 / 12.3 with two, 11.2 / 11.4 / 11.7 with one; 8 sequences, 32 heads on 8 of 128: 9.8 / 13.2 / 18.9, 9.8 / 14.3 / 18.5
-// and 12.4 / 15.4 / 23.1.
-constexpr int kUncut = 4;
-__host__ __device__ constexpr int few_least(int reach) { return reach <= kUncut * kFewKeys * kFewWaves ? kUncut : 2; }
+// Blocks that splits are made for: as many as run at a time.  Of the large ones that is one a compute unit (with 256 / 512 the chunk takes 524 / 556, the prompts 206 / 231).
+// Of the small ones LDS decides: two, and one of those that hold two stages of bf16 for heads above 64 (with 512 / 256 for these: one token behind 131071 124 / 115 us, 32 sequences of
+// 4099 with 5 new tokens 122 / 114, 8 of 1000 24 / 18, 64 of 8192 435 / 435, all with 32 heads on 8 of 128).
+constexpr int few_lds(int D, bool e4m3) {
+    const int tiles = kFewWaves * (e4m3 ? 1 : 2) * 2 * kFewKeys * 2 * D, joined = kFewWaves * 32 * (D + 4) * 4 + kFewWaves * 32 * 8;
+    return tiles > joined ? tiles : joined;
+}
+constexpr int kManyTarget = 256;
+constexpr int few_target(int D, bool e4m3) { return few_lds(D, e4m3) <= 80 * 1024 ? 512 : 256; }
+// Steps of 128 keys that a split of the small ones has at least.  A table of up to four is not cut, which saves the join.  Behind a wider one the join is launched, whatever the lengths
+// are, and the longest sequence decides: up to two steps stay whole, up to sixteen are cut into single ones, more into two at least, since a join takes longer the more
+// there is to join.  One token behind 200 / 500 / 1000 / 4000 in a table of 4096 (a captured step, us): 12 heads of 64 10.8 / 11.7 / 11.9 / 13.9, with one step everywhere 11.4 / 11.6 / 11.9 /
+// 14.9, with two 10.8 / 12.5 / 12.6 / 13.9; 32 heads on 8 of 128 12.8 / 13.3 / 13.5 / 15.5, 12.8 / 13.0 / 13.3 / 16.3 and 12.9 / 14.5 / 14.7 / 15.5.
+constexpr int kUncut = 4, kWhole = 2, kSingle = 16;
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kSlack = 8.0f;                                 // how far, in powers of two, a running maximum may lag behind
 
@@ -102,12 +108,16 @@ __device__ bool find(const Attend &a, uint32_t index, uint32_t target, Item &it)
     const int lane = threadIdx.x % kWave;
     Share mine = share_of<ROWS, KEYS>(a, lane);
     int64_t work = (int64_t)mine.tiles * mine.units;
+    uint32_t most = mine.units;
     for (int s0 = kWave; s0 < a.p.seqs; s0 += kWave) {
         const Share h = share_of<ROWS, KEYS>(a, s0 + lane);
         work += (int64_t)h.tiles * h.units;
+        most = max(most, h.units);
     }
     const int64_t per64 = (wave_add(work) * a.p.kv_heads + target - 1) / target;
-    const uint32_t per = (uint32_t)min(max(per64, (int64_t)(KEYS == kFewKeys * kFewWaves ? few_least(a.p.reach) : 1)), (int64_t)INT32_MAX);
+    const int longest = __any(most > kSingle) ? kSingle + 1 : __any(most > kWhole) ? kSingle : kWhole;           // (as far as it matters)
+    const int least = KEYS != kFewKeys * kFewWaves ? 1 : a.p.reach <= kUncut * KEYS ? kUncut : longest > kWhole && longest <= kSingle ? 1 : 2;
+    const uint32_t per = (uint32_t)min(max(per64, (int64_t)least), (int64_t)INT32_MAX);
     uint32_t parts0 = 0;
     int64_t slots0 = 0;
     for (int s0 = 0; s0 < a.p.seqs; s0 += kWave) {
@@ -564,11 +574,6 @@ __device__ __forceinline__ void make_finite(uint32_t vt, int first, int step, in
 __device__ __forceinline__ uint32_t lds_base(uint8_t *lds) { return (uint32_t)(uintptr_t)(lds_u8 *)lds; }
 
 // ---------------------------------------------------------------------------------------------------------------- few rows
-constexpr int few_lds(int D, bool e4m3) {
-    const int tiles = kFewWaves * (e4m3 ? 1 : 2) * 2 * kFewKeys * 2 * D, joined = kFewWaves * 32 * (D + 4) * 4 + kFewWaves * 32 * 8;
-    return tiles > joined ? tiles : joined;
-}
-
 template <int D, bool E4M3>
 __global__ __launch_bounds__(kFewWaves *kWave, E4M3 ? 2 : 1) void attend_few_kernel(Attend a) {
     extern __shared__ __attribute__((aligned(1024))) uint8_t lds[];
@@ -577,7 +582,7 @@ __global__ __launch_bounds__(kFewWaves *kWave, E4M3 ? 2 : 1) void attend_few_ker
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
     clear_rest(a, blockIdx.x, gridDim.x, kFewWaves * kWave);
     Item it;
-    if (!find<kFewRows, kStep, false>(a, blockIdx.x / a.p.kv_heads, kFewTarget, it)) return;
+    if (!find<kFewRows, kStep, false>(a, blockIdx.x / a.p.kv_heads, few_target(D, E4M3), it)) return;
     const Range range = range_of<kFewRows, kStep>(a, it);
     const int rows = it.run.n * a.group, row0 = it.tile * kFewRows, row = row0 + lane % 32, before = it.length - it.run.n;
     const int pos = before + row / a.group, pos0 = before + row0 / a.group, pos1 = before + min(row0 + kFewRows - 1, rows - 1) / a.group;
@@ -999,20 +1004,21 @@ int launch(Attend &a, const Plan &plan, int64_t most_rows, float *workspace, hip
     }
     if (plan.few) {
         a.least_rows = 0, a.most_rows = plan.many ? plan.least : INT32_MAX;
-        a.partial = workspace, a.slots = slots_of(kFewTarget);
-        const dim3 grid(blocks(plan.many ? seqs : seqs + rows / kFewRows, kFewTarget));         // (beside the other kernel: a tile a sequence)
+        const int target = few_target(D, a.p.e4m3);
+        a.partial = workspace, a.slots = slots_of(target);
+        const dim3 grid(blocks(plan.many ? seqs : seqs + rows / kFewRows, target));         // (beside the other kernel: a tile a sequence)
         if (a.p.e4m3) hipLaunchKernelGGL((attend_few_kernel<D, true>), grid, dim3(kFewWaves * kWave), few_lds(D, true), stream, a);
         else hipLaunchKernelGGL((attend_few_kernel<D, false>), grid, dim3(kFewWaves * kWave), few_lds(D, false), stream, a);
-        if (a.p.reach > kFewKeys * kFewWaves * few_least(a.p.reach))
-            hipLaunchKernelGGL((attend_join_kernel<D, kFewRows, kFewKeys * kFewWaves, kJoinFew>), dim3(joins(kFewTarget), (unsigned)(((most_rows < kFewRows ? most_rows : kFewRows) + kJoinFew - 1) / kJoinFew)), dim3(256), 0, stream, a,
-                               (uint32_t)kFewTarget);
+        if (a.p.reach > kUncut * kFewKeys * kFewWaves)
+            hipLaunchKernelGGL((attend_join_kernel<D, kFewRows, kFewKeys * kFewWaves, kJoinFew>), dim3(joins(target), (unsigned)(((most_rows < kFewRows ? most_rows : kFewRows) + kJoinFew - 1) / kJoinFew)), dim3(256), 0, stream, a,
+                               (uint32_t)target);
     }
     return check_launch("odl_fp8_paged_attention");
 }
 
-int64_t workspace_of(const Plan &plan, int dim) {
-    const int D = dim > 64 ? 128 : 64;
-    return (plan.many ? floats_of(kManyRows, kManyTarget, D) : 0) + (plan.few ? floats_of(kFewRows, kFewTarget, D) : 0);
+int64_t workspace_of(const Plan &plan, const Paged &p) {
+    const int D = p.dim > 64 ? 128 : 64;
+    return (plan.many ? floats_of(kManyRows, kManyTarget, D) : 0) + (plan.few ? floats_of(kFewRows, few_target(D, p.e4m3), D) : 0);
 }
 
 }  // namespace
@@ -1020,7 +1026,7 @@ int64_t workspace_of(const Plan &plan, int dim) {
 extern "C" int64_t odl_fp8_paged_attention_workspace(int64_t heads, int64_t most_new, const odl_fp8_paged_cache *cache, const odl_fp8_paged_batch *batch) {
     Paged p;
     if (check("odl_fp8_paged_attention_workspace", heads, most_new, cache, batch, p)) return -1;
-    return workspace_of(plan_of(heads / p.kv_heads, p.rows, p.seqs, most_new < p.rows ? most_new : p.rows), p.dim);
+    return workspace_of(plan_of(heads / p.kv_heads, p.rows, p.seqs, most_new < p.rows ? most_new : p.rows), p);
 }
 
 extern "C" int odl_fp8_paged_attention(const void *q, const int64_t *q_strides, int64_t heads, int64_t most_new, const odl_fp8_paged_cache *cache,
@@ -1039,8 +1045,8 @@ extern "C" int odl_fp8_paged_attention(const void *q, const int64_t *q_strides, 
     a.heads = (int)heads, a.group = (int)(heads / a.p.kv_heads), a.window = window == 0 || window > INT32_MAX / 2 ? INT32_MAX / 2 : (int)window;
     a.scale = scale, a.softcap = softcap, a.out = static_cast<uint16_t *>(out);
     const Plan plan = plan_of(a.group, a.p.rows, a.p.seqs, most_new < a.p.rows ? most_new : a.p.rows);
-    if (!workspace || workspace_floats < workspace_of(plan, a.p.dim) || (reinterpret_cast<uintptr_t>(workspace) & 15))
-        return set_error(ODL_ERR_ARG, "%s: a workspace of %lld floats, 16-byte aligned", who, (long long)workspace_of(plan, a.p.dim));
+    if (!workspace || workspace_floats < workspace_of(plan, a.p) || (reinterpret_cast<uintptr_t>(workspace) & 15))
+        return set_error(ODL_ERR_ARG, "%s: a workspace of %lld floats, 16-byte aligned", who, (long long)workspace_of(plan, a.p));
     hipStream_t stream = reinterpret_cast<hipStream_t>(stream_);
     const int64_t most_rows = (most_new < 1 ? 1 : most_new < a.p.rows ? most_new : a.p.rows) * a.group;
     // heads of up to 96: a quarter of the products of 128 less (the prompts above 206 -> 192 us; the kernel for few rows waits for memory, and has one form)

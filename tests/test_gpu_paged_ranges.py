@@ -126,3 +126,14 @@ def test_rows_in_front_of_the_first_sequence_answer_0(new, lengths):
         assert (got[:2] == 0).all() and (got[-1:] == 0).all()
         assert_near(got, want, far)
     assert (append_kv(c.q, c.k, c.v, c.keys, c.values, *c.batch())[:2] == 0).all()
+
+
+@pytest.mark.parametrize("length", [1, 129, 257, 511, 512, 700, 2048, 2049])
+@pytest.mark.parametrize("cache", [BF16, E4M3])
+@pytest.mark.parametrize("dim,heads,kv", [(64, 12, 12), (128, 8, 2)])
+def test_tables_of_any_width(length, cache, dim, heads, kv):
+    """Which work is cut, and how, changes nothing: as wide as the context, one page wider, and much wider than it."""
+    need = -(-length // 16)
+    for width in (need, need + 1, 32, 33, 64, 65, 300):
+        if width >= need:
+            attend(Case([1], [length], heads, kv, dim, 16, cache, seed=length, width=width), max_new=1)

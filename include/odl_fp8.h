@@ -46,7 +46,7 @@ enum odl_status {
 };
 
 /* ABI version of this header; bumped when a signature changes or an entry point is added. */
-#define ODL_FP8_ABI_VERSION 32
+#define ODL_FP8_ABI_VERSION 33
 int odl_fp8_abi_version(void);
 
 /*
@@ -803,6 +803,11 @@ int odl_fp8_append_kv(const void *q, const int64_t *q_strides, const void *k, co
                       int64_t heads, const odl_fp8_paged_cache *cache, const odl_fp8_paged_batch *batch, const float *cos, const float *sin,
                       int64_t positions, int64_t half, int interleaved, const float *q_weight, const float *k_weight, double eps, void *q_out,
                       odl_stream_t stream);
+/* The same with weights of the norms in fp32 or bf16 (weight_dtype, of both), at any alignment; bf16 is widened exactly. */
+int odl_fp8_append_kv_typed(const void *q, const int64_t *q_strides, const void *k, const int64_t *k_strides, const void *v, const int64_t *v_strides,
+                            int64_t heads, const odl_fp8_paged_cache *cache, const odl_fp8_paged_batch *batch, const float *cos, const float *sin,
+                            int64_t positions, int64_t half, int interleaved, const void *q_weight, const void *k_weight, int weight_dtype, double eps,
+                            void *q_out, odl_stream_t stream);
 
 /*
  * Attention of the new tokens over the cache, which holds them.  Row at position p, of a head whose keys are those of head / (heads / kv_heads):

@@ -62,9 +62,10 @@ struct Append {
     Paged p;
     const uint16_t *q, *k, *v;
     int64_t q_row, q_head, k_row, k_head, v_row, v_head;       // strides in elements
-    const float *cos, *sin, *q_weight, *k_weight;
+    const float *cos, *sin;
+    const void *q_weight, *k_weight;
     double eps;
-    int heads, half, interleaved;
+    int heads, half, interleaved, weight_bf16;
     uint16_t *out;
 };
 
@@ -97,7 +98,7 @@ __global__ __launch_bounds__(256) void append_kv_kernel(Append a) {
     float x[8];
 #pragma unroll
     for (int i = 0; i < 4; ++i) { x[2 * i] = bf16_lo(raw[i]); x[2 * i + 1] = bf16_hi(raw[i]); }
-    const float *weight = is_q ? a.q_weight : is_v ? nullptr : a.k_weight;
+    const void *weight = is_q ? a.q_weight : is_v ? nullptr : a.k_weight;
     if (a.q_weight || a.k_weight) {
         double sum = 0.0;
 #pragma unroll
@@ -107,7 +108,14 @@ __global__ __launch_bounds__(256) void append_kv_kernel(Append a) {
         if (weight && live) {
             const float r = (float)(1.0 / sqrt(sum / (double)p.dim + a.eps));
             float w[8];
-            __builtin_memcpy(w, weight + c * 8, sizeof(w));
+            if (a.weight_bf16) {
+                uint32_t two[4];
+                __builtin_memcpy(two, static_cast<const uint16_t *>(weight) + c * 8, sizeof(two));
+#pragma unroll
+                for (int i = 0; i < 4; ++i) { w[2 * i] = bf16_lo(two[i]); w[2 * i + 1] = bf16_hi(two[i]); }
+            } else {
+                __builtin_memcpy(w, static_cast<const float *>(weight) + c * 8, sizeof(w));
+            }
 #pragma unroll
             for (int i = 0; i < 8; ++i) x[i] = x[i] * r * w[i];
         }
@@ -166,10 +174,10 @@ __global__ __launch_bounds__(256) void append_kv_kernel(Append a) {
 
 using namespace odl;
 
-extern "C" int odl_fp8_append_kv(const void *q, const int64_t *q_strides, const void *k, const int64_t *k_strides, const void *v,
-                                 const int64_t *v_strides, int64_t heads, const odl_fp8_paged_cache *cache, const odl_fp8_paged_batch *batch,
-                                 const float *cos, const float *sin, int64_t positions, int64_t half, int interleaved, const float *q_weight,
-                                 const float *k_weight, double eps, void *q_out, odl_stream_t stream_) {
+extern "C" int odl_fp8_append_kv_typed(const void *q, const int64_t *q_strides, const void *k, const int64_t *k_strides, const void *v,
+                                       const int64_t *v_strides, int64_t heads, const odl_fp8_paged_cache *cache, const odl_fp8_paged_batch *batch,
+                                       const float *cos, const float *sin, int64_t positions, int64_t half, int interleaved, const void *q_weight,
+                                       const void *k_weight, int weight_dtype, double eps, void *q_out, odl_stream_t stream_) {
     static const char who[] = "odl_fp8_append_kv";
     Append a;
     if (const int rc = take_paged(who, cache, batch, a.p)) return rc;
@@ -177,6 +185,7 @@ extern "C" int odl_fp8_append_kv(const void *q, const int64_t *q_strides, const 
     if (half < 0 || 2 * half > a.p.dim || half % (interleaved ? 4 : 8)) return set_error(ODL_ERR_SHAPE, "%s: a rotation of %lld pairs in heads of %d (half a head at most, a multiple of %d)", who, (long long)half, a.p.dim, interleaved ? 4 : 8);
     if (half > 0 && (!cos || !sin)) return set_error(ODL_ERR_ARG, "%s: null pointer for the angles", who);
     if (half > 0 && positions < a.p.reach) return set_error(ODL_ERR_SHAPE, "%s: angles of %lld positions for a page table of %d", who, (long long)positions, a.p.reach);
+    if (weight_dtype != ODL_F32 && weight_dtype != ODL_BF16) return set_error(ODL_ERR_ARG, "%s: weights of dtype %d", who, weight_dtype);
     const int64_t rows = batch->rows;
     if (const int rc = check_strides(who, "q", q, q_strides, rows)) return rc;
     if (const int rc = check_strides(who, "k", k, k_strides, rows)) return rc;
@@ -185,9 +194,17 @@ extern "C" int odl_fp8_append_kv(const void *q, const int64_t *q_strides, const 
     if (!q_out || !aligned16(q_out)) return set_error(ODL_ERR_ARG, "%s: q_out must be a 16-byte aligned address", who);
     a.q = static_cast<const uint16_t *>(q), a.k = static_cast<const uint16_t *>(k), a.v = static_cast<const uint16_t *>(v);
     a.q_row = q_strides[0], a.q_head = q_strides[1], a.k_row = k_strides[0], a.k_head = k_strides[1], a.v_row = v_strides[0], a.v_head = v_strides[1];
-    a.cos = cos, a.sin = sin, a.q_weight = q_weight, a.k_weight = k_weight, a.eps = eps;
+    a.cos = cos, a.sin = sin, a.q_weight = q_weight, a.k_weight = k_weight, a.weight_bf16 = weight_dtype == ODL_BF16, a.eps = eps;
     a.heads = (int)heads, a.half = (int)half, a.interleaved = interleaved != 0, a.out = static_cast<uint16_t *>(q_out);
     const int64_t count = heads + 2 * a.p.kv_heads;
     hipLaunchKernelGGL(append_kv_kernel, dim3((unsigned)rows, (unsigned)((count + kRows - 1) / kRows)), dim3(256), 0, reinterpret_cast<hipStream_t>(stream_), a);
     return check_launch(who);
+}
+
+extern "C" int odl_fp8_append_kv(const void *q, const int64_t *q_strides, const void *k, const int64_t *k_strides, const void *v,
+                                 const int64_t *v_strides, int64_t heads, const odl_fp8_paged_cache *cache, const odl_fp8_paged_batch *batch,
+                                 const float *cos, const float *sin, int64_t positions, int64_t half, int interleaved, const float *q_weight,
+                                 const float *k_weight, double eps, void *q_out, odl_stream_t stream) {
+    return odl_fp8_append_kv_typed(q, q_strides, k, k_strides, v, v_strides, heads, cache, batch, cos, sin, positions, half, interleaved, q_weight,
+                                   k_weight, ODL_F32, eps, q_out, stream);
 }

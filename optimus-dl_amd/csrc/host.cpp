@@ -61,7 +61,7 @@ decltype(&odl_fp8_token_logprobs) logprobs_c;
 decltype(&odl_fp8_token_logprobs_bwd) logprobs_bwd_c;
 decltype(&odl_fp8_fp4_linear_runs) fp4_runs_c;
 decltype(&odl_fp8_fp4_linear) fp4_linear_c;
-decltype(&odl_fp8_append_kv) append_kv_c;
+decltype(&odl_fp8_append_kv_typed) append_kv_c;
 decltype(&odl_fp8_paged_attention_workspace) paged_workspace_c;
 decltype(&odl_fp8_paged_attention) paged_attention_c;
 decltype(&odl_fp8_verify_drafts_workspace) verify_workspace_c;
@@ -110,7 +110,7 @@ void bind(const py::dict &d) {
     take(logprobs_bwd_c, d, "odl_fp8_token_logprobs_bwd");
     take(fp4_runs_c, d, "odl_fp8_fp4_linear_runs");
     take(fp4_linear_c, d, "odl_fp8_fp4_linear");
-    take(append_kv_c, d, "odl_fp8_append_kv");
+    take(append_kv_c, d, "odl_fp8_append_kv_typed");
     take(paged_workspace_c, d, "odl_fp8_paged_attention_workspace");
     take(paged_attention_c, d, "odl_fp8_paged_attention");
     take(verify_workspace_c, d, "odl_fp8_verify_drafts_workspace");
@@ -629,11 +629,17 @@ py::object append_kv(const Tensor &q, const Tensor &k, const Tensor &v, const Te
         positions = cos->size(0), half = cos->size(1);
         if (!floats(*cos, positions * half) || !floats(*sin, positions * half) || cos->device() != q.device() || sin->device() != q.device()) return none();
     }
-    for (const OptTensor *w : {&qw, &kw})
-        if (*w && (!floats(**w, c.head_dim) || (*w)->dim() != 1 || (*w)->device() != q.device() || wants_gradient(*w))) return none();
+    int weights = -1;                            // the type of both
+    for (const OptTensor *w : {&qw, &kw}) {
+        if (!*w) continue;
+        const int type = src_of(**w);
+        if (type < 0 || (weights >= 0 && type != weights) || !dense(**w) || (*w)->numel() != c.head_dim || (*w)->dim() != 1 || (*w)->device() != q.device() || wants_gradient(*w))
+            return none();
+        weights = type;
+    }
     Tensor out = at::empty({q.size(0), q.size(1), q.size(2)}, q.options());
     const int rc = call(append_kv_c, ptr(q), q.strides().data(), ptr(k), k.strides().data(), ptr(v), v.strides().data(), q.size(1), &c, &b, ptr(cos), ptr(sin),
-                        positions, half, (int)interleaved, ptr(qw), ptr(kw), eps, ptr(out), str(stream));
+                        positions, half, (int)interleaved, ptr(qw), ptr(kw), weights < 0 ? (int)ODL_F32 : weights, eps, ptr(out), str(stream));
     return rc ? none() : py::cast(out);
 }
 

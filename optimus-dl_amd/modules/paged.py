@@ -143,7 +143,7 @@ def append_kv(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, keys: torch.Ten
     ``p % page size`` of page ``pages[s, p // page size]``.  pages, offsets, lengths int32.
 
     cos, sin: fp32 [positions, pairs], of every position that the table reaches; the first 2 * pairs elements of a head are rotated, as pairs (2 i, 2 i + 1)
-    where ``interleaved``, else (i, pairs + i).  q_weight, k_weight [head_dim]: norms by root mean square in front of the rotation.
+    where ``interleaved``, else (i, pairs + i).  q_weight, k_weight [head_dim]: norms by root mean square in front of the rotation, in fp32 or bf16 without a cast.
     Rows of no sequence, in front of the first or behind the last, are not read: their queries are 0.  Tokens whose page is none of the cache are not written, those behind the
     table's reach neither, and their queries are 0.  Two rows of a call must not share a slot.
 

@@ -26,7 +26,7 @@ DT_BF16, DT_F32 = 0, 1
 AMAX_MAX, AMAX_MOST_RECENT = 0, 1
 FP8_MAX = {E4M3: 448.0, E5M2: 57344.0}
 TORCH_FP8 = {E4M3: torch.float8_e4m3fn, E5M2: torch.float8_e5m2}
-ABI_VERSION = 32
+ABI_VERSION = 33
 _OUT_DTYPES = {torch.bfloat16: DT_BF16, torch.float32: DT_F32}
 AMAX_PARTS = 512                       # ODL_FP8_AMAX_PARTS
 
@@ -113,6 +113,7 @@ EXPORTS = (
     "odl_fp8_fp4_linear",
     "odl_fp8_fp4_quantise",
     "odl_fp8_append_kv",
+    "odl_fp8_append_kv_typed",
     "odl_fp8_paged_attention_workspace",
     "odl_fp8_paged_attention",
     "odl_fp8_verify_drafts_workspace",
@@ -227,6 +228,7 @@ def load() -> ctypes.CDLL:
         L.odl_fp8_residual_norm.argtypes = [vp, i32, vp, i32, vp, vp, vp, i64, i64, i64, f32, f32, f32, vp, vp, vp, vp, vp]
         L.odl_fp8_residual_norm_bwd.argtypes = [vp, vp, vp, i32, vp, i32, vp, vp, vp, i64, i64, i64, f32, vp, vp, vp, vp, vp, vp, vp, vp, vp]
         L.odl_fp8_append_kv.argtypes = [vp, vp, vp, vp, vp, vp, i64, vp, vp, vp, vp, i64, i64, i32, vp, vp, ctypes.c_double, vp, vp]
+        L.odl_fp8_append_kv_typed.argtypes = [vp, vp, vp, vp, vp, vp, i64, vp, vp, vp, vp, i64, i64, i32, vp, vp, i32, ctypes.c_double, vp, vp]
         L.odl_fp8_paged_attention_workspace.argtypes = [i64, i64, vp, vp]
         L.odl_fp8_paged_attention_workspace.restype = i64
         L.odl_fp8_paged_attention.argtypes = [vp, vp, i64, i64, vp, vp, f32, i64, f32, vp, vp, i64, vp]
@@ -1975,11 +1977,14 @@ def append_kv(q, k, v, keys, values, pages, offsets, lengths, cos=None, sin=None
                 raise NativeError(f"append_kv: angles {tuple(cos.shape)} and {tuple(sin.shape)}, expected [positions, pairs] of both")
             cos, sin = (_f32_dev(t, t.numel(), "append_kv angles") for t in (cos, sin))
             positions, half = cos.shape
-        q_weight, k_weight = (_f32_vector(w, dim, q.device, "append_kv " + n) for w, n in ((q_weight, "q_weight"), (k_weight, "k_weight")))
+        weights = [w for w in (q_weight, k_weight) if w is not None]
+        dtype = DT_BF16 if weights and all(w.dtype == torch.bfloat16 and w.is_contiguous() and w.numel() == dim for w in weights) else DT_F32
+        if dtype == DT_F32:
+            q_weight, k_weight = (_f32_vector(w, dim, q.device, "append_kv " + n) for w, n in ((q_weight, "q_weight"), (k_weight, "k_weight")))
         out = torch.empty(q.shape, dtype=torch.bfloat16, device=q.device)
         p = lambda t: None if t is None else t.data_ptr()
-        _check(load().odl_fp8_append_kv(p(q), _strides(q), p(k), _strides(k), p(v), _strides(v), q.shape[1], ctypes.byref(cache), ctypes.byref(batch),
-                                        p(cos), p(sin), positions, half, int(interleaved), p(q_weight), p(k_weight), float(eps), p(out), _stream()),
+        _check(load().odl_fp8_append_kv_typed(p(q), _strides(q), p(k), _strides(k), p(v), _strides(v), q.shape[1], ctypes.byref(cache), ctypes.byref(batch),
+                                              p(cos), p(sin), positions, half, int(interleaved), p(q_weight), p(k_weight), dtype, float(eps), p(out), _stream()),
                "odl_fp8_append_kv")
     return out
 

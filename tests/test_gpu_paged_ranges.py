@@ -4,6 +4,7 @@ import math
 import pytest
 import torch
 
+from optimus_dl_amd import native
 from optimus_dl_amd.modules.paged import append_kv, paged_attention
 from tests.paged_helpers import BF16, E4M3, Case, assert_near, bits
 from tests.paged_oracle import attention_rows
@@ -137,3 +138,28 @@ def test_tables_of_any_width(length, cache, dim, heads, kv):
     for width in (need, need + 1, 32, 33, 64, 65, 300):
         if width >= need:
             attend(Case([1], [length], heads, kv, dim, 16, cache, seed=length, width=width), max_new=1)
+
+
+@pytest.mark.parametrize("cache", [BF16, E4M3])
+def test_norms_with_bf16_weights_take_the_short_way(cache):
+    """A model in bf16 has bf16 weights: widened by the kernel, bit by bit what fp32 copies of them give; weights of two types, or spread in memory, the long way."""
+    def run(q_weight, k_weight, plain):
+        c = Case([1, 3, 17], [1, 40, 33], 6, 2, 96, 16, cache, seed=15).to(CUDA)
+        args = c.q, c.k, c.v, c.keys, c.values, *c.batch()
+        if plain:
+            out = native.plain_append_kv(*args, None, None, True, q_weight, k_weight, 1e-5, c.key_scale, c.value_scale)
+            assert out is not None
+        else:
+            out = append_kv(*args, q_weight=q_weight, k_weight=k_weight, eps=1e-5, **c.scales())
+        return [bits(t) for t in (out, c.keys, c.values)]
+
+    g = torch.Generator().manual_seed(16)
+    wide = [(1 + 0.2 * torch.randn(97, generator=g)).bfloat16().cuda() for _ in range(2)]
+    for first in (0, 1):                                                             # (aligned to 16 bytes, and to 2)
+        wq, wk = (w[first:first + 96] for w in wide)
+        want = run(wq.float(), wk.float(), True)
+        spread = torch.stack((wq, wq), 1)[:, 0]
+        for a, b, plain in ((wq, wk, True), (wq.float(), wk, False), (wq, wk, False), (spread, wk, False)):
+            assert all(torch.equal(x, y) for x, y in zip(run(a, b, plain), want))
+    only = run(wq, None, True), run(wq.float(), None, True)
+    assert all(torch.equal(x, y) for x, y in zip(*only))

@@ -9,7 +9,7 @@ For inference: inputs that want gradients are refused.
 
 from __future__ import annotations
 
-
+from itertools import accumulate
 from typing import NamedTuple
 
 import torch
@@ -252,6 +252,7 @@ class PagedKVCache:
         self.value_scale = torch.full((n_layer, kv_heads), value_scale, dtype=torch.float32, device=self.device) if scales else None
         self._free = list(range(pages - 1, -1, -1))
         self._pages: dict[int, list[int]] = {}
+        self._rows: dict[int, torch.Tensor] = {}       # the same as rows of a table, 0 behind the last
         self._length: dict[int, int] = {}
         self._next = 0
         self._angles: dict[tuple, tuple] = {}
@@ -259,7 +260,7 @@ class PagedKVCache:
     def add(self) -> int:
         """A new sequence without tokens."""
         s, self._next = self._next, self._next + 1
-        self._pages[s], self._length[s] = [], 0
+        self._pages[s], self._length[s], self._rows[s] = [], 0, torch.zeros(self.width, dtype=torch.int32)
         return s
 
     def length(self, sequence: int) -> int:
@@ -275,12 +276,13 @@ class PagedKVCache:
             raise ValueError(f"sequence {sequence} has {self._length[sequence]} tokens, not {length}")
         self._length[sequence] = length
         kept = -(-length // self.page_size)
+        self._rows[sequence][kept:len(self._pages[sequence])] = 0
         while len(self._pages[sequence]) > kept:
             self._free.append(self._pages[sequence].pop())
 
     def remove(self, sequence: int) -> None:
         self.shorten(sequence, 0)
-        del self._pages[sequence], self._length[sequence]
+        del self._pages[sequence], self._length[sequence], self._rows[sequence]
 
     def batch(self, sequences: "list[int]", new: "list[int]") -> PagedBatch:
         """Room for ``new`` more tokens of each of ``sequences``, and the batch of them in this order.  Refused as a whole where pages run out."""
@@ -293,16 +295,19 @@ class PagedKVCache:
             need.append(-(-(self._length[s] + n) // self.page_size) - len(self._pages[s]))
         if sum(need) > len(self._free):
             raise RuntimeError(f"{sum(need)} pages wanted, {len(self._free)} are free")
-        table = torch.zeros((len(sequences), self.width), dtype=torch.int32)
-        offsets, lengths = [0], []
-        for i, (s, n, k) in enumerate(zip(sequences, new, need)):
-            self._pages[s] += [self._free.pop() for _ in range(k)]
+        for s, n, k in zip(sequences, new, need):
             self._length[s] += n
-            table[i, :len(self._pages[s])] = torch.tensor(self._pages[s], dtype=torch.int32)
-            offsets.append(offsets[-1] + n)
-            lengths.append(self._length[s])
-        ints = lambda v: torch.tensor(v, dtype=torch.int32).to(self.device)
-        return PagedBatch(table.to(self.device), ints(offsets), ints(lengths), max(new, default=0))
+            if k > 0:
+                pages = [self._free.pop() for _ in range(k)]
+                held = len(self._pages[s])
+                self._rows[s][held:held + k] = torch.tensor(pages, dtype=torch.int32)
+                self._pages[s] += pages
+        seqs, offsets = len(sequences), list(accumulate(new, initial=0))
+        numbers = torch.tensor(offsets + [self._length[s] for s in sequences], dtype=torch.int32)
+        # one tensor of everything, which goes to the GPU in one copy
+        everything = torch.cat([self._rows[s] for s in sequences] + [numbers]).to(self.device)
+        table, offsets, lengths = everything.split((seqs * self.width, seqs + 1, seqs))
+        return PagedBatch(table.view(seqs, self.width), offsets, lengths, max(new, default=0))
 
     def layer(self, i: int, batch: PagedBatch) -> PagedLayer:
         scale = lambda t: None if t is None else t[i]

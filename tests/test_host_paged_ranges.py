@@ -1,7 +1,7 @@
 """The paged cache on the CPU where numbers are odd or 0."""
 import torch
 
-from optimus_dl_amd.modules.paged import append_kv, paged_attention
+from optimus_dl_amd.modules.paged import PagedKVCache, append_kv, paged_attention
 from tests.paged_helpers import E4M3, Case, bits
 
 
@@ -29,3 +29,33 @@ def test_rows_without_a_score_above_minus_infinity_answer_0_beside_odd_values():
     c.keys[int(c.pages[1, 1])] = 0.0             # the second sequence's last token
     y = paged_attention(c.q, c.keys, c.values, *c.batch())
     assert (y[:2] == 0).all() and (y[2, :, 3] == torch.inf).all() and y[2, :, 4].isnan().all() and y[2, :, 5:].isfinite().all()
+
+
+def test_a_batch_looks_at_new_pages_alone(monkeypatch):
+    """A decode step of long sequences: what is built in Python is the new pages, an offset and a length each, and not the whole table; the table says the same."""
+    cache = PagedKVCache(1, 1, 16, pages=700, page_size=4, max_tokens=128, device="cpu", dtype=torch.float32)
+    s = [cache.add() for _ in range(20)]
+    lengths = [100 + i for i in range(20)]
+    cache.batch(s, lengths)
+    built, made = [], torch.tensor
+    monkeypatch.setattr(torch, "tensor", lambda v, *a, **k: built.append(len(v)) or made(v, *a, **k))
+    for step in range(6):
+        if step == 3:
+            cache.shorten(s[4], 3)
+            cache.remove(s[7])
+            s[7] = cache.add()
+            lengths[4], lengths[7] = 3, 0
+        built.clear()
+        batch = cache.batch(s, [1] * 20)
+        lengths = [n + 1 for n in lengths]
+        assert sum(built) <= 20 + 41
+        assert batch.lengths.tolist() == lengths and batch.offsets.tolist() == list(range(21))
+        for row, i in zip(batch.pages.tolist(), s):
+            assert row == cache._pages[i] + [0] * (32 - len(cache._pages[i])) and len(cache._pages[i]) == -(-cache.length(i) // 4)
+    held = [p for i in s for p in cache._pages[i]]
+    assert len(set(held)) == len(held) == 700 - cache.free_pages
+    before = batch.pages.clone()
+    cache.shorten(s[0], 0)
+    assert torch.equal(batch.pages, before)              # (a batch that was made stays as it is)
+    empty = cache.batch([], [])
+    assert empty.pages.shape == (0, 32) and empty.offsets.tolist() == [0] and empty.lengths.shape == (0,) and empty.max_new == 0

@@ -315,7 +315,7 @@ class PagedKVCache:
 
     def angles(self, tables, head_dim: int, theta: float) -> tuple[torch.Tensor, torch.Tensor]:
         """``tables(head_dim, positions, theta, device)`` for every position that the tables reach, made once."""
-        key = (head_dim, theta)
+        key = (tables, head_dim, theta)
         if key not in self._angles:
             on_gpu = self.device.type == "cuda"
             if on_gpu and torch.cuda.is_current_stream_capturing():

@@ -59,3 +59,19 @@ def test_a_batch_looks_at_new_pages_alone(monkeypatch):
     assert torch.equal(batch.pages, before)              # (a batch that was made stays as it is)
     empty = cache.batch([], [])
     assert empty.pages.shape == (0, 32) and empty.offsets.tolist() == [0] and empty.lengths.shape == (0,) and empty.max_new == 0
+
+
+def test_angles_belong_to_the_function_that_makes_them():
+    cache = PagedKVCache(1, 1, 16, pages=2, page_size=4, device="cpu")
+    made = []
+
+    def first(dim, positions, theta, device):
+        made.append(1)
+        return torch.ones(positions, dim // 2), torch.zeros(positions, dim // 2)
+
+    def second(dim, positions, theta, device):
+        return torch.zeros(positions, dim // 2), torch.ones(positions, dim // 2)
+
+    for _ in range(2):
+        assert (cache.angles(first, 16, 1e4)[0] == 1).all() and (cache.angles(second, 16, 1e4)[0] == 0).all()
+    assert len(made) == 1

@@ -191,6 +191,7 @@ extern "C" int odl_fp8_append_kv_typed(const void *q, const int64_t *q_strides, 
     if (const int rc = check_strides(who, "k", k, k_strides, rows)) return rc;
     if (const int rc = check_strides(who, "v", v, v_strides, rows)) return rc;
     if (rows == 0) return ODL_OK;
+    if (rows * 256 > UINT32_MAX) return set_error(ODL_ERR_SHAPE, "%s: more rows than a launch has blocks (below 2^24)", who);
     if (!q_out || !aligned16(q_out)) return set_error(ODL_ERR_ARG, "%s: q_out must be a 16-byte aligned address", who);
     a.q = static_cast<const uint16_t *>(q), a.k = static_cast<const uint16_t *>(k), a.v = static_cast<const uint16_t *>(v);
     a.q_row = q_strides[0], a.q_head = q_strides[1], a.k_row = k_strides[0], a.k_head = k_strides[1], a.v_row = v_strides[0], a.v_head = v_strides[1];

@@ -989,13 +989,17 @@ template <int D, int C>
 int launch(Attend &a, const Plan &plan, int64_t most_rows, float *workspace, hipStream_t stream) {
     const int64_t kv = a.p.kv_heads, rows = (int64_t)a.p.rows * a.group, seqs = a.p.seqs < a.p.rows ? a.p.seqs : a.p.rows;
     // no more tiles than sequences (those that fill no tile) and rows / tile; splits that begin anew: see `find`
-    auto blocks = [&](int64_t tiles, int target) { return (unsigned)((target / kv + 1 + tiles) * kv); };
+    auto blocks = [&](int64_t tiles, int target) { return (target / kv + 1 + tiles) * kv; };
     auto joins = [&](int target) { return (unsigned)((target / kv + 1) * kv); };
+    const int few = few_target(D, a.p.e4m3);
+    const int64_t many_blocks = blocks(seqs + rows / kManyRows, kManyTarget), few_blocks = blocks(plan.many ? seqs : seqs + rows / kFewRows, few);         // (beside the other kernel: a tile a sequence)
+    if ((plan.many && many_blocks * kManyWaves * kWave > UINT32_MAX) || (plan.few && few_blocks * kFewWaves * kWave > UINT32_MAX))
+        return set_error(ODL_ERR_SHAPE, "odl_fp8_paged_attention: more tiles of rows than a launch has blocks (times key heads, below 2^24 of few rows and 2^23 of many)");
     if (plan.many) {
         a.least_rows = plan.least, a.most_rows = INT32_MAX;
         a.partial = workspace, a.slots = slots_of(kManyTarget);
         const int clear = !plan.few;
-        const dim3 grid(blocks(seqs + rows / kManyRows, kManyTarget));
+        const dim3 grid((unsigned)many_blocks);
         if (a.p.e4m3) hipLaunchKernelGGL((attend_many_kernel<D, C, true>), grid, dim3(kManyWaves * kWave), many_lds(D), stream, a, clear);
         else hipLaunchKernelGGL((attend_many_kernel<D, C, false>), grid, dim3(kManyWaves * kWave), many_lds(D), stream, a, clear);
         if (a.p.reach > kManyKeys)
@@ -1004,14 +1008,13 @@ int launch(Attend &a, const Plan &plan, int64_t most_rows, float *workspace, hip
     }
     if (plan.few) {
         a.least_rows = 0, a.most_rows = plan.many ? plan.least : INT32_MAX;
-        const int target = few_target(D, a.p.e4m3);
-        a.partial = workspace, a.slots = slots_of(target);
-        const dim3 grid(blocks(plan.many ? seqs : seqs + rows / kFewRows, target));         // (beside the other kernel: a tile a sequence)
+        a.partial = workspace, a.slots = slots_of(few);
+        const dim3 grid((unsigned)few_blocks);
         if (a.p.e4m3) hipLaunchKernelGGL((attend_few_kernel<D, true>), grid, dim3(kFewWaves * kWave), few_lds(D, true), stream, a);
         else hipLaunchKernelGGL((attend_few_kernel<D, false>), grid, dim3(kFewWaves * kWave), few_lds(D, false), stream, a);
         if (a.p.reach > kUncut * kFewKeys * kFewWaves)
-            hipLaunchKernelGGL((attend_join_kernel<D, kFewRows, kFewKeys * kFewWaves, kJoinFew>), dim3(joins(target), (unsigned)(((most_rows < kFewRows ? most_rows : kFewRows) + kJoinFew - 1) / kJoinFew)), dim3(256), 0, stream, a,
-                               (uint32_t)target);
+            hipLaunchKernelGGL((attend_join_kernel<D, kFewRows, kFewKeys * kFewWaves, kJoinFew>), dim3(joins(few), (unsigned)(((most_rows < kFewRows ? most_rows : kFewRows) + kJoinFew - 1) / kJoinFew)), dim3(256), 0, stream, a,
+                               (uint32_t)few);
     }
     return check_launch("odl_fp8_paged_attention");
 }

@@ -1,6 +1,10 @@
 """The paged cache on the CPU where numbers are odd or 0."""
+import ctypes
+
+import pytest
 import torch
 
+from optimus_dl_amd import native
 from optimus_dl_amd.modules.paged import PagedKVCache, append_kv, paged_attention
 from tests.paged_helpers import E4M3, Case, bits
 
@@ -75,3 +79,20 @@ def test_angles_belong_to_the_function_that_makes_them():
     for _ in range(2):
         assert (cache.angles(first, 16, 1e4)[0] == 1).all() and (cache.angles(second, 16, 1e4)[0] == 0).all()
     assert len(made) == 1
+
+
+@pytest.mark.parametrize("rows,heads,seqs,append_fits,attention_fits", [((1 << 24) - 1, 2, 3, True, True), (1 << 24, 2, 3, False, True), (1 << 20, 32, 1 << 20, True, False)])
+def test_entries_refuse_more_blocks_than_a_launch_has(rows, heads, seqs, append_fits, attention_fits):
+    """Pointers that nothing follows: what is refused is refused in front of a launch.  What fits goes on to the checks behind, and to an address that is refused."""
+    if not native.is_built():
+        pytest.skip("library not built")
+    L = native.load()
+    kv = heads // 2
+    cache = native._PagedCache(4096, 4096, None, None, 10, kv, 16, 64)
+    cache.key_strides[:] = cache.value_strides[:] = (1024 * kv, 1024, 64)
+    batch = native._PagedBatch(4096, 4096, 4096, seqs, rows, 5, 5)
+    refs, q, k = (ctypes.byref(cache), ctypes.byref(batch)), (ctypes.c_int64 * 2)(heads * 64, 64), (ctypes.c_int64 * 2)(kv * 64, 64)
+    code = L.odl_fp8_append_kv(4096, q, 4096, k, 4096, k, heads, *refs, 4096, 4096, 80, 16, 1, None, None, 1e-6, 4104 if append_fits else 4096, None)
+    assert code in (1, 2) and (b"aligned" if append_fits else b"blocks") in L.odl_fp8_last_error()
+    code = L.odl_fp8_paged_attention(4096, q, heads, 1, *refs, 1.0, 0, 0.0, 4104 if attention_fits else 4096, 4096, 1 << 40, None)
+    assert code in (1, 2) and (b"aligned" if attention_fits else b"blocks") in L.odl_fp8_last_error()

@@ -210,12 +210,8 @@ class PagedBatch(NamedTuple):
     def positions(self, rows: int) -> torch.Tensor:
         """The position of every row's token, 0 for rows behind the last sequence."""
         row, offsets = torch.arange(rows, device=self.offsets.device), self.offsets.long()
-        if offsets.numel() == 1:
-            return torch.zeros_like(row)
-        seq = torch.searchsorted(offsets[1:], row, right=True)
-        live, seq = seq < offsets.numel() - 1, seq.clamp(max=offsets.numel() - 2)
-        position = self.lengths.long()[seq] - offsets[seq + 1] + row
-        return torch.where(live, position.clamp(min=0), torch.zeros_like(row))
+        first = torch.nn.functional.pad(self.lengths - offsets[1:], (0, 1), value=-rows)         # position 0's row, negative; none behind the last sequence
+        return first[torch.searchsorted(offsets[1:], row, right=True)].add_(row).clamp_(min=0)
 
 
 class PagedLayer(NamedTuple):

@@ -5,7 +5,7 @@ import pytest
 import torch
 
 from optimus_dl_amd import native
-from optimus_dl_amd.modules.paged import PagedKVCache, append_kv, paged_attention
+from optimus_dl_amd.modules.paged import PagedBatch, PagedKVCache, append_kv, paged_attention
 from tests.paged_helpers import E4M3, Case, bits
 
 
@@ -96,3 +96,23 @@ def test_entries_refuse_more_blocks_than_a_launch_has(rows, heads, seqs, append_
     assert code in (1, 2) and (b"aligned" if append_fits else b"blocks") in L.odl_fp8_last_error()
     code = L.odl_fp8_paged_attention(4096, q, heads, 1, *refs, 1.0, 0, 0.0, 4104 if attention_fits else 4096, 4096, 1 << 40, None)
     assert code in (1, 2) and (b"aligned" if attention_fits else b"blocks") in L.odl_fp8_last_error()
+
+
+def test_positions_take_few_operations():
+    """Every step of a model with learned positions makes them: each operation is a launch."""
+    from torch.utils._python_dispatch import TorchDispatchMode
+
+    class Count(TorchDispatchMode):
+        def __torch_dispatch__(self, func, types, args=(), kwargs=None):
+            out = func(*args, **(kwargs or {}))
+            self.made = getattr(self, "made", 0) + (not func.is_view and "empty" not in str(func))
+            return out
+
+    ints = lambda v: torch.tensor(v, dtype=torch.int32)
+    for offsets, lengths in (([0, 3, 3, 4, 9], [10, 7, 1, 5]), ([0], []), ([0, 0], [5]), ([0, 2], [1]), ([0, 1, 2, 3], [2 ** 30, 1, 2 ** 30])):
+        batch = PagedBatch(ints([[0]] * len(lengths)), ints(offsets), ints(lengths))
+        with Count() as count:
+            got = batch.positions(offsets[-1] + 3)
+        want = [max(n - (offsets[s + 1] - r), 0) for s, n in enumerate(lengths) for r in range(offsets[s], offsets[s + 1])] + [0] * 3
+        assert got.dtype == torch.int64 and got.tolist() == want and count.made <= 9
+    assert batch.positions(0).shape == (0,)

@@ -163,3 +163,42 @@ def test_norms_with_bf16_weights_take_the_short_way(cache):
             assert all(torch.equal(x, y) for x, y in zip(run(a, b, plain), want))
     only = run(wq, None, True), run(wq.float(), None, True)
     assert all(torch.equal(x, y) for x, y in zip(*only))
+
+
+@pytest.mark.parametrize("cache", [BF16, E4M3])
+@pytest.mark.parametrize("dim,heads,kv", [(64, 16, 2), (128, 16, 2), (96, 16, 2)])
+def test_splits_of_more_than_64_tiles(cache, dim, heads, kv):
+    """A prompt whose splits have more tiles than are looked up at a time (64 of 64 keys), some of its pages none."""
+    c = Case([2048], [9000], heads, kv, dim, 16, cache, seed=10)
+    c.pages[0, 270], c.pages[0, 300] = -1, c.keys.shape[0]
+    attend(c, rows=[0, 1, 31, 255, 256, 700, 1300, 1791, 1792, 2000, 2046, 2047])
+
+
+@pytest.mark.parametrize("cache", [BF16, E4M3])
+@pytest.mark.parametrize("heads,dim", [(1, 128), (2, 64)])
+def test_tiles_of_more_than_64_splits(cache, heads, dim):
+    """Forty tokens of one key head behind 20000: a tile in more splits than weights are kept of at a time."""
+    attend(Case([40], [20040], heads, 1, dim, 16, cache, seed=11))
+
+
+@pytest.mark.parametrize("new,lengths,heads,kv", CUT + [([1, 4], [300, 70], 4, 2), ([70, 2], [200, 33], 4, 2)])
+def test_odd_values_and_codes(new, lengths, heads, kv):
+    """NaN among codes of keys and values, infinities in bf16: in tokens that all rows of a sequence see, that some see, and that none does; uncut and cut."""
+    n, length = new[0], lengths[0]
+    for cache in (BF16, E4M3):
+        c = Case(new, lengths, heads, kv, 64, 16, cache, seed=12)
+        put = lambda t, p, h, d, x: t.view(torch.uint8 if cache == E4M3 else BF16)[int(c.pages[0, p // 16]), h, p % 16].__setitem__(d, x)
+        nan = 0x7f if cache == E4M3 else math.nan
+        put(c.values, 100, 0, 3, nan)                                                 # all rows of one key head
+        put(c.values, length - 1, kv - 1, 5, nan)                                     # the last token's row alone
+        if cache == BF16:
+            put(c.values, 130, 0, 7, math.inf)
+            put(c.values, length - 1, 0, 9, -math.inf)
+        got = attend(c)
+        assert got[0, 0, 3].isnan() and got[n - 1, heads - 1, 5].isnan()
+        assert n == 1 or got[n - 2, heads - 1, 5].isfinite()
+        c = Case(new, lengths, heads, kv, 64, 16, cache, seed=13)
+        put(c.keys, length - 1, 0, 2, nan)                                            # a score of NaN, in the last token's row of a key head
+        c.to(CUDA)
+        got = paged_attention(c.q, c.keys, c.values, *c.batch()) if cache == BF16 else paged_attention(c.q, c.keys, c.values, *c.batch(), **c.scales())
+        assert got[n - 1, :heads // kv].isnan().all() and got[:n - 1].isfinite().all() and got[n:].isfinite().all() and got[n - 1, heads // kv:].isfinite().all()

@@ -31,7 +31,7 @@ def refuse_transforms(what: str) -> None:
 
 
 def _check(what: str, q, keys, values, pages, offsets, lengths, key_scale, value_scale) -> None:
-    if keys.dim() != 4 or values.shape != keys.shape or values.dtype != keys.dtype:
+    if keys.dim() != 4 or not (keys.shape[1] and keys.shape[3]) or values.shape != keys.shape or values.dtype != keys.dtype:
         raise ValueError(f"{what}: keys {keys.dtype} {tuple(keys.shape)} and values {values.dtype} {tuple(values.shape)}, expected [pages, kv heads, page size, "
                          "head_dim] of one type")
     if q.dim() != 3 or q.shape[2] != keys.shape[3] or q.shape[1] % keys.shape[1]:
@@ -281,7 +281,10 @@ class PagedKVCache:
         del self._pages[sequence], self._length[sequence], self._rows[sequence]
 
     def batch(self, sequences: "list[int]", new: "list[int]") -> PagedBatch:
-        """Room for ``new`` more tokens of each of ``sequences``, and the batch of them in this order.  Refused as a whole where pages run out."""
+        """Room for ``new`` more tokens of each of ``sequences``, and the batch of them in this order.  Refused as a whole where pages run out.
+
+        The tokens count from here on.  Where the step that puts them into the cache raises, ``shorten`` takes them out again; until then later steps
+        would see what their pages held before."""
         if len(sequences) != len(new) or len(set(sequences)) != len(sequences) or any(n < 0 for n in new):
             raise ValueError(f"{len(sequences)} sequences, each once, and {len(new)} numbers of new tokens")
         need = []

@@ -5,6 +5,7 @@ import pytest
 import torch
 
 from optimus_dl_amd import native
+from optimus_dl_amd.modules.model import GPT2, GPT2Config
 from optimus_dl_amd.modules.paged import PagedBatch, PagedKVCache, append_kv, paged_attention
 from tests.paged_helpers import E4M3, Case, bits
 
@@ -116,3 +117,26 @@ def test_positions_take_few_operations():
         want = [max(n - (offsets[s + 1] - r), 0) for s, n in enumerate(lengths) for r in range(offsets[s], offsets[s + 1])] + [0] * 3
         assert got.dtype == torch.int64 and got.tolist() == want and count.made <= 9
     assert batch.positions(0).shape == (0,)
+
+
+def test_caches_without_heads_or_of_empty_heads_are_refused():
+    ints = lambda v: torch.tensor(v, dtype=torch.int32)
+    for heads, dim in ((0, 16), (1, 0)):
+        q, cache = torch.zeros(1, 2, dim), torch.zeros(1, heads, 4, dim)
+        batch = ints([[0]]), ints([0, 1]), ints([1])
+        for call in (lambda: paged_attention(q, cache, cache, *batch), lambda: append_kv(q, q[:, :heads], q[:, :heads], cache, cache, *batch)):
+            with pytest.raises(ValueError, match="kv heads"):
+                call()
+
+
+def test_tokens_of_a_step_that_raised_are_taken_out_again():
+    model = GPT2(GPT2Config(vocab_size=32, n_embd=32, n_head=2, n_layer=1, block_size=16)).eval()
+    cache = model.new_cache(pages=4, page_size=4)
+    s, ids = cache.add(), torch.arange(9)
+    model.step(ids[:5], cache, cache.batch([s], [5]))
+    batch = cache.batch([s], [2])
+    with pytest.raises(IndexError):
+        model.step(ids[5:7] + 100, cache, batch)
+    cache.shorten(s, cache.length(s) - 2)
+    got = model.step(ids[5:9], cache, cache.batch([s], [4]))["logits"]
+    assert torch.allclose(got, model(ids[None])["logits"][0, 5:].detach(), atol=1e-5)

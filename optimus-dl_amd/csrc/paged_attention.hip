@@ -489,11 +489,13 @@ struct Caps {
     float c, in, out;
     bool negative;
 };
+template <bool CAP>
 __device__ __forceinline__ Caps caps_of(const Attend &a, int kv_head) {
+    auto one = [](float v) { return bits_to_float((uint32_t)__builtin_amdgcn_readfirstlane((int)float_to_bits(v))); };       // (the same in all lanes: a scalar register)
     const float of_keys = a.p.key_scale ? a.p.key_scale[kv_head] : 1.0f, scale = a.scale * __builtin_fabsf(of_keys);
-    if (a.softcap > 0.0f) return {1.0f, 2.0f * kLog2e * scale / a.softcap, a.softcap * kLog2e, of_keys < 0.0f};
+    if (CAP) return {1.0f, one(2.0f * kLog2e * scale / a.softcap), one(a.softcap * kLog2e), of_keys < 0.0f};
     const float c = scale * kLog2e;
-    return {c == 0.0f ? __FLT_DENORM_MIN__ : c, 0.0f, 0.0f, of_keys < 0.0f};
+    return {one(c == 0.0f ? __FLT_DENORM_MIN__ : c), 0.0f, 0.0f, of_keys < 0.0f};
 }
 
 // ---------------------------------------------------------------------------------------------------------------- keys and values on their way to LDS
@@ -574,7 +576,7 @@ __device__ __forceinline__ void make_finite(uint32_t vt, int first, int step, in
 __device__ __forceinline__ uint32_t lds_base(uint8_t *lds) { return (uint32_t)(uintptr_t)(lds_u8 *)lds; }
 
 // ---------------------------------------------------------------------------------------------------------------- few rows
-template <int D, bool E4M3>
+template <int D, bool E4M3, bool CAP>
 __global__ __launch_bounds__(kFewWaves *kWave, E4M3 ? 2 : 1) void attend_few_kernel(Attend a) {
     extern __shared__ __attribute__((aligned(1024))) uint8_t lds[];
     constexpr int kTile = kFewKeys * 2 * D, kStages = E4M3 ? 1 : 2, kStep = kFewKeys * kFewWaves;
@@ -586,7 +588,7 @@ __global__ __launch_bounds__(kFewWaves *kWave, E4M3 ? 2 : 1) void attend_few_ker
     const Range range = range_of<kFewRows, kStep>(a, it);
     const int rows = it.run.n * a.group, row0 = it.tile * kFewRows, row = row0 + lane % 32, before = it.length - it.run.n;
     const int pos = before + row / a.group, pos0 = before + row0 / a.group, pos1 = before + min(row0 + kFewRows - 1, rows - 1) / a.group;
-    const Caps caps = caps_of(a, head);
+    const Caps caps = caps_of<CAP>(a, head);
     const int32_t *table = a.p.table + it.seq * a.p.table_stride;
     Rows32<D, 1> w;
     w.load_q(a, it.run, row, head, E4M3 && caps.negative);
@@ -603,7 +605,7 @@ __global__ __launch_bounds__(kFewWaves *kWave, E4M3 ? 2 : 1) void attend_few_ker
         }
         if (pass == kFinite) make_finite(kt + kTile, lane, kWave, kTile / 16);
         w.scores(kt);
-        if (a.softcap > 0.0f) w.cap(caps.in, caps.out);
+        if (CAP) w.cap(caps.in, caps.out);
         if (held != ~0u || base + kFewKeys - 1 > pos0 || base <= pos1 - a.window) w.hide(seen >> h4);
         w.weights(caps.c);
         w.sums(kt + kTile);
@@ -730,7 +732,7 @@ struct Eight {
     }
 };
 
-template <int D, int C, bool E4M3>
+template <int D, int C, bool E4M3, bool CAP>
 __global__ __launch_bounds__(kManyWaves *kWave) void attend_many_kernel(Attend a, int clear) {
     extern __shared__ __attribute__((aligned(1024))) uint8_t lds[];
     constexpr int kTile = kManyKeys * 2 * D, kMine = kManyKeys / kManyWaves;
@@ -743,7 +745,7 @@ __global__ __launch_bounds__(kManyWaves *kWave) void attend_many_kernel(Attend a
     const Range range = range_of<kManyRows, kManyKeys>(a, it);
     const int rows = it.run.n * a.group, row0 = it.tile * kManyRows + 32 * wave, row = row0 + lane % 32, before = it.length - it.run.n;
     const int pos = before + row / a.group, pos0 = before + row0 / a.group, pos1 = before + min(row0 + 31, rows - 1) / a.group;
-    const Caps caps = caps_of(a, head);
+    const Caps caps = caps_of<CAP>(a, head);
     const int32_t *table = a.p.table + it.seq * a.p.table_stride;
     const int tiles = (range.end - range.first + kManyKeys - 1) / kManyKeys;
     Rows32<D, 2, C> w;
@@ -845,7 +847,7 @@ __global__ __launch_bounds__(kManyWaves *kWave) void attend_many_kernel(Attend a
         turn();
         for (int t = 0; t < tiles; ++t) {
             const int base = base_of(t);
-            if (a.softcap > 0.0f) w.cap(caps.in, caps.out);
+            if (CAP) w.cap(caps.in, caps.out);
             if (held[0] != ~0ull || base + kManyKeys - 1 > pos0 || base <= pos1 - a.window) w.hide(seen_of(pos, base, a.window, held[0]) >> h4);
             w.weights(caps.c);
             fetch(t + 2, keys + b2, values + b1);
@@ -985,7 +987,7 @@ int check(const char *who, int64_t heads, int64_t most_new, const odl_fp8_paged_
     return ODL_OK;
 }
 
-template <int D, int C>
+template <int D, int C, bool CAP>
 int launch(Attend &a, const Plan &plan, int64_t most_rows, float *workspace, hipStream_t stream) {
     const int64_t kv = a.p.kv_heads, rows = (int64_t)a.p.rows * a.group, seqs = a.p.seqs < a.p.rows ? a.p.seqs : a.p.rows;
     // no more tiles than sequences (those that fill no tile) and rows / tile; splits that begin anew: see `find`
@@ -1000,8 +1002,8 @@ int launch(Attend &a, const Plan &plan, int64_t most_rows, float *workspace, hip
         a.partial = workspace, a.slots = slots_of(kManyTarget);
         const int clear = !plan.few;
         const dim3 grid((unsigned)many_blocks);
-        if (a.p.e4m3) hipLaunchKernelGGL((attend_many_kernel<D, C, true>), grid, dim3(kManyWaves * kWave), many_lds(D), stream, a, clear);
-        else hipLaunchKernelGGL((attend_many_kernel<D, C, false>), grid, dim3(kManyWaves * kWave), many_lds(D), stream, a, clear);
+        if (a.p.e4m3) hipLaunchKernelGGL((attend_many_kernel<D, C, true, CAP>), grid, dim3(kManyWaves * kWave), many_lds(D), stream, a, clear);
+        else hipLaunchKernelGGL((attend_many_kernel<D, C, false, CAP>), grid, dim3(kManyWaves * kWave), many_lds(D), stream, a, clear);
         if (a.p.reach > kManyKeys)
             hipLaunchKernelGGL((attend_join_kernel<D, kManyRows, kManyKeys, kJoinMany>), dim3(joins(kManyTarget), kManyRows / kJoinMany), dim3(256), 0, stream, a, (uint32_t)kManyTarget);
         workspace += floats_of(kManyRows, kManyTarget, D);
@@ -1010,8 +1012,8 @@ int launch(Attend &a, const Plan &plan, int64_t most_rows, float *workspace, hip
         a.least_rows = 0, a.most_rows = plan.many ? plan.least : INT32_MAX;
         a.partial = workspace, a.slots = slots_of(few);
         const dim3 grid((unsigned)few_blocks);
-        if (a.p.e4m3) hipLaunchKernelGGL((attend_few_kernel<D, true>), grid, dim3(kFewWaves * kWave), few_lds(D, true), stream, a);
-        else hipLaunchKernelGGL((attend_few_kernel<D, false>), grid, dim3(kFewWaves * kWave), few_lds(D, false), stream, a);
+        if (a.p.e4m3) hipLaunchKernelGGL((attend_few_kernel<D, true, CAP>), grid, dim3(kFewWaves * kWave), few_lds(D, true), stream, a);
+        else hipLaunchKernelGGL((attend_few_kernel<D, false, CAP>), grid, dim3(kFewWaves * kWave), few_lds(D, false), stream, a);
         if (a.p.reach > kUncut * kFewKeys * kFewWaves)
             hipLaunchKernelGGL((attend_join_kernel<D, kFewRows, kFewKeys * kFewWaves, kJoinFew>), dim3(joins(few), (unsigned)(((most_rows < kFewRows ? most_rows : kFewRows) + kJoinFew - 1) / kJoinFew)), dim3(256), 0, stream, a,
                                (uint32_t)few);
@@ -1053,7 +1055,8 @@ extern "C" int odl_fp8_paged_attention(const void *q, const int64_t *q_strides, 
     hipStream_t stream = reinterpret_cast<hipStream_t>(stream_);
     const int64_t most_rows = (most_new < 1 ? 1 : most_new < a.p.rows ? most_new : a.p.rows) * a.group;
     // heads of up to 96: a quarter of the products of 128 less (the prompts above 206 -> 192 us; the kernel for few rows waits for memory, and has one form)
-    if (a.p.dim > 96) return launch<128, 128>(a, plan, most_rows, workspace, stream);
-    if (a.p.dim > 64) return launch<128, 96>(a, plan, most_rows, workspace, stream);
-    return launch<64, 64>(a, plan, most_rows, workspace, stream);
+    // Kernels with a cap are apart: its code in the loop costs the others 1 to 4 per cent (one token behind 200, 12 heads of 64: 7.9 and 8.2 us; the chunk above 519 and 527).
+#define ODL_ATTEND(D, C) (softcap > 0.0f ? launch<D, C, true>(a, plan, most_rows, workspace, stream) : launch<D, C, false>(a, plan, most_rows, workspace, stream))
+    return a.p.dim > 96 ? ODL_ATTEND(128, 128) : a.p.dim > 64 ? ODL_ATTEND(128, 96) : ODL_ATTEND(64, 64);
+#undef ODL_ATTEND
 }

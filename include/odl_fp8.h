@@ -813,7 +813,9 @@ int odl_fp8_append_kv_typed(const void *q, const int64_t *q_strides, const void 
  * Attention of the new tokens over the cache, which holds them.  Row at position p, of a head whose keys are those of head / (heads / kv_heads):
  *   s_i = scale * q . key_i,  softcap > 0: s_i = softcap * tanh(s_i / softcap),  for max(0, p - window + 1) <= i <= p  (window 0: from 0)
  *   out = sum_i e^(s_i - m) value_i / sum_i e^(s_i - m)
- * Products of bf16 (E4M3 codes are widened exactly) with fp32 sums; weights round to bf16 in front of the second product.  Sums and maxima fp32.
+ * Products of bf16 (E4M3 codes are widened exactly) with fp32 sums; weights round to bf16 in front of the second product.  Sums and maxima fp32: of values times weights
+ * of up to 2^8 before they are divided, so that values beyond 2^120 / (number of keys) may pass fp32's range.  A cap of up to 256 is off by 5 * 2^-24 of itself
+ * at most, a larger one by some 2^-24 of the score.
  * Keys and values that a row does not see do not reach it, NaN and infinities included.  A row that sees nothing, or no score above -inf, and rows that belong to
  * nobody, answer 0.  q [rows, heads, head_dim] bf16 with strides as above; out bf16 [rows, heads, head_dim].
  * most_new: the most new tokens of a sequence where the caller knows it, else `rows`: chooses kernels, results do not depend on its truth.

@@ -12,11 +12,11 @@
 // part is its own (`find`): lengths never pass the host.
 //
 // Measured (calls in a row, host included; a large copy moves 5.1 TB/s on this card, a large product in bf16 makes 1206 TFLOP/s):
-//   few   64 sequences of up to 8192 tokens, 32 heads on 8 of 128, bf16               311 us   5.1 TB/s
-//         1 sequence of 131072 tokens, the same heads                                 115 us   4.7 TB/s  (of which the join 5 to 15)
-//         32 sequences of 4099, 5 new tokens of each, E4M3                             72 us   3.8 TB/s  (codes pass registers; the join 10)
-//   many  2048 new tokens behind 14336, 32 heads on 8 of 128                          500 us   1030 TFLOP/s  (the card runs at some 2.0 GHz meanwhile)
-//         12 prompts of up to 1000 tokens behind up to 3000, 16 heads on 4 of 96, capped, a window of 1500: 188 us  (288 tiles on 256 compute units: two rounds)
+//   few   64 sequences of up to 8192 tokens, 32 heads on 8 of 128, bf16               298 us   5.4 TB/s  (E4M3 191, 4.2: codes pass registers)
+//         1 sequence of 131072 tokens, the same heads                                 110 us   4.9 TB/s  (of which the join 5 to 10; E4M3 71)
+//         32 sequences of 4099, 5 new tokens of each, E4M3                             69 us   3.9 TB/s  (the join 10; bf16 110)
+//   many  2048 new tokens behind 14336, 32 heads on 8 of 128                          497 us   1037 TFLOP/s  (the card runs at some 2.0 GHz meanwhile; E4M3 564, capped 670)
+//         12 prompts of up to 1000 tokens behind up to 3000, 16 heads on 4 of 96, capped, a window of 1500: 171 us  (288 tiles on 256 compute units: two rounds; without the cap 128)
 // A sequence with up to 32 rows a key head fills one tile of the first kernel; from there on that would read the cache again for every 32 rows.
 #include "paged.h"
 

@@ -91,7 +91,8 @@ def verify_drafts(logits: torch.Tensor, tokens: torch.Tensor, offsets: torch.Ten
     n_vocab: columns in use.  A draft that is no token does not hold.  A row with NaN or +inf, or of -inf only, stops its sequence: token -1, logprob
     NaN.  Rows behind the last sequence answer -1 and 0.
 
-    bf16 and fp32 logits on the GPU (rows at any distance and alignment): three launches, sums in 64 bits, so that tokens do not depend on how a row is cut."""
+    bf16 and fp32 logits on the GPU (rows at any distance and alignment): three launches, sums in 64 bits, so that how a row is cut, by the
+    number of rows, settles one draw in some 10^13 otherwise."""
     if logits.is_cuda and untransformed():
         r = native.plain_verify_drafts(logits, tokens, offsets, uniforms, draft_logits, temperature, n_vocab)
         if r is not None:
